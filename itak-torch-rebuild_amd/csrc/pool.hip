@@ -4,6 +4,7 @@
 // All validation happens here, in the reference's order, before anything is enqueued.
 #include "../../include/itak_hip_kv.h"
 #include "internal.h"
+#include "errors.h"
 #include "host_ring.h"
 #include "host_turns.h"
 #include "load_room.h"
@@ -72,13 +73,6 @@ struct LayerInfo {
     uint64_t window = 0;  // attention window; 0 on a global layer
     uint32_t ring = 0;    // storage rows of the ring (a multiple of 32); 0 on a global layer
 };
-
-struct ErrorState {
-    std::string message;
-    itak_error_info info{};
-};
-
-thread_local ErrorState g_create_error;
 
 // ---- the split workspace of the allocation-free entry point --------------------------------
 // itak_attention_step_device_noalloc may not allocate, so its split workspace is this array:
@@ -202,136 +196,6 @@ struct itak_pool {
 };
 
 namespace {
-
-// ------------------------------------------------------------------------------ debug channel
-// attention::diag (crates/attention/src/diag.rs:13-33,71-79): off by default; the switch or
-// ITAK_HIP_KV_DEBUG in the environment (any value but "0" or empty, looked up at every event as
-// the reference looks its variable up) turns one stderr line per event on.
-std::atomic<bool> g_debug_enabled{false};
-
-bool diag_enabled() {
-    if (g_debug_enabled.load(std::memory_order_relaxed)) return true;
-    const char *v = getenv("ITAK_HIP_KV_DEBUG");
-    return v && v[0] != '\0' && !(v[0] == '0' && v[1] == '\0');
-}
-
-__attribute__((format(printf, 1, 2))) void diag_emit(const char *fmt, ...) {
-    char buf[1024];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof(buf), fmt, ap);
-    va_end(ap);
-    fprintf(stderr, "[itak_hip_kv::diag] %s\n", buf);
-}
-
-#define ITAK_DIAG(...)                          \
-    do {                                        \
-        if (diag_enabled()) diag_emit(__VA_ARGS__); \
-    } while (0)
-
-// ------------------------------------------------------------------------------ errors
-
-itak_status set_error(ErrorState &e, int32_t code, const char *what, uint64_t a, uint64_t b,
-                      uint64_t c, uint64_t d, const char *fmt, ...) {
-    e.info = itak_error_info{};
-    e.info.code = code;
-    if (what) snprintf(e.info.what, sizeof(e.info.what), "%s", what);
-    e.info.a = a;
-    e.info.b = b;
-    e.info.c = c;
-    e.info.d = d;
-    char buf[1024];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof(buf), fmt, ap);
-    va_end(ap);
-    e.message = buf;
-    ITAK_DIAG("refused code=%d: %s", int(code), buf);  // every refusal says why
-    return code;
-}
-
-#define ULL(x) static_cast<unsigned long long>(x)
-
-// The Display texts of AttentionError (crates/attention/src/error.rs:129-214).
-itak_status zero_dimension(ErrorState &e, const char *what) {
-    return set_error(e, ITAK_ZERO_DIMENSION, what, 0, 0, 0, 0, "%s must be positive, got 0", what);
-}
-itak_status invalid_window(ErrorState &e, uint64_t window) {
-    return set_error(e, ITAK_INVALID_WINDOW, nullptr, window, 0, 0, 0,
-                     "sliding window must be positive, got %llu", ULL(window));
-}
-itak_status size_overflow(ErrorState &e, const char *what) {
-    return set_error(e, ITAK_SIZE_OVERFLOW, what, 0, 0, 0, 0, "%s: element count overflows usize",
-                     what);
-}
-itak_status shape_mismatch(ErrorState &e, const char *what, uint64_t expected, uint64_t actual) {
-    return set_error(e, ITAK_SHAPE_MISMATCH, what, expected, actual, 0, 0,
-                     "%s: got %llu, expected %llu", what, ULL(actual), ULL(expected));
-}
-itak_status invalid_layer(ErrorState &e, uint64_t layer, uint64_t layer_count) {
-    return set_error(e, ITAK_INVALID_LAYER, nullptr, layer, layer_count, 0, 0,
-                     "layer %llu out of range, cache has %llu layers", ULL(layer),
-                     ULL(layer_count));
-}
-itak_status out_of_order(ErrorState &e, uint64_t layer, uint64_t expected, uint64_t actual) {
-    return set_error(e, ITAK_OUT_OF_ORDER_POSITION, nullptr, layer, expected, actual, 0,
-                     "layer %llu appends must be in order: expected position %llu, got %llu",
-                     ULL(layer), ULL(expected), ULL(actual));
-}
-itak_status non_divisible(ErrorState &e, uint64_t q_heads, uint64_t kv_heads) {
-    return set_error(e, ITAK_NON_DIVISIBLE_HEADS, nullptr, q_heads, kv_heads, 0, 0,
-                     "%llu query heads do not divide evenly across %llu KV heads", ULL(q_heads),
-                     ULL(kv_heads));
-}
-itak_status no_visible_keys(ErrorState &e, uint64_t position) {
-    return set_error(e, ITAK_NO_VISIBLE_KEYS, nullptr, position, 0, 0, 0,
-                     "query at position %llu has no visible keys", ULL(position));
-}
-itak_status checkpoint_busy(ErrorState &e) {
-    return set_error(e, ITAK_CHECKPOINT_BUSY, nullptr, 0, 0, 0, 0,
-                     "a checkpoint is already outstanding on this cache; release it before "
-                     "taking another");
-}
-itak_status stale_checkpoint(ErrorState &e, uint64_t serial) {
-    return set_error(e, ITAK_STALE_CHECKPOINT, nullptr, serial, 0, 0, 0,
-                     "checkpoint %llu is not this cache's live checkpoint (already released or "
-                     "foreign)",
-                     ULL(serial));
-}
-itak_status range_exceeded(ErrorState &e, uint64_t layer, uint64_t position, uint64_t limit) {
-    return set_error(e, ITAK_CHECKPOINT_RANGE_EXCEEDED, nullptr, layer, position, limit, 0,
-                     "layer %llu append at position %llu is outside the live checkpoint's saved "
-                     "range (first unsaved position %llu); refusing so a later rewind cannot meet "
-                     "a slot it cannot restore",
-                     ULL(layer), ULL(position), ULL(limit));
-}
-itak_status not_fresh(ErrorState &e, uint64_t layer, uint64_t appended) {
-    return set_error(e, ITAK_BULK_RESTORE_NOT_FRESH, nullptr, layer, appended, 0, 0,
-                     "layer %llu already holds %llu appended positions; bulk restore installs "
-                     "into a fresh layer only",
-                     ULL(layer), ULL(appended));
-}
-itak_status rewind_range(ErrorState &e, uint64_t layer, uint64_t base, uint64_t appended,
-                         uint64_t target) {
-    return set_error(e, ITAK_REWIND_OUT_OF_RANGE, nullptr, layer, base, appended, target,
-                     "rewind target %llu is outside layer %llu's checkpoint range [%llu, %llu]",
-                     ULL(target), ULL(layer), ULL(base), ULL(appended));
-}
-itak_status hip_error(ErrorState &e, hipError_t code, const char *doing) {
-    return set_error(e, ITAK_HIP_ERROR, doing, uint64_t(code), 0, 0, 0, "%s: HIP error %d (%s)",
-                     doing, int(code), hipGetErrorString(code));
-}
-itak_status invalid_argument(ErrorState &e, const char *what) {
-    return set_error(e, ITAK_INVALID_ARGUMENT, what, 0, 0, 0, 0, "invalid argument: %s", what);
-}
-itak_status capacity_exceeded(ErrorState &e, uint64_t layer, uint64_t need, uint64_t capacity) {
-    return set_error(e, ITAK_CAPACITY_EXCEEDED, nullptr, layer, need, capacity, 0,
-                     "layer %llu would hold %llu positions but the pool's slots hold %llu",
-                     ULL(layer), ULL(need), ULL(capacity));
-}
-itak_status unsupported(ErrorState &e, const char *what) {
-    return set_error(e, ITAK_UNSUPPORTED, what, 0, 0, 0, 0, "unsupported: %s", what);
-}
 
 #define HIP_TRY(pool, call, doing)                                   \
     do {                                                             \
@@ -1354,17 +1218,17 @@ extern "C" {
 uint32_t itak_abi_version(void) { return 1; }
 
 const char *itak_last_error(const itak_pool *pool) {
-    return pool ? pool->err.message.c_str() : g_create_error.message.c_str();
+    return pool ? pool->err.message.c_str() : thread_error().message.c_str();
 }
 
 itak_status itak_last_error_info(const itak_pool *pool, itak_error_info *out) {
     if (!out) return ITAK_INVALID_ARGUMENT;
-    *out = pool ? pool->err.info : g_create_error.info;
+    *out = pool ? pool->err.info : thread_error().info;
     return ITAK_OK;
 }
 
 itak_status itak_pool_create(const itak_pool_config *config, itak_pool **out) {
-    ErrorState &e = g_create_error;
+    ErrorState &e = thread_error();
     if (!out) return invalid_argument(e, "out is null");
     *out = nullptr;
     if (!config) return invalid_argument(e, "config is null");
@@ -2048,7 +1912,7 @@ uint64_t itak_kv_checksum_blocks(const void *bytes, uint64_t count) {
 itak_status itak_itkv_validate(const itak_itkv_header *header, const itak_itkv_layer *layers,
                                uint64_t blocks, const uint64_t *key_floats,
                                const uint64_t *value_floats) {
-    ErrorState &e = g_create_error;
+    ErrorState &e = thread_error();
     if (!header || (blocks && (!layers || !key_floats || !value_floats)))
         return invalid_argument(e, "header, layers or the float counts are null");
     ItkvError err;
@@ -2063,7 +1927,7 @@ itak_status itak_itkv_encode(const itak_itkv_header *header, const char *fingerp
                              const float *const *keys, const uint64_t *key_floats,
                              const float *const *values, const uint64_t *value_floats, void *out,
                              uint64_t capacity, uint64_t *written) {
-    ErrorState &e = g_create_error;
+    ErrorState &e = thread_error();
     itak_status st = itak_itkv_validate(header, layers, blocks, key_floats, value_floats);
     if (st != ITAK_OK) return st;
     if (!written) return invalid_argument(e, "written is null");
@@ -2098,7 +1962,7 @@ itak_status itak_itkv_encode(const itak_itkv_header *header, const char *fingerp
 
 itak_status itak_itkv_decode(const void *bytes, uint64_t len, itak_itkv_header *header,
                              itak_itkv_layer *layers, uint64_t layers_capacity) {
-    ErrorState &e = g_create_error;
+    ErrorState &e = thread_error();
     if (!bytes || !header) return invalid_argument(e, "bytes or header is null");
     ItkvHeader h;
     std::vector<ItkvLayer> ls;
@@ -3335,7 +3199,7 @@ itak_status itak_probe_read_device(itak_pool *pool, const void *src_dev, uint64_
 }
 
 void itak_set_debug_enabled(int32_t enabled) {
-    g_debug_enabled.store(enabled != 0, std::memory_order_relaxed);
+    set_diag_enabled(enabled != 0);
 }
 int32_t itak_debug_enabled(void) { return diag_enabled() ? 1 : 0; }
 
