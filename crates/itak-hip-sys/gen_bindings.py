@@ -13,7 +13,7 @@ OUT = os.path.join(HERE, "src", "lib.rs")
 
 SCALARS = {
     "itak_status": "itak_status", "int32_t": "i32", "uint32_t": "u32", "uint64_t": "u64",
-    "uint16_t": "u16", "uint8_t": "u8", "float": "f32", "char": "c_char", "void": "c_void",
+    "uint16_t": "u16", "uint8_t": "u8", "int64_t": "i64", "float": "f32", "double": "f64", "char": "c_char", "void": "c_void",
     "int": "i32",
 }
 

@@ -56,6 +56,10 @@ pub const ITAK_POOL_MERGE_IN_LAUNCH: u32 = 2;
 pub const ITAK_POOL_DIE_MERGE: u32 = 4;
 pub const ITAK_POOL_Q_TWO_HALVES: u32 = 8;
 pub const ITAK_POOL_PREP_BY_LAUNCH: u32 = 16;
+pub const ITAK_ELEM_BF16: u32 = 2;
+pub const ITAK_ROTATION_PLAIN: u32 = 0;
+pub const ITAK_ROTATION_LINEAR: u32 = 1;
+pub const ITAK_ROTATION_YARN: u32 = 2;
 
 /// Opaque handle.
 #[repr(C)]
@@ -66,6 +70,18 @@ pub struct itak_pool {
 /// Opaque handle.
 #[repr(C)]
 pub struct itak_store {
+    _private: [u8; 0],
+}
+
+/// Opaque handle.
+#[repr(C)]
+pub struct itak_rotation {
+    _private: [u8; 0],
+}
+
+/// Opaque handle.
+#[repr(C)]
+pub struct itak_paged {
     _private: [u8; 0],
 }
 
@@ -197,6 +213,56 @@ pub struct itak_prep_params {
     pub rotary_dim: u32,
 }
 
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct itak_rotation_config {
+    pub base: f64,
+    pub rotary_dim: u32,
+    pub interleaved: u32,
+    pub scaling: u32,
+    pub device: i32,
+    pub factor: f64,
+    pub original_positions: f64,
+    pub beta_fast: f64,
+    pub beta_slow: f64,
+    pub amplitude: f64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct itak_rows {
+    pub data: *mut c_void,
+    pub elem: u32,
+    pub heads: u32,
+    pub row_stride: u64,
+    pub head_stride: u64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct itak_paged_config {
+    pub layer_count: u32,
+    pub elem: u32,
+    pub num_kv_heads: u64,
+    pub head_dim: u64,
+    pub page_count: u64,
+    pub page_rows: u32,
+    pub max_sequences: u32,
+    pub max_table_pages: u64,
+    pub device: i32,
+    pub flags: u32,
+    pub storage: *mut c_void,
+    pub storage_bytes: u64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct itak_paged_item {
+    pub position: u64,
+    pub rows: u32,
+    pub pages: u32,
+}
+
 #[link(name = "itak_hip_kv")]
 extern "C" {
     pub fn itak_abi_version() -> u32;
@@ -265,6 +331,22 @@ extern "C" {
     pub fn itak_attention_device(pool: *mut itak_pool, layer: u64, items: *const itak_batch_item, item_count: u32, q_dev: *const f32, out_dev: *mut f32, num_q_heads: u64, scale: f32, softcap: f32) -> itak_status;
     pub fn itak_kv_append_device(pool: *mut itak_pool, layer: u64, items: *const itak_batch_item, item_count: u32, k_dev: *const f32, v_dev: *const f32) -> itak_status;
     pub fn itak_convert_f32_to_f16_device(pool: *mut itak_pool, src_dev: *const f32, dst_dev: *mut u16, count: u64) -> itak_status;
+    pub fn itak_rotation_create(config: *const itak_rotation_config, out: *mut *mut itak_rotation) -> itak_status;
+    pub fn itak_rotation_destroy(rotation: *mut itak_rotation);
+    pub fn itak_rotation_frequencies(rotation: *const itak_rotation, frequencies_out: *mut f64, amplitude_out: *mut f64) -> itak_status;
+    pub fn itak_rotate_device(rotation: *const itak_rotation, hip_stream: *mut c_void, head_dim: u64, rows: u64, positions_dev: *const i64, inputs: *const itak_rows, outputs: *const itak_rows, tensors: u32, inverse: u32) -> itak_status;
+    pub fn itak_paged_storage_bytes(config: *const itak_paged_config) -> u64;
+    pub fn itak_paged_create(config: *const itak_paged_config, out: *mut *mut itak_paged) -> itak_status;
+    pub fn itak_paged_destroy(paged: *mut itak_paged);
+    pub fn itak_paged_last_error(paged: *const itak_paged) -> *const c_char;
+    pub fn itak_paged_last_error_info(paged: *const itak_paged, out: *mut itak_error_info) -> itak_status;
+    pub fn itak_paged_set_stream(paged: *mut itak_paged, hip_stream: *mut c_void) -> itak_status;
+    pub fn itak_paged_synchronize(paged: *mut itak_paged) -> itak_status;
+    pub fn itak_paged_storage(paged: *const itak_paged) -> *mut c_void;
+    pub fn itak_paged_set_batch(paged: *mut itak_paged, items: *const itak_paged_item, count: u32, pages: *const u32, page_ids: u64) -> itak_status;
+    pub fn itak_paged_append_device(paged: *mut itak_paged, layer: u64, k: *const itak_rows, v: *const itak_rows, rotation: *const itak_rotation) -> itak_status;
+    pub fn itak_paged_attention_device(paged: *mut itak_paged, layer: u64, q: *const itak_rows, out: *const itak_rows, scale: f32, softcap: f32, window: u64, rotation: *const itak_rotation) -> itak_status;
+    pub fn itak_paged_step_device(paged: *mut itak_paged, layer: u64, q: *const itak_rows, k: *const itak_rows, v: *const itak_rows, out: *const itak_rows, scale: f32, softcap: f32, window: u64, rotation: *const itak_rotation) -> itak_status;
     pub fn itak_set_debug_enabled(enabled: i32);
     pub fn itak_debug_enabled() -> i32;
     pub fn itak_probe_copy_device(pool: *mut itak_pool, src_dev: *const c_void, dst_dev: *mut c_void, bytes: u64) -> itak_status;

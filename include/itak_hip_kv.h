@@ -677,6 +677,153 @@ itak_status itak_kv_append_device(itak_pool *pool, uint64_t layer, const itak_ba
 itak_status itak_convert_f32_to_f16_device(itak_pool *pool, const float *src_dev,
                                            uint16_t *dst_dev, uint64_t count);
 
+/* ---- rotary positions ------------------------------------------------------------------
+   The rotation of queries and keys by their positions, on its own or on the way into a paged cache (below).
+   Channels 2i and 2i+1 (interleaved) or i and i + rotary_dim/2 (half split) of a head turn by the angle
+   position * f(i); channels from rotary_dim on pass through. No counterpart for the scaled forms in the
+   reference, whose rotations (crates/torch-math/src/rope.rs:63-117, rope_interleaved.rs:65-117) are the plain one.
+   Angles are reduced in 64 bits, the products are f32, and what is stored is rounded once to its own type. */
+
+enum { ITAK_ELEM_BF16 = 2 }; /* of tensors and pages below; an itak_pool stores f32 or f16 */
+
+enum {
+    /* f(i) = base^(-2i/rotary_dim). */
+    ITAK_ROTATION_PLAIN = 0,
+    /* f(i) / factor: positions interpolated. */
+    ITAK_ROTATION_LINEAR = 1,
+    /* YaRN: pairs that turn at least beta_fast times over original_positions keep f(i), those that turn at most
+       beta_slow times take f(i) / factor, and between the two a ramp over the pair's index blends them. */
+    ITAK_ROTATION_YARN = 2
+};
+
+typedef struct itak_rotation itak_rotation;
+
+typedef struct itak_rotation_config {
+    double base;               /* > 1 */
+    uint32_t rotary_dim;       /* even, 2 .. 256 */
+    uint32_t interleaved;      /* 1: adjacent pairs, 0: half split */
+    uint32_t scaling;          /* ITAK_ROTATION_* */
+    int32_t device;            /* HIP device ordinal */
+    double factor;             /* >= 1; read unless plain */
+    double original_positions; /* > 0; read by YARN, with the two below: beta_fast > beta_slow > 0 */
+    double beta_fast;          /* 0 = 32 */
+    double beta_slow;          /* 0 = 1 */
+    double amplitude;          /* cosine and sine are multiplied by it; 0 = 1, of YARN 0.1 ln(factor) + 1 */
+} itak_rotation_config;
+
+/* A view of rows x heads x head_dim elements in device memory: element (row, head, channel) lies at
+   row * row_stride + head * head_stride + channel, in elements; 0 for both strides: dense. Rows and heads may lie in any order and
+   with any gaps (slices of one projection's output, heads first); views that start on 16 bytes with strides that
+   are multiples of 16 bytes are read and written 16 bytes at a time, others element by element. A view that is
+   written must not hold the same element twice, and may share memory with one that is read only by being the same view. */
+typedef struct itak_rows {
+    void *data;
+    uint32_t elem;  /* ITAK_ELEM_* */
+    uint32_t heads;
+    uint64_t row_stride;
+    uint64_t head_stride;
+} itak_rows;
+
+/* Computes the frequencies and places them on the device. The handle does not change afterwards: any thread and
+   stream of its device may use it. Of a failure of it and of the two calls below itak_last_error(NULL) tells. */
+itak_status itak_rotation_create(const itak_rotation_config *config, itak_rotation **out);
+/* Waits for the device to be done with it. Not while a captured graph that names it may still be replayed. */
+void itak_rotation_destroy(itak_rotation *rotation);
+/* The rotary_dim / 2 frequencies, radians a position, and the amplitude. Either may be NULL. */
+itak_status itak_rotation_frequencies(const itak_rotation *rotation, double *frequencies_out, double *amplitude_out);
+/* Turns up to four tensors by the same rows' positions in one launch on `hip_stream`: outputs[i] = rotation of inputs[i],
+   each rows x inputs[i].heads x head_dim, an output of its input's type and either the same view or disjoint
+   from it. positions_dev: [rows] int64 on the device, any sign, below 2^31 in magnitude. `inverse` turns back
+   (by the negative angles, the same amplitude): the transpose, which is what the gradients of rotated rows go through. */
+itak_status itak_rotate_device(const itak_rotation *rotation, void *hip_stream, uint64_t head_dim, uint64_t rows,
+                               const int64_t *positions_dev, const itak_rows *inputs, const itak_rows *outputs,
+                               uint32_t tensors, uint32_t inverse);
+
+/* ---- paged cache -----------------------------------------------------------------------
+   Keys and values in pages of page_rows positions each, in any order in one storage, where a pool gives every slot
+   capacity_rows positions of its own. A sequence is a table of page ids; which pages are free, and which
+   sequences share a prefix's pages, is the caller's to keep (a page is copied by copying its bytes in every layer). No counterpart
+   in the reference. The storage is
+
+       [layer][page][side][kv_head][row of the page][channel], side 0 = keys, 1 = values,
+
+   elements of ITAK_ELEM_F16 or ITAK_ELEM_BF16, dense. Position p of a sequence is row p % page_rows of its page p / page_rows.
+   Rows no position stands in are never read for a result and never written.
+
+   Tensors of a call are ITAK_ELEM_F32 or of the pages' own type. Scores, softmax and sums are f32. With tensors of
+   the pages' type the softmax weights are rounded to that type once (f16 2^-11, bf16 2^-8 relative to each) and
+   the output once; with f32 tensors queries and weights enter the matrix pipe as several halves each,
+   which leaves 2^-22 of them (bf16: 2^-24 of queries, 2^-16 of weights). An f16 query's or key's channel beyond 65504 is infinite.
+   A row that is not finite reaches the outputs of exactly the queries that see its position; one difference is left on f16 pages: a weight
+   below about 2^-32 of its row's largest is zero, and zero times an infinite value is NaN.
+   Results do not depend on the pages' order or on what other sequences the batch holds beyond rounding (sums are cut
+   into other pieces), and are the same from call to call.
+
+   A handle is used from one thread at a time, on the stream it was given (itak_paged_set_stream), as an itak_pool is; its
+   calls, and replays of graphs that hold them, share one batch and one workspace and are to run one after another. */
+
+typedef struct itak_paged itak_paged;
+
+typedef struct itak_paged_config {
+    uint32_t layer_count;
+    uint32_t elem;            /* ITAK_ELEM_F16 or ITAK_ELEM_BF16 */
+    uint64_t num_kv_heads;
+    uint64_t head_dim;        /* a multiple of 8, up to 256 */
+    uint64_t page_count;      /* below 2^31 */
+    uint32_t page_rows;       /* a power of two, 16 .. 1024 */
+    uint32_t max_sequences;   /* of one batch, up to 1024 */
+    uint64_t max_table_pages; /* page ids of one batch over all its sequences; 0 = page_count */
+    int32_t device;           /* HIP device ordinal */
+    uint32_t flags;           /* 0 */
+    void *storage;            /* device memory that starts on 16 bytes, the caller's to keep until the handle is gone;
+                                 NULL = allocated (and zeroed) by the handle */
+    uint64_t storage_bytes;   /* bytes at `storage`: at least itak_paged_storage_bytes */
+} itak_paged_config;
+
+/* One sequence of a batch: `rows` new positions behind the `position` it holds, and how many of the batch's page ids are
+   its own: exactly the pages of position + rows positions, or more. */
+typedef struct itak_paged_item {
+    uint64_t position; /* position + rows below 2^31 */
+    uint32_t rows;     /* 0: the sequence takes no part */
+    uint32_t pages;
+} itak_paged_item;
+
+/* Bytes of storage a configuration needs; 0 for one that itak_paged_create refuses. */
+uint64_t itak_paged_storage_bytes(const itak_paged_config *config);
+itak_status itak_paged_create(const itak_paged_config *config, itak_paged **out);
+void itak_paged_destroy(itak_paged *paged);
+/* As itak_last_error and itak_last_error_info, of a paged cache's calls (NULL: of this thread's last failed create). */
+const char *itak_paged_last_error(const itak_paged *paged);
+itak_status itak_paged_last_error_info(const itak_paged *paged, itak_error_info *out);
+itak_status itak_paged_set_stream(itak_paged *paged, void *hip_stream);
+itak_status itak_paged_synchronize(itak_paged *paged);
+/* Where the storage lies on the device. */
+void *itak_paged_storage(const itak_paged *paged);
+/* The batch that the calls below work on, until the next: `count` items, their page ids in order behind one another in
+   `pages` (host memory, `page_ids` of them). A forward sets it once and then goes through its layers. Refused, with the batch
+   before it left in force: ids beyond the pages, too few pages for an item's positions, and a page that new rows go to and that
+   any other place of any table names as well (shared pages are to be copied before they are written). Enqueued on
+   the handle's stream: calls before it see the batch before it, and replays of a graph the batch that is set when they
+   run. Not while that stream is being captured. Graphs need the same number of items with the same rows
+   each as when they were captured, and as many page ids as max_table_pages allows; positions and pages may be others. */
+itak_status itak_paged_set_batch(itak_paged *paged, const itak_paged_item *items, uint32_t count, const uint32_t *pages,
+                                 uint64_t page_ids);
+/* Writes the batch's new rows of `layer` into their pages: k and v are [sum rows][num_kv_heads][head_dim], items in
+   order; with `rotation` the keys are turned by their positions on the way. */
+itak_status itak_paged_append_device(itak_paged *paged, uint64_t layer, const itak_rows *k, const itak_rows *v,
+                                     const itak_rotation *rotation);
+/* Attention of the batch's new positions over the pages, which hold their rows already: query row r of an item attends at
+   position p = item.position + r over max(0, p + 1 - window) .. p (window 0: from 0 on). q and out are
+   [sum rows][heads][head_dim] of the same type, heads a multiple of num_kv_heads (at most 64 times as many); with `rotation` the queries are
+   turned by their positions first (a type of 16 bits is rounded once more for it). scale = NaN selects 1/sqrt(head_dim);
+   softcap > 0 caps each scaled score as cap*tanh(s/cap), 0 disables it. */
+itak_status itak_paged_attention_device(itak_paged *paged, uint64_t layer, const itak_rows *q, const itak_rows *out,
+                                        float scale, float softcap, uint64_t window, const itak_rotation *rotation);
+/* The two in turn: append, then attend, with queries and keys rotated in the append's launch. */
+itak_status itak_paged_step_device(itak_paged *paged, uint64_t layer, const itak_rows *q, const itak_rows *k,
+                                   const itak_rows *v, const itak_rows *out, float scale, float softcap, uint64_t window,
+                                   const itak_rotation *rotation);
+
 /* ---- debug channel ------------------------------------------------------------------- */
 
 /* attention::diag (crates/attention/src/diag.rs:13-33,71-79): one line per cache and

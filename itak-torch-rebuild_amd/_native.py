@@ -33,7 +33,8 @@ STATUS_NAMES = {
     32: "SnapshotTokenMismatch", 33: "EntryTooLarge", 34: "InvalidConfig", 35: "Io",
 }
 KV_ERROR_FIRST, KV_ERROR_LAST = 21, 35
-ELEM_F32, ELEM_F16 = 0, 1
+ELEM_F32, ELEM_F16, ELEM_BF16 = 0, 1, 2
+ROTATION_PLAIN, ROTATION_LINEAR, ROTATION_YARN = 0, 1, 2
 LAYER_GLOBAL, LAYER_WINDOWED = 0, 1
 POOL_SCRUB_ON_TRUNCATE = 1
 POOL_MERGE_IN_LAUNCH = 2
@@ -114,6 +115,28 @@ class StoreStats(C.Structure):
 class PrefixHit(C.Structure):
     _fields_ = [("token_count", C.c_uint64), ("snapshot", C.c_void_p),
                 ("snapshot_len", C.c_uint64), ("file_name", C.c_char * 96)]
+
+
+class RotationConfig(C.Structure):
+    _fields_ = [("base", C.c_double), ("rotary_dim", C.c_uint32), ("interleaved", C.c_uint32), ("scaling", C.c_uint32),
+                ("device", C.c_int32), ("factor", C.c_double), ("original_positions", C.c_double), ("beta_fast", C.c_double),
+                ("beta_slow", C.c_double), ("amplitude", C.c_double)]
+
+
+class Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("elem", C.c_uint32), ("heads", C.c_uint32), ("row_stride", C.c_uint64),
+                ("head_stride", C.c_uint64)]
+
+
+class PagedConfig(C.Structure):
+    _fields_ = [("layer_count", C.c_uint32), ("elem", C.c_uint32), ("num_kv_heads", C.c_uint64), ("head_dim", C.c_uint64),
+                ("page_count", C.c_uint64), ("page_rows", C.c_uint32), ("max_sequences", C.c_uint32),
+                ("max_table_pages", C.c_uint64), ("device", C.c_int32), ("flags", C.c_uint32), ("storage", C.c_void_p),
+                ("storage_bytes", C.c_uint64)]
+
+
+class PagedItem(C.Structure):
+    _fields_ = [("position", C.c_uint64), ("rows", C.c_uint32), ("pages", C.c_uint32)]
 
 
 _P = C.c_void_p
@@ -199,6 +222,23 @@ PROTOTYPES = {
     "itak_probe_read_device": (_i32, [_P, _P, _u64]),
     "itak_probe_empty_launch": (_i32, [_P]),
     "itak_probe_mfma": (_i32, [_P, _u32, _u32, _P, _P]),
+    "itak_rotation_create": (_i32, [C.POINTER(RotationConfig), C.POINTER(_P)]),
+    "itak_rotation_destroy": (None, [_P]),
+    "itak_rotation_frequencies": (_i32, [_P, _P, C.POINTER(C.c_double)]),
+    "itak_rotate_device": (_i32, [_P, _P, _u64, _u64, _P, C.POINTER(Rows), C.POINTER(Rows), _u32, _u32]),
+    "itak_paged_storage_bytes": (_u64, [C.POINTER(PagedConfig)]),
+    "itak_paged_create": (_i32, [C.POINTER(PagedConfig), C.POINTER(_P)]),
+    "itak_paged_destroy": (None, [_P]),
+    "itak_paged_last_error": (C.c_char_p, [_P]),
+    "itak_paged_last_error_info": (_i32, [_P, C.POINTER(ErrorInfo)]),
+    "itak_paged_set_stream": (_i32, [_P, _P]),
+    "itak_paged_synchronize": (_i32, [_P]),
+    "itak_paged_storage": (_P, [_P]),
+    "itak_paged_set_batch": (_i32, [_P, C.POINTER(PagedItem), _u32, _P, _u64]),
+    "itak_paged_append_device": (_i32, [_P, _u64, C.POINTER(Rows), C.POINTER(Rows), _P]),
+    "itak_paged_attention_device": (_i32, [_P, _u64, C.POINTER(Rows), C.POINTER(Rows), _f32, _f32, _u64, _P]),
+    "itak_paged_step_device": (_i32, [_P, _u64, C.POINTER(Rows), C.POINTER(Rows), C.POINTER(Rows), C.POINTER(Rows), _f32, _f32,
+                                      _u64, _P]),
     "itak_set_debug_enabled": (None, [_i32]),
     "itak_debug_enabled": (_i32, []),
 }

@@ -1,0 +1,206 @@
+// What the kernels of a paged cache share: its geometry, the batch in device memory, and how attention cuts it.
+#pragma once
+
+#include "rotation.h"
+
+#include "paged_table.h"
+
+namespace itak {
+
+constexpr float kPagedLog2e = 1.4426950408889634f;
+
+// Strides in elements; side = keys or values of a page, all its heads.
+struct PagedGeom {
+    uint32_t kv_heads;
+    uint32_t head_dim;
+    uint32_t page_shift;  // log2(page_rows)
+    uint32_t ids_at;      // first page id's word in the batch
+    uint64_t head_stride; // page_rows * head_dim
+    uint64_t side_stride;
+    uint64_t page_stride;
+};
+
+struct PagedAppend {
+    PagedGeom g;
+    const uint32_t *batch;
+    uint16_t *layer_base;
+    RowsView k, v;
+    RotationView r;
+    uint32_t q_heads;      // 0: keys and values only
+    RowsView q, q_out;
+    uint32_t pieces;       // of a row: queries', keys', values'
+    uint32_t per_group;
+};
+// `page_elem`, `elem`: ITAK_ELEM_* of the pages and the tensors; `by_8`: pieces of eight channels.
+hipError_t launch_paged_append(uint32_t page_elem, uint32_t elem, bool by_8, const PagedAppend &a, uint32_t rows,
+                               hipStream_t stream);
+
+// Attention. A query vector is one query head's row; the `group` query heads of a KV head times an item's rows are that KV
+// head's vectors, vector v being row v / group, head v % group. A tile is `kTile` of them, a unit a tile of one KV head of one
+// item: its work is the 32-key blocks from the window of the item's first row to the item's last position. All units' blocks
+// in one line (items in order, in an item tile by tile, in a tile head by head) are dealt out evenly: workgroup w takes blocks w * share
+// .. (w + 1) * share of the line, over unit borders, so that a batch of any lengths keeps every compute unit busy to the end
+// and the grid does not depend on the lengths. A unit that one workgroup has whole is written out by it; of the others every workgroup
+// leaves its partial in slot w + (unit's index), which no two parts share, and the merge launch joins them.
+// The cut is worked out on the device from the batch's lengths, so a captured launch is right for whatever batch is set when it runs.
+struct PagedAttn {
+    PagedGeom g;
+    const uint32_t *batch;
+    const uint16_t *layer_base;
+    RowsView q, out;
+    uint32_t rows;       // of the batch the launch was made for
+    uint32_t items;
+    uint32_t group;      // query heads a KV head
+    uint32_t tile;       // vectors
+    uint32_t groups;     // workgroups
+    uint32_t least;      // blocks a workgroup takes at least
+    uint32_t units;      // of the batch the launch was made for
+    uint32_t v_from, v_to; // the launch takes the items of v_from .. v_to vectors a KV head
+    uint32_t q_on_16;    // every 8 channels of q start on 16 bytes
+    uint32_t out_on_16;
+    float scale_log2;    // scale * log2(e); with a softcap 2 * log2(e) * scale / cap
+    float cap_log2;      // cap * log2(e), 0: none
+    uint32_t window;
+    uint32_t parts;      // kernel of many rows: workgroups a unit is dealt to; 0: the line above
+    const void *zeros;   // 16 bytes of them
+    float *ws_acc;       // [slots][tile][padded head_dim]
+    float2 *ws_ml;       // [slots][tile]: maximum (log2 domain), sum
+};
+// The kernel of few rows (paged_few_kernel.h): tiles of `sets` times 16 vectors, 1, 2 or 4 (up to 128 channels).
+constexpr uint32_t kPagedSet = 16;
+// Workgroups a compute unit holds: two where a lane does with 256 registers.
+__host__ __device__ constexpr uint32_t paged_few_groups_per_cu(uint32_t padded, uint32_t elem, uint32_t sets) {
+    return padded <= 128 && elem != ITAK_ELEM_F32 && sets == 1 ? 2 : 1;
+}
+hipError_t launch_paged_few_f16(uint32_t sets, const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_few_f16_f32(uint32_t sets, const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_few_bf16(uint32_t sets, const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_few_bf16_f32(uint32_t sets, const PagedAttn &a, hipStream_t stream);
+// The kernel of many rows (paged_chunk_kernel.h): tiles of 128 or 256 vectors.
+__host__ __device__ constexpr uint32_t paged_chunk_tile(uint32_t padded, uint32_t elem) {
+    return padded <= 128 && elem != ITAK_ELEM_F32 ? 256 : 128;
+}
+// (f32 queries of 256 channels in three bf16 pieces are more registers than there are: the kernel of few rows takes them.)
+__host__ __device__ constexpr bool paged_chunk_takes(uint32_t padded, uint32_t page_elem, uint32_t elem) {
+    return !(padded == 256 && page_elem == ITAK_ELEM_BF16 && elem == ITAK_ELEM_F32);
+}
+hipError_t launch_paged_chunk_f16(const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_chunk_f16_f32(const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_chunk_bf16(const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_chunk_bf16_f32(const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_merge(uint32_t elem, const PagedAttn &a, hipStream_t stream);
+// head_dim as the kernels hold it.
+__host__ __device__ constexpr uint32_t paged_padded(uint32_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+
+// ---- on the device ----------------------------------------------------------------------------
+
+struct PagedSpan {
+    uint32_t position, rows, row0, table;
+    uint32_t first;   // first 32-key block its rows see
+    uint32_t blocks;  // of a unit
+    uint32_t tiles;
+    uint32_t start;   // of its blocks in the line of all units'
+    uint32_t unit0;   // its first unit's index
+};
+
+__host__ __device__ inline uint32_t paged_first_block(uint32_t position, uint32_t window) {
+    return window && position + 1 > window ? (position + 1 - window) / 32 : 0;
+}
+
+#if defined(__HIPCC__)
+
+// Walks the items of a batch, 64 at a time, one a lane.
+struct PagedLine {
+    const PagedAttn &a;
+    uint32_t n, lane;
+
+    __device__ __forceinline__ PagedLine(const PagedAttn &args) : a(args) {
+        n = min(a.batch[0], a.items);
+        lane = __lane_id();
+    }
+    // Lane's item of a chunk, and blocks and units in all of it. Items beyond the launch's rows are left out (a batch that is not
+    // what a captured launch was made for).
+    __device__ __forceinline__ PagedSpan mine(uint32_t at, uint32_t &work, uint32_t &units) const {
+        PagedSpan s{};
+        work = units = 0;
+        if (at + lane < n) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(a.batch + kPagedItem0 + 4 * (at + lane));
+            const uint32_t vectors = w.y * a.group;
+            if (w.z + w.y <= a.rows && vectors >= a.v_from && vectors <= a.v_to) {
+                s.position = w.x, s.rows = w.y, s.row0 = w.z, s.table = w.w;
+                s.first = paged_first_block(w.x, a.window);
+                s.blocks = (w.x + w.y + 31) / 32 - s.first;
+                s.tiles = (vectors + a.tile - 1) / a.tile;
+                units = s.tiles * a.g.kv_heads;
+                work = units * s.blocks;
+            }
+        }
+        return s;
+    }
+    static __device__ __forceinline__ uint32_t scan(uint32_t x) {  // inclusive, over the wavefront
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t y = __shfl_up(x, d);
+            x += (__lane_id() >= uint32_t(d)) ? y : 0;
+        }
+        return x;
+    }
+    __device__ __forceinline__ uint32_t total() const {
+        uint32_t all = 0;
+        for (uint32_t at = 0; at < n; at += 64) {
+            uint32_t work, units;
+            mine(at, work, units);
+            all += n == 1 ? __builtin_amdgcn_readfirstlane(work) : __builtin_amdgcn_readlane(scan(work), 63);
+        }
+        return all;
+    }
+    // The item that FOUND(item, work before it, work of it) holds for, one of them at most, with `start` and `unit0` filled in.
+    template <typename F>
+    __device__ __forceinline__ bool find(PagedSpan &out, F found) const {
+        uint32_t before = 0, units_before = 0;
+        for (uint32_t at = 0; at < n; at += 64) {
+            uint32_t work, units;
+            PagedSpan s = mine(at, work, units);
+            uint32_t upto = work, units_upto = units;
+            if (n > 1) upto = scan(work), units_upto = scan(units);
+            s.start = before + upto - work;
+            s.unit0 = units_before + units_upto - units;
+            const uint64_t mask = __builtin_amdgcn_ballot_w64(work != 0 && found(s, work));
+            if (mask) {
+                const uint32_t l = __builtin_ctzll(mask);
+#define ITAK_FIELD(f) out.f = __builtin_amdgcn_readlane(s.f, l)
+                ITAK_FIELD(position), ITAK_FIELD(rows), ITAK_FIELD(row0), ITAK_FIELD(table), ITAK_FIELD(first);
+                ITAK_FIELD(blocks), ITAK_FIELD(tiles), ITAK_FIELD(start), ITAK_FIELD(unit0);
+#undef ITAK_FIELD
+                return true;
+            }
+            before += __builtin_amdgcn_readlane(upto, n == 1 ? 0 : 63);
+            units_before += __builtin_amdgcn_readlane(units_upto, n == 1 ? 0 : 63);
+        }
+        return false;
+    }
+};
+__device__ __forceinline__ uint32_t paged_share(const PagedAttn &a, uint32_t total) {
+    return max(a.least, (total + a.groups - 1) / a.groups);
+}
+
+// The batch's item that holds row `row`: its position, first row and table. All lanes ask together.
+__device__ __forceinline__ bool paged_item_of_row(const uint32_t *batch, uint32_t row, uint4 &item) {
+    const uint32_t n = batch[0], lane = __lane_id();
+    for (uint32_t at = 0; at < n; at += 64) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (at + lane < n) w = *reinterpret_cast<const uint4 *>(batch + kPagedItem0 + 4 * (at + lane));
+        const uint64_t mask = __builtin_amdgcn_ballot_w64(row >= w.z && row - w.z < w.y);
+        if (mask) {
+            const uint32_t l = __builtin_ctzll(mask);
+            item.x = __builtin_amdgcn_readlane(w.x, l), item.y = __builtin_amdgcn_readlane(w.y, l);
+            item.z = __builtin_amdgcn_readlane(w.z, l), item.w = __builtin_amdgcn_readlane(w.w, l);
+            return true;
+        }
+    }
+    return false;
+}
+
+#endif
+
+}  // namespace itak

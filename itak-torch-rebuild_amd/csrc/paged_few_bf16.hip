@@ -1,0 +1,10 @@
+// The kernel of few rows over bf16 pages, bf16 tensors.
+#include "paged_few_kernel.h"
+
+namespace itak {
+
+hipError_t launch_paged_few_bf16(uint32_t sets, const PagedAttn &a, hipStream_t stream) {
+    return launch_few<ITAK_ELEM_BF16, ITAK_ELEM_BF16, 1, 1>(sets, a, stream);
+}
+
+}  // namespace itak

@@ -75,11 +75,12 @@ class StepFailed(Exception):
         super().__init__(f"{step}: {detail}")
 
 
-def _raise_last(handle, step: Optional[str] = None):
+def _raise_last(handle, step: Optional[str] = None, lib_error=None):
     lib = N.load()
+    last_error, last_info = lib_error or (lib.itak_last_error, lib.itak_last_error_info)
     info = N.ErrorInfo()
-    lib.itak_last_error_info(handle, C.byref(info))
-    message = (lib.itak_last_error(handle) or b"").decode()
+    last_info(handle, C.byref(info))
+    message = (last_error(handle) or b"").decode()
     name = N.STATUS_NAMES.get(info.code, f"Status{info.code}")
     if name == "StepFailed":
         raise StepFailed(step or info.what.decode() or "attention", message)
