@@ -41,9 +41,19 @@ def sources():
 NO_STAMPS = {"attn_prefill_f16_dims.hip"}
 
 
+# Kernels that hold more than 256 registers a lane beside matrix accumulators which vector code also works on: left to itself the
+# compiler keeps the accumulators in the accumulation registers and copies them out and back in every turn of the loop (the kernel
+# of many rows over pages: 1,650 us for a chunk of 2,048 rows over 30,720, 256 copies a block).
+MFMA_IN_VECTOR_REGISTERS = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+
+
+def source_flags(src: str):
+    return MFMA_IN_VECTOR_REGISTERS if src.startswith(("paged_chunk", "paged_few")) else []
+
+
 def _compile(src: str, timeline: bool = False) -> str:
     obj = os.path.join(OBJ_DIR + ("_timeline" if timeline else ""), src.replace(".hip", ".o"))
-    cmd = [HIPCC, *FLAGS, *(["-DITAK_TIMELINE"] if timeline and src not in NO_STAMPS else []), "-c",
+    cmd = [HIPCC, *FLAGS, *source_flags(src), *(["-DITAK_TIMELINE"] if timeline and src not in NO_STAMPS else []), "-c",
            os.path.join(CSRC, src), "-o", obj]
     res = subprocess.run(cmd, capture_output=True, text=True)
     noise = "is not a recognized feature for this target"

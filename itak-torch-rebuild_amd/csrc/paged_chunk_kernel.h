@@ -52,19 +52,25 @@ __device__ __forceinline__ void wait_loads() {  // s_waitcnt vmcnt(n), other cou
     __builtin_amdgcn_s_waitcnt(0x0f70 | (n & 15) | ((n >> 4) << 14));
 }
 
-template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP, int COLS, int GROUPS>
+// Sub-blocks of 32 keys a stage of the ring holds, and stages.
+constexpr int chunk_subs(int dp) { return dp <= 128 ? 2 : 1; }
+constexpr int chunk_stages(int dp) { return dp == 256 ? 4 : 4; }
+constexpr size_t chunk_lds(int dp) { return size_t(chunk_stages(dp)) * chunk_subs(dp) * 2 * 32 * 2 * dp; }
+
+template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP, int COLS, int GROUPS, bool CAP>
 __global__ __launch_bounds__(kChunkWaves * 64, GROUPS) void paged_chunk_kernel(PagedAttn a) {
     typedef typename Elem<ELEM>::type T;
     constexpr int kTile = kChunkWaves * 32 * COLS;
     constexpr int kSteps = DP / 16;               // products of a score tile
     constexpr int kOut = DP / 32;                 // output tiles of 32 channels
     constexpr int kRowBytes = 2 * DP;
-    constexpr int kBlockBytes = 32 * kRowBytes;   // of one side
-    constexpr int kStageBytes = 2 * kBlockBytes;
-    constexpr int kStages = DP == 256 ? 3 : 4;
+    constexpr int kBlockBytes = 32 * kRowBytes;   // of one side of a sub-block
+    constexpr int kSubBytes = 2 * kBlockBytes;
+    constexpr int kSubs = chunk_subs(DP), kStages = chunk_stages(DP), kStageBytes = kSubs * kSubBytes;
     constexpr int kRowPieces = DP / 8;            // 16-byte pieces of a row
     constexpr int kLoadRows = 512 / DP;           // rows a load of one wavefront moves
-    constexpr int kLoads = DP / 64;               // loads a wavefront issues for a side of a block
+    constexpr int kLoads = DP / 64;               // loads a wavefront issues for a side of a sub-block
+    constexpr int kStageLoads = 2 * kLoads * kSubs;
     extern __shared__ __attribute__((aligned(16))) unsigned char ring[];
     __shared__ uint32_t lds_flag;
 
@@ -128,14 +134,14 @@ __global__ __launch_bounds__(kChunkWaves * 64, GROUPS) void paged_chunk_kernel(P
         p.id[1] = ids[min((32 * kb + 16) >> a.g.page_shift, last_page)];
         return p;
     };
-    // Block kb into its stage. Past the end the last block comes once more into a stage nobody reads: the loads in flight stay the same.
-    auto issue = [&](uint32_t kb, uint32_t stage, const Pages &pages) {
+    // Block kb to its place in the ring. Past the end the last block comes once more: the loads in flight stay the same.
+    auto issue = [&](uint32_t kb, uint32_t place, const Pages &pages) {
         const uint32_t at = min(kb, max(kb_end, kb0 + 1) - 1);
         uint64_t base[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half)
             base[half] = head_base + pages.id[half] * a.g.page_stride * 2 + uint64_t((32 * at + 16 * half) & page_mask) * (d * 2);
-        const uint32_t dst = ring_base + stage * kStageBytes + wave * 1024;
+        const uint32_t dst = ring_base + place + wave * 1024;
 #pragma unroll
         for (int side = 0; side < 2; ++side)
 #pragma unroll
@@ -163,38 +169,20 @@ __global__ __launch_bounds__(kChunkWaves * 64, GROUPS) void paged_chunk_kernel(P
         my_pos[c] = span.position + row;
         my_lo[c] = lowest_visible(my_pos[c], a.window, 0);
         const T *src = static_cast<const T *>(a.q.data) + uint64_t(span.row0 + row) * a.q.row_stride + hq * a.q.head_stride;
+        typename QueryRaw<ELEM>::type raw[kSteps];
+        if (a.q_on_16) {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const bool in = v < vectors && (EXACT || 16 * s + 8 * h < d);
-            const T *p = src + (EXACT || 16 * s + 8 * h < d ? 16 * s + 8 * h : 0);
-            if constexpr (ELEM != ITAK_ELEM_F32) {
-                u32x4 x;
-                if (a.q_on_16) {
-                    x = *reinterpret_cast<const u32x4 *>(p);
-                } else {
-                    const uint16_t *u = reinterpret_cast<const uint16_t *>(p);
+            for (int s = 0; s < kSteps; ++s)
+                raw[s] = load_query<ELEM, true>(src + (EXACT || 16 * s + 8 * h < d ? 16 * s + 8 * h : 0));
+        } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = u[2 * e] | (uint32_t(u[2 * e + 1]) << 16);
-                }
-                q[c][0][s] = in ? x : u32x4{0, 0, 0, 0};
-            } else {
-                float x[8];
-                if (a.q_on_16) {
-                    const floatx4 lo = *reinterpret_cast<const floatx4 *>(p), hi = *reinterpret_cast<const floatx4 *>(p + 4);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = lo[e], x[4 + e] = hi[e];
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = p[e];
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = in ? x[e] : 0.0f;
-                u32x4 pieces[NQ];
-                split_8<PAGE, NQ>(x, pieces);
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) q[c][n][s] = pieces[n];
-            }
+            for (int s = 0; s < kSteps; ++s)
+                raw[s] = load_query<ELEM, false>(src + (EXACT || 16 * s + 8 * h < d ? 16 * s + 8 * h : 0));
         }
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+            split_query<PAGE, ELEM, NQ>(raw[s], v < vectors && (EXACT || 16 * s + 8 * h < d),
+                                        [&](int n, u32x4 x) { q[c][n][s] = x; });
     }
     // (The compiler cannot count the ring's loads: every load of its own has to be in before the first of them.)
     wait_loads<0>();
@@ -216,74 +204,50 @@ __global__ __launch_bounds__(kChunkWaves * 64, GROUPS) void paged_chunk_kernel(P
             for (int r = 0; r < 16; ++r) o[c][t][r] = 0.0f;
     }
 
-    {
-        Pages pages[kStages - 1];
+    // Operands out of a sub-block at LDS address `at`.
+    auto k_operand = [&](uint32_t at, int i) {
+        return *reinterpret_cast<const __attribute__((address_space(3))) u32x4 *>((uintptr_t)(at + (k_at ^ (i * 32))));
+    };
+    auto v_operand = [&](uint32_t at, int t, int m) {
+        u32x4 v;
 #pragma unroll
-        for (int s = 0; s < kStages - 1; ++s) pages[s] = pages_of(kb0 + s);
-#pragma unroll
-        for (int s = 0; s < kStages - 1; ++s) issue(kb0 + s, s, pages[s]);
-    }
-    Pages ahead = pages_of(kb0 + kStages - 1);
-    uint32_t stage = 0;
-    for (uint32_t kb = kb0; kb < kb_end; ++kb) {
-        // This wavefront's loads of block kb have landed (those of the next blocks may still fly); behind the barrier everybody's have,
-        // and everybody is done with block kb - 1, whose stage the next loads overwrite.
-        wait_loads<2 * kLoads * (kStages - 2)>();
-        __builtin_amdgcn_s_barrier();
-        issue(kb + kStages - 1, stage == 0 ? kStages - 1 : stage - 1, ahead);
-        ahead = pages_of(kb + kStages);
-        unsigned char *const block = ring + stage * kStageBytes;
-        if (32 * kb < tile_lo || 32 * kb + 32 > tile_hi) {
-            // Rows no query of the tile sees may hold anything: their values are zeroed. (At most the first and the last block.)
-            for (uint32_t p = tid; p < 32 * kRowPieces; p += kChunkWaves * 64) {
-                const uint32_t key = 32 * kb + p / kRowPieces;
-                if (key < tile_lo || key >= tile_hi) *reinterpret_cast<u32x4 *>(block + kBlockBytes + p * 16) = u32x4{0, 0, 0, 0};
-            }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-            __builtin_amdgcn_s_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+        for (int u = 0; u < 2; ++u) {
+            const shortx4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) shortx4 *)(uintptr_t)(at + (v_at ^ (t * 64)) + (16 * m + 8 * u) * kRowBytes));
+            const uint2 y = __builtin_bit_cast(uint2, x);
+            v[2 * u] = y.x, v[2 * u + 1] = y.y;
         }
-        stage = stage + 1 == kStages ? 0 : stage + 1;
-        if (32 * kb >= some_hi || 32 * kb + 32 <= some_lo) continue;
-        const bool edge = 32 * kb < every_lo || 32 * kb + 32 > every_hi;
-
-        floatx16 s[COLS];
+        return v;
+    };
+    // A lane's scores of a block, relative to the reference, and the largest of a column.
+    float x[COLS][16];
+    auto scaled = [&](float s, int c) {
+        if constexpr (CAP)
+            return softcap_of_exp2_arg(s * a.scale_log2, a.cap_log2, ref[c]);
+        else
+            return __builtin_fmaf(s, a.scale_log2, -ref[c]);
+    };
+    // Masks the scores of block kb where a row does not see all of it, and moves references that they pass.
+    auto settle = [&](uint32_t kb, float (&most)[COLS]) {
+        if (32 * kb < every_lo || 32 * kb + 32 > every_hi) {
 #pragma unroll
-        for (int c = 0; c < COLS; ++c)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[c][r] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            const u32x4 k = *reinterpret_cast<const u32x4 *>(block + (k_at ^ (i * 32)));
-#pragma unroll
-            for (int c = 0; c < COLS; ++c)
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) s[c] = mfma_32x32x16<PAGE>(k, q[c][n][i], s[c]);
-        }
-        u32x4 p[COLS][NP][2];
-#pragma unroll
-        for (int c = 0; c < COLS; ++c) {
-            float x[16];
-            if (a.cap_log2 != 0.0f) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = softcap_of_exp2_arg(s[c][r] * a.scale_log2, a.cap_log2, ref[c]);
-            } else {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(s[c][r], a.scale_log2, -ref[c]);
-            }
-            if (edge) {
+            for (int c = 0; c < COLS; ++c) {
+                most[c] = -INFINITY;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const uint32_t key = 32 * kb + 8 * (r / 4) + 4 * h + r % 4;
-                    if (key > my_pos[c] || key < my_lo[c]) x[r] = -INFINITY;
+                    if (key > my_pos[c] || key < my_lo[c]) x[c][r] = -INFINITY;
+                    most[c] = fmaxf(most[c], x[c][r]);
                 }
             }
-            float most = max3(x[0], x[1], x[2]);
+        }
+        bool over = false;
 #pragma unroll
-            for (int r = 3; r < 15; r += 2) most = max3(most, x[r], x[r + 1]);
-            most = fmaxf(most, x[15]);
-            if (__builtin_amdgcn_ballot_w64(most > threshold[c]) != 0) {
-                const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
+        for (int c = 0; c < COLS; ++c) over = over || most[c] > threshold[c];
+        if (__builtin_amdgcn_ballot_w64(over) != 0) {
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) {
+                const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(most[c]), __float_as_uint(most[c]), false, false);
                 const float m = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
                 const bool live = threshold[c] != -INFINITY;
                 float delta = live ? fmaxf(m, 0.0f) : m;
@@ -295,40 +259,167 @@ __global__ __launch_bounds__(kChunkWaves * 64, GROUPS) void paged_chunk_kernel(P
 #pragma unroll
                 for (int t = 0; t < kOut; ++t) o[c][t] *= alpha;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] -= delta;
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = fast_exp2(x[r]);
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                float e[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r) e[r] = x[8 * m + r];
-                sum[c] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-                u32x4 pieces[NP];
-                split_8<PAGE, NP>(e, pieces);
-#pragma unroll
-                for (int n = 0; n < NP; ++n) p[c][n][m] = pieces[n];
+                for (int r = 0; r < 16; ++r) x[c][r] -= delta;
             }
         }
+    };
+    // Rows of block kb no query of the tile sees may hold anything: their values are zeroed in LDS, where the block lies at `at`.
+    auto clear = [&](uint32_t kb, uint32_t at) {
+        for (uint32_t p = tid; p < 32 * kRowPieces; p += kChunkWaves * 64) {
+            const uint32_t key = 32 * kb + p / kRowPieces;
+            if (key < tile_lo || key >= tile_hi)
+                *reinterpret_cast<__attribute__((address_space(3))) u32x4 *>((uintptr_t)(at + kBlockBytes + p * 16)) = u32x4{0, 0, 0, 0};
+        }
+    };
+    // The blocks of a stage that have such rows: at most the tile's first and last, and what comes past the end in their stage.
+    auto clear_stage = [&](uint32_t kb, uint32_t at) {
+        bool any = false;
 #pragma unroll
-        for (int t = 0; t < kOut; ++t)
+        for (int u = 0; u < kSubs; ++u)
+            if (32 * (kb + u) < tile_lo || 32 * (kb + u) + 32 > tile_hi) clear(kb + u, at + u * kSubBytes), any = true;
+        if (any) {
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+        }
+    };
+
+    // Stages of the ring fill ahead of the one at hand; its last places are never read where the blocks end inside one.
+    const uint32_t stages = (kb_end - kb0 + kSubs - 1) / kSubs;
+    Pages ahead[kSubs];
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                u32x4 v;
+    for (int s = 0; s < kStages - 1; ++s)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const uint32_t at = (v_at ^ (t * 64)) + (16 * m + 8 * u) * kRowBytes;
-                    const shortx4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) shortx4 *)(uintptr_t)((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)block + at));
-                    const uint2 y = __builtin_bit_cast(uint2, x);
-                    v[2 * u] = y.x, v[2 * u + 1] = y.y;
+        for (int u = 0; u < kSubs; ++u) issue(kb0 + s * kSubs + u, s * kStageBytes + u * kSubBytes, pages_of(kb0 + s * kSubs + u));
+#pragma unroll
+    for (int u = 0; u < kSubs; ++u) ahead[u] = pages_of(kb0 + (kStages - 1) * kSubs + u);
+    u32x4 k[kSteps];
+    if (stages) {
+        // The first block's scores by themselves, and the operands of the second block's.
+        wait_loads<kStageLoads * (kStages - 2)>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        clear_stage(kb0, ring_base);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) k[i] = k_operand(ring_base, i);
+        float most[COLS];
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+            floatx16 s;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) s = mfma_32x32x16<PAGE>(k[i], q[c][n][i], s);
+            most[c] = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[c][r] = scaled(s[r], c), most[c] = fmaxf(most[c], x[c][r]);
+        }
+        settle(kb0, most);
+        if constexpr (kSubs > 1) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) k[i] = k_operand(ring_base + kSubBytes, i);
+        }
+    }
+    uint32_t at = ring_base, next = ring_base + kStageBytes, free_at = (kStages - 1) * kStageBytes;
+    for (uint32_t g = 0; g < stages; ++g) {
+        // This wavefront's loads of the next stage have landed (those of the stages behind it may still fly); behind the barrier
+        // everybody's have, and everybody is done with the stage before this one, which the loads that go out now overwrite.
+        wait_loads<kStageLoads * (kStages - 3)>();
+        __builtin_amdgcn_s_barrier();
+        const uint32_t kb = kb0 + g * kSubs;
+#pragma unroll
+        for (int u = 0; u < kSubs; ++u) issue(kb + (kStages - 1) * kSubs + u, free_at + u * kSubBytes, ahead[u]);
+#pragma unroll
+        for (int u = 0; u < kSubs; ++u) ahead[u] = pages_of(kb + kStages * kSubs + u);
+        clear_stage(kb + kSubs, next);
+        if constexpr (kSubs == 1) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) k[i] = k_operand(next, i);
+        }
+#pragma unroll
+        for (int u = 0; u < kSubs; ++u) {
+            const uint32_t here = at + u * kSubBytes;
+            // Where the operands of the scores after the next lie.
+            const uint32_t k_next = u + 2 < kSubs ? at + (u + 2) * kSubBytes : next + (u + 2 - kSubs) * kSubBytes;
+            // Three stretches, each of products beside vector work of about their length: the next block's scores beside three quarters
+            // of this block's exponentials, the first half of P.V beside the rest, the second half beside the next scores' scaling.
+            constexpr int kAll = 16 * COLS, kFirst = kAll * 3 / 4;
+            floatx16 s[COLS];
+#pragma unroll
+            for (int c = 0; c < COLS; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[c][r] = 0.0f;
+            u32x4 p[COLS][NP][2];
+            u32x4 v[kOut][2];
+            auto weigh = [&](int e) {  // exponential e: halves of the keys, columns, keys
+                const int m = e / (8 * COLS), c = e / 8 % COLS, r = 8 * m + e % 8;
+                x[c][r] = fast_exp2(x[c][r]);
+                if (e % 8 == 7) {
+                    float w[8];
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) w[y] = x[c][8 * m + y];
+                    sum[c] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+                    u32x4 pieces[NP];
+                    split_8<PAGE, NP>(w, pieces);
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) p[c][n][m] = pieces[n];
                 }
+            };
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
                 for (int c = 0; c < COLS; ++c)
 #pragma unroll
-                    for (int n = 0; n < NP; ++n) o[c][t] = mfma_32x32x16<PAGE>(v, p[c][n][m], o[c][t]);
+                    for (int n = 0; n < NQ; ++n) s[c] = mfma_32x32x16<PAGE>(k[i], q[c][n][i], s[c]);
+#pragma unroll
+                for (int e = i * kFirst / kSteps; e < (i + 1) * kFirst / kSteps; ++e) weigh(e);
+                if (i >= kSteps - 2 * kOut) v[(i - (kSteps - 2 * kOut)) % kOut][(i - (kSteps - 2 * kOut)) / kOut] =
+                    v_operand(here, (i - (kSteps - 2 * kOut)) % kOut, (i - (kSteps - 2 * kOut)) / kOut);
+                __builtin_amdgcn_sched_barrier(0);
             }
+#pragma unroll
+            for (int t = 0; t < kOut; ++t) {
+#pragma unroll
+                for (int c = 0; c < COLS; ++c)
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) o[c][t] = mfma_32x32x16<PAGE>(v[t][0], p[c][n][0], o[c][t]);
+#pragma unroll
+                for (int e = kFirst + t * (kAll - kFirst) / kOut; e < kFirst + (t + 1) * (kAll - kFirst) / kOut; ++e) weigh(e);
+                if (kSubs > 1) {
+                    k[2 * t] = k_operand(k_next, 2 * t);
+                    k[2 * t + 1] = k_operand(k_next, 2 * t + 1);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            float most[COLS];
+#pragma unroll
+            for (int t = 0; t < kOut; ++t) {
+#pragma unroll
+                for (int c = 0; c < COLS; ++c)
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) o[c][t] = mfma_32x32x16<PAGE>(v[t][1], p[c][n][1], o[c][t]);
+#pragma unroll
+                for (int e = t * kAll / kOut; e < (t + 1) * kAll / kOut; ++e) {
+                    const int c = e / 16, r = e % 16;
+                    x[c][r] = scaled(s[c][r], c);
+                    if (r == 0)
+                        most[c] = x[c][0];
+                    else if (r % 2 == 0)
+                        most[c] = max3(most[c], x[c][r - 1], x[c][r]);
+                    else if (r == 15)
+                        most[c] = fmaxf(most[c], x[c][15]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (kb + u + 1 < kb_end) settle(kb + u + 1, most);
+            if (kb + u + 1 >= kb_end) break;
+        }
+        const uint32_t was = at;
+        at = next;
+        free_at = was - ring_base;
+        next = next + kStageBytes == ring_base + kStages * kStageBytes ? ring_base : next + kStageBytes;
     }
     wait_loads<0>();  // (the surplus loads)
 
@@ -392,13 +483,15 @@ hipError_t launch_chunk_as(const PagedAttn &a, hipStream_t stream) {
     else {
     constexpr int kCols = int(paged_chunk_tile(DP, ELEM)) / (kChunkWaves * 32);
     constexpr int kGroups = DP == 64 ? 2 : 1;
-    constexpr size_t lds = size_t(DP == 256 ? 3 : 4) * 2 * 32 * 2 * DP;
-    auto kernel = paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kCols, kGroups>;
-    static const hipError_t granted =
-        hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
-    if (granted != hipSuccess) return granted;
-    launch_kernel(kernel, a.units * a.parts, kChunkWaves * 64, lds, stream, a);
-    return hipGetLastError();
+    auto run = [&](auto kernel) {
+        static const hipError_t granted =
+            hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(chunk_lds(DP)));
+        if (granted != hipSuccess) return granted;
+        launch_kernel(kernel, a.units * a.parts, kChunkWaves * 64, chunk_lds(DP), stream, a);
+        return hipGetLastError();
+    };
+    return a.cap_log2 != 0.0f ? run(paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kCols, kGroups, true>)
+                              : run(paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kCols, kGroups, false>);
     }
 }
 template <int PAGE, int ELEM, int NQ, int NP>

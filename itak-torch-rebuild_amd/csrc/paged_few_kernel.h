@@ -110,42 +110,27 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, ELEM, S
         for (int n = 0; n < SETS; ++n) {
             const T *src = static_cast<const T *>(a.q.data) + uint64_t(span.row0 + my_row[n]) * a.q.row_stride +
                            my_head[n] * a.q.head_stride;
+            // (Of queries in LDS every wavefront brings its share of the steps.)
+            constexpr int kMine = kQInLds ? (S::kSteps + kFewWaves - 1) / kFewWaves : S::kSteps;
+            typename QueryRaw<ELEM>::type raw[kMine];
+            auto step = [&](int m) { return kQInLds ? m * kFewWaves + wave : uint32_t(m); };
+            auto chan = [&](int m) { return EXACT || 32 * step(m) + 8 * g < d ? min(32 * step(m) + 8 * g, uint32_t(DP) - 8) : 0u; };
+            if (a.q_on_16) {
 #pragma unroll
-            for (int s = 0; s < S::kSteps; ++s) {
-                if (kQInLds && uint32_t(s) % kFewWaves != wave) continue;
-                const bool in = v0 + n * kSet + i < vectors && (EXACT || 32 * s + 8 * g < d);
-                const T *p = src + k_chan[s];
-                if constexpr (ELEM != ITAK_ELEM_F32) {
-                    u32x4 x;
-                    if (a.q_on_16) {
-                        x = *reinterpret_cast<const u32x4 *>(p);
-                    } else {
-                        const uint16_t *u = reinterpret_cast<const uint16_t *>(p);
+                for (int m = 0; m < kMine; ++m) raw[m] = load_query<ELEM, true>(src + chan(m));
+            } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) x[e] = u[2 * e] | (uint32_t(u[2 * e + 1]) << 16);
-                    }
-                    x = in ? x : u32x4{0, 0, 0, 0};
+                for (int m = 0; m < kMine; ++m) raw[m] = load_query<ELEM, false>(src + chan(m));
+            }
+#pragma unroll
+            for (int m = 0; m < kMine; ++m) {
+                if (kQInLds && step(m) >= uint32_t(S::kSteps)) continue;
+                split_query<PAGE, ELEM, NQ>(raw[m], v0 + n * kSet + i < vectors && (EXACT || 32 * step(m) + 8 * g < d), [&](int piece, u32x4 x) {
                     if constexpr (kQInLds)
-                        lds_q[(n * S::kSteps + s) * 64 + lane] = x;
+                        lds_q[((n * NQ + piece) * S::kSteps + step(m)) * 64 + lane] = x;
                     else
-                        q[n][s] = x;
-                } else {
-                    float x[8];
-                    if (a.q_on_16) {
-                        const floatx4 lo = *reinterpret_cast<const floatx4 *>(p), hi = *reinterpret_cast<const floatx4 *>(p + 4);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x[e] = lo[e], x[4 + e] = hi[e];
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) x[e] = p[e];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = in ? x[e] : 0.0f;
-                    u32x4 pieces[NQ];
-                    split_8<PAGE, NQ>(x, pieces);
-#pragma unroll
-                    for (int m = 0; m < NQ; ++m) lds_q[((n * NQ + m) * S::kSteps + s) * 64 + lane] = pieces[m];
-                }
+                        q[n][m] = x;
+                });
             }
         }
         if constexpr (kQInLds) __syncthreads();

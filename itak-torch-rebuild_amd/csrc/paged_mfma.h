@@ -38,22 +38,50 @@ __device__ __forceinline__ void split_8(const float (&x)[8], u32x4 (&out)[PIECES
     }
 }
 
-// Bit 15 or 31 of the result is set if the half there is an infinity or a NaN (its exponent field all ones: one more carries).
-template <int PAGE>
-__device__ __forceinline__ uint32_t not_finite_2(uint32_t x) {
-    return PAGE == ITAK_ELEM_F16 ? (x & 0x7c007c00u) + 0x04000400u : (x & 0x7f807f80u) + 0x00800080u;
-}
-
-// The halves that are neither, zero in place of the others.
-template <int PAGE>
-__device__ __forceinline__ u32x4 finite_only(u32x4 x) {
-    u32x4 y;
+// Eight channels of a query as they are loaded, on 16 bytes or element by element, and as operands: `in` = false gives zeros.
+template <int ELEM>
+struct QueryRaw {
+    typedef u32x4 type;
+};
+typedef float floatx8 __attribute__((ext_vector_type(8)));
+template <>
+struct QueryRaw<ITAK_ELEM_F32> {
+    typedef floatx8 type;
+};
+template <int ELEM, bool ON_16>
+__device__ __forceinline__ typename QueryRaw<ELEM>::type load_query(const typename Elem<ELEM>::type *p) {
+    typename QueryRaw<ELEM>::type x;
+    if constexpr (ELEM == ITAK_ELEM_F32) {
+        if constexpr (ON_16) {
+            const floatx4 lo = *reinterpret_cast<const floatx4 *>(p), hi = *reinterpret_cast<const floatx4 *>(p + 4);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const uint32_t bad = not_finite_2<PAGE>(x[c]) & 0x80008000u;
-        y[c] = x[c] & ~((bad >> 15) * 0xffffu);
+            for (int e = 0; e < 4; ++e) x[e] = lo[e], x[4 + e] = hi[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = p[e];
+        }
+    } else if constexpr (ON_16) {
+        x = *reinterpret_cast<const u32x4 *>(p);
+    } else {
+        const uint16_t *u = reinterpret_cast<const uint16_t *>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = u[2 * e] | (uint32_t(u[2 * e + 1]) << 16);
     }
-    return y;
+    return x;
+}
+template <int PAGE, int ELEM, int NQ, typename F>
+__device__ __forceinline__ void split_query(const typename QueryRaw<ELEM>::type &raw, bool in, F store) {
+    if constexpr (ELEM == ITAK_ELEM_F32) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = in ? raw[e] : 0.0f;
+        u32x4 pieces[NQ];
+        split_8<PAGE, NQ>(x, pieces);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) store(n, pieces[n]);
+    } else {
+        store(0, in ? raw : u32x4{0, 0, 0, 0});
+    }
 }
 
 // The maximum over the four lanes that hold one column of S.
