@@ -76,10 +76,12 @@ hipError_t launch_paged_few_f16(uint32_t sets, const PagedAttn &a, hipStream_t s
 hipError_t launch_paged_few_f16_f32(uint32_t sets, const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_few_bf16(uint32_t sets, const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_few_bf16_f32(uint32_t sets, const PagedAttn &a, hipStream_t stream);
-// The kernel of many rows (paged_chunk_kernel.h): tiles of 128 or 256 vectors.
-__host__ __device__ constexpr uint32_t paged_chunk_tile(uint32_t padded, uint32_t elem) {
-    return padded <= 128 && elem != ITAK_ELEM_F32 ? 256 : 128;
+// The kernel of many rows (paged_chunk_kernel.h): 32 vectors a wavefront, four or eight wavefronts a tile.
+__host__ __device__ constexpr uint32_t paged_chunk_waves(uint32_t padded, uint32_t elem) {
+    return padded == 64 || (padded == 128 && elem != ITAK_ELEM_F32) ? 8 : 4;
 }
+// Workgroups a compute unit holds (by LDS and registers).
+__host__ __device__ constexpr uint32_t paged_chunk_groups_per_cu(uint32_t) { return 1; }
 // (f32 queries of 256 channels in three bf16 pieces are more registers than there are: the kernel of few rows takes them.)
 __host__ __device__ constexpr bool paged_chunk_takes(uint32_t padded, uint32_t page_elem, uint32_t elem) {
     return !(padded == 256 && page_elem == ITAK_ELEM_BF16 && elem == ITAK_ELEM_F32);

@@ -129,6 +129,7 @@ itak_status check_config(ErrorState &e, const itak_paged_config *c, PagedGeom &g
     g.side_stride = g.head_stride * g.kv_heads;
     g.page_stride = 2 * g.side_stride;
     uint64_t all = 0;
+    if (g.page_stride >= (1ull << 31)) return size_overflow(e, "a page of one layer");  // (4 GiB)
     if (__builtin_mul_overflow(g.page_stride, c->page_count, &layer_stride) ||
         __builtin_mul_overflow(layer_stride, uint64_t(c->layer_count), &all) || __builtin_mul_overflow(all, uint64_t(2), &bytes) ||
         bytes > (1ull << 62))
@@ -269,12 +270,12 @@ itak_status run_attention(itak_paged *p, uint64_t layer, const itak_rows &q, con
         HIP_TRY(p, launch_paged_merge(q.elem, a, p->stream), "launch the merge of paged attention");
     }
     if (many) {
-        a.tile = paged_chunk_tile(dp, q.elem);
+        a.tile = 32 * paged_chunk_waves(dp, q.elem);
         a.v_from = few_most + 1, a.v_to = ~0u;
         uint64_t work = 0;
         st = count_units(p, a, work);
         if (st != ITAK_OK) return st;
-        a.parts = chunk_parts(a.units, work, cus * (dp == 64 ? 2 : 1));
+        a.parts = chunk_parts(a.units, work, cus * paged_chunk_groups_per_cu(dp));
         if (a.parts > 1) {
             st = workspace(p, a, uint64_t(a.units) * a.parts, dp);
             if (st != ITAK_OK) return st;

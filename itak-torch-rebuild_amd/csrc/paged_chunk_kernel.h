@@ -28,7 +28,6 @@ namespace {
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
 
-constexpr int kChunkWaves = 4;
 constexpr float kChunkSlack = 8.0f;
 
 template <int PAGE>
@@ -57,10 +56,11 @@ constexpr int chunk_subs(int dp) { return dp <= 128 ? 2 : 1; }
 constexpr int chunk_stages(int dp) { return dp == 256 ? 4 : 4; }
 constexpr size_t chunk_lds(int dp) { return size_t(chunk_stages(dp)) * chunk_subs(dp) * 2 * 32 * 2 * dp; }
 
-template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP, int COLS, int GROUPS, bool CAP>
-__global__ __launch_bounds__(kChunkWaves * 64, GROUPS) void paged_chunk_kernel(PagedAttn a) {
+template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP, bool CAP>
+__global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_kernel(PagedAttn a) {
     typedef typename Elem<ELEM>::type T;
-    constexpr int kTile = kChunkWaves * 32 * COLS;
+    constexpr int kWaves = paged_chunk_waves(DP, ELEM);
+    constexpr int kTile = kWaves * 32;
     constexpr int kSteps = DP / 16;               // products of a score tile
     constexpr int kOut = DP / 32;                 // output tiles of 32 channels
     constexpr int kRowBytes = 2 * DP;
@@ -69,8 +69,9 @@ __global__ __launch_bounds__(kChunkWaves * 64, GROUPS) void paged_chunk_kernel(P
     constexpr int kSubs = chunk_subs(DP), kStages = chunk_stages(DP), kStageBytes = kSubs * kSubBytes;
     constexpr int kRowPieces = DP / 8;            // 16-byte pieces of a row
     constexpr int kLoadRows = 512 / DP;           // rows a load of one wavefront moves
-    constexpr int kLoads = DP / 64;               // loads a wavefront issues for a side of a sub-block
-    constexpr int kStageLoads = 2 * kLoads * kSubs;
+    constexpr int kSideLoads = DP / 16;           // loads of a side of a sub-block, dealt to the wavefronts in turn
+    constexpr int kLoads = 2 * kSideLoads / kWaves; // loads of a wavefront for a sub-block, both sides
+    constexpr int kStageLoads = kLoads * kSubs;
     extern __shared__ __attribute__((aligned(16))) unsigned char ring[];
     __shared__ uint32_t lds_flag;
 
@@ -96,11 +97,9 @@ __global__ __launch_bounds__(kChunkWaves * 64, GROUPS) void paged_chunk_kernel(P
     const uint32_t kb0 = b_first + min(b_all, part * b_part), kb_end = b_first + min(b_all, part * b_part + b_part);
     const uint64_t slot0 = uint64_t(unit * a.parts + part) * kTile;
 
-    // Of this wavefront's vectors: positions some, and positions all of its rows see.
-    const uint32_t wv0 = v0 + wave * 32 * COLS;
-    const uint32_t w_first = min(wv0 / a.group, span.rows - 1), w_last = min((wv0 + 32 * COLS - 1) / a.group, span.rows - 1);
-    const bool active = wv0 < vectors;
-    const uint32_t some_lo = lowest_visible(span.position + w_first, a.window, 0), some_hi = active ? span.position + w_last + 1 : 0;
+    // Positions all of this wavefront's rows see.
+    const uint32_t wv0 = v0 + wave * 32;
+    const uint32_t w_first = min(wv0 / a.group, span.rows - 1), w_last = min((wv0 + 31) / a.group, span.rows - 1);
     const uint32_t every_lo = lowest_visible(span.position + w_last, a.window, 0), every_hi = span.position + w_first + 1;
 
     // Loads: piece `lane` of a load is row lane / kRowPieces of its rows, 16-byte place lane % kRowPieces. The place holds the piece
@@ -109,65 +108,60 @@ __global__ __launch_bounds__(kChunkWaves * 64, GROUPS) void paged_chunk_kernel(P
     const uint32_t l_row = lane / kRowPieces, l_place = lane % kRowPieces;
     auto k_shuffle = [](uint32_t row) { return DP == 64 ? (row >> 1) & 7 : row & 15; };
     auto v_shuffle = [](uint32_t row) { return DP == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3); };
-    uint32_t k_src[kLoads], v_src[kLoads];  // bytes from the half block's first row
+    // Load i of this wavefront: which side, and which of its loads. (The rows of a load lie in one half of the block.)
+    auto side_of = [&](int i) { return kSideLoads >= kWaves ? uint32_t(i / (kSideLoads / kWaves)) : wave / kSideLoads; };
+    auto load_of = [&](int i) { return kSideLoads >= kWaves ? wave + kWaves * (i % (kSideLoads / kWaves)) : wave % kSideLoads; };
+    auto half_of = [&](int i) { return load_of(i) / (16 / kLoadRows); };
+    uint32_t src[kLoads];  // bytes from the half block's first row
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-        const uint32_t row = (wave + 4 * i) * kLoadRows + l_row;
-        const uint32_t kp = l_place ^ k_shuffle(row), vp = l_place ^ v_shuffle(row);
-        k_src[i] = (row & 15) * d * 2 + kp * 16;
-        v_src[i] = (row & 15) * d * 2 + vp * 16;
-        if (!EXACT && kp * 8 >= d) k_src[i] = ~0u;  // (zeros)
-        if (!EXACT && vp * 8 >= d) v_src[i] = ~0u;
+        const uint32_t row = load_of(i) * kLoadRows + l_row;
+        const uint32_t piece = l_place ^ (side_of(i) ? v_shuffle(row) : k_shuffle(row));
+        src[i] = (row & 15) * d * 2 + piece * 16;
+        if (!EXACT && piece * 8 >= d) src[i] = ~0u;  // (zeros)
     }
     const uint32_t ring_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)ring;
     typedef const __attribute__((address_space(4))) uint32_t *ScalarIds;
     const ScalarIds ids = (ScalarIds)(uintptr_t)(a.batch + span.table);
     const uint32_t last_page = (length - 1) >> a.g.page_shift, page_mask = (1u << a.g.page_shift) - 1;
     const uint64_t head_base = reinterpret_cast<uint64_t>(a.layer_base + head * a.g.head_stride);
-    const uint64_t side_bytes = 2 * a.g.side_stride;
+    const uint32_t page_bytes = uint32_t(2 * a.g.page_stride), side_bytes = uint32_t(2 * a.g.side_stride);
+    // The page of this wavefront's load i of block kb.
+    auto page_of = [&](uint32_t kb, int i) { return ids[min((32 * kb + 16 * half_of(i)) >> a.g.page_shift, last_page)]; };
+    constexpr int kIds = kLoads > 2 ? kLoads : 1;  // (up to 128 channels a wavefront's loads lie in the same half)
     struct Pages {
-        uint32_t id[2];
+        uint32_t id[kIds];
     };
     auto pages_of = [&](uint32_t kb) {
         Pages p;
-        p.id[0] = ids[min((32 * kb) >> a.g.page_shift, last_page)];
-        p.id[1] = ids[min((32 * kb + 16) >> a.g.page_shift, last_page)];
+#pragma unroll
+        for (int i = 0; i < kIds; ++i) p.id[i] = page_of(kb, i);
         return p;
     };
     // Block kb to its place in the ring. Past the end the last block comes once more: the loads in flight stay the same.
     auto issue = [&](uint32_t kb, uint32_t place, const Pages &pages) {
         const uint32_t at = min(kb, max(kb_end, kb0 + 1) - 1);
-        uint64_t base[2];
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-            base[half] = head_base + pages.id[half] * a.g.page_stride * 2 + uint64_t((32 * at + 16 * half) & page_mask) * (d * 2);
-        const uint32_t dst = ring_base + place + wave * 1024;
-#pragma unroll
-        for (int side = 0; side < 2; ++side)
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                // (The half a load's rows lie in, the same for all of its lanes.)
-                const uint32_t half = DP == 64 ? wave >> 1 : DP == 128 ? uint32_t(i) : uint32_t(i) >> 1;
-                const uint64_t from = (half ? base[1] : base[0]) + (side ? side_bytes : 0);
-                const uint32_t off = side ? v_src[i] : k_src[i];
-                const uint32_t to = dst + side * kBlockBytes + i * 4096;
-                if constexpr (EXACT)
-                    page_to_lds(from, off, to);
-                else
-                    lane_to_lds(off == ~0u ? reinterpret_cast<uint64_t>(a.zeros) : from + off, to);
-            }
+        for (int i = 0; i < kLoads; ++i) {
+            const uint64_t from = head_base + uint64_t(pages.id[i % kIds]) * page_bytes + ((32 * at + 16 * half_of(i)) & page_mask) * (d * 2) +
+                                  (side_of(i) ? side_bytes : 0);
+            const uint32_t to = ring_base + place + side_of(i) * kBlockBytes + load_of(i) * 1024;
+            if constexpr (EXACT)
+                page_to_lds(from, src[i], to);
+            else
+                lane_to_lds(src[i] == ~0u ? reinterpret_cast<uint64_t>(a.zeros) : from + src[i], to);
+        }
     };
 
     // The queries as B operands: column j, channels 16 s + 8 h .. + 7.
-    u32x4 q[COLS][NQ][kSteps];
-    uint32_t my_pos[COLS], my_lo[COLS];
-#pragma unroll
-    for (int c = 0; c < COLS; ++c) {
-        const uint32_t v = wv0 + 32 * c + j;
+    u32x4 q[NQ][kSteps];
+    uint32_t my_pos, my_lo;
+    {
+        const uint32_t v = wv0 + j;
         const uint32_t row = min(v / a.group, span.rows - 1);
         const uint32_t hq = head * a.group + (v < vectors ? v - row * a.group : 0);
-        my_pos[c] = span.position + row;
-        my_lo[c] = lowest_visible(my_pos[c], a.window, 0);
+        my_pos = span.position + row;
+        my_lo = lowest_visible(my_pos, a.window, 0);
         const T *src = static_cast<const T *>(a.q.data) + uint64_t(span.row0 + row) * a.q.row_stride + hq * a.q.head_stride;
         typename QueryRaw<ELEM>::type raw[kSteps];
         if (a.q_on_16) {
@@ -182,7 +176,15 @@ __global__ __launch_bounds__(kChunkWaves * 64, GROUPS) void paged_chunk_kernel(P
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
             split_query<PAGE, ELEM, NQ>(raw[s], v < vectors && (EXACT || 16 * s + 8 * h < d),
-                                        [&](int n, u32x4 x) { q[c][n][s] = x; });
+                                        [&](int n, u32x4 x) { q[n][s] = x; });
+    }
+    // Of 256 channels queries go to the accumulation registers, which products read as well: there are 256 vector registers, and
+    // what vector code works on fills them. (Left to itself the compiler moves the queries out and back in every block.)
+    if constexpr (DP == 256) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) asm volatile("" : "+a"(q[n][s]));
     }
     // (The compiler cannot count the ring's loads: every load of its own has to be in before the first of them.)
     wait_loads<0>();
@@ -193,16 +195,12 @@ __global__ __launch_bounds__(kChunkWaves * 64, GROUPS) void paged_chunk_kernel(P
     const uint32_t tr_row = 4 * h + ((lane & 15) >> 2);
     const uint32_t v_at = kBlockBytes + tr_row * kRowBytes + ((v_shuffle(tr_row) * 16) ^ (((lane >> 4) & 1) * 32 + (lane & 3) * 8));
 
-    float ref[COLS], threshold[COLS], sum[COLS];
-    floatx16 o[COLS][kOut];
+    float ref = 0.0f, threshold = -INFINITY, sum = 0.0f;
+    floatx16 o[kOut];
 #pragma unroll
-    for (int c = 0; c < COLS; ++c) {
-        ref[c] = 0.0f, threshold[c] = -INFINITY, sum[c] = 0.0f;
+    for (int t = 0; t < kOut; ++t)
 #pragma unroll
-        for (int t = 0; t < kOut; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[c][t][r] = 0.0f;
-    }
+        for (int r = 0; r < 16; ++r) o[t][r] = 0.0f;
 
     // Operands out of a sub-block at LDS address `at`.
     auto k_operand = [&](uint32_t at, int i) {
@@ -219,53 +217,45 @@ __global__ __launch_bounds__(kChunkWaves * 64, GROUPS) void paged_chunk_kernel(P
         }
         return v;
     };
-    // A lane's scores of a block, relative to the reference, and the largest of a column.
-    float x[COLS][16];
-    auto scaled = [&](float s, int c) {
+    // A lane's scores of a block, relative to the reference.
+    float x[16];
+    auto scaled = [&](float s) {
         if constexpr (CAP)
-            return softcap_of_exp2_arg(s * a.scale_log2, a.cap_log2, ref[c]);
+            return softcap_of_exp2_arg(s * a.scale_log2, a.cap_log2, ref);
         else
-            return __builtin_fmaf(s, a.scale_log2, -ref[c]);
+            return __builtin_fmaf(s, a.scale_log2, -ref);
     };
-    // Masks the scores of block kb where a row does not see all of it, and moves references that they pass.
-    auto settle = [&](uint32_t kb, float (&most)[COLS]) {
+    // Masks the scores of block kb where a row does not see all of it, and moves the references that they pass; `most`: the
+    // largest of a lane's.
+    auto settle = [&](uint32_t kb, float most) {
         if (32 * kb < every_lo || 32 * kb + 32 > every_hi) {
+            most = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < COLS; ++c) {
-                most[c] = -INFINITY;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const uint32_t key = 32 * kb + 8 * (r / 4) + 4 * h + r % 4;
-                    if (key > my_pos[c] || key < my_lo[c]) x[c][r] = -INFINITY;
-                    most[c] = fmaxf(most[c], x[c][r]);
-                }
+            for (int r = 0; r < 16; ++r) {
+                const uint32_t key = 32 * kb + 8 * (r / 4) + 4 * h + r % 4;
+                if (key > my_pos || key < my_lo) x[r] = -INFINITY;
+                most = fmaxf(most, x[r]);
             }
         }
-        bool over = false;
+        if (__builtin_amdgcn_ballot_w64(most > threshold) != 0) {
+            const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
+            const float m = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+            const bool live = threshold != -INFINITY;
+            float delta = live ? fmaxf(m, 0.0f) : m;
+            if (m == -INFINITY) delta = 0.0f;
+            const float alpha = live ? fast_exp2(-delta) : 1.0f;
+            ref += delta;
+            if (m != -INFINITY) threshold = kChunkSlack;
+            sum *= alpha;
 #pragma unroll
-        for (int c = 0; c < COLS; ++c) over = over || most[c] > threshold[c];
-        if (__builtin_amdgcn_ballot_w64(over) != 0) {
+            for (int t = 0; t < kOut; ++t) o[t] *= alpha;
 #pragma unroll
-            for (int c = 0; c < COLS; ++c) {
-                const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(most[c]), __float_as_uint(most[c]), false, false);
-                const float m = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
-                const bool live = threshold[c] != -INFINITY;
-                float delta = live ? fmaxf(m, 0.0f) : m;
-                if (m == -INFINITY) delta = 0.0f;
-                const float alpha = live ? fast_exp2(-delta) : 1.0f;
-                ref[c] += delta;
-                if (m != -INFINITY) threshold[c] = kChunkSlack;
-                sum[c] *= alpha;
-#pragma unroll
-                for (int t = 0; t < kOut; ++t) o[c][t] *= alpha;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[c][r] -= delta;
-            }
+            for (int r = 0; r < 16; ++r) x[r] -= delta;
         }
     };
     // Rows of block kb no query of the tile sees may hold anything: their values are zeroed in LDS, where the block lies at `at`.
     auto clear = [&](uint32_t kb, uint32_t at) {
-        for (uint32_t p = tid; p < 32 * kRowPieces; p += kChunkWaves * 64) {
+        for (uint32_t p = tid; p < 32 * kRowPieces; p += kWaves * 64) {
             const uint32_t key = 32 * kb + p / kRowPieces;
             if (key < tile_lo || key >= tile_hi)
                 *reinterpret_cast<__attribute__((address_space(3))) u32x4 *>((uintptr_t)(at + kBlockBytes + p * 16)) = u32x4{0, 0, 0, 0};
@@ -302,20 +292,16 @@ __global__ __launch_bounds__(kChunkWaves * 64, GROUPS) void paged_chunk_kernel(P
         clear_stage(kb0, ring_base);
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) k[i] = k_operand(ring_base, i);
-        float most[COLS];
+        floatx16 s;
 #pragma unroll
-        for (int c = 0; c < COLS; ++c) {
-            floatx16 s;
+        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+        for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i)
+            for (int n = 0; n < NQ; ++n) s = mfma_32x32x16<PAGE>(k[i], q[n][i], s);
+        float most = -INFINITY;
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) s = mfma_32x32x16<PAGE>(k[i], q[c][n][i], s);
-            most[c] = -INFINITY;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) x[c][r] = scaled(s[r], c), most[c] = fmaxf(most[c], x[c][r]);
-        }
+        for (int r = 0; r < 16; ++r) x[r] = scaled(s[r]), most = fmaxf(most, x[r]);
         settle(kb0, most);
         if constexpr (kSubs > 1) {
 #pragma unroll
@@ -345,76 +331,64 @@ __global__ __launch_bounds__(kChunkWaves * 64, GROUPS) void paged_chunk_kernel(P
             const uint32_t k_next = u + 2 < kSubs ? at + (u + 2) * kSubBytes : next + (u + 2 - kSubs) * kSubBytes;
             // Three stretches, each of products beside vector work of about their length: the next block's scores beside three quarters
             // of this block's exponentials, the first half of P.V beside the rest, the second half beside the next scores' scaling.
-            constexpr int kAll = 16 * COLS, kFirst = kAll * 3 / 4;
-            floatx16 s[COLS];
+            constexpr int kFirst = 12;
+            floatx16 s;
 #pragma unroll
-            for (int c = 0; c < COLS; ++c)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[c][r] = 0.0f;
-            u32x4 p[COLS][NP][2];
-            u32x4 v[kOut][2];
-            auto weigh = [&](int e) {  // exponential e: halves of the keys, columns, keys
-                const int m = e / (8 * COLS), c = e / 8 % COLS, r = 8 * m + e % 8;
-                x[c][r] = fast_exp2(x[c][r]);
+            for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+            u32x4 p[NP][2], v[kOut][2];
+            auto weigh = [&](int e) {
+                x[e] = fast_exp2(x[e]);
                 if (e % 8 == 7) {
                     float w[8];
 #pragma unroll
-                    for (int y = 0; y < 8; ++y) w[y] = x[c][8 * m + y];
-                    sum[c] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+                    for (int y = 0; y < 8; ++y) w[y] = x[e - 7 + y];
+                    sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
                     u32x4 pieces[NP];
                     split_8<PAGE, NP>(w, pieces);
 #pragma unroll
-                    for (int n = 0; n < NP; ++n) p[c][n][m] = pieces[n];
+                    for (int n = 0; n < NP; ++n) p[n][e / 8] = pieces[n];
                 }
             };
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
-                for (int c = 0; c < COLS; ++c)
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) s[c] = mfma_32x32x16<PAGE>(k[i], q[c][n][i], s[c]);
+                for (int n = 0; n < NQ; ++n) s = mfma_32x32x16<PAGE>(k[i], q[n][i], s);
 #pragma unroll
                 for (int e = i * kFirst / kSteps; e < (i + 1) * kFirst / kSteps; ++e) weigh(e);
-                if (i >= kSteps - 2 * kOut) v[(i - (kSteps - 2 * kOut)) % kOut][(i - (kSteps - 2 * kOut)) / kOut] =
-                    v_operand(here, (i - (kSteps - 2 * kOut)) % kOut, (i - (kSteps - 2 * kOut)) / kOut);
+                v[i % kOut][i / kOut] = v_operand(here, i % kOut, i / kOut);
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int t = 0; t < kOut; ++t) {
 #pragma unroll
-                for (int c = 0; c < COLS; ++c)
+                for (int n = 0; n < NP; ++n) o[t] = mfma_32x32x16<PAGE>(v[t][0], p[n][0], o[t]);
 #pragma unroll
-                    for (int n = 0; n < NP; ++n) o[c][t] = mfma_32x32x16<PAGE>(v[t][0], p[c][n][0], o[c][t]);
-#pragma unroll
-                for (int e = kFirst + t * (kAll - kFirst) / kOut; e < kFirst + (t + 1) * (kAll - kFirst) / kOut; ++e) weigh(e);
+                for (int e = kFirst + t * (16 - kFirst) / kOut; e < kFirst + (t + 1) * (16 - kFirst) / kOut; ++e) weigh(e);
                 if (kSubs > 1) {
                     k[2 * t] = k_operand(k_next, 2 * t);
                     k[2 * t + 1] = k_operand(k_next, 2 * t + 1);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            float most[COLS];
+            float most = 0.0f;
 #pragma unroll
             for (int t = 0; t < kOut; ++t) {
 #pragma unroll
-                for (int c = 0; c < COLS; ++c)
+                for (int n = 0; n < NP; ++n) o[t] = mfma_32x32x16<PAGE>(v[t][1], p[n][1], o[t]);
 #pragma unroll
-                    for (int n = 0; n < NP; ++n) o[c][t] = mfma_32x32x16<PAGE>(v[t][1], p[c][n][1], o[c][t]);
-#pragma unroll
-                for (int e = t * kAll / kOut; e < (t + 1) * kAll / kOut; ++e) {
-                    const int c = e / 16, r = e % 16;
-                    x[c][r] = scaled(s[c][r], c);
-                    if (r == 0)
-                        most[c] = x[c][0];
-                    else if (r % 2 == 0)
-                        most[c] = max3(most[c], x[c][r - 1], x[c][r]);
+                for (int r = t * 16 / kOut; r < (t + 1) * 16 / kOut; ++r) {
+                    x[r] = scaled(s[r]);
+                    if (r == 2)
+                        most = max3(x[0], x[1], x[2]);
+                    else if (r > 2 && r % 2 == 0)
+                        most = max3(most, x[r - 1], x[r]);
                     else if (r == 15)
-                        most[c] = fmaxf(most[c], x[c][15]);
+                        most = max3(most, x[15], x[15]);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (kb + u + 1 < kb_end) settle(kb + u + 1, most);
             if (kb + u + 1 >= kb_end) break;
+            settle(kb + u + 1, most);
         }
         const uint32_t was = at;
         at = next;
@@ -426,17 +400,15 @@ __global__ __launch_bounds__(kChunkWaves * 64, GROUPS) void paged_chunk_kernel(P
     // A lane holds of its column channels 32 t + 8 (r / 4) + 4 h + r % 4.
     const bool whole = a.parts == 1;
     bool bad = false;
-#pragma unroll
-    for (int c = 0; c < COLS; ++c) {
-        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum[c]), __float_as_uint(sum[c]), false, false);
+    if (wv0 + j < vectors) {
+        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
         const float l = __uint_as_float(both[0]) + __uint_as_float(both[1]);
-        const uint32_t v = wv0 + 32 * c + j;
-        if (v >= vectors) continue;
+        const uint32_t v = wv0 + j;
         float check = l;
 #pragma unroll
         for (int t = 0; t < kOut; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) check += EXACT || 32u * t + 8 * (r / 4) + 4 * h < d ? o[c][t][r] : 0.0f;
+            for (int r = 0; r < 16; ++r) check += EXACT || 32u * t + 8 * (r / 4) + 4 * h < d ? o[t][r] : 0.0f;
         bad = bad || check != check;
         if (whole) {
             const float inv = 1.0f / l;
@@ -451,7 +423,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, GROUPS) void paged_chunk_kernel(P
                     if (!EXACT && ch >= d) continue;
                     Four y;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) y.v[e] = Elem<ELEM>::from_f32(o[c][t][r + e] * inv);
+                    for (int e = 0; e < 4; ++e) y.v[e] = Elem<ELEM>::from_f32(o[t][r + e] * inv);
                     if (a.out_on_16) {
                         *reinterpret_cast<Four *>(dst + ch) = y;
                     } else {
@@ -466,12 +438,12 @@ __global__ __launch_bounds__(kChunkWaves * 64, GROUPS) void paged_chunk_kernel(P
 #pragma unroll
                 for (int r = 0; r < 16; r += 4)
                     *reinterpret_cast<floatx4 *>(a.ws_acc + slot * DP + 32 * t + 2 * r + 4 * h) =
-                        floatx4{o[c][t][r], o[c][t][r + 1], o[c][t][r + 2], o[c][t][r + 3]};
-            if (h == 0) a.ws_ml[slot] = make_float2(threshold[c] == -INFINITY ? -INFINITY : ref[c], l);
+                        floatx4{o[t][r], o[t][r + 1], o[t][r + 2], o[t][r + 3]};
+            if (h == 0) a.ws_ml[slot] = make_float2(threshold == -INFINITY ? -INFINITY : ref, l);
         }
     }
     if (any_of_group(bad, &lds_flag))
-        paged_careful<PAGE, ELEM, DP>(a, span, head, v0, min(v0 + kTile, vectors), wave, kChunkWaves, 32 * kb0, 32 * kb_end,
+        paged_careful<PAGE, ELEM, DP>(a, span, head, v0, min(v0 + kTile, vectors), wave, kWaves, 32 * kb0, 32 * kb_end,
                                       [&](uint32_t v, const float (&acc)[DP / 64], float m, float l) {
                                           paged_write_careful<ELEM, DP>(a, span, head, v, whole, slot0 + v - v0, true, acc, m, l);
                                       });
@@ -481,17 +453,15 @@ template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP>
 hipError_t launch_chunk_as(const PagedAttn &a, hipStream_t stream) {
     if constexpr (!paged_chunk_takes(DP, PAGE, ELEM)) return hipErrorInvalidValue;
     else {
-    constexpr int kCols = int(paged_chunk_tile(DP, ELEM)) / (kChunkWaves * 32);
-    constexpr int kGroups = DP == 64 ? 2 : 1;
     auto run = [&](auto kernel) {
         static const hipError_t granted =
             hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(chunk_lds(DP)));
         if (granted != hipSuccess) return granted;
-        launch_kernel(kernel, a.units * a.parts, kChunkWaves * 64, chunk_lds(DP), stream, a);
+        launch_kernel(kernel, a.units * a.parts, paged_chunk_waves(DP, ELEM) * 64, chunk_lds(DP), stream, a);
         return hipGetLastError();
     };
-    return a.cap_log2 != 0.0f ? run(paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kCols, kGroups, true>)
-                              : run(paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kCols, kGroups, false>);
+    return a.cap_log2 != 0.0f ? run(paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, true>)
+                              : run(paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, false>);
     }
 }
 template <int PAGE, int ELEM, int NQ, int NP>
