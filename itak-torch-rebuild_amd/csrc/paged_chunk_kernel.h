@@ -202,23 +202,21 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[t][r] = 0.0f;
 
-    // Operands out of a sub-block at LDS address `at`.
-    auto k_operand = [&](uint32_t at, int i) {
-        return *reinterpret_cast<const __attribute__((address_space(3))) u32x4 *>((uintptr_t)(at + (k_at ^ (i * 32))));
-    };
-    auto v_operand = [&](uint32_t at, int t, int m) {
+    // Operands out of LDS: a lane's address for each of a row's places, from which the rest is a constant.
+    auto k_operand = [&](uint32_t lane_at) { return *reinterpret_cast<const __attribute__((address_space(3))) u32x4 *>((uintptr_t)lane_at); };
+    auto v_operand = [&](uint32_t lane_at, int m) {
         u32x4 v;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const shortx4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) shortx4 *)(uintptr_t)(at + (v_at ^ (t * 64)) + (16 * m + 8 * u) * kRowBytes));
+                (__attribute__((address_space(3))) shortx4 *)(uintptr_t)(lane_at + (16 * m + 8 * u) * kRowBytes));
             const uint2 y = __builtin_bit_cast(uint2, x);
             v[2 * u] = y.x, v[2 * u + 1] = y.y;
         }
         return v;
     };
     // A lane's scores of a block, relative to the reference.
-    float x[16];
+    floatx16 x;
     auto scaled = [&](float s) {
         if constexpr (CAP)
             return softcap_of_exp2_arg(s * a.scale_log2, a.cap_log2, ref);
@@ -291,7 +289,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
         asm volatile("" ::: "memory");
         clear_stage(kb0, ring_base);
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) k[i] = k_operand(ring_base, i);
+        for (int i = 0; i < kSteps; ++i) k[i] = k_operand(ring_base + (k_at ^ (i * 32)));
         floatx16 s;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.0f;
@@ -305,88 +303,87 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
         settle(kb0, most);
         if constexpr (kSubs > 1) {
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) k[i] = k_operand(ring_base + kSubBytes, i);
+            for (int i = 0; i < kSteps; ++i) k[i] = k_operand(ring_base + (k_at ^ (i * 32)) + kSubBytes);
         }
     }
     uint32_t at = ring_base, next = ring_base + kStageBytes, free_at = (kStages - 1) * kStageBytes;
     for (uint32_t g = 0; g < stages; ++g) {
+        const uint32_t kb = kb0 + g * kSubs;
+        Pages after[kSubs];
+#pragma unroll
+        for (int u = 0; u < kSubs; ++u) after[u] = pages_of(kb + kStages * kSubs + u);
         // This wavefront's loads of the next stage have landed (those of the stages behind it may still fly); behind the barrier
         // everybody's have, and everybody is done with the stage before this one, which the loads that go out now overwrite.
         wait_loads<kStageLoads * (kStages - 3)>();
         __builtin_amdgcn_s_barrier();
-        const uint32_t kb = kb0 + g * kSubs;
 #pragma unroll
         for (int u = 0; u < kSubs; ++u) issue(kb + (kStages - 1) * kSubs + u, free_at + u * kSubBytes, ahead[u]);
+        // (The scalar loads of page ids come in here: while one is out, every wait for an operand from LDS is a wait for all of them.)
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
 #pragma unroll
-        for (int u = 0; u < kSubs; ++u) ahead[u] = pages_of(kb + kStages * kSubs + u);
+        for (int u = 0; u < kSubs; ++u) ahead[u] = after[u];
         clear_stage(kb + kSubs, next);
+        uint32_t k_lane[kSteps], v_lane[kOut];
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) k_lane[i] = next + (k_at ^ (i * 32));
+#pragma unroll
+        for (int t = 0; t < kOut; ++t) v_lane[t] = at + (v_at ^ (t * 64));
         if constexpr (kSubs == 1) {
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) k[i] = k_operand(next, i);
+            for (int i = 0; i < kSteps; ++i) k[i] = k_operand(k_lane[i]);
         }
 #pragma unroll
         for (int u = 0; u < kSubs; ++u) {
-            const uint32_t here = at + u * kSubBytes;
-            // Where the operands of the scores after the next lie.
-            const uint32_t k_next = u + 2 < kSubs ? at + (u + 2) * kSubBytes : next + (u + 2 - kSubs) * kSubBytes;
-            // Three stretches, each of products beside vector work of about their length: the next block's scores beside three quarters
-            // of this block's exponentials, the first half of P.V beside the rest, the second half beside the next scores' scaling.
-            constexpr int kFirst = 12;
+            // Two stretches of products: the next block's scores beside this block's exponentials, then P.V beside the next scores'
+            // scaling and maximum, which are done when the products are: nothing waits at the border of two blocks.
             floatx16 s;
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = 0.0f;
             u32x4 p[NP][2], v[kOut][2];
-            auto weigh = [&](int e) {
-                x[e] = fast_exp2(x[e]);
-                if (e % 8 == 7) {
-                    float w[8];
-#pragma unroll
-                    for (int y = 0; y < 8; ++y) w[y] = x[e - 7 + y];
-                    sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-                    u32x4 pieces[NP];
-                    split_8<PAGE, NP>(w, pieces);
-#pragma unroll
-                    for (int n = 0; n < NP; ++n) p[n][e / 8] = pieces[n];
-                }
-            };
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) s = mfma_32x32x16<PAGE>(k[i], q[n][i], s);
+                v[i % kOut][i / kOut] = v_operand(v_lane[i % kOut] + u * kSubBytes, i / kOut);
 #pragma unroll
-                for (int e = i * kFirst / kSteps; e < (i + 1) * kFirst / kSteps; ++e) weigh(e);
-                v[i % kOut][i / kOut] = v_operand(here, i % kOut, i / kOut);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+                for (int e = i * 16 / kSteps; e < (i + 1) * 16 / kSteps; ++e) {
+                    x[e] = fast_exp2(x[e]);
+                    if (e % 8 == 7) {
+                        float w[8];
 #pragma unroll
-            for (int t = 0; t < kOut; ++t) {
+                        for (int y = 0; y < 8; ++y) w[y] = x[e - 7 + y];
+                        sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+                        u32x4 pieces[NP];
+                        split_8<PAGE, NP>(w, pieces);
 #pragma unroll
-                for (int n = 0; n < NP; ++n) o[t] = mfma_32x32x16<PAGE>(v[t][0], p[n][0], o[t]);
-#pragma unroll
-                for (int e = kFirst + t * (16 - kFirst) / kOut; e < kFirst + (t + 1) * (16 - kFirst) / kOut; ++e) weigh(e);
-                if (kSubs > 1) {
-                    k[2 * t] = k_operand(k_next, 2 * t);
-                    k[2 * t + 1] = k_operand(k_next, 2 * t + 1);
+                        for (int n = 0; n < NP; ++n) p[n][e / 8] = pieces[n];
+                    }
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
             float most = 0.0f;
 #pragma unroll
-            for (int t = 0; t < kOut; ++t) {
+            for (int i = 0; i < 2 * kOut; ++i) {
+                const int t = i % kOut, m = i / kOut;
 #pragma unroll
-                for (int n = 0; n < NP; ++n) o[t] = mfma_32x32x16<PAGE>(v[t][1], p[n][1], o[t]);
+                for (int n = 0; n < NP; ++n) o[t] = mfma_32x32x16<PAGE>(v[t][m], p[n][m], o[t]);
+                // (The scores' last product is on its way for the time of two others.)
+                constexpr int kSlots = 2 * kOut > 4 ? 2 * kOut - 3 : 2, kSkip = 2 * kOut > 4 ? 2 : 1;
 #pragma unroll
-                for (int r = t * 16 / kOut; r < (t + 1) * 16 / kOut; ++r) {
-                    x[r] = scaled(s[r]);
+                for (int r = (i - kSkip) * 16 / kSlots; r < (i - kSkip + 1) * 16 / kSlots; ++r) {
+                    if (r < 0 || r >= 16) continue;
+                    s[r] = scaled(s[r]);
                     if (r == 2)
-                        most = max3(x[0], x[1], x[2]);
+                        most = max3(s[0], s[1], s[2]);
                     else if (r > 2 && r % 2 == 0)
-                        most = max3(most, x[r - 1], x[r]);
+                        most = max3(most, s[r - 1], s[r]);
                     else if (r == 15)
-                        most = max3(most, x[15], x[15]);
+                        most = max3(most, s[15], s[15]);
                 }
+                if (kSubs > 1) k[i] = k_operand(k_lane[i] + u * kSubBytes);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            x = s;
             if (kb + u + 1 >= kb_end) break;
             settle(kb + u + 1, most);
         }
