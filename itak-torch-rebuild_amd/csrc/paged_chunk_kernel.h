@@ -101,6 +101,9 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     const uint32_t wv0 = v0 + wave * 32;
     const uint32_t w_first = min(wv0 / a.group, span.rows - 1), w_last = min((wv0 + 31) / a.group, span.rows - 1);
     const uint32_t every_lo = lowest_visible(span.position + w_last, a.window, 0), every_hi = span.position + w_first + 1;
+    // Blocks all of which they all see: from inner0 on, `inner` of them.
+    const uint32_t inner0 = __builtin_amdgcn_readfirstlane((every_lo + 31) / 32);
+    const uint32_t inner = __builtin_amdgcn_readfirstlane(every_hi / 32 > inner0 ? every_hi / 32 - inner0 : 0);
 
     // Loads: piece `lane` of a load is row lane / kRowPieces of its rows, 16-byte place lane % kRowPieces. The place holds the piece
     // place ^ (the row's shuffle): of keys, so that 16 rows' pieces of one number lie in 16 different places modulo 256 bytes;
@@ -111,7 +114,10 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     // Load i of this wavefront: which side, and which of its loads. (The rows of a load lie in one half of the block.)
     auto side_of = [&](int i) { return kSideLoads >= kWaves ? uint32_t(i / (kSideLoads / kWaves)) : wave / kSideLoads; };
     auto load_of = [&](int i) { return kSideLoads >= kWaves ? wave + kWaves * (i % (kSideLoads / kWaves)) : wave % kSideLoads; };
-    auto half_of = [&](int i) { return load_of(i) / (16 / kLoadRows); };
+    auto half_of = [&](int i) {
+        constexpr int kHalf = 16 / kLoadRows;  // loads of a half of a side
+        return kSideLoads > kWaves || kWaves == 4 ? uint32_t(kWaves * (i % (kSideLoads / kWaves)) / kHalf) : load_of(i) / kHalf;
+    };
     uint32_t src[kLoads];  // bytes from the half block's first row
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
@@ -121,30 +127,32 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
         if (!EXACT && piece * 8 >= d) src[i] = ~0u;  // (zeros)
     }
     const uint32_t ring_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)ring;
-    typedef const __attribute__((address_space(4))) uint32_t *ScalarIds;
-    const ScalarIds ids = (ScalarIds)(uintptr_t)(a.batch + span.table);
     const uint32_t last_page = (length - 1) >> a.g.page_shift, page_mask = (1u << a.g.page_shift) - 1;
     const uint64_t head_base = reinterpret_cast<uint64_t>(a.layer_base + head * a.g.head_stride);
     const uint32_t page_bytes = uint32_t(2 * a.g.page_stride), side_bytes = uint32_t(2 * a.g.side_stride);
-    // The page of this wavefront's load i of block kb.
-    auto page_of = [&](uint32_t kb, int i) { return ids[min((32 * kb + 16 * half_of(i)) >> a.g.page_shift, last_page)]; };
-    constexpr int kIds = kLoads > 2 ? kLoads : 1;  // (up to 128 channels a wavefront's loads lie in the same half)
-    struct Pages {
-        uint32_t id[kIds];
-    };
-    auto pages_of = [&](uint32_t kb) {
-        Pages p;
+    // Where the next 64 blocks' halves begin, a block a lane: worked out by vector code every 64 blocks and read lane by lane, where a
+    // scalar load and some sixteen scalar instructions a block would each cost the wavefront an issue slot. A wavefront's loads lie in
+    // one half of a block where it has one or two of them, else in both. (Positions past the end are clamped to the last page: any row of it may be read.)
+    constexpr bool kBothHalves = kLoads > 2;
+    uint64_t begins[kBothHalves ? 2 : 1];
+    auto look_up = [&](uint32_t kb) {
 #pragma unroll
-        for (int i = 0; i < kIds; ++i) p.id[i] = page_of(kb, i);
-        return p;
+        for (int i = 0; i < (kBothHalves ? 2 : 1); ++i) {
+            const uint32_t key = 32 * (kb + lane) + 16 * (kBothHalves ? uint32_t(i) : half_of(0));
+            const uint32_t id = a.batch[span.table + min(key >> a.g.page_shift, last_page)];
+            begins[i] = head_base + uint64_t(id) * page_bytes + (key & page_mask) * (d * 2);
+        }
     };
-    // Block kb to its place in the ring. Past the end the last block comes once more: the loads in flight stay the same.
-    auto issue = [&](uint32_t kb, uint32_t place, const Pages &pages) {
-        const uint32_t at = min(kb, max(kb_end, kb0 + 1) - 1);
+    // Block number n (from kb0 on) to its place in the ring.
+    auto issue = [&](uint32_t n, uint32_t place) {
+        uint64_t begin[kBothHalves ? 2 : 1];
+#pragma unroll
+        for (int i = 0; i < (kBothHalves ? 2 : 1); ++i)
+            begin[i] = uint64_t(uint32_t(__builtin_amdgcn_readlane(uint32_t(begins[i] >> 32), n & 63))) << 32 |
+                       uint32_t(__builtin_amdgcn_readlane(uint32_t(begins[i]), n & 63));
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const uint64_t from = head_base + uint64_t(pages.id[i % kIds]) * page_bytes + ((32 * at + 16 * half_of(i)) & page_mask) * (d * 2) +
-                                  (side_of(i) ? side_bytes : 0);
+            const uint64_t from = begin[kBothHalves ? half_of(i) : 0] + (side_of(i) ? side_bytes : 0);
             const uint32_t to = ring_base + place + side_of(i) * kBlockBytes + load_of(i) * 1024;
             if constexpr (EXACT)
                 page_to_lds(from, src[i], to);
@@ -186,8 +194,6 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) asm volatile("" : "+a"(q[n][s]));
     }
-    // (The compiler cannot count the ring's loads: every load of its own has to be in before the first of them.)
-    wait_loads<0>();
 
     // Where the operands lie in a stage: K row j, piece 2 s + h at ((2 s + h) ^ shuffle) = place0 ^ 2 s; V row 4 h + (lane & 15) / 4
     // (of the four of 16 m + 8 u + ..), channels 32 t + 16 (lane / 16 % 2) + 4 (lane % 4) on.
@@ -226,7 +232,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     // Masks the scores of block kb where a row does not see all of it, and moves the references that they pass; `most`: the
     // largest of a lane's.
     auto settle = [&](uint32_t kb, float most) {
-        if (32 * kb < every_lo || 32 * kb + 32 > every_hi) {
+        if (kb - inner0 >= inner) {
             most = -INFINITY;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -259,28 +265,24 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
                 *reinterpret_cast<__attribute__((address_space(3))) u32x4 *>((uintptr_t)(at + kBlockBytes + p * 16)) = u32x4{0, 0, 0, 0};
         }
     };
-    // The blocks of a stage that have such rows: at most the tile's first and last, and what comes past the end in their stage.
+    // The blocks of a stage that have such rows: at most the tile's first and last.
     auto clear_stage = [&](uint32_t kb, uint32_t at) {
-        bool any = false;
 #pragma unroll
         for (int u = 0; u < kSubs; ++u)
-            if (32 * (kb + u) < tile_lo || 32 * (kb + u) + 32 > tile_hi) clear(kb + u, at + u * kSubBytes), any = true;
-        if (any) {
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-            __builtin_amdgcn_s_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-        }
+            if (32 * (kb + u) < tile_lo || 32 * (kb + u) + 32 > tile_hi) clear(kb + u, at + u * kSubBytes);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
     };
 
     // Stages of the ring fill ahead of the one at hand; its last places are never read where the blocks end inside one.
     const uint32_t stages = (kb_end - kb0 + kSubs - 1) / kSubs;
-    Pages ahead[kSubs];
+    look_up(kb0);
+    wait_loads<0>();  // (the compiler cannot count the ring's loads: every load of its own has to be in before the first of them)
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s)
 #pragma unroll
-        for (int u = 0; u < kSubs; ++u) issue(kb0 + s * kSubs + u, s * kStageBytes + u * kSubBytes, pages_of(kb0 + s * kSubs + u));
-#pragma unroll
-    for (int u = 0; u < kSubs; ++u) ahead[u] = pages_of(kb0 + (kStages - 1) * kSubs + u);
+        for (int u = 0; u < kSubs; ++u) issue(s * kSubs + u, s * kStageBytes + u * kSubBytes);
     u32x4 k[kSteps];
     if (stages) {
         // The first block's scores by themselves, and the operands of the second block's.
@@ -309,20 +311,15 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     uint32_t at = ring_base, next = ring_base + kStageBytes, free_at = (kStages - 1) * kStageBytes;
     for (uint32_t g = 0; g < stages; ++g) {
         const uint32_t kb = kb0 + g * kSubs;
-        Pages after[kSubs];
-#pragma unroll
-        for (int u = 0; u < kSubs; ++u) after[u] = pages_of(kb + kStages * kSubs + u);
         // This wavefront's loads of the next stage have landed (those of the stages behind it may still fly); behind the barrier
         // everybody's have, and everybody is done with the stage before this one, which the loads that go out now overwrite.
         wait_loads<kStageLoads * (kStages - 3)>();
         __builtin_amdgcn_s_barrier();
+        const uint32_t n = (g + kStages - 1) * kSubs;
+        if ((n & 63) == 0) look_up(kb0 + n);
 #pragma unroll
-        for (int u = 0; u < kSubs; ++u) issue(kb + (kStages - 1) * kSubs + u, free_at + u * kSubBytes, ahead[u]);
-        // (The scalar loads of page ids come in here: while one is out, every wait for an operand from LDS is a wait for all of them.)
-        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-#pragma unroll
-        for (int u = 0; u < kSubs; ++u) ahead[u] = after[u];
-        clear_stage(kb + kSubs, next);
+        for (int u = 0; u < kSubs; ++u) issue(n + u, free_at + u * kSubBytes);
+        if (g + 2 == stages) clear_stage(kb + kSubs, next);
         uint32_t k_lane[kSteps], v_lane[kOut];
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) k_lane[i] = next + (k_at ^ (i * 32));
@@ -340,6 +337,12 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = 0.0f;
             u32x4 p[NP][2], v[kOut][2];
+            // The wavefront of a SIMD that is behind goes first: left to itself the SIMD prefers the older one, which then waits at the
+            // barrier while the younger runs alone.
+            if (u == 0)
+                __builtin_amdgcn_s_setprio(3);
+            else
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
@@ -362,6 +365,10 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
                 __builtin_amdgcn_sched_barrier(0);
             }
             float most = 0.0f;
+            if (u == 0 && kSubs > 1)
+                __builtin_amdgcn_s_setprio(2);
+            else
+                __builtin_amdgcn_s_setprio(0);
 #pragma unroll
             for (int i = 0; i < 2 * kOut; ++i) {
                 const int t = i % kOut, m = i / kOut;
