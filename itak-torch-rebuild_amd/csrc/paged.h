@@ -43,6 +43,12 @@ hipError_t launch_paged_append(uint32_t page_elem, uint32_t elem, bool by_8, con
 // and the grid does not depend on the lengths. A unit that one workgroup has whole is written out by it; of the others every workgroup
 // leaves its partial in slot w + (unit's index), which no two parts share, and the merge launch joins them.
 // The cut is worked out on the device from the batch's lengths, so a captured launch is right for whatever batch is set when it runs.
+// Items that travel with a launch: an eager call whose batch has at most this many hands them over by value, and its kernels do not
+// go to memory for them; one that is being captured, or has more, leaves them to the batch in device memory.
+constexpr uint32_t kPagedInline = 8;
+struct PagedItemWords {
+    uint32_t position, rows, row0, table;
+};
 struct PagedAttn {
     PagedGeom g;
     const uint32_t *batch;
@@ -51,7 +57,9 @@ struct PagedAttn {
     uint32_t rows;       // of the batch the launch was made for
     uint32_t items;
     uint32_t group;      // query heads a KV head
-    uint32_t tile;       // vectors
+    uint32_t group_magic; // ceil(2^32 / group): v / group is the high word of v * magic for v below 2^26; group 1: 0
+    uint32_t tile;       // vectors, a power of two
+    uint32_t tile_shift;
     uint32_t groups;     // workgroups
     uint32_t least;      // blocks a workgroup takes at least
     uint32_t units;      // of the batch the launch was made for
@@ -63,14 +71,19 @@ struct PagedAttn {
     uint32_t window;
     uint32_t parts;      // kernel of many rows: workgroups a unit is dealt to; 0: the line above
     const void *zeros;   // 16 bytes of them
+    uint32_t inline_items; // 0: the batch's are read from device memory
+    uint32_t total;      // with inline items: blocks of all units
+    PagedItemWords item[kPagedInline];
     float *ws_acc;       // [slots][tile][padded head_dim]
     float2 *ws_ml;       // [slots][tile]: maximum (log2 domain), sum
 };
+// Workgroups that may share a unit.
+constexpr uint32_t kPagedMostParts = 1024;
 // The kernel of few rows (paged_few_kernel.h): tiles of `sets` times 16 vectors, 1, 2 or 4 (up to 128 channels).
 constexpr uint32_t kPagedSet = 16;
 // Workgroups a compute unit holds: two where a lane does with 256 registers.
-__host__ __device__ constexpr uint32_t paged_few_groups_per_cu(uint32_t padded, uint32_t elem, uint32_t sets) {
-    return padded <= 128 && elem != ITAK_ELEM_F32 && sets == 1 ? 2 : 1;
+__host__ __device__ constexpr uint32_t paged_few_groups_per_cu(uint32_t padded, uint32_t page_elem, uint32_t elem, uint32_t sets) {
+    return padded * sets <= (page_elem == ITAK_ELEM_BF16 && elem == ITAK_ELEM_F32 ? 64 : 128) ? 2 : 1;
 }
 hipError_t launch_paged_few_f16(uint32_t sets, const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_few_f16_f32(uint32_t sets, const PagedAttn &a, hipStream_t stream);
@@ -111,33 +124,40 @@ __host__ __device__ inline uint32_t paged_first_block(uint32_t position, uint32_
 
 #if defined(__HIPCC__)
 
-// Walks the items of a batch, 64 at a time, one a lane.
+__device__ __forceinline__ uint32_t paged_row_of(const PagedAttn &a, uint32_t vector) {
+    return a.group_magic ? __umulhi(vector, a.group_magic) : vector;
+}
+
+// The items a launch takes, in order: where their blocks and units lie in the line. Inline items are walked by scalar code, those in
+// memory 64 at a time, one a lane.
 struct PagedLine {
     const PagedAttn &a;
-    uint32_t n, lane;
 
-    __device__ __forceinline__ PagedLine(const PagedAttn &args) : a(args) {
-        n = min(a.batch[0], a.items);
-        lane = __lane_id();
-    }
-    // Lane's item of a chunk, and blocks and units in all of it. Items beyond the launch's rows are left out (a batch that is not
-    // what a captured launch was made for).
-    __device__ __forceinline__ PagedSpan mine(uint32_t at, uint32_t &work, uint32_t &units) const {
+    __device__ __forceinline__ explicit PagedLine(const PagedAttn &args) : a(args) {}
+    // An item's span, and blocks and units of all of it; none of an item that the launch does not take, and of one beyond the
+    // launch's rows (a batch that is not what a captured launch was made for).
+    __device__ __forceinline__ PagedSpan span_of(const PagedItemWords &w, bool there, uint32_t &work, uint32_t &units) const {
         PagedSpan s{};
         work = units = 0;
-        if (at + lane < n) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(a.batch + kPagedItem0 + 4 * (at + lane));
-            const uint32_t vectors = w.y * a.group;
-            if (w.z + w.y <= a.rows && vectors >= a.v_from && vectors <= a.v_to) {
-                s.position = w.x, s.rows = w.y, s.row0 = w.z, s.table = w.w;
-                s.first = paged_first_block(w.x, a.window);
-                s.blocks = (w.x + w.y + 31) / 32 - s.first;
-                s.tiles = (vectors + a.tile - 1) / a.tile;
-                units = s.tiles * a.g.kv_heads;
-                work = units * s.blocks;
-            }
+        const uint32_t vectors = w.rows * a.group;
+        if (there && w.row0 + w.rows <= a.rows && w.rows && vectors >= a.v_from && vectors <= a.v_to) {
+            s.position = w.position, s.rows = w.rows, s.row0 = w.row0, s.table = w.table;
+            s.first = paged_first_block(w.position, a.window);
+            s.blocks = (w.position + w.rows + 31) / 32 - s.first;
+            s.tiles = (vectors + (1u << a.tile_shift) - 1) >> a.tile_shift;
+            units = s.tiles * a.g.kv_heads;
+            work = units * s.blocks;
         }
         return s;
+    }
+    __device__ __forceinline__ PagedSpan of_lane(uint32_t at, uint32_t n, uint32_t &work, uint32_t &units) const {
+        PagedItemWords w{};
+        const bool there = at + __lane_id() < n;
+        if (there) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(a.batch + kPagedItem0 + 4 * (at + __lane_id()));
+            w.position = x.x, w.rows = x.y, w.row0 = x.z, w.table = x.w;
+        }
+        return span_of(w, there, work, units);
     }
     static __device__ __forceinline__ uint32_t scan(uint32_t x) {  // inclusive, over the wavefront
 #pragma unroll
@@ -147,24 +167,42 @@ struct PagedLine {
         }
         return x;
     }
+    // Blocks of all units.
     __device__ __forceinline__ uint32_t total() const {
+        if (a.inline_items) return a.total;
+        const uint32_t n = min(a.batch[0], a.items);
         uint32_t all = 0;
         for (uint32_t at = 0; at < n; at += 64) {
             uint32_t work, units;
-            mine(at, work, units);
-            all += n == 1 ? __builtin_amdgcn_readfirstlane(work) : __builtin_amdgcn_readlane(scan(work), 63);
+            of_lane(at, n, work, units);
+            all += __builtin_amdgcn_readlane(scan(work), 63);
         }
         return all;
     }
-    // The item that FOUND(item, work before it, work of it) holds for, one of them at most, with `start` and `unit0` filled in.
+    // The item that FOUND(span with `start` and `unit0` filled in, its blocks) holds for, one of them at most.
     template <typename F>
     __device__ __forceinline__ bool find(PagedSpan &out, F found) const {
         uint32_t before = 0, units_before = 0;
+        if (a.inline_items) {
+#pragma unroll
+            for (uint32_t i = 0; i < kPagedInline; ++i) {
+                if (i >= a.inline_items) break;
+                uint32_t work, units;
+                PagedSpan s = span_of(a.item[i], true, work, units);
+                s.start = before, s.unit0 = units_before;
+                if (work != 0 && found(s, work)) {
+                    out = s;
+                    return true;
+                }
+                before += work, units_before += units;
+            }
+            return false;
+        }
+        const uint32_t n = min(a.batch[0], a.items);
         for (uint32_t at = 0; at < n; at += 64) {
             uint32_t work, units;
-            PagedSpan s = mine(at, work, units);
-            uint32_t upto = work, units_upto = units;
-            if (n > 1) upto = scan(work), units_upto = scan(units);
+            PagedSpan s = of_lane(at, n, work, units);
+            const uint32_t upto = scan(work), units_upto = scan(units);
             s.start = before + upto - work;
             s.unit0 = units_before + units_upto - units;
             const uint64_t mask = __builtin_amdgcn_ballot_w64(work != 0 && found(s, work));
@@ -176,8 +214,8 @@ struct PagedLine {
 #undef ITAK_FIELD
                 return true;
             }
-            before += __builtin_amdgcn_readlane(upto, n == 1 ? 0 : 63);
-            units_before += __builtin_amdgcn_readlane(units_upto, n == 1 ? 0 : 63);
+            before += __builtin_amdgcn_readlane(upto, 63);
+            units_before += __builtin_amdgcn_readlane(units_upto, 63);
         }
         return false;
     }

@@ -175,6 +175,8 @@ itak_status check_attention(itak_paged *p, uint64_t layer, const itak_rows *q, c
     return ITAK_OK;
 }
 
+uint32_t shift_of(uint32_t power) { return uint32_t(__builtin_ctz(power)); }
+
 // Units and blocks of the items a launch takes.
 itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work) {
     uint64_t units = 0;
@@ -189,6 +191,7 @@ itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work) {
     }
     if (work >= (1ull << 31) || units >= (1ull << 24)) return size_overflow(p->err, "blocks of the batch's attention");
     a.units = uint32_t(units);
+    a.total = uint32_t(work);
     return ITAK_OK;
 }
 
@@ -230,6 +233,13 @@ itak_status run_attention(itak_paged *p, uint64_t layer, const itak_rows &q, con
     a.rows = p->batch.rows;
     a.items = p->batch.items;
     a.group = group;
+    a.group_magic = group > 1 ? uint32_t((1ull << 32) / group + ((1ull << 32) % group != 0)) : 0;
+    if (uint64_t(a.rows) * group >= (1ull << 26)) return size_overflow(p->err, "query vectors of the batch");
+    // (A call that is being captured is replayed over other batches.)
+    if (a.items <= kPagedInline && !capturing(p->stream)) {
+        a.inline_items = a.items;
+        std::memcpy(a.item, p->batch.head.data() + kPagedItem0, a.items * sizeof(PagedItemWords));
+    }
     a.q_on_16 = rows_on_16(q, d);
     a.out_on_16 = rows_on_16(out, d);
     const float s = std::isnan(scale) ? 1.0f / std::sqrt(float(d)) : scale;
@@ -255,8 +265,9 @@ itak_status run_attention(itak_paged *p, uint64_t layer, const itak_rows &q, con
     if (most_few) {
         const uint32_t sets = most_few <= kPagedSet ? 1 : most_few <= 2 * kPagedSet ? 2 : 4;
         a.tile = sets * kPagedSet;
+        a.tile_shift = shift_of(a.tile);
         a.v_from = 1, a.v_to = chunks ? few_most : ~0u;
-        a.groups = cus * paged_few_groups_per_cu(dp, q.elem, sets);
+        a.groups = std::min(cus * paged_few_groups_per_cu(dp, p->cfg.elem, q.elem, sets), kPagedMostParts);
         a.least = 4;
         a.parts = 0;
         uint64_t work = 0;
@@ -271,6 +282,7 @@ itak_status run_attention(itak_paged *p, uint64_t layer, const itak_rows &q, con
     }
     if (many) {
         a.tile = 32 * paged_chunk_waves(dp, q.elem);
+        a.tile_shift = shift_of(a.tile);
         a.v_from = few_most + 1, a.v_to = ~0u;
         uint64_t work = 0;
         st = count_units(p, a, work);

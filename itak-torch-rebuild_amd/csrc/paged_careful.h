@@ -25,7 +25,7 @@ __device__ __forceinline__ void paged_careful(const PagedAttn &a, const PagedSpa
     const uint32_t *ids = a.batch + span.table;
     auto row_of = [&](uint32_t key) { return base + ids[key >> a.g.page_shift] * a.g.page_stride + uint64_t(key & page_mask) * d; };
     for (uint32_t v = v0 + wave; v < v_end; v += waves) {
-        const uint32_t row = v / a.group, pos = span.position + row;
+        const uint32_t row = paged_row_of(a, v), pos = span.position + row;
         const uint32_t lo = max(lowest_visible(pos, a.window, 0), key0), hi = min(pos + 1, key1);
         const T *q = static_cast<const T *>(a.q.data) + uint64_t(span.row0 + row) * a.q.row_stride +
                      (head * a.group + v - row * a.group) * a.q.head_stride;
@@ -65,7 +65,7 @@ template <int ELEM, int DP>
 __device__ __forceinline__ void paged_write_careful(const PagedAttn &a, const PagedSpan &span, uint32_t head, uint32_t v, bool whole,
                                                     uint64_t slot, bool has_slot, const float (&acc)[DP / 64], float m, float l) {
     typedef typename Elem<ELEM>::type T;
-    const uint32_t lane = __lane_id(), row = v / a.group;
+    const uint32_t lane = __lane_id(), row = paged_row_of(a, v);
     T *dst = static_cast<T *>(a.out.data) + uint64_t(span.row0 + row) * a.out.row_stride +
              (head * a.group + v - row * a.group) * a.out.head_stride;
 #pragma unroll

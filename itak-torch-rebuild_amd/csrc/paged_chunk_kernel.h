@@ -91,7 +91,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     const uint32_t length = span.position + span.rows;
     const uint32_t vectors = span.rows * a.group, v0 = tile * kTile;
     // Keys the tile's rows see, and this workgroup's blocks of them.
-    const uint32_t first_row = v0 / a.group, last_row = min((v0 + kTile - 1) / a.group, span.rows - 1);
+    const uint32_t first_row = paged_row_of(a, v0), last_row = min(paged_row_of(a, v0 + kTile - 1), span.rows - 1);
     const uint32_t tile_lo = lowest_visible(span.position + first_row, a.window, 0), tile_hi = span.position + last_row + 1;
     const uint32_t b_first = tile_lo / 32, b_all = (tile_hi + 31) / 32 - b_first, b_part = (b_all + a.parts - 1) / a.parts;
     const uint32_t kb0 = b_first + min(b_all, part * b_part), kb_end = b_first + min(b_all, part * b_part + b_part);
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
 
     // Positions all of this wavefront's rows see.
     const uint32_t wv0 = v0 + wave * 32;
-    const uint32_t w_first = min(wv0 / a.group, span.rows - 1), w_last = min((wv0 + 31) / a.group, span.rows - 1);
+    const uint32_t w_first = min(paged_row_of(a, wv0), span.rows - 1), w_last = min(paged_row_of(a, wv0 + 31), span.rows - 1);
     const uint32_t every_lo = lowest_visible(span.position + w_last, a.window, 0), every_hi = span.position + w_first + 1;
     // Blocks all of which they all see: from inner0 on, `inner` of them.
     const uint32_t inner0 = __builtin_amdgcn_readfirstlane((every_lo + 31) / 32);
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     uint32_t my_pos, my_lo;
     {
         const uint32_t v = wv0 + j;
-        const uint32_t row = min(v / a.group, span.rows - 1);
+        const uint32_t row = min(paged_row_of(a, v), span.rows - 1);
         const uint32_t hq = head * a.group + (v < vectors ? v - row * a.group : 0);
         my_pos = span.position + row;
         my_lo = lowest_visible(my_pos, a.window, 0);
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
         bad = bad || check != check;
         if (whole) {
             const float inv = 1.0f / l;
-            const uint32_t row = v / a.group, hq = head * a.group + v - row * a.group;
+            const uint32_t row = paged_row_of(a, v), hq = head * a.group + v - row * a.group;
             T *dst = static_cast<T *>(a.out.data) + uint64_t(span.row0 + row) * a.out.row_stride + hq * a.out.head_stride;
             typedef Piece<T, 4> Four;
 #pragma unroll

@@ -46,7 +46,7 @@ struct FewBlock {
 
 // NQ, NP: pieces of the pages' type that a query and a weight enter the products as. EXACT: head_dim == DP. SETS of 16 vectors.
 template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP, int SETS>
-__global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, ELEM, SETS)) void paged_few_kernel(PagedAttn a) {
+__global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, ELEM, SETS)) void paged_few_kernel(PagedAttn a) {
     typedef FewShape<DP> S;
     typedef typename Elem<ELEM>::type T;
     // (Two blocks of 256 channels beside the accumulators are more than 512 registers, and so are those of 64 vectors and pieces.)
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, ELEM, S
         const uint32_t unit = span.unit0 + local;
         const uint32_t length = span.position + span.rows;
         const uint32_t vectors = span.rows * a.group, v0 = tile * kTile;
-        const uint32_t first_row = v0 / a.group, last_row = min((v0 + kTile - 1) / a.group, span.rows - 1);
+        const uint32_t first_row = paged_row_of(a, v0), last_row = min(paged_row_of(a, v0 + kTile - 1), span.rows - 1);
         // Positions some, and positions every row of the tile sees.
         const uint32_t some_lo = lowest_visible(span.position + first_row, a.window, 0), some_hi = span.position + last_row + 1;
         const uint32_t every_lo = lowest_visible(span.position + last_row, a.window, 0), every_hi = span.position + first_row + 1;
@@ -100,40 +100,9 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, ELEM, S
 #pragma unroll
         for (int n = 0; n < SETS; ++n) {
             const uint32_t v = v0 + n * kSet + i;
-            my_row[n] = min(v / a.group, span.rows - 1);
+            my_row[n] = min(paged_row_of(a, v), span.rows - 1);
             my_head[n] = head * a.group + (v < vectors ? v - my_row[n] * a.group : 0);
         }
-
-        // The queries as B operands.
-        u32x4 q[SETS][S::kSteps];
-#pragma unroll
-        for (int n = 0; n < SETS; ++n) {
-            const T *src = static_cast<const T *>(a.q.data) + uint64_t(span.row0 + my_row[n]) * a.q.row_stride +
-                           my_head[n] * a.q.head_stride;
-            // (Of queries in LDS every wavefront brings its share of the steps.)
-            constexpr int kMine = kQInLds ? (S::kSteps + kFewWaves - 1) / kFewWaves : S::kSteps;
-            typename QueryRaw<ELEM>::type raw[kMine];
-            auto step = [&](int m) { return kQInLds ? m * kFewWaves + wave : uint32_t(m); };
-            auto chan = [&](int m) { return EXACT || 32 * step(m) + 8 * g < d ? min(32 * step(m) + 8 * g, uint32_t(DP) - 8) : 0u; };
-            if (a.q_on_16) {
-#pragma unroll
-                for (int m = 0; m < kMine; ++m) raw[m] = load_query<ELEM, true>(src + chan(m));
-            } else {
-#pragma unroll
-                for (int m = 0; m < kMine; ++m) raw[m] = load_query<ELEM, false>(src + chan(m));
-            }
-#pragma unroll
-            for (int m = 0; m < kMine; ++m) {
-                if (kQInLds && step(m) >= uint32_t(S::kSteps)) continue;
-                split_query<PAGE, ELEM, NQ>(raw[m], v0 + n * kSet + i < vectors && (EXACT || 32 * step(m) + 8 * g < d), [&](int piece, u32x4 x) {
-                    if constexpr (kQInLds)
-                        lds_q[((n * NQ + piece) * S::kSteps + step(m)) * 64 + lane] = x;
-                    else
-                        q[n][m] = x;
-                });
-            }
-        }
-        if constexpr (kQInLds) __syncthreads();
 
         const uint32_t *ids = a.batch + span.table;
         const uint32_t last_page = (length - 1) >> a.g.page_shift;
@@ -146,7 +115,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, ELEM, S
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int s = 0; s < S::kSteps; ++s)
-                    b.k[t][s] = *reinterpret_cast<const u32x4 *>(kp + 4 * t * d + k_chan[s]);
+                    b.k[t][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kp + 4 * t * d + k_chan[s]));
             const uint16_t *vp = a.layer_base + v_page * a.g.page_stride + head_off + a.g.side_stride +
                                  ((32 * kb + 8 * g) & page_mask) * d;
 #pragma unroll
@@ -155,15 +124,56 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, ELEM, S
                 for (int r = 0; r < 8; ++r) {
                     const uint16_t *p = vp + r * d + v_chan[h];
                     if constexpr (S::kWide == 8) {
-                        const u32x4 x = *reinterpret_cast<const u32x4 *>(p);
+                        const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
 #pragma unroll
                         for (int c = 0; c < 4; ++c) b.v[h][r][c] = x[c];
                     } else {
-                        const uint2 x = *reinterpret_cast<const uint2 *>(p);
-                        b.v[h][r][0] = x.x, b.v[h][r][1] = x.y;
+                        const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(p));
+                        b.v[h][r][0] = x[0], b.v[h][r][1] = x[1];
                     }
                 }
         };
+
+        // What the first block takes is asked for in the order of the trips: page ids, the queries, keys and values.
+        const uint32_t kb_end = span.first + from + count;
+        uint32_t kb = span.first + from + wave;
+        uint32_t kp = page_of(32 * kb + 8 * k_group), vp = page_of(32 * kb + 8 * g);
+        u32x4 q[SETS][kQInLds ? 1 : S::kSteps];
+        // (Of queries in LDS every wavefront brings its share of the steps.)
+        constexpr int kMine = kQInLds ? (S::kSteps + kFewWaves - 1) / kFewWaves : S::kSteps;
+        typename QueryRaw<ELEM>::type raw[SETS][kMine];
+        auto step = [&](int m) { return kQInLds ? m * kFewWaves + wave : uint32_t(m); };
+        auto load_queries = [&](auto on_16) {
+#pragma unroll
+            for (int n = 0; n < SETS; ++n) {
+                const T *src = static_cast<const T *>(a.q.data) + uint64_t(span.row0 + my_row[n]) * a.q.row_stride +
+                               my_head[n] * a.q.head_stride;
+#pragma unroll
+                for (int m = 0; m < kMine; ++m)
+                    raw[n][m] = load_query<ELEM, on_16.value>(src + (EXACT || 32 * step(m) + 8 * g < d ? min(32 * step(m) + 8 * g, uint32_t(DP) - 8) : 0u));
+            }
+        };
+        if (a.q_on_16)
+            load_queries(std::true_type{});
+        else
+            load_queries(std::false_type{});
+        FewBlock<DP> block;
+        load(kb, kp, vp, block);  // (of a wavefront without a block whatever the last page holds)
+        kp = page_of(32 * (kb + kFewWaves) + 8 * k_group), vp = page_of(32 * (kb + kFewWaves) + 8 * g);
+        // The queries as B operands.
+#pragma unroll
+        for (int n = 0; n < SETS; ++n)
+#pragma unroll
+            for (int m = 0; m < kMine; ++m) {
+                if (kQInLds && step(m) >= uint32_t(S::kSteps)) continue;
+                split_query<PAGE, ELEM, NQ>(raw[n][m], v0 + n * kSet + i < vectors && (EXACT || 32 * step(m) + 8 * g < d), [&](int piece, u32x4 x) {
+                    if constexpr (kQInLds)
+                        lds_q[((n * NQ + piece) * S::kSteps + step(m)) * 64 + lane] = x;
+                    else
+                        q[n][m] = x;
+                });
+            }
+        if constexpr (kQInLds) __syncthreads();
 
         float ref[SETS], threshold[SETS], sum[SETS];
         floatx4 o[SETS][S::kTiles];
@@ -203,7 +213,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, ELEM, S
                     for (int c = 0; c < S::kSteps; ++c) {
 #pragma unroll
                         for (int m = 0; m < NQ; ++m)
-                            s = mfma_16x16x32<PAGE>(b.k[t][c], kQInLds ? lds_q[((n * NQ + m) * S::kSteps + c) * 64 + lane] : q[n][c], s);
+                            s = mfma_16x16x32<PAGE>(b.k[t][c], kQInLds ? lds_q[((n * NQ + m) * S::kSteps + c) * 64 + lane] : q[n][kQInLds ? 0 : c], s);
                         if constexpr (DP == 256) __builtin_amdgcn_sched_barrier(0);  // (registers)
                     }
 #pragma unroll
@@ -268,29 +278,23 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, ELEM, S
                 }
         };
 
-        {
-            const uint32_t kb_end = span.first + from + count;
-            uint32_t kb = span.first + from + wave;
-            if (kb < kb_end) {
-                FewBlock<DP> block;
-                load(kb, page_of(32 * kb + 8 * k_group), page_of(32 * kb + 8 * g), block);
-                if constexpr (kAhead) {
-                    uint32_t kp = page_of(32 * (kb + kFewWaves) + 8 * k_group), vp = page_of(32 * (kb + kFewWaves) + 8 * g);
-                    for (; kb + kFewWaves < kb_end; kb += kFewWaves) {
-                        FewBlock<DP> next;
-                        load(kb + kFewWaves, kp, vp, next);
-                        kp = page_of(32 * (kb + 2 * kFewWaves) + 8 * k_group), vp = page_of(32 * (kb + 2 * kFewWaves) + 8 * g);
-                        multiply(kb, block);
-                        block = next;
-                    }
+        if (kb < kb_end) {
+            if constexpr (kAhead) {
+                for (; kb + kFewWaves < kb_end; kb += kFewWaves) {
+                    FewBlock<DP> next;
+                    load(kb + kFewWaves, kp, vp, next);
+                    kp = page_of(32 * (kb + 2 * kFewWaves) + 8 * k_group), vp = page_of(32 * (kb + 2 * kFewWaves) + 8 * g);
                     multiply(kb, block);
-                } else {
-                    while (true) {
-                        multiply(kb, block);
-                        kb += kFewWaves;
-                        if (kb >= kb_end) break;
-                        load(kb, page_of(32 * kb + 8 * k_group), page_of(32 * kb + 8 * g), block);
-                    }
+                    block = next;
+                }
+                multiply(kb, block);
+            } else {
+                while (true) {
+                    multiply(kb, block);
+                    kb += kFewWaves;
+                    if (kb >= kb_end) break;
+                    load(kb, kp, vp, block);
+                    kp = page_of(32 * (kb + kFewWaves) + 8 * k_group), vp = page_of(32 * (kb + kFewWaves) + 8 * g);
                 }
             }
         }
@@ -344,7 +348,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, ELEM, S
                 bad = bad || check != check;
                 if (whole) {
                     const float inv = 1.0f / all;
-                    const uint32_t row = v / a.group, hq = head * a.group + v - row * a.group;
+                    const uint32_t row = paged_row_of(a, v), hq = head * a.group + v - row * a.group;
                     T *dst = static_cast<T *>(a.out.data) + uint64_t(span.row0 + row) * a.out.row_stride + hq * a.out.head_stride + c0;
                     typedef Piece<T, 4> Four;
 #pragma unroll

@@ -1,8 +1,8 @@
 // Joins the partials of units that several workgroups shared: out = sum_w 2^(m_w - m) acc_w / sum_w 2^(m_w - m) l_w.
 //
 // A workgroup serves one query head's row. Its unit's place in the line of blocks gives the workgroups that had a part of it, and so
-// their slots. Eight lanes of a quarter of the channels' float4s each take every eighth partial, all loads of a partial's
-// accumulators in flight beside the maxima, and meet in LDS. Two trips to memory and a launch are what it costs.
+// their slots. All loads go out before anything waits: maxima and sums a thread each, accumulators (a float4 a thread and
+// partial) up to eight of a thread's at once; the weights meet in LDS. One trip to memory and a launch are what it costs.
 #include "paged.h"
 
 #include "mfma_common.h"
@@ -18,16 +18,17 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttn a) {
     typedef typename Elem<ELEM>::type T;
     constexpr int kQuads = DP / 4;               // float4s of a partial
     constexpr int kLanes = kThreads / kQuads;    // partials taken at once
+    constexpr int kAtOnce = 8;
     __shared__ floatx4 lds[kLanes][kQuads];
-    __shared__ float lds_l[kLanes], lds_m[kLanes];
+    __shared__ float weights[kPagedMostParts], lds_m[kThreads / 64], lds_l[kThreads / 64];
     const uint32_t tid = threadIdx.x, row = blockIdx.x, hq = blockIdx.y;
     const PagedLine line(a);
     const uint32_t share = a.parts ? 0 : paged_share(a, line.total());
     PagedSpan span;
     if (!line.find(span, [=](const PagedSpan &s, uint32_t) { return row >= s.row0 && row - s.row0 < s.rows; })) return;
-    const uint32_t head = hq / a.group, v = (row - span.row0) * a.group + (hq - head * a.group);
+    const uint32_t head = paged_row_of(a, hq), v = (row - span.row0) * a.group + (hq - head * a.group);
     // (The kernel of many rows counts an item's tiles from the last.)
-    const uint32_t tile = v / a.tile, local = (a.parts ? span.tiles - 1 - tile : tile) * a.g.kv_heads + head;
+    const uint32_t tile = v >> a.tile_shift, local = (a.parts ? span.tiles - 1 - tile : tile) * a.g.kv_heads + head;
     const uint32_t unit = span.unit0 + local;
     // Slots first .. last of the unit's partials, from slot `base` on.
     uint32_t first = 0, last = a.parts - 1;
@@ -39,37 +40,50 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttn a) {
         first = from / share, last = (from + span.blocks - 1) / share, base = unit;
         if (first == last || last + unit >= a.groups + a.units) return;  // written whole
     }
-    const uint32_t quad = tid % kQuads, part = tid / kQuads;
-    float m = -INFINITY, l = 0.0f;
-    floatx4 acc = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t w = first + part; w <= last; w += kLanes) {
-        const uint64_t slot = (base + w) * a.tile + (v - tile * a.tile);
-        const float2 ml = a.ws_ml[slot];
-        const floatx4 x = *reinterpret_cast<const floatx4 *>(a.ws_acc + slot * DP + quad * 4);
-        if (ml.x == -INFINITY) {
-            l += ml.y;  // nothing visible (0), or scores that are no numbers
-            continue;
-        }
-        const float next = fmaxf(m, ml.x), old = m == -INFINITY ? 0.0f : fast_exp2(m - next), now = fast_exp2(ml.x - next);
-        l = l * (m == -INFINITY ? 1.0f : old) + now * ml.y;
-        acc = acc * old + x * now;
-        m = next;
+    const uint32_t quad = tid % kQuads, part = tid / kQuads, parts = last - first + 1;
+    base = (base + first) * a.tile + (v - (tile << a.tile_shift));
+    const float *const acc_at = a.ws_acc + base * DP + quad * 4;
+    auto acc_of = [&](uint32_t w) { return *reinterpret_cast<const floatx4 *>(acc_at + uint64_t(w) * a.tile * DP); };
+    floatx4 early[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) early[u] = acc_of(min(part + u * kLanes, parts - 1));
+    float2 ml[kPagedMostParts / kThreads];
+    float m = -INFINITY;
+#pragma unroll
+    for (uint32_t u = 0; u < kPagedMostParts / kThreads; ++u) {
+        ml[u] = make_float2(-INFINITY, 0.0f);
+        if (tid + u * kThreads < parts) ml[u] = a.ws_ml[base + uint64_t(tid + u * kThreads) * a.tile];
+        m = fmaxf(m, ml[u].x);
     }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if ((tid & 63) == 0) lds_m[tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(lds_m[0], lds_m[1]), fmaxf(lds_m[2], lds_m[3]));
+    float l = 0.0f;
+#pragma unroll
+    for (uint32_t u = 0; u < kPagedMostParts / kThreads; ++u) {
+        // (A maximum of minus infinity: nothing visible, a sum of 0, or scores that are no numbers, which the sum then is.)
+        const float weight = ml[u].x == -INFINITY ? 0.0f : fast_exp2(ml[u].x - m);
+        l += ml[u].x == -INFINITY ? ml[u].y : weight * ml[u].y;
+        if (tid + u * kThreads < parts) weights[tid + u * kThreads] = weight;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+    if ((tid & 63) == 0) lds_l[tid >> 6] = l;
+    __syncthreads();
+    const float total = (lds_l[0] + lds_l[1]) + (lds_l[2] + lds_l[3]);
+    floatx4 acc = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u)
+        if (part + u * kLanes < parts) acc += early[u] * weights[part + u * kLanes];
+    for (uint32_t w = part + kAtOnce * kLanes; w < parts; w += kLanes) acc += acc_of(w) * weights[w];
     lds[part][quad] = acc;
-    if (quad == 0) lds_l[part] = l, lds_m[part] = m;
     __syncthreads();
     if (tid >= kQuads) return;
-    float most = -INFINITY;
-#pragma unroll
-    for (int p = 0; p < kLanes; ++p) most = fmaxf(most, lds_m[p]);
-    float total = 0.0f;
     floatx4 sum = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int p = 0; p < kLanes; ++p) {
-        const float weight = lds_m[p] == -INFINITY ? 0.0f : fast_exp2(lds_m[p] - most);
-        total += lds_m[p] == -INFINITY ? lds_l[p] : weight * lds_l[p];
-        sum += lds[p][tid] * weight;
-    }
+    for (int p = 0; p < kLanes; ++p) sum += lds[p][tid];
     const float inv = 1.0f / total;
     const uint32_t c = tid * 4;
     if (c >= a.g.head_dim) return;

@@ -7,6 +7,7 @@
 namespace itak {
 
 typedef __bf16 bfloat8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 // S += A . B, A 16 x 32 and B 32 x 16: lane (i, g) holds row i of A (column i of B), elements 8g .. 8g + 7, and of S column i,
 // rows 4g .. 4g + 3.
