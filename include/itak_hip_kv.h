@@ -715,7 +715,7 @@ typedef struct itak_rotation_config {
    row * row_stride + head * head_stride + channel, in elements; 0 for both strides: dense. Rows and heads may lie in any order and
    with any gaps (slices of one projection's output, heads first); views that start on 16 bytes with strides that
    are multiples of 16 bytes are read and written 16 bytes at a time, others element by element. A view that is
-   written must not hold the same element twice, and may share memory with one that is read only by being the same view. */
+   written must not hold the same element twice, and shares no memory with one that is read (but for rotations in place). */
 typedef struct itak_rows {
     void *data;
     uint32_t elem;  /* ITAK_ELEM_* */
@@ -753,7 +753,7 @@ itak_status itak_rotate_device(const itak_rotation *rotation, void *hip_stream, 
    Tensors of a call are ITAK_ELEM_F32 or of the pages' own type. Scores, softmax and sums are f32. With tensors of
    the pages' type the softmax weights are rounded to that type once (f16 2^-11, bf16 2^-8 relative to each) and
    the output once; with f32 tensors queries and weights enter the matrix pipe as several halves each,
-   which leaves 2^-22 of them (bf16: 2^-24 of queries, 2^-16 of weights). An f16 query's or key's channel beyond 65504 is infinite.
+   which leaves 2^-22 of them (bf16: 2^-24). An f16 query's or key's channel beyond 65504 is infinite.
    A row that is not finite reaches the outputs of exactly the queries that see its position; one difference is left on f16 pages: a weight
    below about 2^-32 of its row's largest is zero, and zero times an infinite value is NaN.
    Results do not depend on the pages' order or on what other sequences the batch holds beyond rounding (sums are cut

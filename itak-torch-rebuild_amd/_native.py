@@ -250,6 +250,7 @@ class NoFront:
     """In place of the front module: every call is left to ctypes."""
 
     step = prep_step = truncate = compute = gqa = staticmethod(lambda *_: -1)
+    rotate = set_batch = append = paged_attention = paged_step = staticmethod(lambda *_: -1)
 
 
 def load_front(lib, cache_type):
@@ -266,6 +267,10 @@ def load_front(lib, cache_type):
     front.bind(cache_type, *(C.cast(getattr(lib, name), C.c_void_p).value for name in (
         "itak_attention_step_device", "itak_attention_prep_step_device", "itak_kv_truncate",
         "itak_compute_attention", "itak_gqa_attention")))
+    from .paged import Rows as rows_type
+    front.bind_paged(rows_type, *(C.cast(getattr(lib, name), C.c_void_p).value for name in (
+        "itak_rotate_device", "itak_paged_set_batch", "itak_paged_append_device", "itak_paged_attention_device",
+        "itak_paged_step_device")))
     return front
 
 

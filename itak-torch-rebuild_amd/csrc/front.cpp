@@ -7,8 +7,8 @@
 // layers of one row at 4,096 7.65 -> 6.3 us, of preparing steps 8.65 -> 6.9, f32 8.2 -> 6.6.
 //
 // Only plain arguments are taken here: exact ints, floats and bools, items in lists or tuples, C-contiguous float32
-// arrays. Whatever else a caller passes (numpy scalars, pointer objects, other sequences) is answered with kNotPlain before
-// anything is called, and hip_compute.py then makes the same call through ctypes with that module's conversions.
+// arrays, views and page tables as paged.py makes them. Whatever else a caller passes (numpy scalars, pointer objects, other sequences) is answered with kNotPlain before
+// anything is called, and hip_compute.py or paged.py then makes the same call through ctypes with that module's conversions.
 //
 // The library's functions are bound by address (bind), so that this module serves whichever build is loaded.
 #define PY_SSIZE_T_CLEAN
@@ -19,6 +19,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <cstring>
 
 #include "../../include/itak_hip_kv.h"
 
@@ -32,8 +33,14 @@ decltype(&itak_attention_prep_step_device) prep_step_fn;
 decltype(&itak_kv_truncate) truncate_fn;
 decltype(&itak_compute_attention) compute_fn;
 decltype(&itak_gqa_attention) gqa_fn;
+decltype(&itak_rotate_device) rotate_fn;
+decltype(&itak_paged_set_batch) set_batch_fn;
+decltype(&itak_paged_append_device) append_fn;
+decltype(&itak_paged_attention_device) paged_attention_fn;
+decltype(&itak_paged_step_device) paged_step_fn;
 PyTypeObject *cache_type;  // hip_compute.KvCache
-PyObject *slot_name;
+PyTypeObject *rows_type;   // paged.Rows
+PyObject *slot_name, *address_name;
 
 // An exact int as ctypes takes it for an unsigned 64-bit argument or a pointer: modulo 2^64.
 bool plain_u64(PyObject *o, uint64_t &v) {
@@ -122,6 +129,28 @@ bool plain_array(PyObject *o, const float *&data, uint64_t &size) {
     if (PyArray_TYPE(a) != NPY_FLOAT32 || !PyArray_ISCARRAY_RO(a)) return false;
     size = uint64_t(PyArray_SIZE(a));
     data = size ? static_cast<const float *>(PyArray_DATA(a)) : nullptr;
+    return true;
+}
+// A paged.Rows: where its itak_rows lies.
+bool plain_rows(PyObject *o, const itak_rows *&rows) {
+    if (Py_TYPE(o) != rows_type) return false;
+    PyObject *at = PyObject_GetAttr(o, address_name);
+    if (!at) {
+        PyErr_Clear();
+        return false;
+    }
+    const bool ok = plain_ptr(at, rows) && rows;
+    Py_DECREF(at);
+    return ok;
+}
+// A C-contiguous run of 32-bit words.
+bool plain_words(PyObject *o, const void *&data, Py_ssize_t &n) {
+    if (!PyArray_CheckExact(o)) return false;
+    PyArrayObject *a = reinterpret_cast<PyArrayObject *>(o);
+    const int type = PyArray_TYPE(a);
+    if ((type != NPY_UINT32 && type != NPY_INT32) || PyArray_NDIM(a) != 1 || !PyArray_ISCARRAY_RO(a)) return false;
+    n = PyArray_SIZE(a);
+    data = PyArray_DATA(a);
     return true;
 }
 PyObject *not_plain() { return PyLong_FromLong(kNotPlain); }
@@ -249,19 +278,163 @@ PyObject *gqa(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return PyLong_FromLong(st);
 }
 
-// bind(KvCache, address of each of the five functions above, in their order)
+bool bound_type(PyObject *o) {
+    if (!PyType_Check(o)) PyErr_SetString(PyExc_TypeError, "a type comes first");
+    return PyType_Check(o);
+}
+bool bound_addresses(PyObject *const *a, uint64_t (&at)[5]) {
+    for (int i = 0; i < 5; ++i)
+        if (!plain_within(a[i], 64, at[i]) || at[i] == 0) {
+            PyErr_SetString(PyExc_TypeError, "an address is an int that is not zero");
+            return false;
+        }
+    return true;
+}
+
+// rotate(rotation, stream, head_dim, rows, positions, inputs, outputs, inverse) -> status
+PyObject *rotate(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (!arity(n, 8)) return nullptr;
+    constexpr Py_ssize_t kMostTensors = 4;
+    itak_rotation *rotation;
+    void *stream;
+    uint64_t head_dim, rows;
+    const int64_t *positions;
+    PyObject **in_at, **out_at;
+    Py_ssize_t ins, outs;
+    itak_rows in[kMostTensors], out[kMostTensors];
+    if (!plain_ptr(a[0], rotation) || !plain_ptr(a[1], stream) || !plain_u64(a[2], head_dim) || !plain_u64(a[3], rows) ||
+        !plain_ptr(a[4], positions) || !plain_sequence(a[5], in_at, ins) || !plain_sequence(a[6], out_at, outs) || ins != outs ||
+        ins > kMostTensors || !PyBool_Check(a[7]))
+        return not_plain();
+    for (Py_ssize_t i = 0; i < ins; ++i) {
+        const itak_rows *x, *y;
+        if (!plain_rows(in_at[i], x) || !plain_rows(out_at[i], y)) return not_plain();
+        in[i] = *x, out[i] = *y;
+    }
+    itak_status st;
+    Py_BEGIN_ALLOW_THREADS
+    st = rotate_fn(rotation, stream, head_dim, rows, positions, in, out, uint32_t(ins), a[7] == Py_True ? 1 : 0);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(st);
+}
+
+// set_batch(paged, items, tables) -> status
+PyObject *set_batch(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (!arity(n, 3)) return nullptr;
+    itak_paged *paged;
+    PyObject **item_at, **table_at;
+    Py_ssize_t items, tables;
+    itak_paged_item item[kMostItems];
+    const void *run[kMostItems];
+    if (!plain_ptr(a[0], paged) || !plain_sequence(a[1], item_at, items) || !plain_sequence(a[2], table_at, tables) ||
+        items != tables || items > kMostItems)
+        return not_plain();
+    uint64_t all = 0;
+    for (Py_ssize_t i = 0; i < items; ++i) {
+        uint64_t rows;
+        Py_ssize_t pages;
+        if (!PyTuple_CheckExact(item_at[i]) || PyTuple_GET_SIZE(item_at[i]) != 2 ||
+            !plain_within(PyTuple_GET_ITEM(item_at[i], 0), 64, item[i].position) ||
+            !plain_within(PyTuple_GET_ITEM(item_at[i], 1), 32, rows) || !plain_words(table_at[i], run[i], pages) ||
+            pages > Py_ssize_t(0xffffffffu))
+            return not_plain();
+        item[i].rows = uint32_t(rows), item[i].pages = uint32_t(pages);
+        all += uint64_t(pages);
+    }
+    // (A batch of one sequence is read where it lies.)
+    uint32_t *joined = nullptr;
+    const uint32_t *ids = items && all ? static_cast<const uint32_t *>(run[0]) : nullptr;
+    if (items > 1 && all) {
+        joined = static_cast<uint32_t *>(PyMem_Malloc(all * sizeof(uint32_t)));
+        if (!joined) return PyErr_NoMemory();
+        uint64_t at = 0;
+        for (Py_ssize_t i = 0; i < items; at += item[i].pages, ++i)
+            if (item[i].pages) std::memcpy(joined + at, run[i], item[i].pages * sizeof(uint32_t));
+        ids = joined;
+    }
+    itak_status st;
+    Py_BEGIN_ALLOW_THREADS
+    st = set_batch_fn(paged, item, uint32_t(items), ids, all);
+    Py_END_ALLOW_THREADS
+    PyMem_Free(joined);
+    return PyLong_FromLong(st);
+}
+
+// append(paged, layer, k, v, rotation) -> status
+PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (!arity(n, 5)) return nullptr;
+    itak_paged *paged;
+    uint64_t layer;
+    const itak_rows *k, *v;
+    itak_rotation *rotation;
+    if (!plain_ptr(a[0], paged) || !plain_u64(a[1], layer) || !plain_rows(a[2], k) || !plain_rows(a[3], v) ||
+        !plain_ptr(a[4], rotation))
+        return not_plain();
+    itak_status st;
+    Py_BEGIN_ALLOW_THREADS
+    st = append_fn(paged, layer, k, v, rotation);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(st);
+}
+
+// paged_attention(paged, layer, q, out, scale, softcap, window, rotation) -> status
+PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (!arity(n, 8)) return nullptr;
+    itak_paged *paged;
+    uint64_t layer, window;
+    const itak_rows *q, *out;
+    float scale, softcap;
+    itak_rotation *rotation;
+    if (!plain_ptr(a[0], paged) || !plain_u64(a[1], layer) || !plain_rows(a[2], q) || !plain_rows(a[3], out) ||
+        !plain_scale(a[4], scale) || !plain_float(a[5], softcap) || !plain_u64(a[6], window) || !plain_ptr(a[7], rotation))
+        return not_plain();
+    itak_status st;
+    Py_BEGIN_ALLOW_THREADS
+    st = paged_attention_fn(paged, layer, q, out, scale, softcap, window, rotation);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(st);
+}
+
+// paged_step(paged, layer, q, k, v, out, scale, softcap, window, rotation) -> status
+PyObject *paged_step(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (!arity(n, 10)) return nullptr;
+    itak_paged *paged;
+    uint64_t layer, window;
+    const itak_rows *q, *k, *v, *out;
+    float scale, softcap;
+    itak_rotation *rotation;
+    if (!plain_ptr(a[0], paged) || !plain_u64(a[1], layer) || !plain_rows(a[2], q) || !plain_rows(a[3], k) ||
+        !plain_rows(a[4], v) || !plain_rows(a[5], out) || !plain_scale(a[6], scale) || !plain_float(a[7], softcap) ||
+        !plain_u64(a[8], window) || !plain_ptr(a[9], rotation))
+        return not_plain();
+    itak_status st;
+    Py_BEGIN_ALLOW_THREADS
+    st = paged_step_fn(paged, layer, q, k, v, out, scale, softcap, window, rotation);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(st);
+}
+
+// bind_paged(Rows, address of each of the five functions above, in their order)
+PyObject *bind_paged(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (!arity(n, 6)) return nullptr;
+    uint64_t at[5];
+    if (!bound_type(a[0]) || !bound_addresses(a + 1, at)) return nullptr;
+    Py_INCREF(a[0]);
+    Py_XDECREF(reinterpret_cast<PyObject *>(rows_type));
+    rows_type = reinterpret_cast<PyTypeObject *>(a[0]);
+    rotate_fn = reinterpret_cast<decltype(rotate_fn)>(uintptr_t(at[0]));
+    set_batch_fn = reinterpret_cast<decltype(set_batch_fn)>(uintptr_t(at[1]));
+    append_fn = reinterpret_cast<decltype(append_fn)>(uintptr_t(at[2]));
+    paged_attention_fn = reinterpret_cast<decltype(paged_attention_fn)>(uintptr_t(at[3]));
+    paged_step_fn = reinterpret_cast<decltype(paged_step_fn)>(uintptr_t(at[4]));
+    Py_RETURN_NONE;
+}
+
+// bind(KvCache, address of step's, prep_step's, truncate's, compute's and gqa's function)
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (!arity(n, 6)) return nullptr;
     uint64_t at[5];
-    if (!PyType_Check(a[0])) {
-        PyErr_SetString(PyExc_TypeError, "the cache's type comes first");
-        return nullptr;
-    }
-    for (int i = 0; i < 5; ++i)
-        if (!plain_within(a[i + 1], 64, at[i]) || at[i] == 0) {
-            PyErr_SetString(PyExc_TypeError, "an address is an int that is not zero");
-            return nullptr;
-        }
+    if (!bound_type(a[0]) || !bound_addresses(a + 1, at)) return nullptr;
     Py_INCREF(a[0]);
     Py_XDECREF(reinterpret_cast<PyObject *>(cache_type));
     cache_type = reinterpret_cast<PyTypeObject *>(a[0]);
@@ -279,6 +452,9 @@ PyMethodDef method(const char *name) {
 }
 PyMethodDef methods[] = {method<bind>("bind"), method<step>("step"),       method<prep_step>("prep_step"),
                          method<truncate>("truncate"), method<compute>("compute"), method<gqa>("gqa"),
+                         method<bind_paged>("bind_paged"), method<rotate>("rotate"), method<set_batch>("set_batch"),
+                         method<append>("append"), method<paged_attention>("paged_attention"),
+                         method<paged_step>("paged_step"),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_itak_front", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
@@ -287,5 +463,6 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_itak_front", nullptr, -1, methods
 PyMODINIT_FUNC PyInit__itak_front(void) {
     import_array();
     slot_name = PyUnicode_InternFromString("slot");
-    return slot_name ? PyModule_Create(&module) : nullptr;
+    address_name = PyUnicode_InternFromString("at");
+    return slot_name && address_name ? PyModule_Create(&module) : nullptr;
 }

@@ -168,6 +168,7 @@ itak_status check_attention(itak_paged *p, uint64_t layer, const itak_rows *q, c
     if (st == ITAK_OK) st = check_tensor(p, "q", q, 0, ~0u, false);
     if (st == ITAK_OK) st = check_tensor(p, "out", out, q->heads, q->elem, true);
     if (st != ITAK_OK) return st;
+    if (p->batch.rows && q->data == out->data) return invalid_argument(p->err, "out shares its memory with q");
     if (q->heads % p->cfg.num_kv_heads) return non_divisible(p->err, q->heads, p->cfg.num_kv_heads);
     if (q->heads / p->cfg.num_kv_heads > 64) return unsupported(p->err, "more than 64 query heads a KV head");
     if (std::isinf(scale)) return invalid_argument(p->err, "scale is infinite");

@@ -14,6 +14,7 @@ from typing import Optional, Sequence, Tuple
 import numpy as np
 
 from . import _native as N
+from . import hip_compute
 from .hip_compute import _check, _ptr, _raise_last
 
 _ELEMS = {"f32": N.ELEM_F32, "f16": N.ELEM_F16, "bf16": N.ELEM_BF16}
@@ -25,11 +26,12 @@ _NAN = math.nan
 class Rows:
     """A view of rows x heads x channels on the device (itak_rows): pointer, type, heads, strides in elements."""
 
-    __slots__ = ("raw", "ref", "keep")
+    __slots__ = ("raw", "ref", "at", "keep")
 
     def __init__(self, ptr: int, elem: str, heads: int, row_stride: int = 0, head_stride: int = 0, keep=None):
         self.raw = N.Rows(ptr, _ELEMS[elem] if isinstance(elem, str) else elem, heads, row_stride, head_stride)
         self.ref = C.byref(self.raw)
+        self.at = C.addressof(self.raw)  # the view as the front module takes it
         self.keep = keep  # what owns the memory
 
     @staticmethod
@@ -49,6 +51,14 @@ class Rows:
                     head_stride if heads > 1 else channels, keep=tensor)
 
 
+def _turning(rotation: Optional["Rotation"]) -> Optional[C.c_void_p]:
+    if rotation is None:
+        return None
+    if not rotation._h:
+        raise ValueError("the rotation is closed")
+    return rotation._h
+
+
 class Rotation:
     """Rotary positions (itak_rotation): `rotary_dim` channels of a head turn by position * frequency, pair by pair; adjacent
     pairs with `interleaved`, else half split. scaling "linear" divides the frequencies by `factor`, "yarn" only those of
@@ -58,7 +68,8 @@ class Rotation:
                  factor: float = 1.0, original_positions: float = 0.0, beta_fast: float = 32.0, beta_slow: float = 1.0,
                  amplitude: Optional[float] = None, device: int = 0):
         self._h = None
-        self._lib = N.load()
+        self._hv = None  # the handle as the front module takes it
+        self._lib = hip_compute._load()
         if scaling not in _SCALINGS:
             raise ValueError(f"scaling {scaling!r} is none of {', '.join(_SCALINGS)}")
         cfg = N.RotationConfig(base, rotary_dim, 1 if interleaved else 0, _SCALINGS[scaling], device, factor, original_positions,
@@ -66,13 +77,13 @@ class Rotation:
         handle = C.c_void_p()
         if self._lib.itak_rotation_create(C.byref(cfg), C.byref(handle)) != N.OK:
             _raise_last(None)
-        self._h = handle
+        self._h, self._hv = handle, handle.value
         self.rotary_dim = rotary_dim
 
     def close(self) -> None:
         if self._h:
             self._lib.itak_rotation_destroy(self._h)
-            self._h = None
+            self._h = self._hv = None
 
     def __del__(self):
         try:
@@ -90,12 +101,15 @@ class Rotation:
                       stream: int = 0, inverse: bool = False) -> None:
         """outputs[i] = inputs[i] turned by the rows' positions (int64 on the device), up to four tensors in one launch on
         `stream`; `inverse` turns back, which is what gradients of rotated rows go through."""
-        n = len(inputs)
-        if len(outputs) != n:
-            raise ValueError("rotate_device: as many outputs as inputs")
-        table = N.Rows * n
-        if self._lib.itak_rotate_device(self._h, stream, head_dim, rows, positions_ptr, table(*[r.raw for r in inputs]),
-                                        table(*[r.raw for r in outputs]), n, 1 if inverse else 0) != N.OK:
+        status = hip_compute._front.rotate(self._hv, stream, head_dim, rows, positions_ptr, inputs, outputs, inverse)
+        if status < 0:  # arguments that the front module leaves to ctypes
+            n = len(inputs)
+            if len(outputs) != n:
+                raise ValueError("rotate_device: as many outputs as inputs")
+            table = N.Rows * n
+            status = self._lib.itak_rotate_device(_turning(self), stream, head_dim, rows, positions_ptr, table(*[r.raw for r in inputs]),
+                                                  table(*[r.raw for r in outputs]), n, 1 if inverse else 0)
+        if status:
             _raise_last(None)
 
 
@@ -107,13 +121,14 @@ class PagedKv:
                  page_count: int, max_sequences: int = 64, max_table_pages: int = 0, device: int = 0, storage_ptr: int = 0,
                  storage_bytes: int = 0):
         self._h = None
-        self._lib = N.load()
+        self._hv = 0  # the handle as the front module takes it
+        self._lib = hip_compute._load()
         cfg = self._config(layers, num_kv_heads, head_dim, elem, page_rows, page_count, max_sequences, max_table_pages, device,
                            storage_ptr, storage_bytes)
         handle = C.c_void_p()
         if self._lib.itak_paged_create(C.byref(cfg), C.byref(handle)) != N.OK:
             _raise_last(None)
-        self._h = handle
+        self._h, self._hv = handle, handle.value
         self.page_rows = page_rows
 
     @staticmethod
@@ -136,7 +151,7 @@ class PagedKv:
     def close(self) -> None:
         if self._h:
             self._lib.itak_paged_destroy(self._h)
-            self._h = None
+            self._h, self._hv = None, 0
 
     def __del__(self):
         try:
@@ -155,14 +170,23 @@ class PagedKv:
 
     def set_batch(self, items: Sequence[Tuple[int, int]], pages: Sequence[Sequence[int]]) -> None:
         """The sequences of the next forward: (positions held, new rows) of each, and its page ids in order."""
+        status = hip_compute._front.set_batch(self._hv, items, pages)
+        if status >= 0:
+            self._done(status)
+            return
         n = len(items)
         if len(pages) != n:
             raise ValueError("set_batch: one table of pages a sequence")
         raw = (N.PagedItem * n)()
         for at, (position, rows), table in zip(raw, items, pages):
+            if not (0 <= position < 1 << 64 and 0 <= rows < 1 << 32):  # (a field would take them modulo its size)
+                raise ValueError(f"set_batch: ({position}, {rows}) is no position and rows")
             at.position, at.rows, at.pages = position, rows, len(table)
         if n and isinstance(pages[0], np.ndarray):
-            ids = np.ascontiguousarray(np.concatenate(pages) if n > 1 else pages[0], dtype=np.uint32)
+            ids = np.concatenate(pages)
+            if ids.size and (ids.dtype.kind not in "iu" or ids.min() < 0 or ids.max() > 0xFFFFFFFF):
+                raise ValueError("set_batch: page ids are integers of 32 bits")
+            ids = np.ascontiguousarray(ids, dtype=np.uint32)
             ptr, count = _ptr(ids), ids.size
         else:
             ids = array("I")
@@ -173,22 +197,30 @@ class PagedKv:
 
     def append_device(self, layer: int, k: Rows, v: Rows, rotation: Optional[Rotation] = None) -> None:
         """The batch's new rows into their pages, keys turned by their positions if `rotation` is given."""
-        status = self._lib.itak_paged_append_device(self._h, layer, k.ref, v.ref, rotation._h if rotation else None)
+        status = hip_compute._front.append(self._hv, layer, k, v, 0 if rotation is None else rotation._hv)
+        if status < 0:
+            status = self._lib.itak_paged_append_device(self._h, layer, k.ref, v.ref, _turning(rotation))
         if status:
             self._done(status)
 
     def attention_device(self, layer: int, q: Rows, out: Rows, *, scale: Optional[float] = None, softcap: float = 0.0,
                          window: int = 0, rotation: Optional[Rotation] = None) -> None:
         """Attention of the batch's new positions over pages that hold their rows already."""
-        status = self._lib.itak_paged_attention_device(self._h, layer, q.ref, out.ref, _NAN if scale is None else scale, softcap,
-                                                       window, rotation._h if rotation else None)
+        status = hip_compute._front.paged_attention(self._hv, layer, q, out, scale, softcap, window,
+                                                    0 if rotation is None else rotation._hv)
+        if status < 0:
+            status = self._lib.itak_paged_attention_device(self._h, layer, q.ref, out.ref, _NAN if scale is None else scale, softcap,
+                                                           window, _turning(rotation))
         if status:
             self._done(status)
 
     def attention_step_device(self, layer: int, q: Rows, k: Rows, v: Rows, out: Rows, *, scale: Optional[float] = None,
                               softcap: float = 0.0, window: int = 0, rotation: Optional[Rotation] = None) -> None:
         """Append the batch's new rows, then attend; queries and keys turned first if `rotation` is given."""
-        status = self._lib.itak_paged_step_device(self._h, layer, q.ref, k.ref, v.ref, out.ref, _NAN if scale is None else scale,
-                                                  softcap, window, rotation._h if rotation else None)
+        status = hip_compute._front.paged_step(self._hv, layer, q, k, v, out, scale, softcap, window,
+                                               0 if rotation is None else rotation._hv)
+        if status < 0:
+            status = self._lib.itak_paged_step_device(self._h, layer, q.ref, k.ref, v.ref, out.ref, _NAN if scale is None else scale,
+                                                      softcap, window, _turning(rotation))
         if status:
             self._done(status)
