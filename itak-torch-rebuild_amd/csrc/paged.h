@@ -73,7 +73,8 @@ struct PagedAttn {
     const void *zeros;   // 16 bytes of them
     uint32_t inline_items; // 0: the batch's are read from device memory
     uint32_t total;      // with inline items: blocks of all units
-    PagedItemWords item[kPagedInline];
+    PagedItemWords item[kPagedInline];  // those behind the last: row0, start and unit0 are ~0
+    uint32_t start[kPagedInline], unit0[kPagedInline];  // where an item's blocks and units begin in the line
     float *ws_acc;       // [slots][tile][padded head_dim]
     float2 *ws_ml;       // [slots][tile]: maximum (log2 domain), sum
 };
@@ -128,8 +129,17 @@ __device__ __forceinline__ uint32_t paged_row_of(const PagedAttn &a, uint32_t ve
     return a.group_magic ? __umulhi(vector, a.group_magic) : vector;
 }
 
-// The items a launch takes, in order: where their blocks and units lie in the line. Inline items are walked by scalar code, those in
-// memory 64 at a time, one a lane.
+// Asks for all of the arguments at once: the compiler asks where it needs them, a trip to memory for every 64 bytes that come
+// first there (of the few rows' kernel four in a row, some 3,000 clocks before the first page id).
+__device__ __forceinline__ void paged_fetch_arguments(const PagedAttn &a) {
+    static_assert(sizeof(PagedAttn) <= 9 * 64 && kPagedInline == 8, "a word of every 64 bytes is named");
+    asm volatile("" ::"s"(a.batch), "s"(a.layer_base), "s"(a.q.data), "s"(a.out.data), "s"(a.rows), "s"(a.units), "s"(a.v_to), "s"(a.window),
+                 "s"(a.zeros), "s"(a.total), "s"(a.item[1].row0), "s"(a.item[5].row0), "s"(a.start[1]), "s"(a.unit0[1]), "s"(a.ws_acc),
+                 "s"(a.ws_ml));
+}
+
+// The items a launch takes, in order: where their blocks and units lie in the line. Those in memory are looked at 64 at a time, one
+// a lane.
 struct PagedLine {
     const PagedAttn &a;
 
@@ -179,24 +189,25 @@ struct PagedLine {
         }
         return all;
     }
-    // The item that FOUND(span with `start` and `unit0` filled in, its blocks) holds for, one of them at most.
-    template <typename F>
-    __device__ __forceinline__ bool find(PagedSpan &out, F found) const {
+    // The item that block, unit or row x of the line belongs to; none if it is no item's, or of one that the launch does not take.
+    enum By { kBlock, kUnit, kRow };
+    template <By BY>
+    __device__ __forceinline__ bool find(PagedSpan &out, uint32_t x) const {
+        auto holds = [&](const PagedSpan &s, uint32_t work, uint32_t units) {
+            if (BY == kBlock) return x >= s.start && x - s.start < work;
+            if (BY == kUnit) return x >= s.unit0 && x - s.unit0 < units;
+            return work != 0 && x >= s.row0 && x - s.row0 < s.rows;
+        };
         uint32_t before = 0, units_before = 0;
         if (a.inline_items) {
+            uint32_t at = 0;  // (of several that begin there all but the last are empty)
 #pragma unroll
-            for (uint32_t i = 0; i < kPagedInline; ++i) {
-                if (i >= a.inline_items) break;
-                uint32_t work, units;
-                PagedSpan s = span_of(a.item[i], true, work, units);
-                s.start = before, s.unit0 = units_before;
-                if (work != 0 && found(s, work)) {
-                    out = s;
-                    return true;
-                }
-                before += work, units_before += units;
-            }
-            return false;
+            for (uint32_t i = 1; i < kPagedInline; ++i)
+                at = x >= (BY == kBlock ? a.start[i] : BY == kUnit ? a.unit0[i] : a.item[i].row0) ? i : at;
+            uint32_t work, units;
+            out = span_of(a.item[at], true, work, units);
+            out.start = a.start[at], out.unit0 = a.unit0[at];
+            return holds(out, work, units);
         }
         const uint32_t n = min(a.batch[0], a.items);
         for (uint32_t at = 0; at < n; at += 64) {
@@ -205,7 +216,7 @@ struct PagedLine {
             const uint32_t upto = scan(work), units_upto = scan(units);
             s.start = before + upto - work;
             s.unit0 = units_before + units_upto - units;
-            const uint64_t mask = __builtin_amdgcn_ballot_w64(work != 0 && found(s, work));
+            const uint64_t mask = __builtin_amdgcn_ballot_w64(holds(s, work, units));
             if (mask) {
                 const uint32_t l = __builtin_ctzll(mask);
 #define ITAK_FIELD(f) out.f = __builtin_amdgcn_readlane(s.f, l)

@@ -171,6 +171,7 @@ itak_status check_attention(itak_paged *p, uint64_t layer, const itak_rows *q, c
     if (p->batch.rows && q->data == out->data) return invalid_argument(p->err, "out shares its memory with q");
     if (q->heads % p->cfg.num_kv_heads) return non_divisible(p->err, q->heads, p->cfg.num_kv_heads);
     if (q->heads / p->cfg.num_kv_heads > 64) return unsupported(p->err, "more than 64 query heads a KV head");
+    if (q->heads > 65535) return unsupported(p->err, "more than 65535 query heads");
     if (std::isinf(scale)) return invalid_argument(p->err, "scale is infinite");
     if (!(softcap >= 0.0f) || std::isinf(softcap)) return invalid_argument(p->err, "softcap must be finite and >= 0");
     return ITAK_OK;
@@ -182,9 +183,11 @@ uint32_t shift_of(uint32_t power) { return uint32_t(__builtin_ctz(power)); }
 itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work) {
     uint64_t units = 0;
     work = 0;
+    for (uint32_t i = 0; i < kPagedInline; ++i) a.start[i] = a.unit0[i] = ~0u;
     for (uint32_t i = 0; i < a.items; ++i) {
         const uint32_t *it = p->batch.head.data() + kPagedItem0 + 4 * i;
         const uint64_t vectors = uint64_t(it[1]) * a.group;
+        if (i < a.inline_items) a.start[i] = uint32_t(work), a.unit0[i] = uint32_t(units);
         if (vectors < a.v_from || vectors > a.v_to) continue;
         const uint64_t tiles = (vectors + a.tile - 1) / a.tile * a.g.kv_heads;
         units += tiles;
@@ -239,6 +242,7 @@ itak_status run_attention(itak_paged *p, uint64_t layer, const itak_rows &q, con
     // (A call that is being captured is replayed over other batches.)
     if (a.items <= kPagedInline && !capturing(p->stream)) {
         a.inline_items = a.items;
+        for (PagedItemWords &w : a.item) w.row0 = ~0u;
         std::memcpy(a.item, p->batch.head.data() + kPagedItem0, a.items * sizeof(PagedItemWords));
     }
     a.q_on_16 = rows_on_16(q, d);

@@ -85,7 +85,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     const uint32_t part = blockIdx.x / units, unit = blockIdx.x - part * units;
     const PagedLine line(a);
     PagedSpan span;
-    if (!line.find(span, [=](const PagedSpan &s, uint32_t) { return unit >= s.unit0 && unit - s.unit0 < s.tiles * a.g.kv_heads; })) return;
+    if (!line.find<PagedLine::kUnit>(span, unit)) return;
     const uint32_t local = unit - span.unit0, turn = local / a.g.kv_heads, head = local - turn * a.g.kv_heads;
     const uint32_t tile = span.tiles - 1 - turn;
     const uint32_t length = span.position + span.rows;

@@ -53,14 +53,19 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
     constexpr bool kAhead = DP <= 128 && !(SETS == 4 && DP == 128 && NQ > 1);
     constexpr int kTile = SETS * kSet;
     constexpr int kStride = DP + 4;  // floats from one vector to the next in LDS
-    __shared__ float lds_o[kFewWaves][kSet][kStride];
-    __shared__ float2 lds_ml[kFewWaves][kTile];
-    __shared__ uint32_t lds_flag;
     // Queries in several pieces, and those of a large tile, lie in LDS, where the four wavefronts share them, and not in
     // registers that the rows need.
     constexpr bool kQInLds = NQ > 1 || SETS * DP >= 512;
-    __shared__ u32x4 lds_q[kQInLds ? SETS * NQ * S::kSteps * 64 : 1];
+    constexpr uint32_t kQBytes = kQInLds ? SETS * NQ * S::kSteps * 64 * sizeof(u32x4) : 0;
+    constexpr uint32_t kOBytes = kFewWaves * kTile * kStride * sizeof(float);
+    // (The queries' place is the wavefronts' results' in the end.)
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kQBytes > kOBytes ? kQBytes : kOBytes];
+    __shared__ float2 lds_ml[kFewWaves][kTile];
+    __shared__ uint32_t lds_flag;
+    u32x4 *const lds_q = reinterpret_cast<u32x4 *>(lds);
+    auto lds_o = reinterpret_cast<float (*)[kTile][kStride]>(lds);
 
+    paged_fetch_arguments(a);
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const uint32_t g = lane >> 4, i = lane & 15;
     const uint32_t d = EXACT ? DP : a.g.head_dim;
@@ -84,7 +89,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
 
     while (at < end) {
         PagedSpan span;
-        if (!line.find(span, [=](const PagedSpan &s, uint32_t work) { return at >= s.start && at - s.start < work; })) break;
+        if (!line.find<PagedLine::kBlock>(span, at)) break;
         const uint32_t local = (at - span.start) / span.blocks, from = (at - span.start) - local * span.blocks;
         const uint32_t count = min(span.blocks - from, end - at);
         const uint32_t tile = local / a.g.kv_heads, head = local - tile * a.g.kv_heads;
@@ -299,14 +304,14 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
             }
         }
 
-        // The four wavefronts' softmaxes meet, 16 vectors at a time. A lane holds of its column, for r = 0 .. 3, the channels
+        // The four wavefronts' softmaxes meet. A lane holds of its column, for r = 0 .. 3, the channels
         // kWide * (4g + r) + t of every run.
         const bool whole = count == span.blocks;
         bool bad = false;
 #pragma unroll
         for (int n = 0; n < SETS; ++n) {
             const float l = sum_over_groups(sum[n]);
-            __syncthreads();  // (what was there has been read)
+            if (n == 0) __syncthreads();  // (what was there has been read)
             if (g == 0) lds_ml[wave][n * kSet + i] = make_float2(threshold[n] == -INFINITY ? -INFINITY : ref[n], l);
 #pragma unroll
             for (int h = 0; h < S::kHalves; ++h)
@@ -314,9 +319,13 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
                     for (int c = 0; c < S::kWide; c += 4)
-                        *reinterpret_cast<floatx4 *>(&lds_o[wave][i][128 * h + S::kWide * (4 * g + r) + c]) = floatx4{
+                        *reinterpret_cast<floatx4 *>(&lds_o[wave][n * kSet + i][128 * h + S::kWide * (4 * g + r) + c]) = floatx4{
                             o[n][8 * h + c][r], o[n][8 * h + c + 1][r], o[n][8 * h + c + 2][r], o[n][8 * h + c + 3][r]};
-            __syncthreads();
+        }
+        __syncthreads();
+        // (A loop: code that runs once is fetched as slowly as it is long.)
+#pragma unroll 1
+        for (int n = 0; n < SETS; ++n) {
             constexpr int kChunk = DP / 16;  // channels a thread writes
             const uint32_t j = tid >> 4, c0 = (tid & 15) * kChunk;
             const uint32_t v = v0 + n * kSet + j;
@@ -337,7 +346,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
             for (int w = 0; w < kFewWaves; ++w)
 #pragma unroll
                 for (int c = 0; c < kChunk; c += 4) {
-                    const floatx4 x = *reinterpret_cast<const floatx4 *>(&lds_o[w][j][c0 + c]);
+                    const floatx4 x = *reinterpret_cast<const floatx4 *>(&lds_o[w][n * kSet + j][c0 + c]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[c + e] = __builtin_fmaf(weight[w], x[e], acc[c + e]);
                 }

@@ -21,11 +21,12 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttn a) {
     constexpr int kAtOnce = 8;
     __shared__ floatx4 lds[kLanes][kQuads];
     __shared__ float weights[kPagedMostParts], lds_m[kThreads / 64], lds_l[kThreads / 64];
+    paged_fetch_arguments(a);
     const uint32_t tid = threadIdx.x, row = blockIdx.x, hq = blockIdx.y;
     const PagedLine line(a);
     const uint32_t share = a.parts ? 0 : paged_share(a, line.total());
     PagedSpan span;
-    if (!line.find(span, [=](const PagedSpan &s, uint32_t) { return row >= s.row0 && row - s.row0 < s.rows; })) return;
+    if (!line.find<PagedLine::kRow>(span, row)) return;
     const uint32_t head = paged_row_of(a, hq), v = (row - span.row0) * a.group + (hq - head * a.group);
     // (The kernel of many rows counts an item's tiles from the last.)
     const uint32_t tile = v >> a.tile_shift, local = (a.parts ? span.tiles - 1 - tile : tile) * a.g.kv_heads + head;
