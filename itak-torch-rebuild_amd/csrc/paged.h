@@ -123,6 +123,12 @@ __host__ __device__ inline uint32_t paged_first_block(uint32_t position, uint32_
     return window && position + 1 > window ? (position + 1 - window) / 32 : 0;
 }
 
+// Blocks of the line that a workgroup takes.
+__host__ __device__ inline uint32_t paged_share(const PagedAttn &a, uint32_t total) {
+    const uint32_t even = (total + a.groups - 1) / a.groups;
+    return even > a.least ? even : a.least;
+}
+
 #if defined(__HIPCC__)
 
 __device__ __forceinline__ uint32_t paged_row_of(const PagedAttn &a, uint32_t vector) {
@@ -231,9 +237,6 @@ struct PagedLine {
         return false;
     }
 };
-__device__ __forceinline__ uint32_t paged_share(const PagedAttn &a, uint32_t total) {
-    return max(a.least, (total + a.groups - 1) / a.groups);
-}
 
 // The batch's item that holds row `row`: its position, first row and table. All lanes ask together.
 __device__ __forceinline__ bool paged_item_of_row(const uint32_t *batch, uint32_t row, uint4 &item) {

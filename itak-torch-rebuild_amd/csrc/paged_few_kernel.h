@@ -396,13 +396,15 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
 
 template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP>
 void launch_few_as(uint32_t sets, const PagedAttn &a, hipStream_t stream) {
+    // (Workgroups that would find nothing are left out where the batch is known.)
+    const uint32_t groups = a.inline_items ? (a.total + paged_share(a, a.total) - 1) / paged_share(a, a.total) : a.groups;
     if (sets == 1) {
-        launch_kernel(paged_few_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, 1>, a.groups, kFewWaves * 64, 0, stream, a);
+        launch_kernel(paged_few_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, 1>, groups, kFewWaves * 64, 0, stream, a);
     } else if (sets == 2 || DP > 128) {
-        launch_kernel(paged_few_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, 2>, a.groups, kFewWaves * 64, 0, stream, a);
+        launch_kernel(paged_few_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, 2>, groups, kFewWaves * 64, 0, stream, a);
     } else {
         if constexpr (DP <= 128)
-            launch_kernel(paged_few_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, 4>, a.groups, kFewWaves * 64, 0, stream, a);
+            launch_kernel(paged_few_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, 4>, groups, kFewWaves * 64, 0, stream, a);
     }
 }
 template <int PAGE, int ELEM, int NQ, int NP>
