@@ -39,8 +39,10 @@ hipError_t launch_paged_append(uint32_t page_elem, uint32_t elem, bool by_8, con
 // head's vectors, vector v being row v / group, head v % group. A tile is `kTile` of them, a unit a tile of one KV head of one
 // item: its work is the 32-key blocks from the window of the item's first row to the item's last position. All units' blocks
 // in one line (items in order, in an item tile by tile, in a tile head by head) are dealt out evenly: workgroup w takes blocks w * share
-// .. (w + 1) * share of the line, over unit borders, so that a batch of any lengths keeps every compute unit busy to the end
-// and the grid does not depend on the lengths. A unit that one workgroup has whole is written out by it; of the others every workgroup
+// .. (w + 1) * share of the line, so that a batch of any lengths keeps every compute unit busy to the end and the grid does not
+// depend on the lengths. Where that makes a share little longer, every unit's run is rounded up to a multiple of the share, so that
+// no workgroup has parts of two units one after the other: a part costs some 4 us beside its blocks (one token at 4,096:
+// 8.4 us over borders, 5.0 without). A unit that one workgroup has whole is written out by it; of the others every workgroup
 // leaves its partial in slot w + (unit's index), which no two parts share, and the merge launch joins them.
 // The cut is worked out on the device from the batch's lengths, so a captured launch is right for whatever batch is set when it runs.
 // Items that travel with a launch: an eager call whose batch has at most this many hands them over by value, and its kernels do not
@@ -72,7 +74,8 @@ struct PagedAttn {
     uint32_t parts;      // kernel of many rows: workgroups a unit is dealt to; 0: the line above
     const void *zeros;   // 16 bytes of them
     uint32_t inline_items; // 0: the batch's are read from device memory
-    uint32_t total;      // with inline items: blocks of all units
+    uint32_t total;      // with inline items: the line's length, and its cut
+    uint32_t share, pad;
     PagedItemWords item[kPagedInline];  // those behind the last: row0, start and unit0 are ~0
     uint32_t start[kPagedInline], unit0[kPagedInline];  // where an item's blocks and units begin in the line
     float *ws_acc;       // [slots][tile][padded head_dim]
@@ -114,6 +117,7 @@ struct PagedSpan {
     uint32_t position, rows, row0, table;
     uint32_t first;   // first 32-key block its rows see
     uint32_t blocks;  // of a unit
+    uint32_t run;     // and with the line's rounding
     uint32_t tiles;
     uint32_t start;   // of its blocks in the line of all units'
     uint32_t unit0;   // its first unit's index
@@ -123,11 +127,19 @@ __host__ __device__ inline uint32_t paged_first_block(uint32_t position, uint32_
     return window && position + 1 > window ? (position + 1 - window) / 32 : 0;
 }
 
-// Blocks of the line that a workgroup takes.
-__host__ __device__ inline uint32_t paged_share(const PagedAttn &a, uint32_t total) {
-    const uint32_t even = (total + a.groups - 1) / a.groups;
-    return even > a.least ? even : a.least;
+// How the line is cut: blocks a workgroup takes, and what the units' runs are multiples of (0: of nothing). With rounded runs
+// the workgroups are at most total / share + units, which is why `groups` of them do.
+struct PagedCut {
+    uint32_t share, pad;
+};
+constexpr uint32_t kPagedPart = 8;  // blocks that a share may be longer for being in one unit
+__host__ __device__ inline PagedCut paged_cut(uint32_t total, uint32_t units, uint32_t groups, uint32_t least) {
+    const uint32_t even = (total + groups - 1) / groups, share = even > least ? even : least;
+    if (units >= groups) return {share, 0};
+    const uint32_t left = groups - units, apart = (total + left - 1) / left, own = apart > least ? apart : least;
+    return own <= share + kPagedPart ? PagedCut{own, own} : PagedCut{share, 0};
 }
+__host__ __device__ inline uint32_t paged_run(uint32_t blocks, uint32_t pad) { return pad ? (blocks + pad - 1) / pad * pad : blocks; }
 
 #if defined(__HIPCC__)
 
@@ -148,6 +160,7 @@ __device__ __forceinline__ void paged_fetch_arguments(const PagedAttn &a) {
 // a lane.
 struct PagedLine {
     const PagedAttn &a;
+    uint32_t share = 0, pad = 0, total = 0;
 
     __device__ __forceinline__ explicit PagedLine(const PagedAttn &args) : a(args) {}
     // An item's span, and blocks and units of all of it; none of an item that the launch does not take, and of one beyond the
@@ -162,7 +175,8 @@ struct PagedLine {
             s.blocks = (w.position + w.rows + 31) / 32 - s.first;
             s.tiles = (vectors + (1u << a.tile_shift) - 1) >> a.tile_shift;
             units = s.tiles * a.g.kv_heads;
-            work = units * s.blocks;
+            s.run = paged_run(s.blocks, pad);
+            work = units * s.run;
         }
         return s;
     }
@@ -183,17 +197,22 @@ struct PagedLine {
         }
         return x;
     }
-    // Blocks of all units.
-    __device__ __forceinline__ uint32_t total() const {
-        if (a.inline_items) return a.total;
+    // The cut; before anything that counts blocks.
+    __device__ __forceinline__ void cut() {
+        if (a.inline_items) {
+            share = a.share, pad = a.pad, total = a.total;
+            return;
+        }
         const uint32_t n = min(a.batch[0], a.items);
-        uint32_t all = 0;
+        uint32_t all = 0, all_units = 0;
         for (uint32_t at = 0; at < n; at += 64) {
             uint32_t work, units;
             of_lane(at, n, work, units);
             all += __builtin_amdgcn_readlane(scan(work), 63);
+            all_units += __builtin_amdgcn_readlane(scan(units), 63);
         }
-        return all;
+        const PagedCut c = paged_cut(all, all_units, a.groups, a.least);
+        share = c.share, pad = c.pad, total = pad ? share * a.groups : all;  // (of rounded runs: what lies past the last is nobody's)
     }
     // The item that block, unit or row x of the line belongs to; none if it is no item's, or of one that the launch does not take.
     enum By { kBlock, kUnit, kRow };
@@ -227,7 +246,7 @@ struct PagedLine {
                 const uint32_t l = __builtin_ctzll(mask);
 #define ITAK_FIELD(f) out.f = __builtin_amdgcn_readlane(s.f, l)
                 ITAK_FIELD(position), ITAK_FIELD(rows), ITAK_FIELD(row0), ITAK_FIELD(table), ITAK_FIELD(first);
-                ITAK_FIELD(blocks), ITAK_FIELD(tiles), ITAK_FIELD(start), ITAK_FIELD(unit0);
+                ITAK_FIELD(blocks), ITAK_FIELD(run), ITAK_FIELD(tiles), ITAK_FIELD(start), ITAK_FIELD(unit0);
 #undef ITAK_FIELD
                 return true;
             }

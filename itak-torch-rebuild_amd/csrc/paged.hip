@@ -179,23 +179,34 @@ itak_status check_attention(itak_paged *p, uint64_t layer, const itak_rows *q, c
 
 uint32_t shift_of(uint32_t power) { return uint32_t(__builtin_ctz(power)); }
 
-// Units and blocks of the items a launch takes.
+// Units and blocks of the items a launch takes, how their line is cut, and where in it inline items begin.
 itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work) {
+    auto each = [&](uint32_t pad, auto item) {
+        uint64_t at = 0, units = 0;
+        for (uint32_t i = 0; i < a.items; ++i) {
+            const uint32_t *it = p->batch.head.data() + kPagedItem0 + 4 * i;
+            const uint64_t vectors = uint64_t(it[1]) * a.group;
+            item(i, at, units);
+            if (vectors < a.v_from || vectors > a.v_to) continue;
+            const uint64_t tiles = (vectors + a.tile - 1) / a.tile * a.g.kv_heads;
+            units += tiles;
+            at += tiles * paged_run((it[0] + it[1] + 31) / 32 - paged_first_block(it[0], a.window), pad);
+        }
+        item(a.items, at, units);
+    };
     uint64_t units = 0;
-    work = 0;
-    for (uint32_t i = 0; i < kPagedInline; ++i) a.start[i] = a.unit0[i] = ~0u;
-    for (uint32_t i = 0; i < a.items; ++i) {
-        const uint32_t *it = p->batch.head.data() + kPagedItem0 + 4 * i;
-        const uint64_t vectors = uint64_t(it[1]) * a.group;
-        if (i < a.inline_items) a.start[i] = uint32_t(work), a.unit0[i] = uint32_t(units);
-        if (vectors < a.v_from || vectors > a.v_to) continue;
-        const uint64_t tiles = (vectors + a.tile - 1) / a.tile * a.g.kv_heads;
-        units += tiles;
-        work += tiles * ((it[0] + it[1] + 31) / 32 - paged_first_block(it[0], a.window));
-    }
-    if (work >= (1ull << 31) || units >= (1ull << 24)) return size_overflow(p->err, "blocks of the batch's attention");
+    each(0, [&](uint32_t, uint64_t at, uint64_t u) { work = at, units = u; });
+    if (work >= (1ull << 30) || units >= (1ull << 24)) return size_overflow(p->err, "blocks of the batch's attention");
     a.units = uint32_t(units);
-    a.total = uint32_t(work);
+    if (!a.inline_items) return ITAK_OK;
+    // (The kernel of many rows has no line.)
+    const PagedCut cut = a.parts ? PagedCut{} : paged_cut(uint32_t(work), a.units, a.groups, a.least);
+    a.share = cut.share, a.pad = cut.pad;
+    for (uint32_t i = 0; i < kPagedInline; ++i) a.start[i] = a.unit0[i] = ~0u;
+    each(cut.pad, [&](uint32_t i, uint64_t at, uint64_t u) {
+        if (i < a.inline_items) a.start[i] = uint32_t(at), a.unit0[i] = uint32_t(u);
+        a.total = uint32_t(at);
+    });
     return ITAK_OK;
 }
 
@@ -289,6 +300,7 @@ itak_status run_attention(itak_paged *p, uint64_t layer, const itak_rows &q, con
         a.tile = 32 * paged_chunk_waves(dp, q.elem);
         a.tile_shift = shift_of(a.tile);
         a.v_from = few_most + 1, a.v_to = ~0u;
+        a.parts = 1;
         uint64_t work = 0;
         st = count_units(p, a, work);
         if (st != ITAK_OK) return st;

@@ -69,10 +69,10 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const uint32_t g = lane >> 4, i = lane & 15;
     const uint32_t d = EXACT ? DP : a.g.head_dim;
-    const PagedLine line(a);
-    const uint32_t total = line.total(), share = paged_share(a, total);
-    uint32_t at = blockIdx.x * share;
-    const uint32_t end = min(total, at + share);
+    PagedLine line(a);
+    line.cut();
+    uint32_t at = blockIdx.x * line.share;
+    const uint32_t end = min(line.total, at + line.share);
 
     // Where a lane reads: of a key block the rows 8 (i / 4) + i % 4 (+ 4 for the second tile), channels 8g of every 32; of a value
     // block the rows 8g .. 8g + 7, channels kWide * i of every run. Channels past head_dim are read from channel 0.
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
     while (at < end) {
         PagedSpan span;
         if (!line.find<PagedLine::kBlock>(span, at)) break;
-        const uint32_t local = (at - span.start) / span.blocks, from = (at - span.start) - local * span.blocks;
+        const uint32_t local = (at - span.start) / span.run, from = (at - span.start) - local * span.run;
         const uint32_t count = min(span.blocks - from, end - at);
         const uint32_t tile = local / a.g.kv_heads, head = local - tile * a.g.kv_heads;
         const uint32_t unit = span.unit0 + local;
@@ -390,14 +390,14 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
                                                                             blockIdx.x + unit < a.groups + a.units, acc, m, l);
                                           });
         }
-        at += count;
+        at += line.pad ? line.share : count;
     }
 }
 
 template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP>
 void launch_few_as(uint32_t sets, const PagedAttn &a, hipStream_t stream) {
     // (Workgroups that would find nothing are left out where the batch is known.)
-    const uint32_t groups = a.inline_items ? (a.total + paged_share(a, a.total) - 1) / paged_share(a, a.total) : a.groups;
+    const uint32_t groups = a.inline_items ? (a.total + a.share - 1) / a.share : a.groups;
     if (sets == 1) {
         launch_kernel(paged_few_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, 1>, groups, kFewWaves * 64, 0, stream, a);
     } else if (sets == 2 || DP > 128) {

@@ -23,8 +23,8 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttn a) {
     __shared__ float weights[kPagedMostParts], lds_m[kThreads / 64], lds_l[kThreads / 64];
     paged_fetch_arguments(a);
     const uint32_t tid = threadIdx.x, row = blockIdx.x, hq = blockIdx.y;
-    const PagedLine line(a);
-    const uint32_t share = a.parts ? 0 : paged_share(a, line.total());
+    PagedLine line(a);
+    if (!a.parts) line.cut();
     PagedSpan span;
     if (!line.find<PagedLine::kRow>(span, row)) return;
     const uint32_t head = paged_row_of(a, hq), v = (row - span.row0) * a.group + (hq - head * a.group);
@@ -37,8 +37,8 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttn a) {
     if (a.parts) {
         if (unit >= a.units) return;
     } else {
-        const uint32_t from = span.start + local * span.blocks;
-        first = from / share, last = (from + span.blocks - 1) / share, base = unit;
+        const uint32_t from = span.start + local * span.run;
+        first = from / line.share, last = (from + span.blocks - 1) / line.share, base = unit;
         if (first == last || last + unit >= a.groups + a.units) return;  // written whole
     }
     const uint32_t quad = tid % kQuads, part = tid / kQuads, parts = last - first + 1;
