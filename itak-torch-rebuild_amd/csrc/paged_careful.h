@@ -55,7 +55,6 @@ __device__ __forceinline__ void paged_careful(const PagedAttn &a, const PagedSpa
             for (uint32_t u = 0; u < kCareful; ++u) x[u] = 0.0f;
 #pragma unroll
             for (int c = 0; c < kRuns; ++c)
-#pragma unroll 4
                 for (uint32_t o = 0; o < min(64u, d - min(d, 64u * c)); o += 8) {
                     const Piece<P, 8> y = *reinterpret_cast<const Piece<P, 8> *>(k + 64 * c + o);
 #pragma unroll

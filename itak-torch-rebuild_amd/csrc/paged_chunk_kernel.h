@@ -39,9 +39,10 @@ __device__ __forceinline__ floatx16 mfma_32x32x16(u32x4 a, u32x4 b, floatx16 c) 
 }
 
 // Issued from assembly: the compiler then neither waits for such a load at every LDS read nor needs to, because its only
-// consumer is ordered by the wait and the barrier at the top of each block.
+// consumer is ordered by the wait and the barrier at the top of each block. It does not look for hazards in there either: a scalar
+// register that vector code wrote (readlane: the address) takes five wait states before a load may read it, m0 one.
 __device__ __forceinline__ void page_to_lds(uint64_t base, uint32_t offset, uint32_t lds_addr) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds_addr) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds_addr) : "memory");
 }
 __device__ __forceinline__ void lane_to_lds(uint64_t address, uint32_t lds_addr) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(address), "s"(lds_addr) : "memory");
@@ -258,11 +259,18 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
         }
     };
     // Rows of block kb no query of the tile sees may hold anything: their values are zeroed in LDS, where the block lies at `at`.
+    // (Every lane reads and writes: a branch that turns lanes off would stand amid the fullest registers there are.)
     auto clear = [&](uint32_t kb, uint32_t at) {
-        for (uint32_t p = tid; p < 32 * kRowPieces; p += kWaves * 64) {
-            const uint32_t key = 32 * kb + p / kRowPieces;
-            if (key < tile_lo || key >= tile_hi)
-                *reinterpret_cast<__attribute__((address_space(3))) u32x4 *>((uintptr_t)(at + kBlockBytes + p * 16)) = u32x4{0, 0, 0, 0};
+        constexpr uint32_t kPieces = 32 * kRowPieces, kStep = kWaves * 64;  // (where lanes are more, two do the same)
+#pragma unroll 1
+        for (uint32_t first = 0; first < kPieces; first += kStep) {
+            const uint32_t p = (first + tid) % kPieces;
+            const uint32_t key = 32 * kb + p / kRowPieces, keep = key < tile_lo || key >= tile_hi ? 0 : ~0u;
+            auto *const piece = reinterpret_cast<__attribute__((address_space(3))) u32x4 *>((uintptr_t)(at + kBlockBytes + p * 16));
+            u32x4 x = *piece;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] &= keep;
+            *piece = x;
         }
     };
     // The blocks of a stage that have such rows: at most the tile's first and last.
