@@ -51,9 +51,34 @@ def source_flags(src: str):
     return MFMA_IN_VECTOR_REGISTERS if src.startswith(("paged_chunk", "paged_few")) else []
 
 
+def misplaced(listing) -> list:
+    """Copies of registers that a listing makes at the head of a block before the lanes that a branch or a loop has turned off are
+    turned on again: (kernel, line). Short of registers the compiler has put the copy of one that every lane needs there, into the
+    accumulation registers: the lanes that were off then read whatever the copy's register held before."""
+    found, kernel, early = [], "?", None
+    for n, raw in enumerate(listing, 1):
+        line = raw.split(";")[0].strip()
+        if line.endswith(":"):
+            if line.startswith("_Z"):
+                kernel = line[:-1]
+            early = []
+        elif early is None or not line:
+            continue
+        elif line.startswith("s_or_b64 exec, exec"):
+            found += [(kernel, at) for at in early]
+            early = None
+        elif "saveexec" in line or " exec," in line or line.startswith(("s_cbranch", "s_branch", "s_endpgm")):
+            early = None
+        elif line.startswith(("v_accvgpr", "v_mov_b32")):
+            early.append(n)
+    return found
+
+
 def _compile(src: str, timeline: bool = False) -> str:
     obj = os.path.join(OBJ_DIR + ("_timeline" if timeline else ""), src.replace(".hip", ".o"))
-    cmd = [HIPCC, *FLAGS, *source_flags(src), *(["-DITAK_TIMELINE"] if timeline and src not in NO_STAMPS else []), "-c",
+    # (Kernels that fill the vector registers have copies in the accumulation registers, and their listing is looked through.)
+    crowded = bool(source_flags(src))
+    cmd = [HIPCC, *FLAGS, *source_flags(src), *(["-save-temps=obj"] if crowded else []), *(["-DITAK_TIMELINE"] if timeline and src not in NO_STAMPS else []), "-c",
            os.path.join(CSRC, src), "-o", obj]
     res = subprocess.run(cmd, capture_output=True, text=True)
     noise = "is not a recognized feature for this target"
@@ -76,6 +101,16 @@ def _compile(src: str, timeline: bool = False) -> str:
             size = int(l.split("ScratchSize [bytes/lane]:")[1].split("[")[0])
             if size:
                 raise RuntimeError(f"{src}: kernel {name} spills {size} bytes/lane to scratch")
+    if crowded:
+        stem = obj[:-2] + f"-hip-amdgcn-amd-amdhsa-{ARCH}"
+        with open(stem + ".s") as f:
+            wrong = misplaced(f)
+        folder, names = os.path.split(obj[:-2])
+        for name in os.listdir(folder):
+            if name.startswith((names + "-hip-", names + "-host-", names + ".hip")) or name in (names + ".hipfb", names + ".bc", names + ".s"):
+                os.remove(os.path.join(folder, name))
+        if wrong:
+            raise RuntimeError(f"{src}: {wrong[0][0]} copies registers under lanes that are off (line {wrong[0][1]} of its listing)")
     if err.strip():
         sys.stderr.write(err + "\n")
     return obj
