@@ -226,7 +226,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     floatx16 x;
     auto scaled = [&](float s) {
         if constexpr (CAP)
-            return softcap_of_exp2_arg(s * a.scale_log2, a.cap_log2, ref);
+            return softcapped<ELEM>(s * a.scale_log2, a.cap_log2, ref);
         else
             return __builtin_fmaf(s, a.scale_log2, -ref);
     };

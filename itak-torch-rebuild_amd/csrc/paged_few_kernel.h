@@ -226,7 +226,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
                 }
                 if (a.cap_log2 != 0.0f) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = softcap_of_exp2_arg(x[e] * a.scale_log2, a.cap_log2, ref[n]);
+                    for (int e = 0; e < 8; ++e) x[e] = softcapped<ELEM>(x[e] * a.scale_log2, a.cap_log2, ref[n]);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf(x[e], a.scale_log2, -ref[n]);

@@ -225,6 +225,23 @@ def test_rows_that_are_not_finite_reach_the_queries_that_see_them(pages, tensors
     assert bool(((got - want).abs()[fine] <= tol[fine]).all())
 
 
+# A cap far above the scores changes them little, and one below them much: both leave f32 tensors their precision. (Of 8 channels,
+# where the bound on a product's sum is no wider than that.)
+@pytest.mark.parametrize("pages", ["f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("softcap", [1000.0, 30.0, 2.0])
+def test_a_cap_keeps_the_precision_of_f32(pages, rows, softcap):
+    cache = PC.Cache(pkg(), [300 + rows], kv_heads=2, d=8, pages=pages, page_rows=32, fill="nan", seed=11)
+    items = [(300, rows)]
+    cache.place(0, 0, 0, *(cache.normal(300 + rows, 2, 8).to(PC.DTYPES[pages]) for _ in range(2)))
+    q = cache.normal(rows, 8, 8)
+    out, qd = torch.empty_like(q, device="cuda"), q.cuda()
+    cache.paged.set_batch(items, cache.tables)
+    cache.paged.attention_device(0, view(qd), view(out), softcap=softcap, scale=0.3)
+    torch.cuda.synchronize()
+    check_attention(cache, 0, items, q, out, "f32", softcap=softcap, scale=0.3)
+
+
 # ------------------------------------------------------------------------------------ the step
 
 @pytest.mark.parametrize("pages,tensors", [("f16", "f16"), ("bf16", "bf16"), ("f16", "f32")])
