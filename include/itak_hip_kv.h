@@ -753,9 +753,10 @@ itak_status itak_rotate_device(const itak_rotation *rotation, void *hip_stream, 
    Tensors of a call are ITAK_ELEM_F32 or of the pages' own type. Scores, softmax and sums are f32. With tensors of
    the pages' type the softmax weights are rounded to that type once (f16 2^-11, bf16 2^-8 relative to each) and
    the output once; with f32 tensors queries and weights enter the matrix pipe as several halves each,
-   which leaves 2^-22 of them (bf16: 2^-24). An f16 query's or key's channel beyond 65504 is infinite.
-   A row that is not finite reaches the outputs of exactly the queries that see its position; one difference is left on f16 pages: a weight
-   below about 2^-32 of its row's largest is zero, and zero times an infinite value is NaN.
+   which leaves 2^-22 of them (bf16: 2^-24), over f16 pages at least 2^-29 of a query and 2^-37 of the largest weight. An f16 query's or key's channel beyond 65504 is infinite.
+   A row that is not finite reaches the outputs of exactly the queries that see its position; one difference is left: a weight
+   below 2^-126 of its row's largest is zero, and zero times an infinite value is NaN. Tiles of queries that meet such
+   rows, and f32 queries beyond 4,094 over f16 pages, are computed twice, the second time without the matrix pipe: slowly.
    Results do not depend on the pages' order or on what other sequences the batch holds beyond rounding (sums are cut
    into other pieces), and are the same from call to call.
 

@@ -8,6 +8,7 @@
 namespace itak {
 
 constexpr float kPagedLog2e = 1.4426950408889634f;
+constexpr float kPagedQueryLift = 16.0f;  // paged_mfma.h
 
 // Strides in elements; side = keys or values of a page, all its heads.
 struct PagedGeom {
@@ -68,7 +69,7 @@ struct PagedAttn {
     uint32_t v_from, v_to; // the launch takes the items of v_from .. v_to vectors a KV head
     uint32_t q_on_16;    // every 8 channels of q start on 16 bytes
     uint32_t out_on_16;
-    float scale_log2;    // scale * log2(e); with a softcap 2 * log2(e) * scale / cap
+    float scale_log2;    // scale * log2(e); with a softcap 2 * log2(e) * scale / cap; of lifted queries divided by their lift
     float cap_log2;      // cap * log2(e), 0: none
     uint32_t window;
     uint32_t parts;      // kernel of many rows: workgroups a unit is dealt to; 0: the line above

@@ -174,6 +174,8 @@ itak_status check_attention(itak_paged *p, uint64_t layer, const itak_rows *q, c
     if (q->heads > 65535) return unsupported(p->err, "more than 65535 query heads");
     if (std::isinf(scale)) return invalid_argument(p->err, "scale is infinite");
     if (!(softcap >= 0.0f) || std::isinf(softcap)) return invalid_argument(p->err, "softcap must be finite and >= 0");
+    if (softcap > 0.0f && std::isinf((std::isnan(scale) ? 1.0f : scale) * (2.0f * kPagedLog2e / softcap)))
+        return unsupported(p->err, "a softcap so small that scale / softcap is infinite");
     return ITAK_OK;
 }
 
@@ -260,6 +262,7 @@ itak_status run_attention(itak_paged *p, uint64_t layer, const itak_rows &q, con
     a.out_on_16 = rows_on_16(out, d);
     const float s = std::isnan(scale) ? 1.0f / std::sqrt(float(d)) : scale;
     a.scale_log2 = softcap > 0.0f ? s * (2.0f * kPagedLog2e / softcap) : s * kPagedLog2e;
+    if (p->cfg.elem == ITAK_ELEM_F16 && q.elem == ITAK_ELEM_F32) a.scale_log2 /= kPagedQueryLift;
     a.cap_log2 = softcap * kPagedLog2e;
     a.window = uint32_t(std::min<uint64_t>(window, 1ull << 31));
     a.zeros = p->batch_dev + p->zeros_at;

@@ -28,8 +28,6 @@ namespace {
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
 
-constexpr float kChunkSlack = 8.0f;
-
 template <int PAGE>
 __device__ __forceinline__ floatx16 mfma_32x32x16(u32x4 a, u32x4 b, floatx16 c) {
     if constexpr (PAGE == ITAK_ELEM_F16)
@@ -246,11 +244,11 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
             const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
             const float m = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
             const bool live = threshold != -INFINITY;
-            float delta = live ? fmaxf(m, 0.0f) : m;
+            float delta = live ? fmaxf(m - kWeightLift, 0.0f) : m - kWeightLift;
             if (m == -INFINITY) delta = 0.0f;
             const float alpha = live ? fast_exp2(-delta) : 1.0f;
             ref += delta;
-            if (m != -INFINITY) threshold = kChunkSlack;
+            if (m != -INFINITY) threshold = kWeightMost;
             sum *= alpha;
 #pragma unroll
             for (int t = 0; t < kOut; ++t) o[t] *= alpha;

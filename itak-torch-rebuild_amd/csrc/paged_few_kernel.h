@@ -24,9 +24,6 @@ namespace {
 
 constexpr int kFewWaves = 4;
 constexpr int kSet = kPagedSet;  // vectors of one column tile
-// A maximum is moved only when a score passes it by more than this many powers of two: the rescaling of the accumulators then
-// leaves the common path. Weights stay below 2^8, and weights of 2^-32 of the largest are still values of f16 (2^-24).
-constexpr float kFewSlack = 8.0f;
 
 // Rows and channels of a 32-key block as a lane holds them: DP = head_dim padded to 64, 128 or 256.
 template <int DP>
@@ -244,11 +241,11 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
                 if (__builtin_amdgcn_ballot_w64(most > threshold[n]) != 0) {
                     const float m = max_over_groups(most);
                     const bool live = threshold[n] != -INFINITY;
-                    float delta = live ? fmaxf(m, 0.0f) : m;
+                    float delta = live ? fmaxf(m - kWeightLift, 0.0f) : m - kWeightLift;
                     if (m == -INFINITY) delta = 0.0f;
                     const float alpha = live ? fast_exp2(-delta) : 1.0f;
                     ref[n] += delta;
-                    if (m != -INFINITY) threshold[n] = kFewSlack;
+                    if (m != -INFINITY) threshold[n] = kWeightMost;
                     sum[n] *= alpha;
 #pragma unroll
                     for (int t = 0; t < S::kTiles; ++t) o[n][t] *= alpha;

@@ -19,6 +19,15 @@ __device__ __forceinline__ floatx4 mfma_16x16x32(u32x4 a, u32x4 b, floatx4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bfloat8, a), __builtin_bit_cast(bfloat8, b), c, 0, 0, 0);
 }
 
+// A row's reference is kept 12 below its largest score (log2 domain): weights are up to 2^15, where f16 ends at 2^16, so that of f16
+// pieces those down to 2^-26 of the largest keep their precision and what is lost of a smaller one is 2^-37 of the largest. It
+// moves only when a score passes it by more than 15: the rescaling of the accumulators then leaves the common path.
+constexpr float kWeightLift = 12.0f, kWeightMost = 15.0f;
+// f32 queries enter f16 products times 16, and the scale makes up for it: f16 ends at 2^-24 below, and a query's last bits do
+// then at 2^-28. (One beyond 4,094 is infinite to the products and is done over in f32, as all that is not finite.)
+template <int PAGE, int ELEM>
+constexpr float kQueryLift = PAGE == ITAK_ELEM_F16 && ELEM == ITAK_ELEM_F32 ? kPagedQueryLift : 1.0f;
+
 // Eight f32 as PIECES vectors of the pages' type whose sum they are: each piece the rounding of what the ones before leave.
 template <int PAGE, int PIECES>
 __device__ __forceinline__ void split_8(const float (&x)[8], u32x4 (&out)[PIECES]) {
@@ -75,7 +84,7 @@ __device__ __forceinline__ void split_query(const typename QueryRaw<ELEM>::type 
     if constexpr (ELEM == ITAK_ELEM_F32) {
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = in ? raw[e] : 0.0f;
+        for (int e = 0; e < 8; ++e) x[e] = in ? raw[e] * kQueryLift<PAGE, ELEM> : 0.0f;
         u32x4 pieces[NQ];
         split_8<PAGE, NQ>(x, pieces);
 #pragma unroll

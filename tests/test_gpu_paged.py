@@ -225,6 +225,54 @@ def test_rows_that_are_not_finite_reach_the_queries_that_see_them(pages, tensors
     assert bool(((got - want).abs()[fine] <= tol[fine]).all())
 
 
+# One key has most of the weight and thousands share the rest evenly, 2^-16 of it each: what a rounding takes of one it takes of all.
+@pytest.mark.parametrize("pages,tensors,off", [("f16", "f16", 2.0 ** -11), ("f16", "f32", 2.0 ** -19), ("bf16", "f32", 2.0 ** -19)])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_many_small_weights_beside_a_large_one(pages, tensors, off, rows):
+    n, d = 20000, 64
+    cache = PC.Cache(pkg(), [n], kv_heads=1, d=d, pages=pages, page_rows=256, fill="nan", seed=2)
+    keys, values = torch.zeros(n, 1, d), torch.full((n, 1, d), 0.75)
+    keys[7, 0, 0] = 11.2  # a score of 11.2 above the others' 0: their weights are e^-11.2 of its
+    keys[7] = keys[7].to(PC.DTYPES[pages]).float()
+    values[7] = -0.5
+    cache.place(0, 0, 0, keys.to(PC.DTYPES[pages]), values.to(PC.DTYPES[pages]))
+    q = torch.zeros(rows, 2, d)
+    q[:, :, 0] = 1.0
+    q = q.to(PC.DTYPES[tensors])
+    out, qd = torch.empty_like(q, device="cuda"), q.cuda()
+    cache.paged.set_batch([(n - rows, rows)], cache.tables)
+    cache.paged.attention_device(0, view(qd), view(out), scale=1.0)
+    torch.cuda.synchronize()
+    # f16: weights are within 2^-11 of themselves in the numerator, where the large one brings at most 0.5 and the others together
+    # at most 0.75 * 0.22, and the output, at most 0.5, is rounded within 2^-11 of itself: below 2^-11 in all. f32: second and
+    # third pieces leave 2^-21 of a weight, and a workgroup adds at most 20 blocks, 2^-24 each in numerator and denominator.
+    w = math.exp(-float(keys[7, 0, 0]))
+    at = torch.arange(n - rows + 1, n + 1).double() - 1
+    want = (-0.5 + 0.75 * w * at) / (1 + w * at)
+    assert bool(((out.cpu().double() - want[:, None, None]).abs() <= off).all())
+
+
+# Small queries before large keys: the scores are what they are of ordinary ones.
+@pytest.mark.parametrize("rows", [1, 40])
+def test_small_f32_queries_keep_their_bits(rows):
+    cache = PC.Cache(pkg(), [200 + rows], kv_heads=2, d=64, page_rows=16, fill="nan", seed=3)
+    items = [(200, rows)]
+    keys, values = (cache.normal(200 + rows, 2, 64) for _ in range(2))
+    cache.place(0, 0, 0, (keys * 64).half(), values.half())
+    q = cache.normal(rows, 4, 64) * 2.0 ** -6
+    out, qd = torch.empty_like(q, device="cuda"), q.cuda()
+    cache.paged.set_batch(items, cache.tables)
+    cache.paged.attention_device(0, view(qd), view(out))
+    torch.cuda.synchronize()
+    at, scale = 0, 1 / math.sqrt(64)
+    k16, v16 = cache.rows(0, 0, 200 + rows)
+    want, spread, most = PC.attention(q, k16, v16, 200, 0, 0.0, scale)
+    # A query channel is off by 2^-22 of itself or by 2^-29: over 64 channels of keys up to 4 * 64, beside the tolerance of any other.
+    extra = 2 * 64 * 4 * 64 * 2.0 ** -29 * scale
+    tol = PC.tolerance(want, spread, most, "f16", "f32", 64, 200 + rows) + spread * extra
+    assert bool(((out.cpu().double() - want).abs() <= tol).all())
+
+
 # A cap far above the scores changes them little, and one below them much: both leave f32 tensors their precision. (Of 8 channels,
 # where the bound on a product's sum is no wider than that.)
 @pytest.mark.parametrize("pages", ["f16", "bf16"])
