@@ -281,18 +281,24 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
     };
 
-    // Stages of the ring fill ahead of the one at hand; its last places are never read where the blocks end inside one.
+    // Stages of the ring fill ahead of the one at hand; the last one's places are never read where the blocks end inside it. Behind
+    // the last stage nothing is asked for, and the waits there are for all that flies.
     const uint32_t stages = (kb_end - kb0 + kSubs - 1) / kSubs;
     look_up(kb0);
     wait_loads<0>();  // (the compiler cannot count the ring's loads: every load of its own has to be in before the first of them)
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s)
+    for (int s = 0; s < kStages - 1; ++s) {
+        if (uint32_t(s) >= stages) break;
 #pragma unroll
         for (int u = 0; u < kSubs; ++u) issue(s * kSubs + u, s * kStageBytes + u * kSubBytes);
+    }
     u32x4 k[kSteps];
     if (stages) {
         // The first block's scores by themselves, and the operands of the second block's.
-        wait_loads<kStageLoads * (kStages - 2)>();
+        if (stages >= kStages - 1)
+            wait_loads<kStageLoads * (kStages - 2)>();
+        else
+            wait_loads<0>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         clear_stage(kb0, ring_base);
@@ -319,12 +325,17 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
         const uint32_t kb = kb0 + g * kSubs;
         // This wavefront's loads of the next stage have landed (those of the stages behind it may still fly); behind the barrier
         // everybody's have, and everybody is done with the stage before this one, which the loads that go out now overwrite.
-        wait_loads<kStageLoads * (kStages - 3)>();
+        if (g + kStages - 1 <= stages)
+            wait_loads<kStageLoads * (kStages - 3)>();
+        else
+            wait_loads<0>();
         __builtin_amdgcn_s_barrier();
-        const uint32_t n = (g + kStages - 1) * kSubs;
-        if ((n & 63) == 0) look_up(kb0 + n);
+        if (g + kStages - 1 < stages) {
+            const uint32_t n = (g + kStages - 1) * kSubs;
+            if ((n & 63) == 0) look_up(kb0 + n);
 #pragma unroll
-        for (int u = 0; u < kSubs; ++u) issue(n + u, free_at + u * kSubBytes);
+            for (int u = 0; u < kSubs; ++u) issue(n + u, free_at + u * kSubBytes);
+        }
         if (g + 2 == stages) clear_stage(kb + kSubs, next);
         uint32_t k_lane[kSteps], v_lane[kOut];
 #pragma unroll
@@ -405,21 +416,24 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
         free_at = was - ring_base;
         next = next + kStageBytes == ring_base + kStages * kStageBytes ? ring_base : next + kStageBytes;
     }
-    wait_loads<0>();  // (the surplus loads)
-
     // A lane holds of its column channels 32 t + 8 (r / 4) + 4 h + r % 4.
-    const bool whole = a.parts == 1;
-    bool bad = false;
-    if (wv0 + j < vectors) {
-        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
-        const float l = __uint_as_float(both[0]) + __uint_as_float(both[1]);
-        const uint32_t v = wv0 + j;
-        float check = l;
+    // (The check comes before the stores: the barriers it takes would wait for them.)
+    const bool whole = a.parts == 1, mine = wv0 + j < vectors;
+    const uint32_t v = wv0 + j;
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+    const float l = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+    float check[4] = {l, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int t = 0; t < kOut; ++t)
+    for (int t = 0; t < kOut; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) check += EXACT || 32u * t + 8 * (r / 4) + 4 * h < d ? o[t][r] : 0.0f;
-        bad = bad || check != check;
+        for (int r = 0; r < 16; ++r) check[r % 4] += EXACT || 32u * t + 8 * (r / 4) + 4 * h < d ? o[t][r] : 0.0f;
+    const float all = (check[0] + check[1]) + (check[2] + check[3]);
+    if (any_of_group(mine && all != all, &lds_flag)) {
+        paged_careful<PAGE, ELEM, DP>(a, span, head, v0, min(v0 + kTile, vectors), wave, kWaves, 32 * kb0, 32 * kb_end,
+                                      [&](uint32_t v, const float (&acc)[DP / 64], float m, float l) {
+                                          paged_write_careful<ELEM, DP>(a, span, head, v, whole, slot0 + v - v0, true, acc, m, l);
+                                      });
+    } else if (mine) {
         if (whole) {
             const float inv = 1.0f / l;
             const uint32_t row = paged_row_of(a, v), hq = head * a.group + v - row * a.group;
@@ -452,11 +466,6 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
             if (h == 0) a.ws_ml[slot] = make_float2(threshold == -INFINITY ? -INFINITY : ref, l);
         }
     }
-    if (any_of_group(bad, &lds_flag))
-        paged_careful<PAGE, ELEM, DP>(a, span, head, v0, min(v0 + kTile, vectors), wave, kWaves, 32 * kb0, 32 * kb_end,
-                                      [&](uint32_t v, const float (&acc)[DP / 64], float m, float l) {
-                                          paged_write_careful<ELEM, DP>(a, span, head, v, whole, slot0 + v - v0, true, acc, m, l);
-                                      });
 }
 
 template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP>
