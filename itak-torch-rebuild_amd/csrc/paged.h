@@ -84,7 +84,7 @@ struct PagedAttn {
 };
 // Workgroups that may share a unit.
 constexpr uint32_t kPagedMostParts = 1024;
-// The kernel of few rows (paged_few_kernel.h): tiles of `sets` times 16 vectors, 1, 2 or 4 (up to 128 channels).
+// The kernel of few rows (paged_few_kernel.h): tiles of `sets` times 16 vectors, 1 or 2.
 constexpr uint32_t kPagedSet = 16;
 // Workgroups a compute unit holds: two where a lane does with 256 registers.
 __host__ __device__ constexpr uint32_t paged_few_groups_per_cu(uint32_t padded, uint32_t page_elem, uint32_t elem, uint32_t sets) {

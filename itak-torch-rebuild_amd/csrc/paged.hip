@@ -268,8 +268,10 @@ itak_status run_attention(itak_paged *p, uint64_t layer, const itak_rows &q, con
     a.zeros = p->batch_dev + p->zeros_at;
     const uint32_t dp = paged_padded(d), cus = std::max(1u, compute_units());
     // Items of few query vectors a KV head and items of many are launches of their own: a prompt's chunk among other
-    // sequences' tokens is common.
-    const uint32_t few_most = dp <= 128 ? 4 * kPagedSet : 2 * kPagedSet;
+    // sequences' tokens is common. Up to 32 vectors are few (4 of 4 rows by 8 heads at 8,192 in f32 22.0 us there and 25.5 in the
+    // kernel of many, 16 in f16 59.3 and 66.5); of 56 the kernel of many is level (4 at 8,192 in f16 25.9 and 25.5) or ahead (in f32 32.7
+    // and 27.8, 64 at 600 47.7 and 26.7), though tiles of four sets of 16 had been made for them.
+    const uint32_t few_most = 2 * kPagedSet;
     const bool chunks = paged_chunk_takes(dp, p->cfg.elem, q.elem);
     uint32_t most_few = 0;
     bool many = false;
@@ -282,7 +284,7 @@ itak_status run_attention(itak_paged *p, uint64_t layer, const itak_rows &q, con
     }
     itak_status st = ITAK_OK;
     if (most_few) {
-        const uint32_t sets = most_few <= kPagedSet ? 1 : most_few <= 2 * kPagedSet ? 2 : 4;
+        const uint32_t sets = most_few <= kPagedSet ? 1 : 2;
         a.tile = sets * kPagedSet;
         a.tile_shift = shift_of(a.tile);
         a.v_from = 1, a.v_to = chunks ? few_most : ~0u;

@@ -1,8 +1,8 @@
-// Attention of few rows over pages: single tokens and short blocks, 16, 32 or 64 query vectors a tile.
+// Attention of few rows over pages: single tokens and short blocks, 16 or 32 query vectors a tile.
 //
 //   o_j = sum_p 2^(s_jp - m_j) v_p / sum_p 2^(s_jp - m_j),  s = log2(e) * (scale q.k, capped), m_j the running maximum
 //
-// Every visible key and value row is read once a tile and multiplied into its columns: 32 to 128 operations a byte, below
+// Every visible key and value row is read once a tile and multiplied into its columns: 32 or 64 operations a byte, below
 // what the matrix pipe does beside the memory, so the bytes bound it, and where they are few the chain of trips to memory: the
 // batch's items, page ids, rows, and the merge.
 //
@@ -46,13 +46,13 @@ template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP, int SETS>
 __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, ELEM, SETS)) void paged_few_kernel(PagedAttn a) {
     typedef FewShape<DP> S;
     typedef typename Elem<ELEM>::type T;
-    // (Two blocks of 256 channels beside the accumulators are more than 512 registers, and so are those of 64 vectors and pieces.)
-    constexpr bool kAhead = DP <= 128 && !(SETS == 4 && DP == 128 && NQ > 1);
+    // (Two blocks of 256 channels beside the accumulators are more than 512 registers.)
+    constexpr bool kAhead = DP <= 128;
     constexpr int kTile = SETS * kSet;
     constexpr int kStride = DP + 4;  // floats from one vector to the next in LDS
     // Queries in several pieces, and those of a large tile, lie in LDS, where the four wavefronts share them, and not in
     // registers that the rows need.
-    constexpr bool kQInLds = NQ > 1 || SETS * DP >= 512;
+    constexpr bool kQInLds = NQ > 1 || SETS * DP > 256;
     constexpr uint32_t kQBytes = kQInLds ? SETS * NQ * S::kSteps * 64 * sizeof(u32x4) : 0;
     constexpr uint32_t kOBytes = kFewWaves * kTile * kStride * sizeof(float);
     // (The queries' place is the wavefronts' results' in the end.)
@@ -397,11 +397,8 @@ void launch_few_as(uint32_t sets, const PagedAttn &a, hipStream_t stream) {
     const uint32_t groups = a.inline_items ? (a.total + a.share - 1) / a.share : a.groups;
     if (sets == 1) {
         launch_kernel(paged_few_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, 1>, groups, kFewWaves * 64, 0, stream, a);
-    } else if (sets == 2 || DP > 128) {
-        launch_kernel(paged_few_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, 2>, groups, kFewWaves * 64, 0, stream, a);
     } else {
-        if constexpr (DP <= 128)
-            launch_kernel(paged_few_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, 4>, groups, kFewWaves * 64, 0, stream, a);
+        launch_kernel(paged_few_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, 2>, groups, kFewWaves * 64, 0, stream, a);
     }
 }
 template <int PAGE, int ELEM, int NQ, int NP>
