@@ -129,13 +129,17 @@ __host__ __device__ inline uint32_t paged_first_block(uint32_t position, uint32_
 }
 
 // How the line is cut: blocks a workgroup takes, and what the units' runs are multiples of (0: of nothing). With rounded runs
-// the workgroups are at most total / share + units, which is why `groups` of them do.
+// the workgroups are at most total / share + units, which is why `groups` of them do; or they are the units, where a unit is
+// not much longer than a share: then nothing is split, and an eager call leaves the merge out.
 struct PagedCut {
     uint32_t share, pad;
 };
-constexpr uint32_t kPagedPart = 8;  // blocks that a share may be longer for being in one unit
-__host__ __device__ inline PagedCut paged_cut(uint32_t total, uint32_t units, uint32_t groups, uint32_t least) {
+// Blocks that a share may be longer for lying in one unit, and for being one (64 of one token at 600 28.6 us cut evenly and
+// 16.8 whole, 100 at 400 37.3 and 21.0; 16 of 8 heads at 4,096, 33 blocks a share, 52.4 and with 43 in one unit 57.3).
+constexpr uint32_t kPagedPart = 8, kPagedWhole = 24;
+__host__ __device__ inline PagedCut paged_cut(uint32_t total, uint32_t units, uint32_t longest, uint32_t groups, uint32_t least) {
     const uint32_t even = (total + groups - 1) / groups, share = even > least ? even : least;
+    if (units <= groups && longest <= share + kPagedWhole && units * 2 >= groups) return {longest, longest};
     if (units >= groups) return {share, 0};
     const uint32_t left = groups - units, apart = (total + left - 1) / left, own = apart > least ? apart : least;
     return own <= share + kPagedPart ? PagedCut{own, own} : PagedCut{share, 0};
@@ -198,6 +202,14 @@ struct PagedLine {
         }
         return x;
     }
+    static __device__ __forceinline__ uint32_t most_of(uint32_t x) {  // over the wavefront
+#define ITAK_MOST(ctrl) x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), ctrl, 0xf, 0xf, true)))
+        ITAK_MOST(0xB1), ITAK_MOST(0x4E), ITAK_MOST(0x141), ITAK_MOST(0x140);  // (of sixteen lanes)
+#undef ITAK_MOST
+        const uint32_t a = __builtin_amdgcn_readlane(x, 0), b = __builtin_amdgcn_readlane(x, 16);
+        const uint32_t c = __builtin_amdgcn_readlane(x, 32), d = __builtin_amdgcn_readlane(x, 48);
+        return max(max(a, b), max(c, d));
+    }
     // The cut; before anything that counts blocks.
     __device__ __forceinline__ void cut() {
         if (a.inline_items) {
@@ -205,14 +217,16 @@ struct PagedLine {
             return;
         }
         const uint32_t n = min(a.batch[0], a.items);
-        uint32_t all = 0, all_units = 0;
+        uint32_t all = 0, all_units = 0, longest = 0;
         for (uint32_t at = 0; at < n; at += 64) {
             uint32_t work, units;
-            of_lane(at, n, work, units);
+            const PagedSpan s = of_lane(at, n, work, units);
             all += __builtin_amdgcn_readlane(scan(work), 63);
             all_units += __builtin_amdgcn_readlane(scan(units), 63);
+            longest = max(longest, s.blocks);
         }
-        const PagedCut c = paged_cut(all, all_units, a.groups, a.least);
+        longest = most_of(longest);
+        const PagedCut c = paged_cut(all, all_units, longest, a.groups, a.least);
         share = c.share, pad = c.pad, total = pad ? share * a.groups : all;  // (of rounded runs: what lies past the last is nobody's)
     }
     // The item that block, unit or row x of the line belongs to; none if it is no item's, or of one that the launch does not take.

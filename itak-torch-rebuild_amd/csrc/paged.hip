@@ -181,8 +181,9 @@ itak_status check_attention(itak_paged *p, uint64_t layer, const itak_rows *q, c
 
 uint32_t shift_of(uint32_t power) { return uint32_t(__builtin_ctz(power)); }
 
-// Units and blocks of the items a launch takes, how their line is cut, and where in it inline items begin.
-itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work) {
+// Units and blocks of the items a launch takes, how their line is cut, and where in it inline items begin; `whole`: no unit is split.
+itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work, bool &whole) {
+    uint32_t longest = 0;
     auto each = [&](uint32_t pad, auto item) {
         uint64_t at = 0, units = 0;
         for (uint32_t i = 0; i < a.items; ++i) {
@@ -191,8 +192,10 @@ itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work) {
             item(i, at, units);
             if (vectors < a.v_from || vectors > a.v_to) continue;
             const uint64_t tiles = (vectors + a.tile - 1) / a.tile * a.g.kv_heads;
+            const uint32_t blocks = (it[0] + it[1] + 31) / 32 - paged_first_block(it[0], a.window);
             units += tiles;
-            at += tiles * paged_run((it[0] + it[1] + 31) / 32 - paged_first_block(it[0], a.window), pad);
+            at += tiles * paged_run(blocks, pad);
+            longest = std::max(longest, blocks);
         }
         item(a.items, at, units);
     };
@@ -200,9 +203,10 @@ itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work) {
     each(0, [&](uint32_t, uint64_t at, uint64_t u) { work = at, units = u; });
     if (work >= (1ull << 30) || units >= (1ull << 24)) return size_overflow(p->err, "blocks of the batch's attention");
     a.units = uint32_t(units);
-    if (!a.inline_items) return ITAK_OK;
     // (The kernel of many rows has no line.)
-    const PagedCut cut = a.parts ? PagedCut{} : paged_cut(uint32_t(work), a.units, a.groups, a.least);
+    const PagedCut cut = a.parts ? PagedCut{} : paged_cut(uint32_t(work), a.units, longest, a.groups, a.least);
+    whole = cut.pad >= longest;
+    if (!a.inline_items) return ITAK_OK;
     a.share = cut.share, a.pad = cut.pad;
     for (uint32_t i = 0; i < kPagedInline; ++i) a.start[i] = a.unit0[i] = ~0u;
     each(cut.pad, [&](uint32_t i, uint64_t at, uint64_t u) {
@@ -253,7 +257,8 @@ itak_status run_attention(itak_paged *p, uint64_t layer, const itak_rows &q, con
     a.group_magic = group > 1 ? uint32_t((1ull << 32) / group + ((1ull << 32) % group != 0)) : 0;
     if (uint64_t(a.rows) * group >= (1ull << 26)) return size_overflow(p->err, "query vectors of the batch");
     // (A call that is being captured is replayed over other batches.)
-    if (a.items <= kPagedInline && !capturing(p->stream)) {
+    const bool captured = capturing(p->stream);
+    if (a.items <= kPagedInline && !captured) {
         a.inline_items = a.items;
         for (PagedItemWords &w : a.item) w.row0 = ~0u;
         std::memcpy(a.item, p->batch.head.data() + kPagedItem0, a.items * sizeof(PagedItemWords));
@@ -283,6 +288,7 @@ itak_status run_attention(itak_paged *p, uint64_t layer, const itak_rows &q, con
             most_few = std::max(most_few, uint32_t(std::min<uint64_t>(vectors, few_most)));
     }
     itak_status st = ITAK_OK;
+    bool whole = false;
     if (most_few) {
         const uint32_t sets = most_few <= kPagedSet ? 1 : 2;
         a.tile = sets * kPagedSet;
@@ -292,14 +298,14 @@ itak_status run_attention(itak_paged *p, uint64_t layer, const itak_rows &q, con
         a.least = 4;
         a.parts = 0;
         uint64_t work = 0;
-        st = count_units(p, a, work);
+        st = count_units(p, a, work, whole);
         if (st == ITAK_OK) st = workspace(p, a, uint64_t(a.groups) + a.units, dp);
         if (st != ITAK_OK) return st;
         const hipError_t he = p->cfg.elem == ITAK_ELEM_F16
                                   ? (q.elem == ITAK_ELEM_F32 ? launch_paged_few_f16_f32 : launch_paged_few_f16)(sets, a, p->stream)
                                   : (q.elem == ITAK_ELEM_F32 ? launch_paged_few_bf16_f32 : launch_paged_few_bf16)(sets, a, p->stream);
         HIP_TRY(p, he, "launch paged attention of few rows");
-        HIP_TRY(p, launch_paged_merge(q.elem, a, p->stream), "launch the merge of paged attention");
+        if (captured || !whole) HIP_TRY(p, launch_paged_merge(q.elem, a, p->stream), "launch the merge of paged attention");
     }
     if (many) {
         a.tile = 32 * paged_chunk_waves(dp, q.elem);
@@ -307,7 +313,7 @@ itak_status run_attention(itak_paged *p, uint64_t layer, const itak_rows &q, con
         a.v_from = few_most + 1, a.v_to = ~0u;
         a.parts = 1;
         uint64_t work = 0;
-        st = count_units(p, a, work);
+        st = count_units(p, a, work, whole);
         if (st != ITAK_OK) return st;
         a.parts = chunk_parts(a.units, work, cus * paged_chunk_groups_per_cu(dp));
         if (a.parts > 1) {
