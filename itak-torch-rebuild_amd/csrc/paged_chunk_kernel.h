@@ -3,20 +3,24 @@
 // 4 d operations a pair of vector and position on the matrix pipe against an exponential, a multiply-add, half a maximum and a
 // conversion of it: the two are of one length, and what bounds the kernel is how far they run beside each other.
 //
-// A workgroup of four wavefronts owns a tile of one KV head; each wavefront keeps 32 * COLS of its vectors, queries and
-// accumulators in registers, and all four walk the tile's keys together in blocks of 32 that lie in LDS. Per block
+// A workgroup of eight wavefronts (four of f32 tensors and of 256 channels) owns a tile of one KV head; each wavefront keeps 32 of its
+// vectors, queries and accumulators in registers, and all walk the tile's keys together in blocks of 32 that lie in LDS. Per block
 //   S^T = K . Q^T, softmax in the lane's own column, O^T += V^T . P^T       (v_mfma_f32_32x32x16)
 // with S^T's rows dealt so that P stays in the registers the scores came in: a lane holds keys 16m + 8u + 4h + e (h = lane / 32) and
 // so must the product's other operand. That one is V row by row as the page has it, turned over on the way out of LDS
 // (ds_read_b64_tr_b16: sixteen lanes read four rows of sixteen channels and each gets four keys of one channel).
-// 64 vectors a wavefront read each block from LDS for 32 bytes a MFMA; with 32, LDS would be as busy as the matrix pipe.
+// The next block's scores are multiplied beside this block's exponentials, and this block's P.V beside the next one's maximum.
+// 32 vectors a wavefront and two wavefronts a SIMD, which fill each other's gaps: 64 vectors and one wavefront read half as much from LDS
+// and took 1,035 us where these take 959 to 980 (2,048 rows by 32 heads over 30,720 and themselves, 128 channels, f16: 1.07 TFLOP, 1.09 to
+// 1.11 PFLOP/s, where a library product of 8,192 cubed reaches 1.14). The matrix pipe is busy 64 % of the time at the 1.77 GHz that the
+// power leaves it; without its LDS reads and loads the loop would take some 800 us.
 //
 // Blocks travel from the pages to LDS without passing through registers (global_load_lds_dwordx4: lane i's 16 bytes go to
 // M0 + 16 i) into a ring of stages, whole rows at a time; the 16-byte pieces of a row are shuffled by the row's number on the way (the source
 // address is free per lane), so that neither the operand reads of K nor the turning reads of V meet a bank twice. A
-// load covers rows of one half of a block only, and pages hold at least 16 rows: its page is one scalar load, a block ahead.
+// load covers rows of one half of a block only, and pages hold at least 16 rows: it has one page, looked up 64 blocks at a time.
 //
-// The maximum is a reference that moves only when a score passes it by 2^8 (see the kernel of few rows).
+// The maximum is a reference that moves only when a score passes it by far (kWeightMost).
 #pragma once
 
 #include "paged_careful.h"
