@@ -40,7 +40,7 @@ decltype(&itak_paged_attention_device) paged_attention_fn;
 decltype(&itak_paged_step_device) paged_step_fn;
 PyTypeObject *cache_type;  // hip_compute.KvCache
 PyTypeObject *rows_type;   // paged.Rows
-PyObject *slot_name, *address_name;
+PyObject *slot_name, *address_name, *rows_name, *channels_name;
 
 // An exact int as ctypes takes it for an unsigned 64-bit argument or a pointer: modulo 2^64.
 bool plain_u64(PyObject *o, uint64_t &v) {
@@ -131,17 +131,24 @@ bool plain_array(PyObject *o, const float *&data, uint64_t &size) {
     data = size ? static_cast<const float *>(PyArray_DATA(a)) : nullptr;
     return true;
 }
-// A paged.Rows: where its itak_rows lies.
-bool plain_rows(PyObject *o, const itak_rows *&rows) {
-    if (Py_TYPE(o) != rows_type) return false;
-    PyObject *at = PyObject_GetAttr(o, address_name);
-    if (!at) {
+bool int_of(PyObject *o, PyObject *name, int64_t &v) {
+    PyObject *x = PyObject_GetAttr(o, name);
+    if (!x) {
         PyErr_Clear();
         return false;
     }
-    const bool ok = plain_ptr(at, rows) && rows;
-    Py_DECREF(at);
+    const bool ok = PyLong_CheckExact(x);
+    if (ok) v = int64_t(PyLong_AsUnsignedLongLongMask(x));
+    Py_DECREF(x);
     return ok;
+}
+// A paged.Rows of at least `need` rows of `head_dim` channels (or of a bare pointer, which says nothing of either): where its itak_rows lies.
+bool plain_rows(PyObject *o, uint64_t need, uint64_t head_dim, const itak_rows *&rows) {
+    int64_t at, have, channels;
+    if (Py_TYPE(o) != rows_type || !int_of(o, address_name, at) || !int_of(o, rows_name, have) || !int_of(o, channels_name, channels))
+        return false;
+    rows = reinterpret_cast<const itak_rows *>(uintptr_t(at));
+    return rows && (have < 0 || (uint64_t(have) >= need && uint64_t(channels) == head_dim));
 }
 // A C-contiguous run of 32-bit words.
 bool plain_words(PyObject *o, const void *&data, Py_ssize_t &n) {
@@ -308,7 +315,7 @@ PyObject *rotate(PyObject *, PyObject *const *a, Py_ssize_t n) {
         return not_plain();
     for (Py_ssize_t i = 0; i < ins; ++i) {
         const itak_rows *x, *y;
-        if (!plain_rows(in_at[i], x) || !plain_rows(out_at[i], y)) return not_plain();
+        if (!plain_rows(in_at[i], rows, head_dim, x) || !plain_rows(out_at[i], rows, head_dim, y)) return not_plain();
         in[i] = *x, out[i] = *y;
     }
     itak_status st;
@@ -360,15 +367,15 @@ PyObject *set_batch(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return PyLong_FromLong(st);
 }
 
-// append(paged, layer, k, v, rotation) -> status
+// append(paged, rows, head_dim, layer, k, v, rotation) -> status
 PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    if (!arity(n, 5)) return nullptr;
+    if (!arity(n, 7)) return nullptr;
     itak_paged *paged;
-    uint64_t layer;
+    uint64_t layer, rows, d;
     const itak_rows *k, *v;
     itak_rotation *rotation;
-    if (!plain_ptr(a[0], paged) || !plain_u64(a[1], layer) || !plain_rows(a[2], k) || !plain_rows(a[3], v) ||
-        !plain_ptr(a[4], rotation))
+    if (!plain_ptr(a[0], paged) || !plain_u64(a[1], rows) || !plain_u64(a[2], d) || !plain_u64(a[3], layer) ||
+        !plain_rows(a[4], rows, d, k) || !plain_rows(a[5], rows, d, v) || !plain_ptr(a[6], rotation))
         return not_plain();
     itak_status st;
     Py_BEGIN_ALLOW_THREADS
@@ -377,16 +384,17 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return PyLong_FromLong(st);
 }
 
-// paged_attention(paged, layer, q, out, scale, softcap, window, rotation) -> status
+// paged_attention(paged, rows, head_dim, layer, q, out, scale, softcap, window, rotation) -> status
 PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    if (!arity(n, 8)) return nullptr;
+    if (!arity(n, 10)) return nullptr;
     itak_paged *paged;
-    uint64_t layer, window;
+    uint64_t layer, window, rows, d;
     const itak_rows *q, *out;
     float scale, softcap;
     itak_rotation *rotation;
-    if (!plain_ptr(a[0], paged) || !plain_u64(a[1], layer) || !plain_rows(a[2], q) || !plain_rows(a[3], out) ||
-        !plain_scale(a[4], scale) || !plain_float(a[5], softcap) || !plain_u64(a[6], window) || !plain_ptr(a[7], rotation))
+    if (!plain_ptr(a[0], paged) || !plain_u64(a[1], rows) || !plain_u64(a[2], d) || !plain_u64(a[3], layer) ||
+        !plain_rows(a[4], rows, d, q) || !plain_rows(a[5], rows, d, out) || !plain_scale(a[6], scale) ||
+        !plain_float(a[7], softcap) || !plain_u64(a[8], window) || !plain_ptr(a[9], rotation))
         return not_plain();
     itak_status st;
     Py_BEGIN_ALLOW_THREADS
@@ -395,17 +403,18 @@ PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return PyLong_FromLong(st);
 }
 
-// paged_step(paged, layer, q, k, v, out, scale, softcap, window, rotation) -> status
+// paged_step(paged, rows, head_dim, layer, q, k, v, out, scale, softcap, window, rotation) -> status
 PyObject *paged_step(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    if (!arity(n, 10)) return nullptr;
+    if (!arity(n, 12)) return nullptr;
     itak_paged *paged;
-    uint64_t layer, window;
+    uint64_t layer, window, rows, d;
     const itak_rows *q, *k, *v, *out;
     float scale, softcap;
     itak_rotation *rotation;
-    if (!plain_ptr(a[0], paged) || !plain_u64(a[1], layer) || !plain_rows(a[2], q) || !plain_rows(a[3], k) ||
-        !plain_rows(a[4], v) || !plain_rows(a[5], out) || !plain_scale(a[6], scale) || !plain_float(a[7], softcap) ||
-        !plain_u64(a[8], window) || !plain_ptr(a[9], rotation))
+    if (!plain_ptr(a[0], paged) || !plain_u64(a[1], rows) || !plain_u64(a[2], d) || !plain_u64(a[3], layer) ||
+        !plain_rows(a[4], rows, d, q) || !plain_rows(a[5], rows, d, k) || !plain_rows(a[6], rows, d, v) ||
+        !plain_rows(a[7], rows, d, out) || !plain_scale(a[8], scale) || !plain_float(a[9], softcap) || !plain_u64(a[10], window) ||
+        !plain_ptr(a[11], rotation))
         return not_plain();
     itak_status st;
     Py_BEGIN_ALLOW_THREADS
@@ -464,5 +473,7 @@ PyMODINIT_FUNC PyInit__itak_front(void) {
     import_array();
     slot_name = PyUnicode_InternFromString("slot");
     address_name = PyUnicode_InternFromString("at");
-    return slot_name && address_name ? PyModule_Create(&module) : nullptr;
+    rows_name = PyUnicode_InternFromString("rows");
+    channels_name = PyUnicode_InternFromString("channels");
+    return slot_name && address_name && rows_name && channels_name ? PyModule_Create(&module) : nullptr;
 }

@@ -227,13 +227,15 @@ itak_status workspace(itak_paged *p, PagedAttn &a, uint64_t slots, uint32_t dp) 
 }
 
 // Parts of a unit's keys in the kernel of many rows: as many as fill the device, each part a workgroup that costs some blocks'
-// time beside its own.
+// time beside its own, and more where the merge has more than 64 of them to join (64 vectors over 20,000 16.7 us with 64 parts and 20.2
+// with 256, over 100,000, two of them, 44.3 with 64 and 34.1 with 128).
 uint32_t chunk_parts(uint32_t units, uint64_t work, uint32_t places) {
-    const double blocks = double(work) / units, extra = 8.0;
+    const double blocks = double(work) / units;
     uint32_t best = 1;
     double least = 1e300;
-    for (uint32_t s = 1; s <= 64 && s <= blocks / 2 + 1; ++s) {
-        const double rounds = std::ceil(double(units) * s / places), cost = rounds * (std::ceil(blocks / s) + (s > 1 ? extra : 0.0));
+    for (uint32_t s = 1; s <= 256 && s <= blocks / 2 + 1; ++s) {
+        const double extra = s > 64 ? 24.0 : s > 1 ? 8.0 : 0.0;
+        const double rounds = std::ceil(double(units) * s / places), cost = rounds * (std::ceil(blocks / s) + extra);
         if (cost < least * 0.97) least = cost, best = s;
         if (units * s > 2 * places) break;
     }

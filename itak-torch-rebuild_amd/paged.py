@@ -26,12 +26,14 @@ _NAN = math.nan
 class Rows:
     """A view of rows x heads x channels on the device (itak_rows): pointer, type, heads, strides in elements."""
 
-    __slots__ = ("raw", "ref", "at", "keep")
+    __slots__ = ("raw", "ref", "at", "rows", "channels", "keep")
 
-    def __init__(self, ptr: int, elem: str, heads: int, row_stride: int = 0, head_stride: int = 0, keep=None):
+    def __init__(self, ptr: int, elem: str, heads: int, row_stride: int = 0, head_stride: int = 0, keep=None, rows: int = -1,
+                 channels: int = -1):
         self.raw = N.Rows(ptr, _ELEMS[elem] if isinstance(elem, str) else elem, heads, row_stride, head_stride)
         self.ref = C.byref(self.raw)
         self.at = C.addressof(self.raw)  # the view as the front module takes it
+        self.rows, self.channels = rows, channels  # -1: of a pointer, as many as a call takes it for
         self.keep = keep  # what owns the memory
 
     @staticmethod
@@ -46,9 +48,17 @@ class Rows:
         row_stride, head_stride, channel_stride = tensor.stride()
         if channels > 1 and channel_stride != 1:
             raise ValueError("Rows.of: the channels of a head do not lie side by side")
+        if rows > 1 and heads > 1 and row_stride == 0 and head_stride == 0:  # (both zero stand for a dense view)
+            raise ValueError("Rows.of: the tensor is one head's channels expanded to all rows and heads")
         # (A stride that is never taken may be anything; written out, a single row of a single head is not taken for dense.)
         return Rows(tensor.data_ptr(), elem, heads, row_stride if rows > 1 else heads * max(head_stride, channels),
-                    head_stride if heads > 1 else channels, keep=tensor)
+                    head_stride if heads > 1 else channels, tensor, rows, channels)
+
+
+def _holds(views: Sequence[Rows], rows: int, channels: int) -> None:
+    for v in views:
+        if v.rows >= 0 and (v.rows < rows or v.channels != channels):
+            raise ValueError(f"a tensor of {v.rows} rows of {v.channels} channels where {rows} of {channels} are taken")
 
 
 def _turning(rotation: Optional["Rotation"]) -> Optional[C.c_void_p]:
@@ -106,6 +116,7 @@ class Rotation:
             n = len(inputs)
             if len(outputs) != n:
                 raise ValueError("rotate_device: as many outputs as inputs")
+            _holds((*inputs, *outputs), rows, head_dim)
             table = N.Rows * n
             status = self._lib.itak_rotate_device(_turning(self), stream, head_dim, rows, positions_ptr, table(*[r.raw for r in inputs]),
                                                   table(*[r.raw for r in outputs]), n, 1 if inverse else 0)
@@ -130,6 +141,8 @@ class PagedKv:
             _raise_last(None)
         self._h, self._hv = handle, handle.value
         self.page_rows = page_rows
+        self.head_dim = head_dim
+        self._rows = 0  # of the batch
 
     @staticmethod
     def _config(layers, num_kv_heads, head_dim, elem, page_rows, page_count, max_sequences=1, max_table_pages=0, device=0,
@@ -173,6 +186,7 @@ class PagedKv:
         status = hip_compute._front.set_batch(self._hv, items, pages)
         if status >= 0:
             self._done(status)
+            self._rows = sum([rows for _, rows in items])
             return
         n = len(items)
         if len(pages) != n:
@@ -194,11 +208,14 @@ class PagedKv:
                 ids.extend(table)
             ptr, count = ids.buffer_info()
         self._done(self._lib.itak_paged_set_batch(self._h, raw, n, ptr if count else None, count))
+        self._rows = sum(int(rows) for _, rows in items)
 
     def append_device(self, layer: int, k: Rows, v: Rows, rotation: Optional[Rotation] = None) -> None:
         """The batch's new rows into their pages, keys turned by their positions if `rotation` is given."""
-        status = hip_compute._front.append(self._hv, layer, k, v, 0 if rotation is None else rotation._hv)
+        status = hip_compute._front.append(self._hv, self._rows, self.head_dim, layer, k, v,
+                                           0 if rotation is None else rotation._hv)
         if status < 0:
+            _holds((k, v), self._rows, self.head_dim)
             status = self._lib.itak_paged_append_device(self._h, layer, k.ref, v.ref, _turning(rotation))
         if status:
             self._done(status)
@@ -206,9 +223,10 @@ class PagedKv:
     def attention_device(self, layer: int, q: Rows, out: Rows, *, scale: Optional[float] = None, softcap: float = 0.0,
                          window: int = 0, rotation: Optional[Rotation] = None) -> None:
         """Attention of the batch's new positions over pages that hold their rows already."""
-        status = hip_compute._front.paged_attention(self._hv, layer, q, out, scale, softcap, window,
+        status = hip_compute._front.paged_attention(self._hv, self._rows, self.head_dim, layer, q, out, scale, softcap, window,
                                                     0 if rotation is None else rotation._hv)
         if status < 0:
+            _holds((q, out), self._rows, self.head_dim)
             status = self._lib.itak_paged_attention_device(self._h, layer, q.ref, out.ref, _NAN if scale is None else scale, softcap,
                                                            window, _turning(rotation))
         if status:
@@ -217,9 +235,10 @@ class PagedKv:
     def attention_step_device(self, layer: int, q: Rows, k: Rows, v: Rows, out: Rows, *, scale: Optional[float] = None,
                               softcap: float = 0.0, window: int = 0, rotation: Optional[Rotation] = None) -> None:
         """Append the batch's new rows, then attend; queries and keys turned first if `rotation` is given."""
-        status = hip_compute._front.paged_step(self._hv, layer, q, k, v, out, scale, softcap, window,
+        status = hip_compute._front.paged_step(self._hv, self._rows, self.head_dim, layer, q, k, v, out, scale, softcap, window,
                                                0 if rotation is None else rotation._hv)
         if status < 0:
+            _holds((q, k, v, out), self._rows, self.head_dim)
             status = self._lib.itak_paged_step_device(self._h, layer, q.ref, k.ref, v.ref, out.ref, _NAN if scale is None else scale,
                                                       softcap, window, _turning(rotation))
         if status:

@@ -20,15 +20,15 @@ def test_only_plain_arguments_are_taken():
     f, P = front(), pkg()
     x = P.Rows(1 << 20, "f16", 2)
     ids = np.array([3, 1], np.uint32)
-    assert f.append(0, 0, x, x, 0) == REFUSED
-    assert f.paged_attention(0, 0, x, x, None, 0.0, 0, 0) == f.paged_attention(0, 0, x, x, 0.5, 0, 7, 0) == REFUSED
-    assert f.paged_step(0, 0, x, x, x, x, None, 0.0, 0, 0) == REFUSED
+    assert f.append(0, 1, 64, 0, x, x, 0) == REFUSED
+    assert f.paged_attention(0, 1, 64, 0, x, x, None, 0.0, 0, 0) == f.paged_attention(0, 1, 64, 0, x, x, 0.5, 0, 7, 0) == REFUSED
+    assert f.paged_step(0, 1, 64, 0, x, x, x, x, None, 0.0, 0, 0) == REFUSED
     assert f.set_batch(0, [(0, 1), (4, 2)], [ids, ids[:1]]) == f.set_batch(0, ((0, 1),), (ids.astype(np.int32),)) == f.set_batch(0, [], []) == REFUSED
     assert f.rotate(0, 0, 64, 1, 0, [x], (x,), False) == REFUSED
     for odd in (x.raw, None, 5):
-        assert f.append(0, 0, odd, x, 0) == f.paged_attention(0, 0, x, odd, None, 0.0, 0, 0) == -1
-        assert f.paged_step(0, 0, x, x, odd, x, None, 0.0, 0, 0) == f.rotate(0, 0, 64, 1, 0, [odd], [x], False) == -1
-    assert f.append(0, 0, x, x, None) == f.append(0, np.int64(0), x, x, 0) == -1  # (None: a rotation that is closed)
+        assert f.append(0, 1, 64, 0, odd, x, 0) == f.paged_attention(0, 1, 64, 0, x, odd, None, 0.0, 0, 0) == -1
+        assert f.paged_step(0, 1, 64, 0, x, x, odd, x, None, 0.0, 0, 0) == f.rotate(0, 0, 64, 1, 0, [odd], [x], False) == -1
+    assert f.append(0, 1, 64, 0, x, x, None) == f.append(0, 1, 64, np.int64(0), x, x, 0) == -1  # (None: a rotation that is closed)
     assert f.rotate(0, 0, 64, 1, 0, [x] * 5, [x] * 5, False) == f.rotate(0, 0, 64, 1, 0, [x], [], False) == f.rotate(0, 0, 64, 1, 0, [x], [x], 1) == -1
     for tables in ([[3, 1]], [ids.astype(np.int64)], [np.array([[3, 1]], np.uint32)], [np.arange(4, dtype=np.uint32)[::2]],
                    [ids.astype(">u4")], ids, [ids, ids], []):
@@ -36,8 +36,13 @@ def test_only_plain_arguments_are_taken():
     for items in ([[0, 1]], [(0, -1)], [(0, 1 << 32)], [(-1, 1)], [(np.int64(0), 1)], [(0, 1, 2)]):
         assert f.set_batch(0, items, [ids]) == -1
     assert f.set_batch(0, [(0, 1)] * 65, [ids] * 65) == -1
+    known = P.Rows(1 << 20, "f16", 2, 128, 64, rows=3, channels=64)  # of a tensor: how much there is of it is known
+    assert f.append(0, 3, 64, 0, known, x, 0) == f.append(0, 1, 64, 0, known, known, 0) == REFUSED
+    for rows, channels in ((4, 64), (3, 128), (3, 32)):
+        assert f.append(0, rows, channels, 0, x, known, 0) == f.paged_attention(0, rows, channels, 0, known, x, None, 0.0, 0, 0) == -1
+        assert f.paged_step(0, rows, channels, 0, x, x, x, known, None, 0.0, 0, 0) == f.rotate(0, 0, channels, rows, 0, [known], [x], False) == -1
     with pytest.raises(TypeError):
-        f.append(0, 0, x, x)
+        f.append(0, 1, 64, 0, x, x)
 
 
 @pytest.mark.gpu
@@ -86,6 +91,18 @@ def test_what_neither_way_can_mean_is_refused(monkeypatch, plain):
     cache.paged.set_batch([(5, 1)], cache.tables)
     before = cache.storage.clone()
     x, y, z = P.Rows.of(q), P.Rows.of(k), P.Rows.of(out)
+    two, wide = torch.zeros(2, 1, 64, device="cuda").half(), torch.zeros(1, 1, 128, device="cuda").half()
+    cache.paged.set_batch([(5, 2)], cache.tables)  # (of which the tensors above have one row)
+    for call in (lambda: cache.paged.append_device(0, y, P.Rows.of(two)),
+                 lambda: cache.paged.attention_device(0, x, P.Rows.of(two)),
+                 lambda: cache.paged.attention_step_device(0, P.Rows.of(two), P.Rows.of(two), y, P.Rows.of(two)),
+                 lambda: cache.paged.attention_device(0, P.Rows.of(two), P.Rows.of(wide)),
+                 lambda: P.Rotation(64).rotate_device([x], [z], 0, 2, 64),
+                 lambda: P.Rotation(64).rotate_device([x], [z], 0, 1, 128),
+                 lambda: P.Rows.of(torch.zeros(1, 1, 64, device="cuda").expand(3, 2, 64))):
+        with pytest.raises(ValueError):
+            call()
+    cache.paged.set_batch([(5, 1)], cache.tables)
     for call in (lambda: cache.paged.append_device(0, y, y, rotation),
                  lambda: cache.paged.attention_device(0, x, z, rotation=rotation),
                  lambda: cache.paged.attention_step_device(0, x, y, y, z, rotation=rotation),
