@@ -43,6 +43,19 @@ def test_many_sequences(count, kv_heads, q_heads, d, rows, pages, tensors):
     assert bool((out[total] == 5.0).all())
 
 
+# One KV head, so that a unit's keys are all the work there is: more parts of it than a wavefront of the merge has lanes.
+@pytest.mark.parametrize("q_heads,tensors", [(64, "f16"), (64, "f32"), (8, "f16")])
+def test_one_unit_in_many_parts(q_heads, tensors):
+    cache = filled([90001], kv_heads=1, d=64, page_rows=256, seed=q_heads)
+    q = cache.normal(1, q_heads, 64).to(PC.DTYPES[tensors])
+    qd = q.cuda()
+    out = torch.empty_like(qd)
+    cache.paged.set_batch([(90000, 1)], cache.tables)
+    cache.paged.attention_device(0, view(qd), view(out))
+    torch.cuda.synchronize()
+    check_attention(cache, 0, [(90000, 1)], q, out, tensors)
+
+
 def test_appends_of_many_sequences():
     items = [((53 * i) % 90, (i * 7) % 4) for i in range(150)]
     cache = PC.Cache(pkg(), [p + r for p, r in items], kv_heads=2, d=64, page_rows=16, max_sequences=150)
