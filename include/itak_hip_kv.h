@@ -755,8 +755,9 @@ itak_status itak_rotate_device(const itak_rotation *rotation, void *hip_stream, 
    the output once; with f32 tensors queries and weights enter the matrix pipe as several halves each,
    which leaves 2^-22 of them (bf16: 2^-24), over f16 pages at least 2^-29 of a query and 2^-37 of the largest weight. An f16 query's or key's channel beyond 65504 is infinite.
    A row that is not finite reaches the outputs of exactly the queries that see its position; one difference is left: a weight
-   below 2^-126 of its row's largest is zero, and zero times an infinite value is NaN. Tiles of queries that meet such
-   rows, and f32 queries beyond 4,094 over f16 pages, are computed twice, the second time without the matrix pipe: slowly.
+   below 2^-126 of its row's largest is zero, and zero times an infinite value is NaN. Finite values give finite outputs, up to the
+   ends of bf16. Tiles of queries that meet rows that are not finite or bf16 values from about 2^100 on, and f32 queries beyond 4,094
+   over f16 pages, are computed twice, the second time without the matrix pipe: slowly.
    Results do not depend on the pages' order or on what other sequences the batch holds beyond rounding (sums are cut
    into other pieces), and are the same from call to call.
 

@@ -2,8 +2,11 @@
 //
 // The kernels multiply whole tiles: a masked key's zero weight meets the key's value row, a query's pieces meet every key, and
 // 0 x inf is NaN where the row of a masked key is never read by the definition. That is looked for once, in a unit's result:
-// without an infinity or a NaN in its inputs none is NaN, and no infinity comes out other than as it should. A unit that holds
-// one is computed again here, row by row and key by key in f32, with nothing read that the row does not see.
+// without an infinity or a NaN in its inputs none is NaN. Over f16 pages no infinity comes out other than as it should either: 2^31
+// values up to 2^16 with weights up to 2^15 are 2^62. Values of bf16 end where f32 does, and a sum of them with weights up to 2^15
+// may pass that though the mean does not, so infinities are looked for as well. A unit that holds
+// one is computed again here, row by row and key by key in f32, with nothing read that the row does not see, and
+// so scaled that no sum leaves f32's range.
 #pragma once
 
 #include "paged_mfma.h"
@@ -16,7 +19,18 @@ __device__ __forceinline__ float lane_of(float x, uint32_t lane) {
     return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane));
 }
 
-// A wavefront's vectors of v0 .. v_end over the keys [key0, key1): WRITE(vector, accumulators of channels 64 c + lane, maximum in
+// Whether a unit is to be computed here: by a sum over what it gave.
+template <int PAGE>
+__device__ __forceinline__ bool to_be_done_over(float check) {
+    return PAGE == ITAK_ELEM_F16 ? check != check : !(__builtin_fabsf(check) < INFINITY);
+}
+
+// What comes out has its reference so far above the largest score (log2 domain): 2^31 values below 2^128 with weights up to 2^-32 stay
+// below 2^127. The factor goes to the values: a weight that it made zero would make an infinite value NaN. (Over f16 pages there is no need.)
+template <int PAGE>
+constexpr float kCarefulDrop = PAGE == ITAK_ELEM_F16 ? 0.0f : 32.0f;
+
+// A wavefront's vectors of v0 .. v_end over the keys [key0, key1): WRITE(vector, accumulators of channels 64 c + lane, reference in
 // the log2 domain, sum). kCareful vectors at once, so that a row is fetched once for them, and 64 keys: a lane has the scores
 // of one key; then the lanes are channels.
 constexpr uint32_t kCareful = 4;
@@ -27,6 +41,7 @@ __device__ __forceinline__ void paged_careful(const PagedAttn &a, const PagedSpa
     typedef typename Elem<PAGE>::type P;
     constexpr int kRuns = DP / 64;
     constexpr uint32_t kAtOnce = 8;
+    constexpr float kDown = PAGE == ITAK_ELEM_F16 ? 1.0f : 0x1p-32f;  // 2^-kCarefulDrop
     const uint32_t lane = __lane_id(), d = a.g.head_dim, page_mask = (1u << a.g.page_shift) - 1;
     const P *const base = reinterpret_cast<const P *>(a.layer_base) + head * a.g.head_stride;
     const uint32_t *ids = a.batch + span.table;
@@ -91,7 +106,7 @@ __device__ __forceinline__ void paged_careful(const PagedAttn &a, const PagedSpa
                     const uint64_t high = uint32_t(__builtin_amdgcn_readlane(uint32_t(row_at >> 32), j + t));
                     const P *value = reinterpret_cast<const P *>(high << 32 | low);
 #pragma unroll
-                    for (int c = 0; c < kRuns; ++c) y[t][c] = 64 * c + lane < d ? Elem<PAGE>::to_f32(value[64 * c + lane]) : 0.0f;
+                    for (int c = 0; c < kRuns; ++c) y[t][c] = 64 * c + lane < d ? Elem<PAGE>::to_f32(value[64 * c + lane]) * kDown : 0.0f;
                 }
 #pragma unroll
                 for (uint32_t t = 0; t < kKeys; ++t)
@@ -110,7 +125,7 @@ __device__ __forceinline__ void paged_careful(const PagedAttn &a, const PagedSpa
         for (uint32_t u = 0; u < kCareful; ++u) {
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) sum[u] += __shfl_xor(sum[u], o);
-            if (v + u < v_end) write(v + u, acc[u], m[u], sum[u]);
+            if (v + u < v_end) write(v + u, acc[u], m[u] + kCarefulDrop<PAGE>, sum[u] * kDown);
         }
     }
 }

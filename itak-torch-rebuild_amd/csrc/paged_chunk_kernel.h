@@ -248,7 +248,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
             const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
             const float m = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
             const bool live = threshold != -INFINITY;
-            float delta = live ? fmaxf(m - kWeightLift, 0.0f) : m - kWeightLift;
+            float delta = live ? fmaxf(m - kWeightLift<PAGE>, 0.0f) : m - kWeightLift<PAGE>;
             if (m == -INFINITY) delta = 0.0f;
             const float alpha = live ? fast_exp2(-delta) : 1.0f;
             ref += delta;
@@ -432,7 +432,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
 #pragma unroll
         for (int r = 0; r < 16; ++r) check[r % 4] += EXACT || 32u * t + 8 * (r / 4) + 4 * h < d ? o[t][r] : 0.0f;
     const float all = (check[0] + check[1]) + (check[2] + check[3]);
-    if (any_of_group(mine && all != all, &lds_flag)) {
+    if (any_of_group(mine && to_be_done_over<PAGE>(all), &lds_flag)) {
         paged_careful<PAGE, ELEM, DP>(a, span, head, v0, min(v0 + kTile, vectors), wave, kWaves, 32 * kb0, 32 * kb_end,
                                       [&](uint32_t v, const float (&acc)[DP / 64], float m, float l) {
                                           paged_write_careful<ELEM, DP>(a, span, head, v, whole, slot0 + v - v0, true, acc, m, l);

@@ -245,7 +245,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
                 if (__builtin_amdgcn_ballot_w64(most > threshold[n]) != 0) {
                     const float m = max_over_groups(most);
                     const bool live = threshold[n] != -INFINITY;
-                    float delta = live ? fmaxf(m - kWeightLift, 0.0f) : m - kWeightLift;
+                    float delta = live ? fmaxf(m - kWeightLift<PAGE>, 0.0f) : m - kWeightLift<PAGE>;
                     if (m == -INFINITY) delta = 0.0f;
                     const float alpha = live ? fast_exp2(-delta) : 1.0f;
                     ref[n] += delta;
@@ -355,7 +355,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
                 float check = all;
 #pragma unroll
                 for (int c = 0; c < kChunk; ++c) check += EXACT || c0 + c < d ? acc[c] : 0.0f;
-                bad = bad || check != check;
+                bad = bad || to_be_done_over<PAGE>(check);
                 if (whole) {
                     const float inv = 1.0f / all;
                     const uint32_t row = paged_row_of(a, v), hq = head * a.group + v - row * a.group;

@@ -1,4 +1,5 @@
-// Joins the partials of units that several workgroups shared: out = sum_w 2^(m_w - m) acc_w / sum_w 2^(m_w - m) l_w.
+// Joins the partials of units that several workgroups shared: out = sum_w 2^(m_w - m) acc_w / sum_w 2^(m_w - m) l_w. Weights are divided by the
+// sum before they meet the accumulators: acc_w / l_w is a mean of values, and no sum of the parts leaves f32's range if they do not.
 //
 // A workgroup serves one query head's row. Its unit's place in the line of blocks gives the workgroups that had a part of it, and so
 // their slots. All loads go out before anything waits: maxima and sums a lane each, accumulators (a float4 a thread and
@@ -52,7 +53,6 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttn a) {
     // (A maximum of minus infinity: nothing visible, a sum of 0, or scores that are no numbers, which the sum then is.)
     auto weight_of = [](float2 x, float m) { return x.x == -INFINITY ? 0.0f : fast_exp2(x.x - m); };
     auto sum_of = [](float2 x, float weight) { return x.x == -INFINITY ? x.y : weight * x.y; };
-    float total;
     floatx4 acc = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     if (parts <= 64) {
         // Every wavefront has all of them, one a lane.
@@ -71,11 +71,11 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttn a) {
         l += dpp_lane<0x4E>(l);
         l += dpp_lane<0x141>(l);
         l += dpp_lane<0x140>(l);
-        total = sum_over_groups(l);
+        const float share = weight * (1.0f / sum_over_groups(l));
         const uint32_t most = 64 / kLanes;  // of a thread's
 #pragma unroll
         for (uint32_t u = 0; u < most; ++u) {
-            const float w = __shfl(weight, part + u * kLanes);
+            const float w = __shfl(share, part + u * kLanes);
             if (u >= kAtOnce && u * kLanes >= parts) break;
             const floatx4 x = u < kAtOnce ? early[u] : acc_of(min(part + u * kLanes, parts - 1));
             if (part + u * kLanes < parts) acc += x * w;
@@ -105,11 +105,11 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttn a) {
         for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
         if ((tid & 63) == 0) lds_l[tid >> 6] = l;
         __syncthreads();
-        total = (lds_l[0] + lds_l[1]) + (lds_l[2] + lds_l[3]);
+        const float inv = 1.0f / ((lds_l[0] + lds_l[1]) + (lds_l[2] + lds_l[3]));
 #pragma unroll
         for (int u = 0; u < kAtOnce; ++u)
-            if (part + u * kLanes < parts) acc += early[u] * weights[part + u * kLanes];
-        for (uint32_t w = part + kAtOnce * kLanes; w < parts; w += kLanes) acc += acc_of(w) * weights[w];
+            if (part + u * kLanes < parts) acc += early[u] * (weights[part + u * kLanes] * inv);
+        for (uint32_t w = part + kAtOnce * kLanes; w < parts; w += kLanes) acc += acc_of(w) * (weights[w] * inv);
     }
     lds[part][quad] = acc;
     __syncthreads();
@@ -117,13 +117,12 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttn a) {
     floatx4 sum = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int p = 0; p < kLanes; ++p) sum += lds[p][tid];
-    const float inv = 1.0f / total;
     const uint32_t c = tid * 4;
     if (c >= a.g.head_dim) return;
     T *dst = static_cast<T *>(a.out.data) + uint64_t(row) * a.out.row_stride + hq * a.out.head_stride + c;
     Piece<T, 4> y;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y.v[e] = Elem<ELEM>::from_f32(sum[e] * inv);
+    for (int e = 0; e < 4; ++e) y.v[e] = Elem<ELEM>::from_f32(sum[e]);
     if (a.out_on_16) {
         *reinterpret_cast<Piece<T, 4> *>(dst) = y;
     } else {

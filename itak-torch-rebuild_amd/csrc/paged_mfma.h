@@ -19,10 +19,13 @@ __device__ __forceinline__ floatx4 mfma_16x16x32(u32x4 a, u32x4 b, floatx4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bfloat8, a), __builtin_bit_cast(bfloat8, b), c, 0, 0, 0);
 }
 
-// A row's reference is kept 12 below its largest score (log2 domain): weights are up to 2^15, where f16 ends at 2^16, so that of f16
-// pieces those down to 2^-26 of the largest keep their precision and what is lost of a smaller one is 2^-37 of the largest. It
+// Over f16 pages a row's reference is kept 12 below its largest score (log2 domain): weights are up to 2^15, where f16 ends at 2^16, so that of
+// f16 pieces those down to 2^-26 of the largest keep their precision and what is lost of a smaller one is 2^-37 of the largest. bf16
+// has f32's range and values of it may end where the accumulators do: no lift. The reference
 // moves only when a score passes it by more than 15: the rescaling of the accumulators then leaves the common path.
-constexpr float kWeightLift = 12.0f, kWeightMost = 15.0f;
+template <int PAGE>
+constexpr float kWeightLift = PAGE == ITAK_ELEM_F16 ? 12.0f : 0.0f;
+constexpr float kWeightMost = 15.0f;
 // f32 queries enter f16 products times 16, and the scale makes up for it: f16 ends at 2^-24 below, and a query's last bits do
 // then at 2^-28. (One beyond 4,094 is infinite to the products and is done over in f32, as all that is not finite.)
 template <int PAGE, int ELEM>
