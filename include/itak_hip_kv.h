@@ -818,7 +818,8 @@ itak_status itak_paged_append_device(itak_paged *paged, uint64_t layer, const it
    position p = item.position + r over max(0, p + 1 - window) .. p (window 0: from 0 on). q and out are
    [sum rows][heads][head_dim] of the same type, heads a multiple of num_kv_heads (at most 64 times as many); with `rotation` the queries are
    turned by their positions first (a type of 16 bits is rounded once more for it). scale = NaN selects 1/sqrt(head_dim);
-   softcap > 0 caps each scaled score as cap*tanh(s/cap), 0 disables it. */
+   softcap > 0 caps each scaled score as cap*tanh(s/cap), 0 disables it; refused are caps so small that scale / softcap is infinite and so
+   large, from some 10^36 on at ordinary scales, that it is below f32's normal numbers. */
 itak_status itak_paged_attention_device(itak_paged *paged, uint64_t layer, const itak_rows *q, const itak_rows *out,
                                         float scale, float softcap, uint64_t window, const itak_rotation *rotation);
 /* The two in turn: append, then attend, with queries and keys rotated in the append's launch. */

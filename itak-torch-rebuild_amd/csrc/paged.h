@@ -9,6 +9,11 @@ namespace itak {
 
 constexpr float kPagedLog2e = 1.4426950408889634f;
 constexpr float kPagedQueryLift = 16.0f;  // paged_mfma.h
+constexpr float kPagedCapShort = 256.0f * kPagedLog2e;  // paged_mfma.h
+// Whether capped scores are worked out by the series (`cap_log2` > 0).
+__host__ __device__ constexpr bool paged_cap_by_series(uint32_t elem, float cap_log2) {
+    return elem == ITAK_ELEM_F32 || cap_log2 > kPagedCapShort;
+}
 
 // Strides in elements; side = keys or values of a page, all its heads.
 struct PagedGeom {

@@ -5,6 +5,7 @@
 #include "errors.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstring>
 #include <new>
@@ -163,6 +164,13 @@ uint16_t *layer_base(const itak_paged *p, uint64_t layer) {
     return reinterpret_cast<uint16_t *>(p->storage) + layer * p->layer_stride;
 }
 
+// What the kernels multiply products by: to scores in the log2 domain, with a softcap to the argument of its exponential.
+float score_scale(const itak_paged *p, uint32_t elem, float scale, float softcap) {
+    const float s = std::isnan(scale) ? 1.0f / std::sqrt(float(p->cfg.head_dim)) : scale;
+    const float x = softcap > 0.0f ? s * (2.0f * kPagedLog2e / softcap) : s * kPagedLog2e;
+    return p->cfg.elem == ITAK_ELEM_F16 && elem == ITAK_ELEM_F32 ? x / kPagedQueryLift : x;
+}
+
 itak_status check_attention(itak_paged *p, uint64_t layer, const itak_rows *q, const itak_rows *out, float scale, float softcap) {
     itak_status st = check_layer(p, layer);
     if (st == ITAK_OK) st = check_tensor(p, "q", q, 0, ~0u, false);
@@ -174,8 +182,14 @@ itak_status check_attention(itak_paged *p, uint64_t layer, const itak_rows *q, c
     if (q->heads > 65535) return unsupported(p->err, "more than 65535 query heads");
     if (std::isinf(scale)) return invalid_argument(p->err, "scale is infinite");
     if (!(softcap >= 0.0f) || std::isinf(softcap)) return invalid_argument(p->err, "softcap must be finite and >= 0");
-    if (softcap > 0.0f && std::isinf((std::isnan(scale) ? 1.0f : scale) * (2.0f * kPagedLog2e / softcap)))
-        return unsupported(p->err, "a softcap so small that scale / softcap is infinite");
+    if (softcap > 0.0f) {
+        const float cap_scale = score_scale(p, q->elem, scale, softcap);
+        if (!std::isfinite(cap_scale)) return unsupported(p->err, "a softcap so small that scale / softcap is infinite");
+        // (Of smaller caps such a scale makes the scores zero.)
+        if (softcap > 0x1p24f && cap_scale != 0.0f && std::fabs(cap_scale) < FLT_MIN)
+            return unsupported(p->err, "a softcap so large that scale / softcap is none of f32's normal numbers");
+        if (std::isinf(softcap * kPagedLog2e)) return unsupported(p->err, "a softcap beyond 2e38");
+    }
     return ITAK_OK;
 }
 
@@ -267,9 +281,7 @@ itak_status run_attention(itak_paged *p, uint64_t layer, const itak_rows &q, con
     }
     a.q_on_16 = rows_on_16(q, d);
     a.out_on_16 = rows_on_16(out, d);
-    const float s = std::isnan(scale) ? 1.0f / std::sqrt(float(d)) : scale;
-    a.scale_log2 = softcap > 0.0f ? s * (2.0f * kPagedLog2e / softcap) : s * kPagedLog2e;
-    if (p->cfg.elem == ITAK_ELEM_F16 && q.elem == ITAK_ELEM_F32) a.scale_log2 /= kPagedQueryLift;
+    a.scale_log2 = score_scale(p, q.elem, scale, softcap);
     a.cap_log2 = softcap * kPagedLog2e;
     a.window = uint32_t(std::min<uint64_t>(window, 1ull << 31));
     a.zeros = p->batch_dev + p->zeros_at;

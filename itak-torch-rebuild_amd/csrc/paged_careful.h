@@ -83,7 +83,7 @@ __device__ __forceinline__ void paged_careful(const PagedAttn &a, const PagedSpa
             for (uint32_t u = 0; u < kCareful; ++u) {
                 every = every && at >= lo[u] && at + n <= hi[u];
                 x[u] *= a.scale_log2 * kQueryLift<PAGE, ELEM>;
-                if (a.cap_log2 != 0.0f) x[u] = softcapped<ELEM>(x[u], a.cap_log2, 0.0f);
+                if (a.cap_log2 != 0.0f) x[u] = softcapped<true>(x[u], a.cap_log2, 0.0f);
                 const bool seen = lane < n && key >= lo[u] && key < hi[u];
                 float most = seen ? fmaxf(m[u], x[u]) : m[u];
 #pragma unroll

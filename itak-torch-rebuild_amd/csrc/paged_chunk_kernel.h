@@ -59,7 +59,9 @@ constexpr int chunk_subs(int dp) { return dp <= 128 ? 2 : 1; }
 constexpr int chunk_stages(int dp) { return dp == 256 ? 4 : 4; }
 constexpr size_t chunk_lds(int dp) { return size_t(chunk_stages(dp)) * chunk_subs(dp) * 2 * 32 * 2 * dp; }
 
-template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP, bool CAP>
+// Scores without a cap, capped by the short form, capped by the series (paged_cap_by_series).
+enum ChunkCap { kNoCap, kShortCap, kSeriesCap };
+template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP, ChunkCap CAP>
 __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_kernel(PagedAttn a) {
     typedef typename Elem<ELEM>::type T;
     constexpr int kWaves = paged_chunk_waves(DP, ELEM);
@@ -227,8 +229,8 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     // A lane's scores of a block, relative to the reference.
     floatx16 x;
     auto scaled = [&](float s) {
-        if constexpr (CAP)
-            return softcapped<ELEM>(s * a.scale_log2, a.cap_log2, ref);
+        if constexpr (CAP != kNoCap)
+            return softcapped<CAP == kSeriesCap>(s * a.scale_log2, a.cap_log2, ref);
         else
             return __builtin_fmaf(s, a.scale_log2, -ref);
     };
@@ -483,8 +485,10 @@ hipError_t launch_chunk_as(const PagedAttn &a, hipStream_t stream) {
         launch_kernel(kernel, a.units * a.parts, paged_chunk_waves(DP, ELEM) * 64, chunk_lds(DP), stream, a);
         return hipGetLastError();
     };
-    return a.cap_log2 != 0.0f ? run(paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, true>)
-                              : run(paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, false>);
+    if (a.cap_log2 == 0.0f) return run(paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kNoCap>);
+    if constexpr (ELEM != ITAK_ELEM_F32)
+        if (!paged_cap_by_series(ELEM, a.cap_log2)) return run(paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kShortCap>);
+    return run(paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kSeriesCap>);
     }
 }
 template <int PAGE, int ELEM, int NQ, int NP>

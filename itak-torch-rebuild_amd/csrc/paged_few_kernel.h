@@ -226,8 +226,13 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
                     for (int r = 0; r < 4; ++r) x[4 * t + r] = s[r];
                 }
                 if (a.cap_log2 != 0.0f) {
+                    if (paged_cap_by_series(ELEM, a.cap_log2)) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = softcapped<ELEM>(x[e] * a.scale_log2, a.cap_log2, ref[n]);
+                        for (int e = 0; e < 8; ++e) x[e] = softcapped<true>(x[e] * a.scale_log2, a.cap_log2, ref[n]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = softcapped<false>(x[e] * a.scale_log2, a.cap_log2, ref[n]);
+                    }
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf(x[e], a.scale_log2, -ref[n]);

@@ -111,12 +111,13 @@ __device__ __forceinline__ float sum_over_groups(float v) {
     return __uint_as_float(c[0]) + __uint_as_float(c[1]);
 }
 
-// A capped score relative to `shift`: c tanh(y) - shift, y = a ln 2 / 2, in the log2 domain (softcap_of_exp2_arg). Of f32 tensors
-// a small score is to be as exact as one without a cap, where 1 - 2 / (2^a + 1) leaves 2^-24 of the cap: up to |y| = 0.45 the
-// series y (1 - y^2 / 3 + 2 y^4 / 15 - ..) to y^13, whose next term is below 2^-25 of the value.
-template <int ELEM>
+// A capped score relative to `shift`: c tanh(y) - shift, y = a ln 2 / 2, in the log2 domain (softcap_of_exp2_arg). Where a small score is
+// to be as exact as one without a cap (SERIES), and 1 - 2 / (2^a + 1) leaves some 2^-23 of the cap: up to |y| = 0.45 the
+// series y (1 - y^2 / 3 + 2 y^4 / 15 - ..) to y^13, whose next term is below 2^-25 of the value. That is for f32 tensors, and of 16 bits for
+// caps beyond kPagedCapShort, below which the short form's error is a tenth of what a weight's rounding to f16 takes.
+template <bool SERIES>
 __device__ __forceinline__ float softcapped(float a, float c, float shift) {
-    if constexpr (ELEM != ITAK_ELEM_F32) return softcap_of_exp2_arg(a, c, shift);
+    if constexpr (!SERIES) return softcap_of_exp2_arg(a, c, shift);
     const float y = a * 0.34657359f, z = y * y;
     float p = __builtin_fmaf(z, 21844.0f / 6081075.0f, -1382.0f / 155925.0f);
     p = __builtin_fmaf(z, p, 62.0f / 2835.0f);
