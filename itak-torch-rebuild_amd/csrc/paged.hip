@@ -230,13 +230,27 @@ itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work, bool &whole
     return ITAK_OK;
 }
 
-itak_status workspace(itak_paged *p, PagedAttn &a, uint64_t slots, uint32_t dp) {
-    const uint64_t acc = slots * a.tile * dp * sizeof(float);
+// What a call's attention launches: found out, and its memory had, before the call enqueues anything.
+struct AttnPlan {
+    PagedAttn few{}, many{};
+    uint32_t sets = 0;       // of the kernel of few rows; 0: it has no items
+    bool merge_few = false;
+    bool has_many = false;
+};
+
+// The partials of both launches lie in one place: they run one after the other.
+itak_status workspace(itak_paged *p, AttnPlan &plan, uint32_t dp) {
+    auto slots = [](const PagedAttn &a) { return a.parts ? (a.parts > 1 ? uint64_t(a.units) * a.parts : 0) : uint64_t(a.groups) + a.units; };
+    auto sums = [&](const PagedAttn &a) { return slots(a) * a.tile * dp * sizeof(float); };
+    uint64_t need = 0;
+    for (const PagedAttn *a : {&plan.few, &plan.many}) need = std::max(need, sums(*a) + slots(*a) * a->tile * sizeof(float2));
     void *ws = p->ws;
-    const itak_status st = grow(p, &ws, &p->ws_bytes, acc + slots * a.tile * sizeof(float2), "split workspace");
+    const itak_status st = grow(p, &ws, &p->ws_bytes, need, "split workspace");
     p->ws = static_cast<float *>(ws);
-    a.ws_acc = p->ws;
-    a.ws_ml = reinterpret_cast<float2 *>(reinterpret_cast<unsigned char *>(p->ws) + acc);
+    for (PagedAttn *a : {&plan.few, &plan.many}) {
+        a->ws_acc = p->ws;
+        a->ws_ml = reinterpret_cast<float2 *>(reinterpret_cast<unsigned char *>(p->ws) + sums(*a));
+    }
     return st;
 }
 
@@ -257,11 +271,11 @@ uint32_t chunk_parts(uint32_t units, uint64_t work, uint32_t places) {
 }
 
 // q is as it attends: turned where it has to be.
-itak_status run_attention(itak_paged *p, uint64_t layer, const itak_rows &q, const itak_rows &out, float scale, float softcap,
-                          uint64_t window) {
+itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, const itak_rows &out, float scale, float softcap,
+                           uint64_t window, AttnPlan &plan) {
     const uint32_t d = uint32_t(p->cfg.head_dim);
     const uint32_t group = uint32_t(q.heads / p->cfg.num_kv_heads);
-    PagedAttn a{};
+    PagedAttn &a = plan.few;
     a.g = p->g;
     a.batch = p->batch_dev;
     a.layer_base = layer_base(p, layer);
@@ -301,44 +315,49 @@ itak_status run_attention(itak_paged *p, uint64_t layer, const itak_rows &q, con
         else
             most_few = std::max(most_few, uint32_t(std::min<uint64_t>(vectors, few_most)));
     }
-    itak_status st = ITAK_OK;
     bool whole = false;
+    uint64_t work = 0;
+    if (many) {
+        PagedAttn &b = plan.many = a;
+        plan.has_many = true;
+        b.tile = 32 * paged_chunk_waves(dp, q.elem);
+        b.tile_shift = shift_of(b.tile);
+        b.v_from = few_most + 1, b.v_to = ~0u;
+        b.parts = 1;
+        const itak_status st = count_units(p, b, work, whole);
+        if (st != ITAK_OK) return st;
+        b.parts = chunk_parts(b.units, work, cus * paged_chunk_groups_per_cu(dp));
+    }
     if (most_few) {
-        const uint32_t sets = most_few <= kPagedSet ? 1 : 2;
-        a.tile = sets * kPagedSet;
+        plan.sets = most_few <= kPagedSet ? 1 : 2;
+        a.tile = plan.sets * kPagedSet;
         a.tile_shift = shift_of(a.tile);
         a.v_from = 1, a.v_to = chunks ? few_most : ~0u;
-        a.groups = std::min(cus * paged_few_groups_per_cu(dp, p->cfg.elem, q.elem, sets), kPagedMostParts);
+        a.groups = std::min(cus * paged_few_groups_per_cu(dp, p->cfg.elem, q.elem, plan.sets), kPagedMostParts);
         a.least = 4;
         a.parts = 0;
-        uint64_t work = 0;
-        st = count_units(p, a, work, whole);
-        if (st == ITAK_OK) st = workspace(p, a, uint64_t(a.groups) + a.units, dp);
+        const itak_status st = count_units(p, a, work, whole);
         if (st != ITAK_OK) return st;
-        const hipError_t he = p->cfg.elem == ITAK_ELEM_F16
-                                  ? (q.elem == ITAK_ELEM_F32 ? launch_paged_few_f16_f32 : launch_paged_few_f16)(sets, a, p->stream)
-                                  : (q.elem == ITAK_ELEM_F32 ? launch_paged_few_bf16_f32 : launch_paged_few_bf16)(sets, a, p->stream);
-        HIP_TRY(p, he, "launch paged attention of few rows");
-        if (captured || !whole) HIP_TRY(p, launch_paged_merge(q.elem, a, p->stream), "launch the merge of paged attention");
+        plan.merge_few = captured || !whole;
     }
-    if (many) {
-        a.tile = 32 * paged_chunk_waves(dp, q.elem);
-        a.tile_shift = shift_of(a.tile);
-        a.v_from = few_most + 1, a.v_to = ~0u;
-        a.parts = 1;
-        uint64_t work = 0;
-        st = count_units(p, a, work, whole);
-        if (st != ITAK_OK) return st;
-        a.parts = chunk_parts(a.units, work, cus * paged_chunk_groups_per_cu(dp));
-        if (a.parts > 1) {
-            st = workspace(p, a, uint64_t(a.units) * a.parts, dp);
-            if (st != ITAK_OK) return st;
-        }
+    return workspace(p, plan, dp);
+}
+
+itak_status run_attention(itak_paged *p, uint32_t elem, const AttnPlan &plan) {
+    if (plan.sets) {
+        const hipError_t he =
+            p->cfg.elem == ITAK_ELEM_F16
+                ? (elem == ITAK_ELEM_F32 ? launch_paged_few_f16_f32 : launch_paged_few_f16)(plan.sets, plan.few, p->stream)
+                : (elem == ITAK_ELEM_F32 ? launch_paged_few_bf16_f32 : launch_paged_few_bf16)(plan.sets, plan.few, p->stream);
+        HIP_TRY(p, he, "launch paged attention of few rows");
+        if (plan.merge_few) HIP_TRY(p, launch_paged_merge(elem, plan.few, p->stream), "launch the merge of paged attention");
+    }
+    if (plan.has_many) {
         const hipError_t he = p->cfg.elem == ITAK_ELEM_F16
-                                  ? (q.elem == ITAK_ELEM_F32 ? launch_paged_chunk_f16_f32 : launch_paged_chunk_f16)(a, p->stream)
-                                  : (q.elem == ITAK_ELEM_F32 ? launch_paged_chunk_bf16_f32 : launch_paged_chunk_bf16)(a, p->stream);
+                                  ? (elem == ITAK_ELEM_F32 ? launch_paged_chunk_f16_f32 : launch_paged_chunk_f16)(plan.many, p->stream)
+                                  : (elem == ITAK_ELEM_F32 ? launch_paged_chunk_bf16_f32 : launch_paged_chunk_bf16)(plan.many, p->stream);
         HIP_TRY(p, he, "launch paged attention of many rows");
-        if (a.parts > 1) HIP_TRY(p, launch_paged_merge(q.elem, a, p->stream), "launch the merge of paged attention");
+        if (plan.many.parts > 1) HIP_TRY(p, launch_paged_merge(elem, plan.many, p->stream), "launch the merge of paged attention");
     }
     return ITAK_OK;
 }
@@ -558,12 +577,11 @@ itak_status itak_paged_attention_device(itak_paged *paged, uint64_t layer, const
     HIP_TRY(paged, scope.status(), "set the device");
     try {
         itak_rows turned = *q;
-        if (rotation) {
-            st = turned_rows(paged, *q, turned);
-            if (st == ITAK_OK) st = run_append_queries(paged, *q, turned, rotation);
-            if (st != ITAK_OK) return st;
-        }
-        return run_attention(paged, layer, turned, *out, scale, softcap, window);
+        AttnPlan plan;
+        if (rotation) st = turned_rows(paged, *q, turned);
+        if (st == ITAK_OK) st = plan_attention(paged, layer, turned, *out, scale, softcap, window, plan);
+        if (st == ITAK_OK && rotation) st = run_append_queries(paged, *q, turned, rotation);
+        return st == ITAK_OK ? run_attention(paged, q->elem, plan) : st;
     } catch (const std::bad_alloc &) {
         return invalid_argument(paged->err, "out of host memory");
     }
@@ -582,11 +600,11 @@ itak_status itak_paged_step_device(itak_paged *paged, uint64_t layer, const itak
     HIP_TRY(paged, scope.status(), "set the device");
     try {
         itak_rows turned = *q;
+        AttnPlan plan;
         if (rotation) st = turned_rows(paged, *q, turned);
-        if (st != ITAK_OK) return st;
-        st = run_append(paged, layer, *k, *v, rotation, rotation ? q : nullptr, &turned);
-        if (st != ITAK_OK) return st;
-        return run_attention(paged, layer, turned, *out, scale, softcap, window);
+        if (st == ITAK_OK) st = plan_attention(paged, layer, turned, *out, scale, softcap, window, plan);
+        if (st == ITAK_OK) st = run_append(paged, layer, *k, *v, rotation, rotation ? q : nullptr, &turned);
+        return st == ITAK_OK ? run_attention(paged, q->elem, plan) : st;
     } catch (const std::bad_alloc &) {
         return invalid_argument(paged->err, "out of host memory");
     }
