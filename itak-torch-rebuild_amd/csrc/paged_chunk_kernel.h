@@ -23,6 +23,7 @@
 // The maximum is a reference that moves only when a score passes it by far (kWeightMost).
 #pragma once
 
+#include "lds_grant.h"
 #include "paged_careful.h"
 
 namespace itak {
@@ -474,21 +475,27 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     }
 }
 
+template <auto Kernel, int ELEM, int DP>
+hipError_t launch_chunk_kernel(const PagedAttn &a, hipStream_t stream) {
+    int device = -1;
+    (void)hipGetDevice(&device);
+    const hipError_t granted = granted_once<Kernel>(device, [] {
+        return hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(chunk_lds(DP)));
+    });
+    if (granted != hipSuccess) return granted;
+    launch_kernel(Kernel, a.units * a.parts, paged_chunk_waves(DP, ELEM) * 64, chunk_lds(DP), stream, a);
+    return hipGetLastError();
+}
 template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP>
 hipError_t launch_chunk_as(const PagedAttn &a, hipStream_t stream) {
-    if constexpr (!paged_chunk_takes(DP, PAGE, ELEM)) return hipErrorInvalidValue;
-    else {
-    auto run = [&](auto kernel) {
-        static const hipError_t granted =
-            hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(chunk_lds(DP)));
-        if (granted != hipSuccess) return granted;
-        launch_kernel(kernel, a.units * a.parts, paged_chunk_waves(DP, ELEM) * 64, chunk_lds(DP), stream, a);
-        return hipGetLastError();
-    };
-    if (a.cap_log2 == 0.0f) return run(paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kNoCap>);
-    if constexpr (ELEM != ITAK_ELEM_F32)
-        if (!paged_cap_by_series(ELEM, a.cap_log2)) return run(paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kShortCap>);
-    return run(paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kSeriesCap>);
+    if constexpr (!paged_chunk_takes(DP, PAGE, ELEM)) {
+        return hipErrorInvalidValue;
+    } else {
+        if (a.cap_log2 == 0.0f) return launch_chunk_kernel<&paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kNoCap>, ELEM, DP>(a, stream);
+        if constexpr (ELEM != ITAK_ELEM_F32)
+            if (!paged_cap_by_series(ELEM, a.cap_log2))
+                return launch_chunk_kernel<&paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kShortCap>, ELEM, DP>(a, stream);
+        return launch_chunk_kernel<&paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kSeriesCap>, ELEM, DP>(a, stream);
     }
 }
 template <int PAGE, int ELEM, int NQ, int NP>
