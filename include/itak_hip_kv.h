@@ -732,7 +732,7 @@ void itak_rotation_destroy(itak_rotation *rotation);
 /* The rotary_dim / 2 frequencies, radians a position, and the amplitude. Either may be NULL. */
 itak_status itak_rotation_frequencies(const itak_rotation *rotation, double *frequencies_out, double *amplitude_out);
 /* Turns up to four tensors by the same rows' positions in one launch on `hip_stream`: outputs[i] = rotation of inputs[i],
-   each rows x inputs[i].heads x head_dim, an output of its input's type and either the same view or disjoint
+   each rows x inputs[i].heads x head_dim (rows below 2^24), an output of its input's type and either the same view or disjoint
    from it. positions_dev: [rows] int64 on the device, any sign, below 2^31 in magnitude. `inverse` turns back
    (by the negative angles, the same amplitude): the transpose, which is what the gradients of rotated rows go through. */
 itak_status itak_rotate_device(const itak_rotation *rotation, void *hip_stream, uint64_t head_dim, uint64_t rows,
@@ -786,7 +786,7 @@ typedef struct itak_paged_config {
    its own: exactly the pages of position + rows positions, or more. */
 typedef struct itak_paged_item {
     uint64_t position; /* position + rows below 2^31 */
-    uint32_t rows;     /* 0: the sequence takes no part */
+    uint32_t rows;     /* 0: the sequence takes no part; of a batch below 2^24 in all */
     uint32_t pages;
 } itak_paged_item;
 

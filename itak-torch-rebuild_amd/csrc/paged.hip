@@ -215,7 +215,9 @@ itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work, bool &whole
     };
     uint64_t units = 0;
     each(0, [&](uint32_t, uint64_t at, uint64_t u) { work = at, units = u; });
-    if (work >= (1ull << 30) || units >= (1ull << 24)) return size_overflow(p->err, "blocks of the batch's attention");
+    // (Of the kernel of many rows a unit is a workgroup of up to 512 threads, and a launch's threads are counted in 32 bits; where units are
+    // dealt to parts they are few.)
+    if (work >= (1ull << 30) || units > (1ull << 32) / 512 - 1) return size_overflow(p->err, "blocks of the batch's attention");
     a.units = uint32_t(units);
     // (The kernel of many rows has no line.)
     const PagedCut cut = a.parts ? PagedCut{} : paged_cut(uint32_t(work), a.units, longest, a.groups, a.least);

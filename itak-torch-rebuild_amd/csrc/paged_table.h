@@ -15,7 +15,8 @@ namespace itak {
 constexpr uint32_t kPagedItem0 = 4;  // the first item's first word
 inline uint32_t paged_ids_at(uint32_t max_sequences) { return kPagedItem0 + 4 * max_sequences; }
 
-constexpr uint64_t kPagedMostRows = 1u << 24;
+// Launches have a workgroup of 256 threads a row, and a launch's threads are counted in 32 bits.
+constexpr uint64_t kPagedMostRows = (1u << 24) - 1;
 
 struct PagedLimits {
     uint64_t page_count;
@@ -74,7 +75,7 @@ inline PagedRefusal make_paged_batch(const PagedLimits &lim, const itak_paged_it
     if (named != page_ids)
         return refuse(ITAK_SHAPE_MISMATCH, "page_ids", named, page_ids,
                       "page_ids: got " + number(page_ids) + ", the items name " + number(named));
-    if (rows > kPagedMostRows) return refuse(ITAK_SIZE_OVERFLOW, "rows", rows, 0, "more than 2^24 rows in a batch");
+    if (rows > kPagedMostRows) return refuse(ITAK_SIZE_OVERFLOW, "rows", rows, 0, "more than 2^24 - 1 rows in a batch");
     for (uint64_t i = 0; i < page_ids; ++i)
         if (pages[i] >= lim.page_count)
             return refuse(ITAK_INVALID_ARGUMENT, "page id", pages[i], lim.page_count,

@@ -18,7 +18,7 @@ namespace {
 
 constexpr uint32_t kMostTensors = 4;
 constexpr int kThreads = 256;
-constexpr uint64_t kMostRows = 1u << 24;  // a workgroup a row: what a launch holds
+constexpr uint64_t kMostRows = (1u << 24) - 1;  // a workgroup a row: a launch's threads are counted in 32 bits
 
 struct RotateArgs {
     RotationView r;
