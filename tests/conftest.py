@@ -23,6 +23,11 @@ def _gpu_present() -> bool:
 
 def pytest_collection_modifyitems(config, items):
     if _gpu_present():
+        import torch
+
+        # A graph that a test leaves in a cycle (a caught exception's frames) is destroyed whenever Python collects, and destroying one waits for
+        # the device, which amid another capture ends the process: what is left is collected before every capture.
+        torch.compiler.config.force_cudagraph_gc = True
         return
     skip = pytest.mark.skip(reason="no GPU in this process")
     for item in items:

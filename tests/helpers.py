@@ -25,6 +25,16 @@ def declared_symbols():
     return sorted(set(re.findall(r"\b(itak_[a-z0-9_]+)\s*\(", text)))
 
 
+def refusal(call):
+    """The variant of the AttentionError that `call` is refused with, or None. (Beside a captured graph: unlike pytest.raises it leaves no
+    cycle with the caller's frame.)"""
+    try:
+        call()
+    except pkg().AttentionError as e:
+        return e.variant
+    return None
+
+
 def normal(rng, *shape):
     return rng.standard_normal(shape, dtype=np.float32)
 
