@@ -807,7 +807,8 @@ void *itak_paged_storage(const itak_paged *paged);
    any other place of any table names as well (shared pages are to be copied before they are written). Enqueued on
    the handle's stream: calls before it see the batch before it, and replays of a graph the batch that is set when they
    run. Not while that stream is being captured. Graphs need the same number of items with the same rows
-   each as when they were captured, and as many page ids as max_table_pages allows; positions and pages may be others. */
+   each as when they were captured, and as many page ids as max_table_pages allows; positions and pages may be others (refused are positions over which
+   a call that was captured would have 2^30 blocks of 32 keys to go through: 2^31 positions of 16 KV heads). */
 itak_status itak_paged_set_batch(itak_paged *paged, const itak_paged_item *items, uint32_t count, const uint32_t *pages,
                                  uint64_t page_ids);
 /* Writes the batch's new rows of `layer` into their pages: k and v are [sum rows][num_kv_heads][head_dim], items in

@@ -34,6 +34,11 @@ struct itak_paged {
     uint64_t ws_bytes = 0;
     void *turned = nullptr;          // a step's rotated queries
     uint64_t turned_bytes = 0;
+    // The most units that an attention call under capture has launched, of calls without a window and with one, whose largest it is.
+    struct Captured {
+        uint64_t units;
+        uint32_t window;
+    } captured[2] = {};
     mutable ErrorState err;
 };
 
@@ -193,6 +198,9 @@ itak_status check_attention(itak_paged *p, uint64_t layer, const itak_rows *q, c
     return ITAK_OK;
 }
 
+// Blocks of all units of a launch: the kernels add them up in 32 bits, rounded up by at most as many again.
+constexpr uint64_t kMostBlocks = 1ull << 30;
+
 uint32_t shift_of(uint32_t power) { return uint32_t(__builtin_ctz(power)); }
 
 // Units and blocks of the items a launch takes, how their line is cut, and where in it inline items begin; `whole`: no unit is split.
@@ -217,7 +225,7 @@ itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work, bool &whole
     each(0, [&](uint32_t, uint64_t at, uint64_t u) { work = at, units = u; });
     // (Of the kernel of many rows a unit is a workgroup of up to 512 threads, and a launch's threads are counted in 32 bits; where units are
     // dealt to parts they are few.)
-    if (work >= (1ull << 30) || units > (1ull << 32) / 512 - 1) return size_overflow(p->err, "blocks of the batch's attention");
+    if (work >= kMostBlocks || units > (1ull << 32) / 512 - 1) return size_overflow(p->err, "blocks of the batch's attention");
     a.units = uint32_t(units);
     // (The kernel of many rows has no line.)
     const PagedCut cut = a.parts ? PagedCut{} : paged_cut(uint32_t(work), a.units, longest, a.groups, a.least);
@@ -342,7 +350,23 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
         if (st != ITAK_OK) return st;
         plan.merge_few = captured || !whole;
     }
-    return workspace(p, plan, dp);
+    const itak_status st = workspace(p, plan, dp);
+    if (st == ITAK_OK && captured) {
+        itak_paged::Captured &c = p->captured[a.window ? 1 : 0];
+        c.units = std::max<uint64_t>({c.units, plan.few.units, plan.many.units});
+        c.window = std::max(c.window, a.window);
+    }
+    return st;
+}
+
+// Whether the captured calls' replays over a batch of these words (of as many units) can count their blocks.
+bool replays_hold(const itak_paged *p, const std::vector<uint32_t> &head) {
+    for (const itak_paged::Captured &c : p->captured)
+        for (size_t at = kPagedItem0; c.units && at < head.size(); at += 4) {
+            const uint32_t blocks = (head[at] + head[at + 1] + 31) / 32 - paged_first_block(head[at], c.window);
+            if (c.units * blocks >= kMostBlocks) return false;
+        }
+    return true;
 }
 
 itak_status run_attention(itak_paged *p, uint32_t elem, const AttnPlan &plan) {
@@ -413,6 +437,7 @@ itak_status set_batch(itak_paged *p, const itak_paged_item *items, uint32_t coun
     if (capturing(p->stream)) return invalid_argument(p->err, "the batch is set while the stream is being captured");
     const PagedRefusal r = make_paged_batch(p->limits, items, count, pages, page_ids, p->marks, p->stamp, p->next);
     if (r.code != ITAK_OK) return set_error(p->err, r.code, r.what, r.a, r.b, 0, 0, "%s", r.text.c_str());
+    if (!replays_hold(p, p->next.head)) return size_overflow(p->err, "blocks of a captured attention over the batch");
     const DeviceScope scope(p->cfg.device);
     HIP_TRY(p, scope.status(), "set the device");
     // The items go up every time, page ids where they are not what the device has: of a sequence that grows, one every
