@@ -23,6 +23,15 @@ _SCALINGS = {"plain": N.ROTATION_PLAIN, "linear": N.ROTATION_LINEAR, "yarn": N.R
 _NAN = math.nan
 
 
+def _filled(kind, *values):
+    """The structure of these values; refused is an integer that its field would take modulo the field's size."""
+    raw = kind(*values)
+    for (name, _), value in zip(kind._fields_, values):
+        if isinstance(value, int) and value != (getattr(raw, name) or 0):
+            raise ValueError(f"{name}: {value} is out of range")
+    return raw
+
+
 class Rows:
     """A view of rows x heads x channels on the device (itak_rows): pointer, type, heads, strides in elements."""
 
@@ -30,6 +39,8 @@ class Rows:
 
     def __init__(self, ptr: int, elem: str, heads: int, row_stride: int = 0, head_stride: int = 0, keep=None, rows: int = -1,
                  channels: int = -1):
+        if not 0 <= heads < 1 << 32:  # (a field would take it modulo its size; strides that far out are refused as they are)
+            raise ValueError(f"heads: {heads} is out of range")
         self.raw = N.Rows(ptr, _ELEMS[elem] if isinstance(elem, str) else elem, heads, row_stride, head_stride)
         self.ref = C.byref(self.raw)
         self.at = C.addressof(self.raw)  # the view as the front module takes it
@@ -82,8 +93,8 @@ class Rotation:
         self._lib = hip_compute._load()
         if scaling not in _SCALINGS:
             raise ValueError(f"scaling {scaling!r} is none of {', '.join(_SCALINGS)}")
-        cfg = N.RotationConfig(base, rotary_dim, 1 if interleaved else 0, _SCALINGS[scaling], device, factor, original_positions,
-                               beta_fast, beta_slow, amplitude or 0.0)
+        cfg = _filled(N.RotationConfig, base, rotary_dim, 1 if interleaved else 0, _SCALINGS[scaling], device, factor,
+                      original_positions, beta_fast, beta_slow, amplitude or 0.0)
         handle = C.c_void_p()
         if self._lib.itak_rotation_create(C.byref(cfg), C.byref(handle)) != N.OK:
             _raise_last(None)
@@ -147,8 +158,8 @@ class PagedKv:
     @staticmethod
     def _config(layers, num_kv_heads, head_dim, elem, page_rows, page_count, max_sequences=1, max_table_pages=0, device=0,
                 storage_ptr=0, storage_bytes=0):
-        return N.PagedConfig(layers, _ELEMS[elem], num_kv_heads, head_dim, page_count, page_rows, max_sequences, max_table_pages,
-                             device, 0, storage_ptr or None, storage_bytes)
+        return _filled(N.PagedConfig, layers, _ELEMS[elem], num_kv_heads, head_dim, page_count, page_rows, max_sequences,
+                       max_table_pages, device, 0, storage_ptr or None, storage_bytes)
 
     @staticmethod
     def bytes_for(layers: int, num_kv_heads: int, head_dim: int, *, elem: str = "f16", page_rows: int = 64,
@@ -159,6 +170,8 @@ class PagedKv:
 
     def _done(self, status: int) -> None:
         if status != N.OK:
+            if not self._h:
+                raise ValueError("the paged cache is closed")
             _raise_last(self._h, lib_error=(self._lib.itak_paged_last_error, self._lib.itak_paged_last_error_info))
 
     def close(self) -> None:
