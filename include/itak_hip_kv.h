@@ -753,7 +753,7 @@ itak_status itak_rotate_device(const itak_rotation *rotation, void *hip_stream, 
    Tensors of a call are ITAK_ELEM_F32 or of the pages' own type. Scores, softmax and sums are f32. With tensors of
    the pages' type the softmax weights are rounded to that type once (f16 2^-11, bf16 2^-8 relative to each) and
    the output once; with f32 tensors queries and weights enter the matrix pipe as several halves each,
-   which leaves 2^-22 of them (bf16: 2^-24), over f16 pages at least 2^-29 of a query and 2^-37 of the largest weight. An f16 query's or key's channel beyond 65504 is infinite.
+   which leaves 2^-22 of them (bf16: 2^-24), over f16 pages at least 2^-29 of a query and 2^-37 of the largest weight. An f16 channel beyond 65504 is infinite.
    A row that is not finite reaches the outputs of exactly the queries that see its position; one difference is left: a weight
    below 2^-126 of its row's largest is zero, and zero times an infinite value is NaN. Finite values give finite outputs, up to the
    ends of bf16. Tiles of queries that meet rows that are not finite or bf16 values from about 2^100 on, and f32 queries beyond 4,094
@@ -808,7 +808,9 @@ void *itak_paged_storage(const itak_paged *paged);
    the handle's stream: calls before it see the batch before it, and replays of a graph the batch that is set when they
    run. Not while that stream is being captured. Graphs need the same number of items with the same rows
    each as when they were captured, and as many page ids as max_table_pages allows; positions and pages may be others (refused are positions over which
-   a call that was captured would have 2^30 blocks of 32 keys to go through: 2^31 positions of 16 KV heads). */
+   a call that was captured would have 2^30 blocks of 32 keys to go through: 2^31 positions of 16 KV heads). Items of more than 32 query vectors a KV
+   head are dealt to as many workgroups as filled the device over the positions they were captured at: capture at the longest that are
+   expected (61 rows replayed over 30,000 positions take 58 us, and 640 if they were captured at position 0). */
 itak_status itak_paged_set_batch(itak_paged *paged, const itak_paged_item *items, uint32_t count, const uint32_t *pages,
                                  uint64_t page_ids);
 /* Writes the batch's new rows of `layer` into their pages: k and v are [sum rows][num_kv_heads][head_dim], items in

@@ -48,7 +48,7 @@ hipError_t launch_paged_append(uint32_t page_elem, uint32_t elem, bool by_8, con
 // .. (w + 1) * share of the line, so that a batch of any lengths keeps every compute unit busy to the end and the grid does not
 // depend on the lengths. Where that makes a share little longer, every unit's run is rounded up to a multiple of the share, so that
 // no workgroup has parts of two units one after the other: a part costs some 4 us beside its blocks (one token at 4,096:
-// 8.4 us over borders, 5.0 without). A unit that one workgroup has whole is written out by it; of the others every workgroup
+// 3.4 us more over borders than the 6.0 to 6.4 that the launch takes). A unit that one workgroup has whole is written out by it; of the others every workgroup
 // leaves its partial in slot w + (unit's index), which no two parts share, and the merge launch joins them.
 // The cut is worked out on the device from the batch's lengths, so a captured launch is right for whatever batch is set when it runs.
 // Items that travel with a launch: an eager call whose batch has at most this many hands them over by value, and its kernels do not
@@ -104,8 +104,9 @@ __host__ __device__ constexpr uint32_t paged_chunk_waves(uint32_t padded, uint32
     return padded == 64 || (padded == 128 && elem != ITAK_ELEM_F32) ? 8 : 4;
 }
 // Workgroups a compute unit holds (by LDS and registers).
-__host__ __device__ constexpr uint32_t paged_chunk_groups_per_cu(uint32_t) { return 1; }
-// (f32 queries of 256 channels in three bf16 pieces are more registers than there are: the kernel of few rows takes them.)
+constexpr uint32_t kPagedChunkGroupsPerCu = 1;
+// (f32 queries of 256 channels in three bf16 pieces are more registers than there are: the kernel of few rows takes them, in tiles of 32 and
+// slowly: 2,048 rows over 30,720 14.4 ms, where f16 pages take 3.6.)
 __host__ __device__ constexpr bool paged_chunk_takes(uint32_t padded, uint32_t page_elem, uint32_t elem) {
     return !(padded == 256 && page_elem == ITAK_ELEM_BF16 && elem == ITAK_ELEM_F32);
 }

@@ -336,7 +336,7 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
         b.parts = 1;
         const itak_status st = count_units(p, b, work, whole);
         if (st != ITAK_OK) return st;
-        b.parts = chunk_parts(b.units, work, cus * paged_chunk_groups_per_cu(dp));
+        b.parts = chunk_parts(b.units, work, cus * kPagedChunkGroupsPerCu);
     }
     if (most_few) {
         plan.sets = most_few <= kPagedSet ? 1 : 2;

@@ -11,9 +11,10 @@
 // (ds_read_b64_tr_b16: sixteen lanes read four rows of sixteen channels and each gets four keys of one channel).
 // The next block's scores are multiplied beside this block's exponentials, and this block's P.V beside the next one's maximum.
 // 32 vectors a wavefront and two wavefronts a SIMD, which fill each other's gaps: 64 vectors and one wavefront read half as much from LDS
-// and took 1,035 us where these take 959 to 980 (2,048 rows by 32 heads over 30,720 and themselves, 128 channels, f16: 1.07 TFLOP, 1.09 to
-// 1.11 PFLOP/s, where a library product of 8,192 cubed reaches 1.14). The matrix pipe is busy 64 % of the time at the 1.77 GHz that the
-// power leaves it; without its LDS reads and loads the loop would take some 800 us.
+// and took 1,035 us where these took 959 to 980 on the same devices and take up to 1,000 on others (2,048 rows by 32 heads over 30,720 and
+// themselves, 128 channels, f16: 1.07 TFLOP, 1.07 to 1.11 PFLOP/s, where a library product of 8,192 cubed reaches 1.14). The matrix pipe is busy 64 % of the time at the 1.77 GHz that the
+// power leaves it; without its LDS reads and loads the loop would take some 800 us. f32 tensors are products times pieces: over f16 two by two,
+// 1,865 us (two times a library product's time are 1,880), over bf16 three by three, 2,510 us.
 //
 // Blocks travel from the pages to LDS without passing through registers (global_load_lds_dwordx4: lane i's 16 bytes go to
 // M0 + 16 i) into a ring of stages, whole rows at a time; the 16-byte pieces of a row are shuffled by the row's number on the way (the source
@@ -57,8 +58,8 @@ __device__ __forceinline__ void wait_loads() {  // s_waitcnt vmcnt(n), other cou
 
 // Sub-blocks of 32 keys a stage of the ring holds, and stages.
 constexpr int chunk_subs(int dp) { return dp <= 128 ? 2 : 1; }
-constexpr int chunk_stages(int dp) { return dp == 256 ? 4 : 4; }
-constexpr size_t chunk_lds(int dp) { return size_t(chunk_stages(dp)) * chunk_subs(dp) * 2 * 32 * 2 * dp; }
+constexpr int kChunkStages = 4;
+constexpr size_t chunk_lds(int dp) { return size_t(kChunkStages) * chunk_subs(dp) * 2 * 32 * 2 * dp; }
 
 // Scores without a cap, capped by the short form, capped by the series (paged_cap_by_series).
 enum ChunkCap { kNoCap, kShortCap, kSeriesCap };
@@ -72,7 +73,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     constexpr int kRowBytes = 2 * DP;
     constexpr int kBlockBytes = 32 * kRowBytes;   // of one side of a sub-block
     constexpr int kSubBytes = 2 * kBlockBytes;
-    constexpr int kSubs = chunk_subs(DP), kStages = chunk_stages(DP), kStageBytes = kSubs * kSubBytes;
+    constexpr int kSubs = chunk_subs(DP), kStages = kChunkStages, kStageBytes = kSubs * kSubBytes;
     constexpr int kRowPieces = DP / 8;            // 16-byte pieces of a row
     constexpr int kLoadRows = 512 / DP;           // rows a load of one wavefront moves
     constexpr int kSideLoads = DP / 16;           // loads of a side of a sub-block, dealt to the wavefronts in turn

@@ -16,7 +16,7 @@
 // The next block's rows are asked for before the block at hand is multiplied, and its page ids a block earlier.
 //
 // Measured, 32 heads over 4 of 128 channels: 16 tokens at up to 16,384 in bf16, 315 MB, 54.5 us, 5.8 TB/s, where a kernel that only reads
-// gets 6.2; one token at 4,096 6.1 us, of which the arguments and the item's place take 1.3, page ids and rows 1, 32 keys' products 0.7
+// gets 6.2; one token at 4,096 6.0 to 6.4 us, of which the arguments and the item's place take 1.3, page ids and rows 1, 32 keys' products 0.7
 // and the meeting of the wavefronts 1.
 #pragma once
 

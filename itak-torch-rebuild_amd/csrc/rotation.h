@@ -140,7 +140,7 @@ __device__ __forceinline__ void move_piece(const typename Elem<FROM>::type *src,
     }
 }
 
-// The checks of a view (rows.hip): null data, an unknown type, no heads, a first stride that lets rows run into one another.
+// The checks of a view (rotation.hip): null data, an unknown type, no heads, a first stride that lets rows run into one another.
 struct ErrorState;
 itak_status check_rows(ErrorState &e, const char *what, const itak_rows *v, uint64_t rows, uint64_t head_dim, bool written);
 // With dense strides filled in.
