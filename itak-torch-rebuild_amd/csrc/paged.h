@@ -9,6 +9,7 @@ namespace itak {
 
 constexpr float kPagedLog2e = 1.4426950408889634f;
 constexpr float kPagedQueryLift = 16.0f;  // paged_mfma.h
+constexpr float kPagedMergeLift = 0x1p32f;  // parts with a negative sum stand for that many times themselves (paged_careful.h)
 constexpr float kPagedCapShort = 256.0f * kPagedLog2e;  // paged_mfma.h
 // Whether capped scores are worked out by the series (`cap_log2` > 0).
 __host__ __device__ constexpr bool paged_cap_by_series(uint32_t elem, float cap_log2) {
@@ -85,7 +86,7 @@ struct PagedAttn {
     PagedItemWords item[kPagedInline];  // those behind the last: row0, start and unit0 are ~0
     uint32_t start[kPagedInline], unit0[kPagedInline];  // where an item's blocks and units begin in the line
     float *ws_acc;       // [slots][tile][padded head_dim]
-    float2 *ws_ml;       // [slots][tile]: maximum (log2 domain), sum
+    float2 *ws_ml;       // [slots][tile]: maximum (log2 domain), sum; negative: of a part that is scaled down by kPagedMergeLift
 };
 // Workgroups that may share a unit.
 constexpr uint32_t kPagedMostParts = 1024;

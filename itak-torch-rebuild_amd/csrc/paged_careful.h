@@ -25,13 +25,13 @@ __device__ __forceinline__ bool to_be_done_over(float check) {
     return PAGE == ITAK_ELEM_F16 ? check != check : !(__builtin_fabsf(check) < INFINITY);
 }
 
-// What comes out has its reference so far above the largest score (log2 domain): 2^31 values below 2^128 with weights up to 2^-32 stay
-// below 2^127. The factor goes to the values: a weight that it made zero would make an infinite value NaN. (Over f16 pages there is no need.)
+// What comes out is scaled by this: 2^31 values below 2^128 with weights up to 2^-32 stay below 2^127. The factor goes to the values: a
+// weight that it made zero would make an infinite value NaN. (Over f16 pages there is no need.)
 template <int PAGE>
-constexpr float kCarefulDrop = PAGE == ITAK_ELEM_F16 ? 0.0f : 32.0f;
+constexpr float kCarefulScale = PAGE == ITAK_ELEM_F16 ? 1.0f : 1.0f / kPagedMergeLift;
 
-// A wavefront's vectors of v0 .. v_end over the keys [key0, key1): WRITE(vector, accumulators of channels 64 c + lane, reference in
-// the log2 domain, sum). kCareful vectors at once, so that a row is fetched once for them, and 64 keys: a lane has the scores
+// A wavefront's vectors of v0 .. v_end over the keys [key0, key1): WRITE(vector, accumulators of channels 64 c + lane, maximum in
+// the log2 domain, sum), accumulators and sum scaled. kCareful vectors at once, so that a row is fetched once for them, and 64 keys: a lane has the scores
 // of one key; then the lanes are channels.
 constexpr uint32_t kCareful = 4;
 template <int PAGE, int ELEM, int DP, typename W>
@@ -41,7 +41,6 @@ __device__ __forceinline__ void paged_careful(const PagedAttn &a, const PagedSpa
     typedef typename Elem<PAGE>::type P;
     constexpr int kRuns = DP / 64;
     constexpr uint32_t kAtOnce = 8;
-    constexpr float kDown = PAGE == ITAK_ELEM_F16 ? 1.0f : 0x1p-32f;  // 2^-kCarefulDrop
     const uint32_t lane = __lane_id(), d = a.g.head_dim, page_mask = (1u << a.g.page_shift) - 1;
     const P *const base = reinterpret_cast<const P *>(a.layer_base) + head * a.g.head_stride;
     const uint32_t *ids = a.batch + span.table;
@@ -106,7 +105,7 @@ __device__ __forceinline__ void paged_careful(const PagedAttn &a, const PagedSpa
                     const uint64_t high = uint32_t(__builtin_amdgcn_readlane(uint32_t(row_at >> 32), j + t));
                     const P *value = reinterpret_cast<const P *>(high << 32 | low);
 #pragma unroll
-                    for (int c = 0; c < kRuns; ++c) y[t][c] = 64 * c + lane < d ? Elem<PAGE>::to_f32(value[64 * c + lane]) * kDown : 0.0f;
+                    for (int c = 0; c < kRuns; ++c) y[t][c] = 64 * c + lane < d ? Elem<PAGE>::to_f32(value[64 * c + lane]) * kCarefulScale<PAGE> : 0.0f;
                 }
 #pragma unroll
                 for (uint32_t t = 0; t < kKeys; ++t)
@@ -125,13 +124,14 @@ __device__ __forceinline__ void paged_careful(const PagedAttn &a, const PagedSpa
         for (uint32_t u = 0; u < kCareful; ++u) {
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) sum[u] += __shfl_xor(sum[u], o);
-            if (v + u < v_end) write(v + u, acc[u], m[u] + kCarefulDrop<PAGE>, sum[u] * kDown);
+            if (v + u < v_end) write(v + u, acc[u], m[u], sum[u] * kCarefulScale<PAGE>);
         }
     }
 }
 
-// What it gives for a vector: out, or its slot of the workspace.
-template <int ELEM, int DP>
+// What it gives for a vector: out, or its slot of the workspace, where a negative sum says that the part is scaled. (The maximum cannot say so: raised
+// by 32 it would lose bits, of scores from 2^29 on all of the 32.)
+template <int PAGE, int ELEM, int DP>
 __device__ __forceinline__ void paged_write_careful(const PagedAttn &a, const PagedSpan &span, uint32_t head, uint32_t v, bool whole,
                                                     uint64_t slot, bool has_slot, const float (&acc)[DP / 64], float m, float l) {
     typedef typename Elem<ELEM>::type T;
@@ -146,7 +146,7 @@ __device__ __forceinline__ void paged_write_careful(const PagedAttn &a, const Pa
         else if (has_slot)
             a.ws_acc[slot * DP + 64 * c + lane] = acc[c];
     }
-    if (!whole && has_slot && lane == 0) a.ws_ml[slot] = make_float2(m, l);
+    if (!whole && has_slot && lane == 0) a.ws_ml[slot] = make_float2(m, kCarefulScale<PAGE> == 1.0f ? l : -l);
 }
 
 // Whether any of a workgroup's threads says so; all of them ask.

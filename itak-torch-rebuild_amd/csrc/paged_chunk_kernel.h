@@ -439,7 +439,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     if (any_of_group(mine && to_be_done_over<PAGE>(all), &lds_flag)) {
         paged_careful<PAGE, ELEM, DP>(a, span, head, v0, min(v0 + kTile, vectors), wave, kWaves, 32 * kb0, 32 * kb_end,
                                       [&](uint32_t v, const float (&acc)[DP / 64], float m, float l) {
-                                          paged_write_careful<ELEM, DP>(a, span, head, v, whole, slot0 + v - v0, true, acc, m, l);
+                                          paged_write_careful<PAGE, ELEM, DP>(a, span, head, v, whole, slot0 + v - v0, true, acc, m, l);
                                       });
     } else if (mine) {
         if (whole) {

@@ -392,7 +392,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
             const uint32_t kb0 = span.first + from;
             paged_careful<PAGE, ELEM, DP>(a, span, head, v0, min(v0 + kTile, vectors), wave, kFewWaves, 32 * kb0, 32 * (kb0 + count),
                                           [&](uint32_t v, const float (&acc)[DP / 64], float m, float l) {
-                                              paged_write_careful<ELEM, DP>(a, span, head, v, whole, uint64_t(blockIdx.x + unit) * kTile + v - v0,
+                                              paged_write_careful<PAGE, ELEM, DP>(a, span, head, v, whole, uint64_t(blockIdx.x + unit) * kTile + v - v0,
                                                                             blockIdx.x + unit < a.groups + a.units, acc, m, l);
                                           });
         }

@@ -51,8 +51,8 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(PagedAttn a) {
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) early[u] = acc_of(min(part + u * kLanes, parts - 1));
     // (A maximum of minus infinity: nothing visible, a sum of 0, or scores that are no numbers, which the sum then is.)
-    auto weight_of = [](float2 x, float m) { return x.x == -INFINITY ? 0.0f : fast_exp2(x.x - m); };
-    auto sum_of = [](float2 x, float weight) { return x.x == -INFINITY ? x.y : weight * x.y; };
+    auto weight_of = [](float2 x, float m) { return x.x == -INFINITY ? 0.0f : fast_exp2(x.x - m) * (x.y < 0.0f ? kPagedMergeLift : 1.0f); };
+    auto sum_of = [](float2 x, float weight) { return x.x == -INFINITY ? x.y : weight * __builtin_fabsf(x.y); };
     floatx4 acc = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     if (parts <= 64) {
         // Every wavefront has all of them, one a lane.

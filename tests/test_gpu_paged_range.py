@@ -71,3 +71,35 @@ def test_infinities_beside_the_largest_values(tensors, position, rows):
     assert torch.equal(got.isinf(), want.isinf()) and torch.equal(got[got.isinf()], want[want.isinf()])
     tol, fine = PC.tolerance(want, spread, most, "bf16", tensors, 64, n), want.isfinite()
     assert bool(((got - want).abs()[fine] <= tol[fine]).all())
+
+
+# Every key scores the same 10^10 and more, beyond which 32 is lost in f32: parts with values that a sum cannot hold and parts without them
+# weigh alike all the same. Of powers of two the score is the scale, 24 bits, times one of them, which f32 holds: weights are 1 to the bit and the
+# output is the mean, whose sums of up to 6,001 values in pieces of 32 and a merge of up to 256 stay within 2^-14, beside the rounding
+# of the output. Of 10^5 squared the product with the scale is rounded, by up to 2^9 where a weight's exponent is the difference of two of
+# them, so that any mean of the values is right.
+@pytest.mark.parametrize("tensors", ["bf16", "f32"])
+@pytest.mark.parametrize("position,rows", [(6000, 1), (3000, 20)])
+@pytest.mark.parametrize("channel", [2.0 ** 17, 1e5])
+def test_parts_weigh_alike_at_large_scores(tensors, position, rows, channel):
+    n = position + rows
+    cache = PC.Cache(pkg(), [n], kv_heads=1, d=64, pages="bf16", page_rows=64, fill="nan")
+    keys, values = torch.zeros(n, 1, 64), torch.ones(n, 1, 64)
+    keys[..., 0] = channel
+    values[n // 2:, 0, 4] = 3e38
+    cache.place(0, 0, 0, keys.bfloat16(), values.bfloat16())
+    q = torch.zeros(rows, 4, 64)
+    q[..., 0] = channel
+    q = q.to(PC.DTYPES[tensors])
+    out, qd = torch.empty_like(q, device="cuda"), q.cuda()
+    cache.paged.set_batch([(position, rows)], cache.tables)
+    cache.paged.attention_device(0, view(qd), view(out), scale=1.0)
+    torch.cuda.synchronize()
+    got, values = out.cpu().double(), cache.rows(0, 0, n)[1].double()
+    tol = 2.0 ** -14 + PC.HALF_STEP[tensors]
+    if channel == 1e5:
+        assert bool((got >= values.amin(0) * (1 - tol)).all()) and bool((got <= values.amax(0) * (1 + tol)).all())
+        return
+    mean = values.cumsum(0)[position:] / torch.arange(position + 1, n + 1).double()[:, None, None]
+    off = float((got / mean - 1).abs().max())
+    assert off <= tol, off
