@@ -793,6 +793,7 @@ typedef struct itak_paged_item {
 /* Bytes of storage a configuration needs; 0 for one that itak_paged_create refuses. */
 uint64_t itak_paged_storage_bytes(const itak_paged_config *config);
 itak_status itak_paged_create(const itak_paged_config *config, itak_paged **out);
+/* Waits for its stream and frees its memory: not while a stream is being captured, nor while a graph that names it may be replayed. */
 void itak_paged_destroy(itak_paged *paged);
 /* As itak_last_error and itak_last_error_info, of a paged cache's calls (NULL: of this thread's last failed create). */
 const char *itak_paged_last_error(const itak_paged *paged);
