@@ -60,6 +60,13 @@ pub const ITAK_ELEM_BF16: u32 = 2;
 pub const ITAK_ROTATION_PLAIN: u32 = 0;
 pub const ITAK_ROTATION_LINEAR: u32 = 1;
 pub const ITAK_ROTATION_YARN: u32 = 2;
+pub const ITAK_TABLE_OK: u32 = 0;
+pub const ITAK_TABLE_POSITION: u32 = 1;
+pub const ITAK_TABLE_PAGES: u32 = 2;
+pub const ITAK_TABLE_ID: u32 = 3;
+pub const ITAK_TABLE_PARENTS: u32 = 4;
+pub const ITAK_TABLE_ROOM: u32 = 5;
+pub const ITAK_TABLE_FREE: u32 = 6;
 
 /// Opaque handle.
 #[repr(C)]
@@ -263,6 +270,18 @@ pub struct itak_paged_item {
     pub pages: u32,
 }
 
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct itak_page_tables {
+    pub table: *mut u32,
+    pub stride: u64,
+    pub pages: *mut i32,
+    pub free_ids: *mut u32,
+    pub free_count: *mut i32,
+    pub sequences: u32,
+    pub reserved: u32,
+}
+
 #[link(name = "itak_hip_kv")]
 extern "C" {
     pub fn itak_abi_version() -> u32;
@@ -347,6 +366,13 @@ extern "C" {
     pub fn itak_paged_append_device(paged: *mut itak_paged, layer: u64, k: *const itak_rows, v: *const itak_rows, rotation: *const itak_rotation) -> itak_status;
     pub fn itak_paged_attention_device(paged: *mut itak_paged, layer: u64, q: *const itak_rows, out: *const itak_rows, scale: f32, softcap: f32, window: u64, rotation: *const itak_rotation) -> itak_status;
     pub fn itak_paged_step_device(paged: *mut itak_paged, layer: u64, q: *const itak_rows, k: *const itak_rows, v: *const itak_rows, out: *const itak_rows, scale: f32, softcap: f32, window: u64, rotation: *const itak_rotation) -> itak_status;
+    pub fn itak_paged_enable_trees(paged: *mut itak_paged, most_rows: u64) -> itak_status;
+    pub fn itak_paged_set_batch_tree(paged: *mut itak_paged, items: *const itak_paged_item, count: u32, pages: *const u32, page_ids: u64, parents: *const i32) -> itak_status;
+    pub fn itak_paged_fit_tables_device(paged: *mut itak_paged, tables: *const itak_page_tables, lengths_dev: *const i32, rows: *const u32, status_dev: *mut i32) -> itak_status;
+    pub fn itak_paged_set_batch_device(paged: *mut itak_paged, tables: *const itak_page_tables, positions_dev: *const i32, rows: *const u32, most_positions: u64, parents_dev: *const i32, status_dev: *mut i32) -> itak_status;
+    pub fn itak_paged_batch_rows_device(paged: *mut itak_paged, positions_dev: *mut i64, slots_dev: *mut i64) -> itak_status;
+    pub fn itak_paged_accept_device(paged: *mut itak_paged, tokens_dev: *const i32, chosen_dev: *const i32, path_dev: *mut i32, next_dev: *mut i32) -> itak_status;
+    pub fn itak_paged_keep_device(paged: *mut itak_paged, path_dev: *const i32, lengths_dev: *mut i32) -> itak_status;
     pub fn itak_set_debug_enabled(enabled: i32);
     pub fn itak_debug_enabled() -> i32;
     pub fn itak_probe_copy_device(pool: *mut itak_pool, src_dev: *const c_void, dst_dev: *mut c_void, bytes: u64) -> itak_status;

@@ -831,6 +831,82 @@ itak_status itak_paged_step_device(itak_paged *paged, uint64_t layer, const itak
                                    const itak_rows *v, const itak_rows *out, float scale, float softcap, uint64_t window,
                                    const itak_rotation *rotation);
 
+/* ---- trees of drafted tokens, and batches that the device makes -----------------------------
+   A sequence's new rows may be a tree: each row with the number of an earlier row of the sequence that it continues, its parent, or -1
+   of one that continues the held positions themselves. Row r lies in the pages at position item.position + r, as any
+   row, and stands in the text at item.position + its depth, the number of rows above it: by that it is turned, and from there a
+   window is counted. It sees the held positions (of its window), the rows above it and itself. Append, attention and step are the calls above: a tree is
+   the batch's. After the forward itak_paged_accept_device walks down the tree, and itak_paged_keep_device moves the
+   accepted rows to where a sequence's next positions lie. No counterpart in the reference, whose drafts are chains
+   (crates/itak-spec/src/session.rs:616-831).
+
+   Lengths, page tables and trees may also lie on the device, where such a walk leaves them: itak_paged_fit_tables_device and
+   itak_paged_set_batch_device take them there, and a whole round can be captured into one graph. */
+
+/* What became of a sequence in the calls that read the device's lengths and tables. */
+enum {
+    ITAK_TABLE_OK = 0,
+    ITAK_TABLE_POSITION = 1, /* a length below 0, or beyond what the call takes */
+    ITAK_TABLE_PAGES = 2,    /* fewer pages than the positions need, or a number of pages that no table has */
+    ITAK_TABLE_ID = 3,       /* a page id beyond the pages */
+    ITAK_TABLE_PARENTS = 4,  /* parents that are no tree's */
+    ITAK_TABLE_ROOM = 5,     /* more page ids than max_table_pages over the batch */
+    ITAK_TABLE_FREE = 6      /* the free list has too few pages, or a number of them that it cannot have */
+};
+
+/* Page tables on the device, the caller's memory: sequence i's pages are table[i * stride ..], pages[i] of them, up to `stride`. The free list
+   is free_ids[0 .. *free_count), of page_count words. */
+typedef struct itak_page_tables {
+    uint32_t *table;
+    uint64_t stride;     /* 1 .. 2^28 */
+    int32_t *pages;      /* [sequences] */
+    uint32_t *free_ids;  /* [page_count]; of itak_paged_fit_tables_device alone, as the next */
+    int32_t *free_count;
+    uint32_t sequences;  /* up to max_sequences */
+    uint32_t reserved;   /* 0 */
+} itak_page_tables;
+
+/* Makes a paged cache one that takes trees, of up to `most_rows` rows a batch (below 2^24; 52 bytes of device memory each). Once; not while its
+   stream is being captured. From then on sequences without rows count among a batch's, and attention that is captured is right for batches with
+   trees and without; what was captured before takes every row for one that sees all before it. */
+itak_status itak_paged_enable_trees(itak_paged *paged, uint64_t most_rows);
+/* itak_paged_set_batch with the parents of all new rows in order: [sum rows] in host memory, each -1 or the number of a row before it among its
+   own item's. An item whose every row continues the one before is no tree but a chain, of any length; a tree has up to 256 rows. A
+   window of an attention or step over the batch is 0 or at least as long as its largest tree has rows. */
+itak_status itak_paged_set_batch_tree(itak_paged *paged, const itak_paged_item *items, uint32_t count, const uint32_t *pages,
+                                      uint64_t page_ids, const int32_t *parents);
+/* Page tables to lengths: sequence i gets or gives back pages until it has those of lengths_dev[i] + rows[i] positions (rows: host memory,
+   [sequences]; NULL: none on top). What is given back is there to be taken in the same call. Pages are taken from the free list's end, by sequences
+   in order and by a sequence in the order of its table, and given back so that taking them again finds the same ones. A sequence is refused,
+   and left as it was, where pages or length are none, and where the list does not hold what it and all sequences before it ask for.
+   status_dev: [sequences] ITAK_TABLE_*, or NULL. One launch, on the handle's stream; it may be captured (rows as they are then). The
+   batch stays as it is. A table names no page twice, and no other sequence's: that is not looked for. */
+itak_status itak_paged_fit_tables_device(itak_paged *paged, const itak_page_tables *tables, const int32_t *lengths_dev, const uint32_t *rows,
+                                         int32_t *status_dev);
+/* The batch from positions and tables on the device: sequence i is an item of rows[i] new rows (host memory, [sequences]) behind positions_dev[i],
+   parents_dev [sum rows] as for itak_paged_set_batch_tree or NULL. A sequence whose position is below 0 or beyond most_positions, whose table
+   has too few pages or names one beyond the pages, or whose parents are no tree's is left out: nothing is written for its rows, in the
+   pages or in outputs. status_dev: [sequences] ITAK_TABLE_*, or NULL. What the host refuses and plans is for most_positions; a window has to be as long
+   as the most rows of an item of up to 256, where there are parents. Pages that take new rows and are named twice are not looked for: such rows are
+   lost. It may be captured, with the rows of then; a batch that a replay sets is not the one that eager calls after it know, so that
+   one is set for those again. */
+itak_status itak_paged_set_batch_device(itak_paged *paged, const itak_page_tables *tables, const int32_t *positions_dev, const uint32_t *rows,
+                                        uint64_t most_positions, const int32_t *parents_dev, int32_t *status_dev);
+/* Of every row of the batch its position in the text (item.position + depth) and its slot: page * page_rows + the row in the page. [sum rows]
+   each, either may be NULL; -1 of rows that the batch has left out. */
+itak_status itak_paged_batch_rows_device(itak_paged *paged, int64_t *positions_dev, int64_t *slots_dev);
+/* The accepted path of every sequence with rows: row 0, then as long as there is one the lowest-numbered child whose token is the one chosen at its
+   parent. tokens_dev: [sum rows] the rows' own tokens; chosen_dev: [sum rows] what the model chose behind each. path_dev: [sum rows], of a sequence
+   its path's row numbers and then -1; next_dev: [sequences of the batch] the choice at the path's last row (of sequences without rows, and left
+   out ones, as it was). The handle takes trees; a batch without them is chains. */
+itak_status itak_paged_accept_device(itak_paged *paged, const int32_t *tokens_dev, const int32_t *chosen_dev, int32_t *path_dev,
+                                     int32_t *next_dev);
+/* Keeps of every sequence the rows that its path names: row path[j] goes to position item.position + j, on every layer. path_dev as above, the row numbers
+   ascending up to the first -1. lengths_dev: [sequences of the batch] item.position + the rows kept, or NULL; -1, and nothing moved, where a path
+   does not ascend or names no row (of sequences without rows, and left out ones, as it was). Rows of the batch behind those kept are no sequence's
+   any more. The batch stays set as it was: another is set before the next forward. */
+itak_status itak_paged_keep_device(itak_paged *paged, const int32_t *path_dev, int32_t *lengths_dev);
+
 /* ---- debug channel ------------------------------------------------------------------- */
 
 /* attention::diag (crates/attention/src/diag.rs:13-33,71-79): one line per cache and

@@ -47,7 +47,7 @@ from .prefix_store import (  # noqa: F401
     prefix_store_enabled,
     prefix_store_enabled_from,
 )
-from .paged import PagedKv, Rotation, Rows  # noqa: F401
+from .paged import PagedKv, PageTables, Rotation, Rows  # noqa: F401
 from .resident import LayerInputCapture, ResidentTarget, SpecRoundRecord  # noqa: F401
 from . import _native  # noqa: F401
 
@@ -60,5 +60,5 @@ __all__ = [
     "EntryMeta", "PrefixHit", "PrefixStore", "StoreConfig", "StoreStats", "max_bytes_from",
     "now_unix", "prefix_store_enabled", "prefix_store_enabled_from",
     "LayerInputCapture", "ResidentTarget", "SpecRoundRecord",
-    "PagedKv", "Rotation", "Rows",
+    "PagedKv", "PageTables", "Rotation", "Rows",
 ]

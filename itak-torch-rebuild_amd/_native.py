@@ -34,6 +34,7 @@ STATUS_NAMES = {
 }
 KV_ERROR_FIRST, KV_ERROR_LAST = 21, 35
 ELEM_F32, ELEM_F16, ELEM_BF16 = 0, 1, 2
+TABLE_OK, TABLE_POSITION, TABLE_PAGES, TABLE_ID, TABLE_PARENTS, TABLE_ROOM, TABLE_FREE = range(7)
 ROTATION_PLAIN, ROTATION_LINEAR, ROTATION_YARN = 0, 1, 2
 LAYER_GLOBAL, LAYER_WINDOWED = 0, 1
 POOL_SCRUB_ON_TRUNCATE = 1
@@ -139,6 +140,11 @@ class PagedItem(C.Structure):
     _fields_ = [("position", C.c_uint64), ("rows", C.c_uint32), ("pages", C.c_uint32)]
 
 
+class PageTables(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("stride", C.c_uint64), ("pages", C.c_void_p), ("free_ids", C.c_void_p),
+                ("free_count", C.c_void_p), ("sequences", C.c_uint32), ("reserved", C.c_uint32)]
+
+
 _P = C.c_void_p
 _u32, _u64, _f32, _i32 = C.c_uint32, C.c_uint64, C.c_float, C.c_int32
 
@@ -239,6 +245,13 @@ PROTOTYPES = {
     "itak_paged_attention_device": (_i32, [_P, _u64, C.POINTER(Rows), C.POINTER(Rows), _f32, _f32, _u64, _P]),
     "itak_paged_step_device": (_i32, [_P, _u64, C.POINTER(Rows), C.POINTER(Rows), C.POINTER(Rows), C.POINTER(Rows), _f32, _f32,
                                       _u64, _P]),
+    "itak_paged_enable_trees": (_i32, [_P, _u64]),
+    "itak_paged_set_batch_tree": (_i32, [_P, C.POINTER(PagedItem), _u32, _P, _u64, _P]),
+    "itak_paged_fit_tables_device": (_i32, [_P, C.POINTER(PageTables), _P, _P, _P]),
+    "itak_paged_set_batch_device": (_i32, [_P, C.POINTER(PageTables), _P, _P, _u64, _P, _P]),
+    "itak_paged_batch_rows_device": (_i32, [_P, _P, _P]),
+    "itak_paged_accept_device": (_i32, [_P, _P, _P, _P, _P]),
+    "itak_paged_keep_device": (_i32, [_P, _P, _P]),
     "itak_set_debug_enabled": (None, [_i32]),
     "itak_debug_enabled": (_i32, []),
 }

@@ -4,6 +4,7 @@
 #include "rotation.h"
 
 #include "paged_table.h"
+#include "paged_tree.h"
 
 namespace itak {
 
@@ -37,6 +38,7 @@ struct PagedAppend {
     RowsView q, q_out;
     uint32_t pieces;       // of a row: queries', keys', values'
     uint32_t per_group;
+    const uint32_t *tree;  // the rows' records (paged_tree.h) of a handle that takes trees, else null
 };
 // `page_elem`, `elem`: ITAK_ELEM_* of the pages and the tensors; `by_8`: pieces of eight channels.
 hipError_t launch_paged_append(uint32_t page_elem, uint32_t elem, bool by_8, const PagedAppend &a, uint32_t rows,
@@ -87,19 +89,25 @@ struct PagedAttn {
     uint32_t start[kPagedInline], unit0[kPagedInline];  // where an item's blocks and units begin in the line
     float *ws_acc;       // [slots][tile][padded head_dim]
     float2 *ws_ml;       // [slots][tile]: maximum (log2 domain), sum; negative: of a part that is scaled down by kPagedMergeLift
+    const uint32_t *tree; // the rows' records (paged_tree.h): of a batch whose rows may be trees, else null
 };
 // Workgroups that may share a unit.
 constexpr uint32_t kPagedMostParts = 1024;
 // The kernel of few rows (paged_few_kernel.h): tiles of `sets` times 16 vectors, 1 or 2.
 constexpr uint32_t kPagedSet = 16;
 // Workgroups a compute unit holds: two where a lane does with 256 registers.
-__host__ __device__ constexpr uint32_t paged_few_groups_per_cu(uint32_t padded, uint32_t page_elem, uint32_t elem, uint32_t sets) {
-    return padded * sets <= (page_elem == ITAK_ELEM_BF16 && elem == ITAK_ELEM_F32 ? 64 : 128) ? 2 : 1;
+__host__ __device__ constexpr uint32_t paged_few_groups_per_cu(uint32_t padded, uint32_t page_elem, uint32_t elem, uint32_t sets, bool tree) {
+    return padded * sets <= (elem == ITAK_ELEM_F32 && (page_elem == ITAK_ELEM_BF16 || tree) ? 64 : 128) ? 2 : 1;
 }
 hipError_t launch_paged_few_f16(uint32_t sets, const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_few_f16_f32(uint32_t sets, const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_few_bf16(uint32_t sets, const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_few_bf16_f32(uint32_t sets, const PagedAttn &a, hipStream_t stream);
+// And of a batch whose rows may be trees (a.tree).
+hipError_t launch_paged_few_tree_f16(uint32_t sets, const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_few_tree_f16_f32(uint32_t sets, const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_few_tree_bf16(uint32_t sets, const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_few_tree_bf16_f32(uint32_t sets, const PagedAttn &a, hipStream_t stream);
 // The kernel of many rows (paged_chunk_kernel.h): 32 vectors a wavefront, four or eight wavefronts a tile.
 __host__ __device__ constexpr uint32_t paged_chunk_waves(uint32_t padded, uint32_t elem) {
     return padded == 64 || (padded == 128 && elem != ITAK_ELEM_F32) ? 8 : 4;
@@ -115,6 +123,10 @@ hipError_t launch_paged_chunk_f16(const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_chunk_f16_f32(const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_chunk_bf16(const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_chunk_bf16_f32(const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_chunk_tree_f16(const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_chunk_tree_f16_f32(const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_chunk_tree_bf16(const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_chunk_tree_bf16_f32(const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_merge(uint32_t elem, const PagedAttn &a, hipStream_t stream);
 // head_dim as the kernels hold it.
 __host__ __device__ constexpr uint32_t paged_padded(uint32_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
@@ -159,13 +171,16 @@ __device__ __forceinline__ uint32_t paged_row_of(const PagedAttn &a, uint32_t ve
     return a.group_magic ? __umulhi(vector, a.group_magic) : vector;
 }
 
+// Whether the rows of the batch at hand have records. (Of a captured launch the batch may be another than it was captured over.)
+__device__ __forceinline__ bool paged_has_trees(const PagedAttn &a) { return a.inline_items || a.batch[2]; }
+
 // Asks for all of the arguments at once: the compiler asks where it needs them, a trip to memory for every 64 bytes that come
 // first there (of the few rows' kernel four in a row, some 3,000 clocks before the first page id).
 __device__ __forceinline__ void paged_fetch_arguments(const PagedAttn &a) {
     static_assert(sizeof(PagedAttn) <= 9 * 64 && kPagedInline == 8, "a word of every 64 bytes is named");
     asm volatile("" ::"s"(a.batch), "s"(a.layer_base), "s"(a.q.data), "s"(a.out.data), "s"(a.rows), "s"(a.units), "s"(a.v_to), "s"(a.window),
                  "s"(a.zeros), "s"(a.total), "s"(a.item[1].row0), "s"(a.item[5].row0), "s"(a.start[1]), "s"(a.unit0[1]), "s"(a.ws_acc),
-                 "s"(a.ws_ml));
+                 "s"(a.ws_ml), "s"(a.tree));
 }
 
 // The items a launch takes, in order: where their blocks and units lie in the line. Those in memory are looked at 64 at a time, one

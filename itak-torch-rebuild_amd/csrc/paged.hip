@@ -1,8 +1,6 @@
 // Host side of the paged cache: the handle, its checks, the batch's way to the device, and which kernels a call launches.
 // Everything is checked before anything is enqueued.
-#include "paged.h"
-
-#include "errors.h"
+#include "paged_handle.h"
 
 #include <algorithm>
 #include <cfloat>
@@ -12,47 +10,10 @@
 
 using namespace itak;
 
-struct itak_paged {
-    itak_paged_config cfg{};
-    PagedGeom g{};
-    PagedLimits limits{};
-    uint64_t layer_stride = 0;  // elements
-    uint64_t bytes = 0;
-    unsigned char *storage = nullptr;
-    bool owns = false;
-    hipStream_t stream = nullptr;
-    uint32_t *batch_dev = nullptr;
-    uint64_t zeros_at = 0;           // words of the batch's memory up to sixteen bytes of zeros
-    PagedBatch batch;                // as it is set
-    PagedBatch next;                 // as it is being made
-    std::vector<uint32_t> ids_there; // page ids as the device has them, all of its table
-    std::vector<uint32_t> marks;
-    uint32_t stamp = 0;
-    // Buffers grow by being replaced, and what was replaced stays until the handle is gone: a captured graph may still name it.
-    std::vector<void *> buffers;
-    float *ws = nullptr;             // split partials
-    uint64_t ws_bytes = 0;
-    void *turned = nullptr;          // a step's rotated queries
-    uint64_t turned_bytes = 0;
-    // The most units that an attention call under capture has launched, of calls without a window and with one, whose largest it is.
-    struct Captured {
-        uint64_t units;
-        uint32_t window;
-    } captured[2] = {};
-    mutable ErrorState err;
-};
-
 namespace {
-
-#define HIP_TRY(paged, call, doing)                                       \
-    do {                                                                  \
-        const hipError_t _e = (call);                                     \
-        if (_e != hipSuccess) return hip_error((paged)->err, _e, doing);  \
-    } while (0)
 
 // Words of a batch on their way to the device travel as the arguments of launches that store them: in the stream's order, with
 // no host memory that has to outlive the call.
-constexpr uint32_t kFewWords = 112, kManyWords = 960;
 template <uint32_t N>
 struct Words {
     uint32_t *dst;
@@ -76,7 +37,9 @@ void send(uint32_t *dst, uint32_t at0, const uint32_t *w0, uint32_t n0, uint32_t
     std::copy(w1, w1 + n1, a.w + n0);
     launch_kernel(paged_words_kernel<N>, 1, 256, 0, stream, a);
 }
-void send_words(uint32_t *dst, uint32_t at0, const uint32_t *w0, uint32_t n0, uint32_t at1, const uint32_t *w1, uint32_t n1,
+}  // namespace
+
+void itak::send_words(uint32_t *dst, uint32_t at0, const uint32_t *w0, uint32_t n0, uint32_t at1, const uint32_t *w1, uint32_t n1,
                 hipStream_t stream) {
     if (n0 + n1 <= kFewWords)
         send<kFewWords>(dst, at0, w0, n0, at1, w1, n1, stream);
@@ -84,10 +47,7 @@ void send_words(uint32_t *dst, uint32_t at0, const uint32_t *w0, uint32_t n0, ui
         send<kManyWords>(dst, at0, w0, n0, at1, w1, n1, stream);
 }
 
-bool capturing(hipStream_t stream) {
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    return hipStreamIsCapturing(stream, &status) != hipSuccess || status != hipStreamCaptureStatusNone;
-}
+namespace {
 
 itak_status grow(itak_paged *p, void **buffer, uint64_t *have, uint64_t need, const char *what) {
     if (need <= *have) return ITAK_OK;
@@ -176,7 +136,8 @@ float score_scale(const itak_paged *p, uint32_t elem, float scale, float softcap
     return p->cfg.elem == ITAK_ELEM_F16 && elem == ITAK_ELEM_F32 ? x / kPagedQueryLift : x;
 }
 
-itak_status check_attention(itak_paged *p, uint64_t layer, const itak_rows *q, const itak_rows *out, float scale, float softcap) {
+itak_status check_attention(itak_paged *p, uint64_t layer, const itak_rows *q, const itak_rows *out, float scale, float softcap,
+                            uint64_t window) {
     itak_status st = check_layer(p, layer);
     if (st == ITAK_OK) st = check_tensor(p, "q", q, 0, ~0u, false);
     if (st == ITAK_OK) st = check_tensor(p, "out", out, q->heads, q->elem, true);
@@ -185,6 +146,9 @@ itak_status check_attention(itak_paged *p, uint64_t layer, const itak_rows *q, c
     if (q->heads % p->cfg.num_kv_heads) return non_divisible(p->err, q->heads, p->cfg.num_kv_heads);
     if (q->heads / p->cfg.num_kv_heads > 64) return unsupported(p->err, "more than 64 query heads a KV head");
     if (q->heads > 65535) return unsupported(p->err, "more than 65535 query heads");
+    if (window && window < p->batch.tree_most)
+        return set_error(p->err, ITAK_UNSUPPORTED, "window", p->batch.tree_most, window, 0, 0,
+                         "unsupported: a window of %llu over a tree of %u rows", ULL(window), p->batch.tree_most);
     if (std::isinf(scale)) return invalid_argument(p->err, "scale is infinite");
     if (!(softcap >= 0.0f) || std::isinf(softcap)) return invalid_argument(p->err, "softcap must be finite and >= 0");
     if (softcap > 0.0f) {
@@ -298,7 +262,9 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
     if (uint64_t(a.rows) * group >= (1ull << 26)) return size_overflow(p->err, "query vectors of the batch");
     // (A call that is being captured is replayed over other batches.)
     const bool captured = capturing(p->stream);
-    if (a.items <= kPagedInline && !captured) {
+    // A handle that takes trees captures launches that find out whether the batch has them.
+    if (p->batch.trees || (captured && p->tree_dev)) a.tree = p->tree_dev;
+    if (a.items <= kPagedInline && !captured && !p->batch.on_device) {
         a.inline_items = a.items;
         for (PagedItemWords &w : a.item) w.row0 = ~0u;
         std::memcpy(a.item, p->batch.head.data() + kPagedItem0, a.items * sizeof(PagedItemWords));
@@ -343,45 +309,58 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
         a.tile = plan.sets * kPagedSet;
         a.tile_shift = shift_of(a.tile);
         a.v_from = 1, a.v_to = chunks ? few_most : ~0u;
-        a.groups = std::min(cus * paged_few_groups_per_cu(dp, p->cfg.elem, q.elem, plan.sets), kPagedMostParts);
+        a.groups = std::min(cus * paged_few_groups_per_cu(dp, p->cfg.elem, q.elem, plan.sets, a.tree != nullptr), kPagedMostParts);
         a.least = 4;
         a.parts = 0;
         const itak_status st = count_units(p, a, work, whole);
         if (st != ITAK_OK) return st;
-        plan.merge_few = captured || !whole;
+        plan.merge_few = captured || p->batch.on_device || !whole;
     }
     const itak_status st = workspace(p, plan, dp);
     if (st == ITAK_OK && captured) {
         itak_paged::Captured &c = p->captured[a.window ? 1 : 0];
         c.units = std::max<uint64_t>({c.units, plan.few.units, plan.many.units});
         c.window = std::max(c.window, a.window);
+        if (a.window && p->tree_dev) c.least_window = c.least_window ? std::min(c.least_window, a.window) : a.window;
     }
     return st;
 }
 
-// Whether the captured calls' replays over a batch of these words (of as many units) can count their blocks.
-bool replays_hold(const itak_paged *p, const std::vector<uint32_t> &head) {
-    for (const itak_paged::Captured &c : p->captured)
+}  // namespace
+
+// Whether the captured calls' replays over a batch (of as many units) can count their blocks, and whether its trees fit their windows.
+bool itak::paged_replays_hold(const itak_paged *p, const PagedBatch &batch) {
+    const std::vector<uint32_t> &head = batch.head;
+    for (const itak_paged::Captured &c : p->captured) {
         for (size_t at = kPagedItem0; c.units && at < head.size(); at += 4) {
             const uint32_t blocks = (head[at] + head[at + 1] + 31) / 32 - paged_first_block(head[at], c.window);
             if (c.units * blocks >= kMostBlocks) return false;
         }
+        if (c.least_window && batch.tree_most > c.least_window) return false;
+    }
     return true;
 }
 
+namespace {
+
 itak_status run_attention(itak_paged *p, uint32_t elem, const AttnPlan &plan) {
+    const bool trees = plan.few.tree != nullptr;
     if (plan.sets) {
         const hipError_t he =
             p->cfg.elem == ITAK_ELEM_F16
-                ? (elem == ITAK_ELEM_F32 ? launch_paged_few_f16_f32 : launch_paged_few_f16)(plan.sets, plan.few, p->stream)
-                : (elem == ITAK_ELEM_F32 ? launch_paged_few_bf16_f32 : launch_paged_few_bf16)(plan.sets, plan.few, p->stream);
+                ? (elem == ITAK_ELEM_F32 ? (trees ? launch_paged_few_tree_f16_f32 : launch_paged_few_f16_f32)
+                                           : (trees ? launch_paged_few_tree_f16 : launch_paged_few_f16))(plan.sets, plan.few, p->stream)
+                : (elem == ITAK_ELEM_F32 ? (trees ? launch_paged_few_tree_bf16_f32 : launch_paged_few_bf16_f32)
+                                         : (trees ? launch_paged_few_tree_bf16 : launch_paged_few_bf16))(plan.sets, plan.few, p->stream);
         HIP_TRY(p, he, "launch paged attention of few rows");
         if (plan.merge_few) HIP_TRY(p, launch_paged_merge(elem, plan.few, p->stream), "launch the merge of paged attention");
     }
     if (plan.has_many) {
         const hipError_t he = p->cfg.elem == ITAK_ELEM_F16
-                                  ? (elem == ITAK_ELEM_F32 ? launch_paged_chunk_f16_f32 : launch_paged_chunk_f16)(plan.many, p->stream)
-                                  : (elem == ITAK_ELEM_F32 ? launch_paged_chunk_bf16_f32 : launch_paged_chunk_bf16)(plan.many, p->stream);
+                                  ? (elem == ITAK_ELEM_F32 ? (trees ? launch_paged_chunk_tree_f16_f32 : launch_paged_chunk_f16_f32)
+                                                           : (trees ? launch_paged_chunk_tree_f16 : launch_paged_chunk_f16))(plan.many, p->stream)
+                                  : (elem == ITAK_ELEM_F32 ? (trees ? launch_paged_chunk_tree_bf16_f32 : launch_paged_chunk_bf16_f32)
+                                                           : (trees ? launch_paged_chunk_tree_bf16 : launch_paged_chunk_bf16))(plan.many, p->stream);
         HIP_TRY(p, he, "launch paged attention of many rows");
         if (plan.many.parts > 1) HIP_TRY(p, launch_paged_merge(elem, plan.many, p->stream), "launch the merge of paged attention");
     }
@@ -394,6 +373,7 @@ itak_status run_append(itak_paged *p, uint64_t layer, const itak_rows &k, const 
     PagedAppend a{};
     a.g = p->g;
     a.batch = p->batch_dev;
+    a.tree = p->tree_dev;
     a.layer_base = layer_base(p, layer);
     a.k = rows_view(k, d);
     a.v = rows_view(v, d);
@@ -416,6 +396,7 @@ itak_status run_append_queries(itak_paged *p, const itak_rows &q, const itak_row
     a.g = p->g;
     a.g.kv_heads = 0;
     a.batch = p->batch_dev;
+    a.tree = p->tree_dev;
     a.r = rotation_view(rotation);
     a.q = rows_view(q, d);
     a.q_out = rows_view(q_out, d);
@@ -433,18 +414,50 @@ itak_status turned_rows(itak_paged *p, const itak_rows &q, itak_rows &out) {
     return st;
 }
 
-itak_status set_batch(itak_paged *p, const itak_paged_item *items, uint32_t count, const uint32_t *pages, uint64_t page_ids) {
+// Whether the parents of a batch's new rows make trees; the largest tree's rows.
+itak_status check_trees(itak_paged *p, const itak_paged_item *items, uint32_t count, const int32_t *parents, uint32_t rows, uint32_t &most) {
+    if (!p->tree_dev) return unsupported(p->err, "a batch of trees of a paged cache that takes none (itak_paged_enable_trees)");
+    if (rows > p->tree_rows)
+        return set_error(p->err, ITAK_CAPACITY_EXCEEDED, "rows of trees", rows, p->tree_rows, 0, 0,
+                         "a batch of trees of %u rows, the paged cache takes %llu", rows, ULL(p->tree_rows));
+    most = 0;
+    for (uint32_t i = 0; i < count; parents += items[i].rows, ++i) {
+        const uint64_t n = items[i].rows, wrong = tree_first_wrong(parents, n);
+        if (wrong < n)
+            return set_error(p->err, ITAK_INVALID_ARGUMENT, "parents", i, wrong, 0, 0,
+                             "invalid argument: item %u: the parent of row %llu is %d, no row before it and not -1", i, ULL(wrong),
+                             int(parents[wrong]));
+        if (tree_is_chain(parents, n)) continue;
+        if (n > kTreeRows)
+            return set_error(p->err, ITAK_UNSUPPORTED, "rows of a tree", i, n, 0, 0,
+                             "unsupported: item %u: a tree of %llu rows, of more than %u only chains are taken", i, ULL(n), kTreeRows);
+        most = std::max(most, uint32_t(n));
+    }
+    return ITAK_OK;
+}
+
+itak_status set_batch(itak_paged *p, const itak_paged_item *items, uint32_t count, const uint32_t *pages, uint64_t page_ids,
+                      const int32_t *parents) {
     if (capturing(p->stream)) return invalid_argument(p->err, "the batch is set while the stream is being captured");
-    const PagedRefusal r = make_paged_batch(p->limits, items, count, pages, page_ids, p->marks, p->stamp, p->next);
+    PagedBatch &next = p->next;
+    const PagedRefusal r = make_paged_batch(p->limits, items, count, pages, page_ids, p->marks, p->stamp, next, p->tree_dev != nullptr);
     if (r.code != ITAK_OK) return set_error(p->err, r.code, r.what, r.a, r.b, 0, 0, "%s", r.text.c_str());
-    if (!replays_hold(p, p->next.head)) return size_overflow(p->err, "blocks of a captured attention over the batch");
+    next.trees = parents != nullptr, next.on_device = false, next.tree_most = 0;
+    if (parents) {
+        const itak_status st = check_trees(p, items, count, parents, next.rows, next.tree_most);
+        if (st != ITAK_OK) return st;
+        next.head[2] = 1;
+    }
+    if (!paged_replays_hold(p, next)) return size_overflow(p->err, "a captured attention over the batch");
     const DeviceScope scope(p->cfg.device);
     HIP_TRY(p, scope.status(), "set the device");
     // The items go up every time, page ids where they are not what the device has: of a sequence that grows, one every
     // page_rows tokens.
-    const std::vector<uint32_t> &head = p->next.head, &ids = p->next.ids;
+    const std::vector<uint32_t> &head = next.head, &ids = next.ids;
     const uint32_t ids_at = p->g.ids_at;
     uint32_t lo = 0, hi = uint32_t(ids.size());
+    if (!p->ids_known || p->ids_never_known) std::fill(p->ids_there.begin(), p->ids_there.end(), ~0u);
+    p->ids_known = true;
     while (lo < hi && p->ids_there[lo] == ids[lo]) ++lo;
     while (hi > lo && p->ids_there[hi - 1] == ids[hi - 1]) --hi;
     // What the device has is unknown from the first launch to the last.
@@ -461,7 +474,16 @@ itak_status set_batch(itak_paged *p, const itak_paged_item *items, uint32_t coun
         send_words(p->batch_dev, ids_at + lo, ids.data() + lo, n, 0, nullptr, 0, p->stream);
         lo += n;
     }
-    if (hipError_t he = hipGetLastError(); he != hipSuccess) {
+    hipError_t he = hipSuccess;
+    if (parents && next.rows) {
+        uint32_t *const there = p->tree_dev + p->tree_rows * kTreeStride;
+        const uint32_t *words = reinterpret_cast<const uint32_t *>(parents);
+        for (uint32_t at = 0; at < next.rows; at += kManyWords)
+            send_words(there, at, words + at, std::min(next.rows - at, kManyWords), 0, nullptr, 0, p->stream);
+        he = launch_paged_records(p->batch_dev, next.items, reinterpret_cast<const int32_t *>(there), p->tree_dev, p->stream);
+    }
+    if (he == hipSuccess) he = hipGetLastError();
+    if (he != hipSuccess) {
         std::fill(p->ids_there.begin(), p->ids_there.end(), ~0u);
         p->batch = PagedBatch{};
         return hip_error(p->err, he, "send a batch to the device");
@@ -512,9 +534,10 @@ itak_status itak_paged_create(const itak_paged_config *config, itak_paged **out)
     const DeviceScope scope(config->device);
     he = scope.status();
     p->zeros_at = (p->g.ids_at + p->cfg.max_table_pages + 3) / 4 * 4;
-    const uint64_t words = (p->zeros_at + 4) * sizeof(uint32_t);
+    const uint64_t words = (p->zeros_at + 4 + config->max_sequences) * sizeof(uint32_t);
     if (he == hipSuccess) he = hipMalloc(reinterpret_cast<void **>(&p->batch_dev), words);
     if (he == hipSuccess) he = hipMemset(p->batch_dev, 0, words);  // (an empty batch)
+    if (he == hipSuccess) p->rows_dev = p->batch_dev + p->zeros_at + 4;
     p->storage = static_cast<unsigned char *>(config->storage);
     p->owns = !config->storage;
     if (he == hipSuccess && p->owns) {
@@ -541,6 +564,7 @@ void itak_paged_destroy(itak_paged *paged) {
     const DeviceScope scope(paged->cfg.device);
     (void)hipStreamSynchronize(paged->stream);
     if (paged->batch_dev) (void)hipFree(paged->batch_dev);
+    if (paged->tree_dev) (void)hipFree(paged->tree_dev);
     if (paged->owns && paged->storage) (void)hipFree(paged->storage);
     for (void *b : paged->buffers) (void)hipFree(b);
     delete paged;
@@ -575,7 +599,18 @@ itak_status itak_paged_set_batch(itak_paged *paged, const itak_paged_item *items
                                  uint64_t page_ids) {
     if (!paged) return ITAK_INVALID_ARGUMENT;
     try {
-        return set_batch(paged, items, count, pages, page_ids);
+        return set_batch(paged, items, count, pages, page_ids, nullptr);
+    } catch (const std::bad_alloc &) {
+        return invalid_argument(paged->err, "out of host memory");
+    }
+}
+
+itak_status itak_paged_set_batch_tree(itak_paged *paged, const itak_paged_item *items, uint32_t count, const uint32_t *pages,
+                                      uint64_t page_ids, const int32_t *parents) {
+    if (!paged) return ITAK_INVALID_ARGUMENT;
+    if (!parents) return invalid_argument(paged->err, "parents are null");
+    try {
+        return set_batch(paged, items, count, pages, page_ids, parents);
     } catch (const std::bad_alloc &) {
         return invalid_argument(paged->err, "out of host memory");
     }
@@ -597,7 +632,7 @@ itak_status itak_paged_append_device(itak_paged *paged, uint64_t layer, const it
 itak_status itak_paged_attention_device(itak_paged *paged, uint64_t layer, const itak_rows *q, const itak_rows *out, float scale,
                                         float softcap, uint64_t window, const itak_rotation *rotation) {
     if (!paged) return ITAK_INVALID_ARGUMENT;
-    itak_status st = check_attention(paged, layer, q, out, scale, softcap);
+    itak_status st = check_attention(paged, layer, q, out, scale, softcap, window);
     if (st == ITAK_OK) st = check_rotation(paged, rotation);
     if (st != ITAK_OK || paged->batch.rows == 0) return st;
     const DeviceScope scope(paged->cfg.device);
@@ -618,7 +653,7 @@ itak_status itak_paged_step_device(itak_paged *paged, uint64_t layer, const itak
                                    const itak_rows *out, float scale, float softcap, uint64_t window,
                                    const itak_rotation *rotation) {
     if (!paged) return ITAK_INVALID_ARGUMENT;
-    itak_status st = check_attention(paged, layer, q, out, scale, softcap);
+    itak_status st = check_attention(paged, layer, q, out, scale, softcap, window);
     if (st == ITAK_OK) st = check_tensor(paged, "k", k, paged->cfg.num_kv_heads, q->elem, false);
     if (st == ITAK_OK) st = check_tensor(paged, "v", v, paged->cfg.num_kv_heads, q->elem, false);
     if (st == ITAK_OK) st = check_rotation(paged, rotation);

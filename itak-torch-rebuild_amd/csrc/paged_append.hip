@@ -21,8 +21,10 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedAppend a) {
     uint4 item;
     if (!paged_item_of_row(a.batch, row, item)) return;  // (the same for the whole workgroup)
     const uint32_t position = item.x + (row - item.z);
+    // (A row of a tree is turned by its depth.)
+    const uint32_t turned_by = a.tree && a.batch[2] ? item.x + tree_depth(a.tree[uint64_t(row) * kTreeStride]) : position;
     const uint32_t page = a.batch[item.w + (position >> a.g.page_shift)];
-    if (tid < a.r.half) cs[tid] = turn_of(a.r, double(position), tid);
+    if (tid < a.r.half) cs[tid] = turn_of(a.r, double(turned_by), tid);
     __syncthreads();
     P *const base = reinterpret_cast<P *>(a.layer_base) + page * a.g.page_stride +
                     uint64_t(position & ((1u << a.g.page_shift) - 1)) * a.g.head_dim;

@@ -34,7 +34,7 @@ constexpr float kCarefulScale = PAGE == ITAK_ELEM_F16 ? 1.0f : 1.0f / kPagedMerg
 // the log2 domain, sum), accumulators and sum scaled. kCareful vectors at once, so that a row is fetched once for them, and 64 keys: a lane has the scores
 // of one key; then the lanes are channels.
 constexpr uint32_t kCareful = 4;
-template <int PAGE, int ELEM, int DP, typename W>
+template <int PAGE, int ELEM, int DP, bool TREE, typename W>
 __device__ __forceinline__ void paged_careful(const PagedAttn &a, const PagedSpan &span, uint32_t head, uint32_t v0, uint32_t v_end,
                                            uint32_t wave, uint32_t waves, uint32_t key0, uint32_t key1, W write) {
     typedef typename Elem<ELEM>::type T;
@@ -44,13 +44,25 @@ __device__ __forceinline__ void paged_careful(const PagedAttn &a, const PagedSpa
     const uint32_t lane = __lane_id(), d = a.g.head_dim, page_mask = (1u << a.g.page_shift) - 1;
     const P *const base = reinterpret_cast<const P *>(a.layer_base) + head * a.g.head_stride;
     const uint32_t *ids = a.batch + span.table;
+    const bool trees = TREE && paged_has_trees(a);
     for (uint32_t v = v0 + wave * kCareful; v < v_end; v += waves * kCareful) {
         uint32_t lo[kCareful], hi[kCareful], from = key1, to = key0;
         float q[kCareful][kRuns], acc[kCareful][kRuns], m[kCareful], sum[kCareful];
+        [[maybe_unused]] const uint32_t *record[kCareful];
+        [[maybe_unused]] uint32_t word[kCareful];
+        // Whether a vector sees a key between its lowest and its highest.
+        auto sees = [&](uint32_t u, uint32_t key) {
+            if constexpr (TREE) return (tree_sees(record[u], word[u], key / 32, span.position / 32) >> key % 32 & 1) != 0;
+            return true;
+        };
 #pragma unroll
         for (uint32_t u = 0; u < kCareful; ++u) {
             const uint32_t mine = min(v + u, v_end - 1), row = paged_row_of(a, mine), pos = span.position + row;
-            lo[u] = max(lowest_visible(pos, a.window, 0), key0), hi[u] = min(pos + 1, key1);
+            if constexpr (TREE) {
+                record[u] = a.tree + uint64_t(span.row0 + row) * kTreeStride;
+                word[u] = trees ? record[u][kTreeDepth] : kTreeChain | row;
+            }
+            lo[u] = max(lowest_visible(TREE ? span.position + tree_depth(word[u]) : pos, a.window, 0), key0), hi[u] = min(pos + 1, key1);
             if (lo[u] < hi[u]) from = min(from, lo[u]), to = max(to, hi[u]);
             const T *src = static_cast<const T *>(a.q.data) + uint64_t(span.row0 + row) * a.q.row_stride +
                            (head * a.group + mine - row * a.group) * a.q.head_stride;
@@ -80,10 +92,10 @@ __device__ __forceinline__ void paged_careful(const PagedAttn &a, const PagedSpa
             bool every = true;  // (vector sees every key of these)
 #pragma unroll
             for (uint32_t u = 0; u < kCareful; ++u) {
-                every = every && at >= lo[u] && at + n <= hi[u];
+                every = every && at >= lo[u] && at + n <= (trees ? min(hi[u], span.position) : hi[u]);
                 x[u] *= a.scale_log2 * kQueryLift<PAGE, ELEM>;
                 if (a.cap_log2 != 0.0f) x[u] = softcapped<true>(x[u], a.cap_log2, 0.0f);
-                const bool seen = lane < n && key >= lo[u] && key < hi[u];
+                const bool seen = lane < n && key >= lo[u] && key < hi[u] && sees(u, key);
                 float most = seen ? fmaxf(m[u], x[u]) : m[u];
 #pragma unroll
                 for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
@@ -111,7 +123,7 @@ __device__ __forceinline__ void paged_careful(const PagedAttn &a, const PagedSpa
                 for (uint32_t t = 0; t < kKeys; ++t)
 #pragma unroll
                     for (uint32_t u = 0; u < kCareful; ++u)
-                        if (kKeys > 1 || (at + j >= lo[u] && at + j < hi[u]))
+                        if (kKeys > 1 || (at + j >= lo[u] && at + j < hi[u] && sees(u, at + j)))
 #pragma unroll
                             for (int c = 0; c < kRuns; ++c) acc[u][c] = __builtin_fmaf(lane_of(p[u], j + t), y[t][c], acc[u][c]);
             };

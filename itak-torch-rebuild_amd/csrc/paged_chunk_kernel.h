@@ -63,7 +63,8 @@ constexpr size_t chunk_lds(int dp) { return size_t(kChunkStages) * chunk_subs(dp
 
 // Scores without a cap, capped by the short form, capped by the series (paged_cap_by_series).
 enum ChunkCap { kNoCap, kShortCap, kSeriesCap };
-template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP, ChunkCap CAP>
+// TREE: rows may be trees, and what a row sees behind the held positions is in its record; the tile's words lie in LDS.
+template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP, ChunkCap CAP, bool TREE>
 __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_kernel(PagedAttn a) {
     typedef typename Elem<ELEM>::type T;
     constexpr int kWaves = paged_chunk_waves(DP, ELEM);
@@ -81,6 +82,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     constexpr int kStageLoads = kLoads * kSubs;
     extern __shared__ __attribute__((aligned(16))) unsigned char ring[];
     __shared__ uint32_t lds_flag;
+    __shared__ uint32_t lds_sees[TREE ? kTreeBlocks : 1][TREE ? kTile : 1];
 
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const uint32_t h = lane >> 5, j = lane & 31;
@@ -99,7 +101,9 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     const uint32_t vectors = span.rows * a.group, v0 = tile * kTile;
     // Keys the tile's rows see, and this workgroup's blocks of them.
     const uint32_t first_row = paged_row_of(a, v0), last_row = min(paged_row_of(a, v0 + kTile - 1), span.rows - 1);
-    const uint32_t tile_lo = lowest_visible(span.position + first_row, a.window, 0), tile_hi = span.position + last_row + 1;
+    // (A row of a tree is turned by less than its number, and may see nothing of the rows before it.)
+    const bool trees = TREE && paged_has_trees(a);
+    const uint32_t tile_lo = lowest_visible(span.position + (trees ? 0 : first_row), a.window, 0), tile_hi = span.position + last_row + 1;
     const uint32_t b_first = tile_lo / 32, b_all = (tile_hi + 31) / 32 - b_first, b_part = (b_all + a.parts - 1) / a.parts;
     const uint32_t kb0 = b_first + min(b_all, part * b_part), kb_end = b_first + min(b_all, part * b_part + b_part);
     const uint64_t slot0 = uint64_t(unit * a.parts + part) * kTile;
@@ -107,7 +111,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     // Positions all of this wavefront's rows see.
     const uint32_t wv0 = v0 + wave * 32;
     const uint32_t w_first = min(paged_row_of(a, wv0), span.rows - 1), w_last = min(paged_row_of(a, wv0 + 31), span.rows - 1);
-    const uint32_t every_lo = lowest_visible(span.position + w_last, a.window, 0), every_hi = span.position + w_first + 1;
+    const uint32_t every_lo = lowest_visible(span.position + w_last, a.window, 0), every_hi = span.position + (trees ? 0 : w_first + 1);
     // Blocks all of which they all see: from inner0 on, `inner` of them.
     const uint32_t inner0 = __builtin_amdgcn_readfirstlane((every_lo + 31) / 32);
     const uint32_t inner = __builtin_amdgcn_readfirstlane(every_hi / 32 > inner0 ? every_hi / 32 - inner0 : 0);
@@ -171,12 +175,26 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     // The queries as B operands: column j, channels 16 s + 8 h .. + 7.
     u32x4 q[NQ][kSteps];
     uint32_t my_pos, my_lo;
+    [[maybe_unused]] const uint32_t tree_block = span.position / 32;
     {
         const uint32_t v = wv0 + j;
         const uint32_t row = min(paged_row_of(a, v), span.rows - 1);
         const uint32_t hq = head * a.group + (v < vectors ? v - row * a.group : 0);
         my_pos = span.position + row;
-        my_lo = lowest_visible(my_pos, a.window, 0);
+        if constexpr (TREE) {
+            const uint32_t *const record = a.tree + uint64_t(span.row0 + row) * kTreeStride;
+            const uint32_t word = trees ? record[kTreeDepth] : kTreeChain | row;
+            my_lo = lowest_visible(span.position + tree_depth(word), a.window, 0);
+            // (The lanes of the two halves hold the same column: each brings every other word. No lane is turned off.)
+            uint32_t sees[kTreeBlocks / 2 + 1];
+#pragma unroll
+            for (uint32_t w = 0; w < kTreeBlocks / 2 + 1; ++w) sees[w] = record[kTreeSees + min(2 * w + h, kTreeBlocks - 1)];
+#pragma unroll
+            for (uint32_t w = 0; w < kTreeBlocks / 2 + 1; ++w)
+                lds_sees[min(2 * w + h, kTreeBlocks - 1)][wave * 32 + j] = word & kTreeChain ? ~0u : sees[w];
+        } else {
+            my_lo = lowest_visible(my_pos, a.window, 0);
+        }
         const T *src = static_cast<const T *>(a.q.data) + uint64_t(span.row0 + row) * a.q.row_stride + hq * a.q.head_stride;
         typename QueryRaw<ELEM>::type raw[kSteps];
         if (a.q_on_16) {
@@ -232,7 +250,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     floatx16 x;
     auto scaled = [&](float s) {
         if constexpr (CAP != kNoCap)
-            return softcapped<CAP == kSeriesCap>(s * a.scale_log2, a.cap_log2, ref);
+            return softcapped<CAP == kSeriesCap, TREE>(s * a.scale_log2, a.cap_log2, ref);
         else
             return __builtin_fmaf(s, a.scale_log2, -ref);
     };
@@ -241,10 +259,12 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     auto settle = [&](uint32_t kb, float most) {
         if (kb - inner0 >= inner) {
             most = -INFINITY;
+            uint32_t sees = ~0u;
+            if (TREE && kb >= tree_block) sees = lds_sees[min(kb - tree_block, kTreeBlocks - 1)][wave * 32 + j] >> 4 * h;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const uint32_t key = 32 * kb + 8 * (r / 4) + 4 * h + r % 4;
-                if (key > my_pos || key < my_lo) x[r] = -INFINITY;
+                if (key > my_pos || key < my_lo || (TREE && !(sees >> (8 * (r / 4) + r % 4) & 1))) x[r] = -INFINITY;
                 most = fmaxf(most, x[r]);
             }
         }
@@ -437,7 +457,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
         for (int r = 0; r < 16; ++r) check[r % 4] += EXACT || 32u * t + 8 * (r / 4) + 4 * h < d ? o[t][r] : 0.0f;
     const float all = (check[0] + check[1]) + (check[2] + check[3]);
     if (any_of_group(mine && to_be_done_over<PAGE>(all), &lds_flag)) {
-        paged_careful<PAGE, ELEM, DP>(a, span, head, v0, min(v0 + kTile, vectors), wave, kWaves, 32 * kb0, 32 * kb_end,
+        paged_careful<PAGE, ELEM, DP, TREE>(a, span, head, v0, min(v0 + kTile, vectors), wave, kWaves, 32 * kb0, 32 * kb_end,
                                       [&](uint32_t v, const float (&acc)[DP / 64], float m, float l) {
                                           paged_write_careful<PAGE, ELEM, DP>(a, span, head, v, whole, slot0 + v - v0, true, acc, m, l);
                                       });
@@ -487,27 +507,27 @@ hipError_t launch_chunk_kernel(const PagedAttn &a, hipStream_t stream) {
     launch_kernel(Kernel, a.units * a.parts, paged_chunk_waves(DP, ELEM) * 64, chunk_lds(DP), stream, a);
     return hipGetLastError();
 }
-template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP>
+template <bool TREE, int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP>
 hipError_t launch_chunk_as(const PagedAttn &a, hipStream_t stream) {
     if constexpr (!paged_chunk_takes(DP, PAGE, ELEM)) {
         return hipErrorInvalidValue;
     } else {
-        if (a.cap_log2 == 0.0f) return launch_chunk_kernel<&paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kNoCap>, ELEM, DP>(a, stream);
+        if (a.cap_log2 == 0.0f) return launch_chunk_kernel<&paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kNoCap, TREE>, ELEM, DP>(a, stream);
         if constexpr (ELEM != ITAK_ELEM_F32)
             if (!paged_cap_by_series(ELEM, a.cap_log2))
-                return launch_chunk_kernel<&paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kShortCap>, ELEM, DP>(a, stream);
-        return launch_chunk_kernel<&paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kSeriesCap>, ELEM, DP>(a, stream);
+                return launch_chunk_kernel<&paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kShortCap, TREE>, ELEM, DP>(a, stream);
+        return launch_chunk_kernel<&paged_chunk_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, kSeriesCap, TREE>, ELEM, DP>(a, stream);
     }
 }
-template <int PAGE, int ELEM, int NQ, int NP>
+template <int PAGE, int ELEM, int NQ, int NP, bool TREE = false>
 hipError_t launch_chunk(const PagedAttn &a, hipStream_t stream) {
     const uint32_t d = a.g.head_dim;
-    return d == 64    ? launch_chunk_as<PAGE, ELEM, 64, true, NQ, NP>(a, stream)
-           : d < 64   ? launch_chunk_as<PAGE, ELEM, 64, false, NQ, NP>(a, stream)
-           : d == 128 ? launch_chunk_as<PAGE, ELEM, 128, true, NQ, NP>(a, stream)
-           : d < 128  ? launch_chunk_as<PAGE, ELEM, 128, false, NQ, NP>(a, stream)
-           : d == 256 ? launch_chunk_as<PAGE, ELEM, 256, true, NQ, NP>(a, stream)
-                      : launch_chunk_as<PAGE, ELEM, 256, false, NQ, NP>(a, stream);
+    return d == 64    ? launch_chunk_as<TREE, PAGE, ELEM, 64, true, NQ, NP>(a, stream)
+           : d < 64   ? launch_chunk_as<TREE, PAGE, ELEM, 64, false, NQ, NP>(a, stream)
+           : d == 128 ? launch_chunk_as<TREE, PAGE, ELEM, 128, true, NQ, NP>(a, stream)
+           : d < 128  ? launch_chunk_as<TREE, PAGE, ELEM, 128, false, NQ, NP>(a, stream)
+           : d == 256 ? launch_chunk_as<TREE, PAGE, ELEM, 256, true, NQ, NP>(a, stream)
+                      : launch_chunk_as<TREE, PAGE, ELEM, 256, false, NQ, NP>(a, stream);
 }
 
 }  // namespace

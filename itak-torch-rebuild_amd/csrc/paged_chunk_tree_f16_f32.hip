@@ -1,0 +1,10 @@
+// The kernel of many rows over f16 pages, f32 tensors, of a batch whose rows may be trees.
+#include "paged_chunk_kernel.h"
+
+namespace itak {
+
+hipError_t launch_paged_chunk_tree_f16_f32(const PagedAttn &a, hipStream_t stream) {
+    return launch_chunk<ITAK_ELEM_F16, ITAK_ELEM_F32, 2, 2, true>(a, stream);
+}
+
+}  // namespace itak

@@ -38,20 +38,23 @@ struct FewShape {
     static constexpr int kTiles = DP / 16;                 // output tiles of 16 channels
 };
 
-template <int DP>
+template <int DP, int TREE_SETS>
 struct FewBlock {
     typedef FewShape<DP> S;
     u32x4 k[2][S::kSteps];
     uint32_t v[S::kHalves][8][S::kWide / 2];
+    uint32_t sees[TREE_SETS ? TREE_SETS : 1];  // what the lane's columns see of the block, where rows may be trees
 };
 
-// NQ, NP: pieces of the pages' type that a query and a weight enter the products as. EXACT: head_dim == DP. SETS of 16 vectors.
-template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP, int SETS>
-__global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, ELEM, SETS)) void paged_few_kernel(PagedAttn a) {
+// NQ, NP: pieces of the pages' type that a query and a weight enter the products as. EXACT: head_dim == DP. SETS of 16 vectors. TREE:
+// rows may be trees, and what a row sees behind the held positions is in its record; those words travel with the rows of the block.
+template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP, int SETS, bool TREE>
+__global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, ELEM, SETS, TREE)) void paged_few_kernel(PagedAttn a) {
     typedef FewShape<DP> S;
     typedef typename Elem<ELEM>::type T;
     // (Two blocks of 256 channels beside the accumulators are more than 512 registers.)
     constexpr bool kAhead = DP <= 128;
+    typedef FewBlock<DP, TREE ? SETS : 0> Block;
     constexpr int kTile = SETS * kSet;
     constexpr int kStride = DP + 4;  // floats from one vector to the next in LDS
     // Queries in several pieces, and those of a large tile, lie in LDS, where the four wavefronts share them, and not in
@@ -87,6 +90,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
         v_chan[h] = EXACT || c < d ? c : 0;
     }
     const uint32_t page_mask = (1u << a.g.page_shift) - 1;
+    const bool trees = TREE && paged_has_trees(a);
 
     while (at < end) {
         PagedSpan span;
@@ -99,22 +103,31 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
         const uint32_t vectors = span.rows * a.group, v0 = tile * kTile;
         const uint32_t first_row = paged_row_of(a, v0), last_row = min(paged_row_of(a, v0 + kTile - 1), span.rows - 1);
         // Positions some, and positions every row of the tile sees.
-        const uint32_t some_lo = lowest_visible(span.position + first_row, a.window, 0), some_hi = span.position + last_row + 1;
-        const uint32_t every_lo = lowest_visible(span.position + last_row, a.window, 0), every_hi = span.position + first_row + 1;
+        // (A row of a tree is turned by less than its number, and may see nothing of the rows before it.)
+        const uint32_t some_lo = lowest_visible(span.position + (trees ? 0 : first_row), a.window, 0), some_hi = span.position + last_row + 1;
+        const uint32_t every_lo = lowest_visible(span.position + last_row, a.window, 0), every_hi = span.position + (trees ? 0 : first_row + 1);
         // A lane's columns.
         uint32_t my_row[SETS], my_head[SETS];
+        [[maybe_unused]] uint32_t my_word[SETS];
 #pragma unroll
         for (int n = 0; n < SETS; ++n) {
             const uint32_t v = v0 + n * kSet + i;
             my_row[n] = min(paged_row_of(a, v), span.rows - 1);
             my_head[n] = head * a.group + (v < vectors ? v - my_row[n] * a.group : 0);
+            if constexpr (TREE) my_word[n] = trees ? a.tree[uint64_t(span.row0 + my_row[n]) * kTreeStride] : kTreeChain | my_row[n];
         }
 
         const uint32_t *ids = a.batch + span.table;
         const uint32_t last_page = (length - 1) >> a.g.page_shift;
         const uint64_t head_off = head * a.g.head_stride;
         auto page_of = [&](uint32_t key) { return ids[min(key >> a.g.page_shift, last_page)]; };
-        auto load = [&](uint32_t kb, uint32_t k_page, uint32_t v_page, FewBlock<DP> &b) {
+        auto load = [&](uint32_t kb, uint32_t k_page, uint32_t v_page, Block &b) {
+            if constexpr (TREE) {
+                if (32 * kb + 32 > span.position)
+#pragma unroll
+                    for (int n = 0; n < SETS; ++n)
+                        b.sees[n] = tree_sees(a.tree + uint64_t(span.row0 + my_row[n]) * kTreeStride, my_word[n], kb, span.position / 32);
+            }
             const uint16_t *kp = a.layer_base + k_page * a.g.page_stride + head_off +
                                  (((32 * kb + 8 * k_group) & page_mask) + k_row) * d;
 #pragma unroll
@@ -163,7 +176,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
             load_queries(std::true_type{});
         else
             load_queries(std::false_type{});
-        FewBlock<DP> block;
+        Block block;
         load(kb, kp, vp, block);  // (of a wavefront without a block whatever the last page holds)
         kp = page_of(32 * (kb + kFewWaves) + 8 * k_group), vp = page_of(32 * (kb + kFewWaves) + 8 * g);
         // The queries as B operands.
@@ -190,7 +203,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
             for (int t = 0; t < S::kTiles; ++t) o[n][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
-        auto multiply = [&](uint32_t kb, FewBlock<DP> &b) {
+        auto multiply = [&](uint32_t kb, Block &b) {
             const uint32_t key = 32 * kb + 8 * g;  // the lane's first
             if constexpr (!EXACT) {
 #pragma unroll
@@ -238,10 +251,12 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
                     for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf(x[e], a.scale_log2, -ref[n]);
                 }
                 if (edge) {
-                    const uint32_t pos = span.position + my_row[n], lo = lowest_visible(pos, a.window, 0);
+                    const uint32_t pos = span.position + my_row[n];
+                    const uint32_t lo = lowest_visible(TREE ? span.position + tree_depth(my_word[n]) : pos, a.window, 0);
+                    const uint32_t sees = TREE && 32 * kb + 32 > span.position ? b.sees[n] >> 8 * g : ~0u;
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        if (key + e > pos || key + e < lo) x[e] = -INFINITY;
+                        if (key + e > pos || key + e < lo || (TREE && !(sees >> e & 1))) x[e] = -INFINITY;
                 }
                 float most = max3(x[0], x[1], x[2]);
                 most = max3(most, x[3], x[4]);
@@ -292,7 +307,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
         if (kb < kb_end) {
             if constexpr (kAhead) {
                 for (; kb + kFewWaves < kb_end; kb += kFewWaves) {
-                    FewBlock<DP> next;
+                    Block next;
                     load(kb + kFewWaves, kp, vp, next);
                     kp = page_of(32 * (kb + 2 * kFewWaves) + 8 * k_group), vp = page_of(32 * (kb + 2 * kFewWaves) + 8 * g);
                     multiply(kb, block);
@@ -390,7 +405,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
         }
         if (any_of_group(bad, &lds_flag)) {
             const uint32_t kb0 = span.first + from;
-            paged_careful<PAGE, ELEM, DP>(a, span, head, v0, min(v0 + kTile, vectors), wave, kFewWaves, 32 * kb0, 32 * (kb0 + count),
+            paged_careful<PAGE, ELEM, DP, TREE>(a, span, head, v0, min(v0 + kTile, vectors), wave, kFewWaves, 32 * kb0, 32 * (kb0 + count),
                                           [&](uint32_t v, const float (&acc)[DP / 64], float m, float l) {
                                               paged_write_careful<PAGE, ELEM, DP>(a, span, head, v, whole, uint64_t(blockIdx.x + unit) * kTile + v - v0,
                                                                             blockIdx.x + unit < a.groups + a.units, acc, m, l);
@@ -400,31 +415,31 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
     }
 }
 
-template <int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP>
+template <bool TREE, int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP>
 void launch_few_as(uint32_t sets, const PagedAttn &a, hipStream_t stream) {
     // (Workgroups that would find nothing are left out where the batch is known.)
     const uint32_t groups = a.inline_items ? (a.total + a.share - 1) / a.share : a.groups;
     if (sets == 1) {
-        launch_kernel(paged_few_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, 1>, groups, kFewWaves * 64, 0, stream, a);
+        launch_kernel(paged_few_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, 1, TREE>, groups, kFewWaves * 64, 0, stream, a);
     } else {
-        launch_kernel(paged_few_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, 2>, groups, kFewWaves * 64, 0, stream, a);
+        launch_kernel(paged_few_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, 2, TREE>, groups, kFewWaves * 64, 0, stream, a);
     }
 }
-template <int PAGE, int ELEM, int NQ, int NP>
+template <int PAGE, int ELEM, int NQ, int NP, bool TREE = false>
 hipError_t launch_few(uint32_t sets, const PagedAttn &a, hipStream_t stream) {
     const uint32_t d = a.g.head_dim;
     if (d == 64)
-        launch_few_as<PAGE, ELEM, 64, true, NQ, NP>(sets, a, stream);
+        launch_few_as<TREE, PAGE, ELEM, 64, true, NQ, NP>(sets, a, stream);
     else if (d < 64)
-        launch_few_as<PAGE, ELEM, 64, false, NQ, NP>(sets, a, stream);
+        launch_few_as<TREE, PAGE, ELEM, 64, false, NQ, NP>(sets, a, stream);
     else if (d == 128)
-        launch_few_as<PAGE, ELEM, 128, true, NQ, NP>(sets, a, stream);
+        launch_few_as<TREE, PAGE, ELEM, 128, true, NQ, NP>(sets, a, stream);
     else if (d < 128)
-        launch_few_as<PAGE, ELEM, 128, false, NQ, NP>(sets, a, stream);
+        launch_few_as<TREE, PAGE, ELEM, 128, false, NQ, NP>(sets, a, stream);
     else if (d == 256)
-        launch_few_as<PAGE, ELEM, 256, true, NQ, NP>(sets, a, stream);
+        launch_few_as<TREE, PAGE, ELEM, 256, true, NQ, NP>(sets, a, stream);
     else
-        launch_few_as<PAGE, ELEM, 256, false, NQ, NP>(sets, a, stream);
+        launch_few_as<TREE, PAGE, ELEM, 256, false, NQ, NP>(sets, a, stream);
     return hipGetLastError();
 }
 

@@ -114,8 +114,9 @@ __device__ __forceinline__ float sum_over_groups(float v) {
 // A capped score relative to `shift`: c tanh(y) - shift, y = a ln 2 / 2, in the log2 domain (softcap_of_exp2_arg). Where a small score is
 // to be as exact as one without a cap (SERIES), and 1 - 2 / (2^a + 1) leaves some 2^-23 of the cap: up to |y| = 0.45 the
 // series y (1 - y^2 / 3 + 2 y^4 / 15 - ..) to y^13, whose next term is below 2^-25 of the value. That is for f32 tensors, and of 16 bits for
-// caps beyond kPagedCapShort, below which the short form's error is a tenth of what a weight's rounding to f16 takes.
-template <bool SERIES>
+// caps beyond kPagedCapShort, below which the short form's error is a tenth of what a weight's rounding to f16 takes. STRAIGHT: both are
+// worked out, where the compiler would make a branch of the choice, which turns lanes off amid the fullest registers.
+template <bool SERIES, bool STRAIGHT = false>
 __device__ __forceinline__ float softcapped(float a, float c, float shift) {
     if constexpr (!SERIES) return softcap_of_exp2_arg(a, c, shift);
     const float y = a * 0.34657359f, z = y * y;
@@ -124,7 +125,12 @@ __device__ __forceinline__ float softcapped(float a, float c, float shift) {
     p = __builtin_fmaf(z, p, -17.0f / 315.0f);
     p = __builtin_fmaf(z, p, 2.0f / 15.0f);
     p = __builtin_fmaf(z, p, -1.0f / 3.0f);
-    const float small = __builtin_fmaf(__builtin_fmaf(y * z, p, y), c, -shift);
+    float small = __builtin_fmaf(__builtin_fmaf(y * z, p, y), c, -shift);
+    if constexpr (STRAIGHT) {
+        float large = softcap_of_exp2_arg(a, c, shift);
+        asm("" : "+v"(small), "+v"(large));
+        return __builtin_fabsf(y) < 0.45f ? small : large;
+    }
     return __builtin_fabsf(y) < 0.45f ? small : softcap_of_exp2_arg(a, c, shift);
 }
 

@@ -9,9 +9,9 @@
 
 namespace itak {
 
-// The batch in device memory: four words (active items, their rows, 0, 0), four words an active item (position, rows, first
-// row among the batch's, the word at which its page ids begin), from ids_at on the page ids. Items without rows are left
-// out, their page ids are not.
+// The batch in device memory: four words (active items, their rows, whether rows have records as paged_tree.h says, 0), four words
+// an active item (position, rows, first row among the batch's, the word at which its page ids begin), from ids_at on the page
+// ids. Items without rows are left out, their page ids are not; of a handle that takes trees an item's number is its sequence's, and none is left out.
 constexpr uint32_t kPagedItem0 = 4;  // the first item's first word
 inline uint32_t paged_ids_at(uint32_t max_sequences) { return kPagedItem0 + 4 * max_sequences; }
 
@@ -38,12 +38,15 @@ struct PagedBatch {
     uint32_t items = 0;          // active ones
     uint32_t rows = 0;           // of all of them
     uint32_t most_rows = 0;      // of one
+    bool trees = false;          // its rows have records
+    uint32_t tree_most = 0;      // rows of its largest tree
+    bool on_device = false;      // lengths and tables are the device's: positions in `head` are the most they may be, and there are no ids
 };
 
 // Fills `batch`, or says why not. `marks` (page_count words, any content that `stamp` is greater than) belongs to the caller and
 // is written; stamp grows by the call.
 inline PagedRefusal make_paged_batch(const PagedLimits &lim, const itak_paged_item *items, uint32_t count, const uint32_t *pages,
-                                     uint64_t page_ids, std::vector<uint32_t> &marks, uint32_t &stamp, PagedBatch &batch) {
+                                     uint64_t page_ids, std::vector<uint32_t> &marks, uint32_t &stamp, PagedBatch &batch, bool keep_idle = false) {
     auto refuse = [](int32_t code, const char *what, uint64_t a, uint64_t b, std::string text) {
         PagedRefusal r;
         r.code = code, r.what = what, r.a = a, r.b = b, r.text = std::move(text);
@@ -109,7 +112,7 @@ inline PagedRefusal make_paged_batch(const PagedLimits &lim, const itak_paged_it
     batch.ids.assign(pages, pages + page_ids);
     uint32_t id = paged_ids_at(lim.max_sequences);
     for (uint32_t i = 0; i < count; id += items[i].pages, ++i) {
-        if (!items[i].rows) continue;
+        if (!items[i].rows && !keep_idle) continue;
         const uint32_t words[4] = {uint32_t(items[i].position), items[i].rows, batch.rows, id};
         batch.head.insert(batch.head.end(), words, words + 4);
         ++batch.items;

@@ -135,6 +135,48 @@ class Rotation:
             _raise_last(None)
 
 
+class PageTables:
+    """Page tables on the device (itak_page_tables), the caller's memory: of each sequence up to `stride` page ids and how many, and the
+    free list."""
+
+    __slots__ = ("raw", "ref", "sequences", "keep")
+
+    def __init__(self, table_ptr: int, stride: int, pages_ptr: int, sequences: int, free_ptr: int = 0, free_count_ptr: int = 0, keep=None):
+        self.raw = _filled(N.PageTables, table_ptr or None, stride, pages_ptr or None, free_ptr or None, free_count_ptr or None, sequences, 0)
+        self.ref = C.byref(self.raw)
+        self.sequences = sequences
+        self.keep = keep  # what owns the memory
+
+    @staticmethod
+    def of(table, pages, free=None, free_count=None) -> "PageTables":
+        """Of int32 tensors on a GPU: table [sequences][stride], pages [sequences], free [page_count], free_count [1]."""
+        for name, t, dims in (("table", table, 2), ("pages", pages, 1), ("free", free, 1), ("free_count", free_count, 1)):
+            if t is not None and not (t.is_cuda and str(t.dtype) == "torch.int32" and t.dim() == dims and t.is_contiguous()):
+                raise ValueError(f"PageTables.of: {name} is no dense int32 tensor of {dims} dimensions on a GPU")
+        if pages.shape[0] != table.shape[0]:
+            raise ValueError(f"PageTables.of: pages of {pages.shape[0]} sequences, tables of {table.shape[0]}")
+        return PageTables(table.data_ptr(), table.shape[1], pages.data_ptr(), table.shape[0], 0 if free is None else free.data_ptr(),
+                          0 if free_count is None else free_count.data_ptr(), (table, pages, free, free_count))
+
+
+def _words(values, kind: str, low: int, high: int, what: str):
+    """Host values as an array of 32-bit words; its address and count."""
+    if isinstance(values, np.ndarray):
+        if values.dtype.kind not in "iu" or values.ndim != 1:
+            raise ValueError(f"{what} are no integers in a row")
+        if values.size and (values.min() < low or values.max() > high):
+            raise ValueError(f"{what} beyond {low} .. {high}")
+        words = np.ascontiguousarray(values, dtype=np.int32 if kind == "i" else np.uint32)
+        return words, _ptr(words) if words.size else None, words.size
+    words = array(kind)
+    try:
+        words.extend(values)
+    except OverflowError:
+        raise ValueError(f"{what} beyond {low} .. {high}") from None
+    ptr, count = words.buffer_info()
+    return words, ptr if count else None, count
+
+
 class PagedKv:
     """Keys and values in pages (itak_paged): storage [layer][page][side][kv_head][page row][channel], side 0 = keys. The storage
     is the caller's (`storage_ptr`, `storage_bytes`: at least `PagedKv.bytes_for(...)`) or the cache's own."""
@@ -194,9 +236,17 @@ class PagedKv:
     def storage_ptr(self) -> int:
         return int(self._lib.itak_paged_storage(self._h) or 0)
 
-    def set_batch(self, items: Sequence[Tuple[int, int]], pages: Sequence[Sequence[int]]) -> None:
-        """The sequences of the next forward: (positions held, new rows) of each, and its page ids in order."""
-        status = hip_compute._front.set_batch(self._hv, items, pages)
+    def enable_trees(self, most_rows: int) -> None:
+        """Lets batches be trees, of up to `most_rows` new rows in all (itak_paged_enable_trees); once."""
+        if not 0 <= most_rows < 1 << 64:
+            raise ValueError(f"most_rows: {most_rows} is out of range")
+        self._done(self._lib.itak_paged_enable_trees(self._h, most_rows))
+
+    def set_batch(self, items: Sequence[Tuple[int, int]], pages: Sequence[Sequence[int]],
+                  parents: Optional[Sequence[int]] = None) -> None:
+        """The sequences of the next forward: (positions held, new rows) of each, and its page ids in order. `parents` makes the new
+        rows trees: of all rows in order the number of the row of the same sequence that it continues, or -1."""
+        status = -1 if parents is not None else hip_compute._front.set_batch(self._hv, items, pages)
         if status >= 0:
             self._done(status)
             self._rows = sum([rows for _, rows in items])
@@ -220,8 +270,50 @@ class PagedKv:
             for table in pages:
                 ids.extend(table)
             ptr, count = ids.buffer_info()
-        self._done(self._lib.itak_paged_set_batch(self._h, raw, n, ptr if count else None, count))
-        self._rows = sum(int(rows) for _, rows in items)
+        all_rows = sum(int(rows) for _, rows in items)
+        if parents is None:
+            self._done(self._lib.itak_paged_set_batch(self._h, raw, n, ptr if count else None, count))
+        else:
+            words, parents_ptr, named = _words(parents, "i", -(1 << 31), (1 << 31) - 1, "parents")
+            if named != all_rows:
+                raise ValueError(f"set_batch: {named} parents of {all_rows} new rows")
+            if parents_ptr is None:
+                parents_ptr = C.addressof(C.c_int32())  # (of no rows: not read)
+            self._done(self._lib.itak_paged_set_batch_tree(self._h, raw, n, ptr if count else None, count, parents_ptr))
+        self._rows = all_rows
+
+    def fit_tables_device(self, tables: PageTables, lengths_ptr: int, rows: Optional[Sequence[int]] = None, status_ptr: int = 0) -> None:
+        """Page tables to lengths on the device (int32 [sequences]), and `rows` new rows on top of each: pages from the free list, or back."""
+        words, rows_ptr, named = _words(rows, "I", 0, (1 << 32) - 1, "rows") if rows is not None else (None, None, tables.sequences)
+        if named != tables.sequences:
+            raise ValueError(f"rows of {named} sequences, tables of {tables.sequences}")
+        self._done(self._lib.itak_paged_fit_tables_device(self._h, tables.ref, lengths_ptr or None, rows_ptr, status_ptr or None))
+
+    def set_batch_device(self, tables: PageTables, positions_ptr: int, rows: Sequence[int], most_positions: int, parents_ptr: int = 0,
+                         status_ptr: int = 0) -> None:
+        """The batch from positions (int32 [sequences]), tables and parents (int32 [sum rows]) on the device; `rows` new rows of each sequence,
+        behind at most `most_positions`."""
+        words, rows_ptr, named = _words(rows, "I", 0, (1 << 32) - 1, "rows")
+        if named != tables.sequences:
+            raise ValueError(f"rows of {named} sequences, tables of {tables.sequences}")
+        if not 0 <= most_positions < 1 << 64:
+            raise ValueError(f"most_positions: {most_positions} is out of range")
+        self._done(self._lib.itak_paged_set_batch_device(self._h, tables.ref, positions_ptr or None, rows_ptr, most_positions,
+                                                         parents_ptr or None, status_ptr or None))
+        self._rows = sum(words.tolist())
+
+    def batch_rows_device(self, positions_ptr: int = 0, slots_ptr: int = 0) -> None:
+        """Every row's position in the text and its row of the storage (page * page_rows + row): int64 [rows] each; -1 of rows left out."""
+        self._done(self._lib.itak_paged_batch_rows_device(self._h, positions_ptr or None, slots_ptr or None))
+
+    def accept_device(self, tokens_ptr: int, chosen_ptr: int, path_ptr: int, next_ptr: int) -> None:
+        """The walk down every tree along the tokens chosen: `path` [rows] its row numbers and then -1, `next` [sequences] the choice at its
+        end (int32 all)."""
+        self._done(self._lib.itak_paged_accept_device(self._h, tokens_ptr or None, chosen_ptr or None, path_ptr or None, next_ptr or None))
+
+    def keep_device(self, path_ptr: int, lengths_ptr: int = 0) -> None:
+        """The rows of every path to the sequence's next positions, on all layers; `lengths` [sequences] the positions held then."""
+        self._done(self._lib.itak_paged_keep_device(self._h, path_ptr or None, lengths_ptr or None))
 
     def append_device(self, layer: int, k: Rows, v: Rows, rotation: Optional[Rotation] = None) -> None:
         """The batch's new rows into their pages, keys turned by their positions if `rotation` is given."""
