@@ -48,7 +48,7 @@ MFMA_IN_VECTOR_REGISTERS = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 
 
 def source_flags(src: str):
-    return MFMA_IN_VECTOR_REGISTERS if src.startswith(("paged_chunk", "paged_few")) else []
+    return MFMA_IN_VECTOR_REGISTERS if src.startswith(("paged_chunk", "paged_few", "paged_trees")) else []
 
 
 def misplaced(listing) -> list:

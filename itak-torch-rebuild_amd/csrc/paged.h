@@ -81,9 +81,10 @@ struct PagedAttn {
     float cap_log2;      // cap * log2(e), 0: none
     uint32_t window;
     uint32_t parts;      // kernel of many rows: workgroups a unit is dealt to; 0: the line above
+    uint32_t apart;      // kernel of trees: no workgroup has parts of two units (paged_cut_apart), and a unit is a tile of all heads
     const void *zeros;   // 16 bytes of them
     uint32_t inline_items; // 0: the batch's are read from device memory
-    uint32_t total;      // with inline items: the line's length, and its cut
+    uint32_t total;      // where the host knows the batch: the line's length, and its cut (else a share of 0)
     uint32_t share, pad;
     PagedItemWords item[kPagedInline];  // those behind the last: row0, start and unit0 are ~0
     uint32_t start[kPagedInline], unit0[kPagedInline];  // where an item's blocks and units begin in the line
@@ -127,6 +128,18 @@ hipError_t launch_paged_chunk_tree_f16(const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_chunk_tree_f16_f32(const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_chunk_tree_bf16(const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_chunk_tree_bf16_f32(const PagedAttn &a, hipStream_t stream);
+// The kernel of trees (paged_trees_kernel.h): 32 vectors a wavefront, eight wavefronts a workgroup where a lane does with 256 registers, else four. A
+// unit is a tile of an item: its heads are workgroups side by side, which the cut does not know of.
+__host__ __device__ constexpr int paged_trees_waves(int padded, int page_elem, int elem) {
+    return padded == 64 || (padded == 128 && !(page_elem == ITAK_ELEM_BF16 && elem == ITAK_ELEM_F32)) ? 8 : 4;
+}
+// Most workgroups that may have parts of units.
+constexpr uint32_t kPagedTreesGroups = 512;
+hipError_t launch_paged_trees_f16(const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_trees_f16_f32(const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_trees_bf16(const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_trees_bf16_f32(const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_join(uint32_t elem, const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_merge(uint32_t elem, const PagedAttn &a, hipStream_t stream);
 // head_dim as the kernels hold it.
 __host__ __device__ constexpr uint32_t paged_padded(uint32_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
@@ -162,6 +175,12 @@ __host__ __device__ inline PagedCut paged_cut(uint32_t total, uint32_t units, ui
     if (units >= groups) return {share, 0};
     const uint32_t left = groups - units, apart = (total + left - 1) / left, own = apart > least ? apart : least;
     return own <= share + kPagedPart ? PagedCut{own, own} : PagedCut{share, 0};
+}
+// The cut of the kernel of trees, whose workgroups have one part of one unit each: at most `groups` of them, which are at least the units.
+__host__ __device__ inline PagedCut paged_cut_apart(uint32_t total, uint32_t units, uint32_t longest, uint32_t groups, uint32_t least) {
+    const uint32_t left = groups > units ? groups - units : 0, even = left ? (total + left - 1) / left : longest;
+    const uint32_t share = even > least ? even : least;
+    return share < longest ? PagedCut{share, share} : PagedCut{longest, longest};
 }
 __host__ __device__ inline uint32_t paged_run(uint32_t blocks, uint32_t pad) { return pad ? (blocks + pad - 1) / pad * pad : blocks; }
 
@@ -201,7 +220,7 @@ struct PagedLine {
             s.first = paged_first_block(w.position, a.window);
             s.blocks = (w.position + w.rows + 31) / 32 - s.first;
             s.tiles = (vectors + (1u << a.tile_shift) - 1) >> a.tile_shift;
-            units = s.tiles * a.g.kv_heads;
+            units = a.apart ? s.tiles : s.tiles * a.g.kv_heads;
             s.run = paged_run(s.blocks, pad);
             work = units * s.run;
         }
@@ -234,7 +253,7 @@ struct PagedLine {
     }
     // The cut; before anything that counts blocks.
     __device__ __forceinline__ void cut() {
-        if (a.inline_items) {
+        if (a.share) {
             share = a.share, pad = a.pad, total = a.total;
             return;
         }
@@ -248,7 +267,7 @@ struct PagedLine {
             longest = max(longest, s.blocks);
         }
         longest = most_of(longest);
-        const PagedCut c = paged_cut(all, all_units, longest, a.groups, a.least);
+        const PagedCut c = a.apart ? paged_cut_apart(all, all_units, longest, a.groups, a.least) : paged_cut(all, all_units, longest, a.groups, a.least);
         share = c.share, pad = c.pad, total = pad ? share * a.groups : all;  // (of rounded runs: what lies past the last is nobody's)
     }
     // The item that block, unit or row x of the line belongs to; none if it is no item's, or of one that the launch does not take.

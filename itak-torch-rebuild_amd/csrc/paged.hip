@@ -167,8 +167,65 @@ constexpr uint64_t kMostBlocks = 1ull << 30;
 
 uint32_t shift_of(uint32_t power) { return uint32_t(__builtin_ctz(power)); }
 
+// How a batch whose rows may be trees is cut: by which kernel, the vectors of a tile, and the blocks of a workgroup's part. The cost of a choice is
+// worked out in clocks: of a workgroup what it takes before its first products and behind its last, its steps, or its blocks on their way from L2
+// where that is more, and its partial's way out; of the launch its rounds and, where units are split, the join and the partials' way there and back.
+struct TreesCut {
+    bool chunk;  // the kernel of many rows
+    uint32_t tile, share;
+};
+TreesCut trees_plan(const PagedBatch &batch, const PagedAttn &a, uint32_t waves, uint32_t chunk_waves, uint32_t dp, uint32_t cus) {
+    struct Run {
+        uint32_t vectors, blocks;
+    };
+    std::vector<Run> runs;
+    uint32_t longest = 1, widest = 1;
+    for (uint32_t i = 0; i < a.items; ++i) {
+        const uint32_t *it = batch.head.data() + kPagedItem0 + 4 * i;
+        const uint64_t vectors = uint64_t(it[1]) * a.group;
+        if (vectors < a.v_from || vectors > a.v_to) continue;
+        const uint32_t blocks = (it[0] + it[1] + 31) / 32 - paged_first_block(it[0], a.window);
+        runs.push_back({uint32_t(vectors), blocks});
+        longest = std::max(longest, blocks), widest = std::max(widest, uint32_t(vectors));
+    }
+    TreesCut best{chunk_waves != 0, 32 * (chunk_waves ? chunk_waves : waves), longest};
+    double lowest = 1e300;
+    auto look = [&](bool chunk, uint32_t sets, uint32_t groups) {
+        const uint32_t tile = 32 * sets;
+        // Clocks of a step, of 128 channels: chunks' wavefronts work at their products and their softmax at once.
+        const double step = (chunk ? 1900.0 : 2450.0) * (waves == 8 || chunk ? 1.0 : 0.6) * dp / 128;
+        for (uint32_t share = longest;;) {
+            uint64_t parts = 0, work = 0;
+            for (const Run &r : runs) {
+                const uint64_t tiles = (r.vectors + tile - 1) / tile;
+                parts += tiles * ((r.blocks + share - 1) / share), work += tiles * r.blocks;
+            }
+            parts *= a.g.kv_heads, work *= a.g.kv_heads;
+            if (parts > kPagedTreesGroups && share != longest) break;
+            const bool split = share < longest;
+            const double load = std::max(280.0, 900.0 * std::min(1.0, double(parts) / cus)) * dp / 128;
+            auto time = [&](double blocks) { return std::max(std::ceil(blocks / groups) * step, blocks * load); };
+            const double beside = chunk ? 13000.0 : 11000.0 + (groups > 1 ? 2000.0 : 1000.0), partial = split ? tile * dp / 16.0 : 0.0;
+            const double alone = time(share) + beside + partial;
+            const double among = double(parts) / cus * (time(double(work) / parts) + beside + partial) + time(share) / 2;
+            const double cost = (parts <= cus ? alone : std::max(alone, among)) + (split ? 8000.0 + parts * tile * dp / 500.0 : 0.0);
+            if (cost < lowest) lowest = cost, best = {chunk, tile, share};
+            if (share <= 2 || parts > 2 * cus) break;
+            // (Shares that are whole steps of the groups.)
+            share = std::max<uint32_t>(2, std::min((share - 1) / groups * groups, share * 7 / 8 / groups * groups));
+        }
+    };
+    // (Eight groups of one set have at least a pair of register quads each to finish.)
+    for (uint32_t sets = dp < 128 ? 2 : 1; sets <= waves; sets *= 2) {
+        if (16 * sets >= widest && sets > (dp < 128 ? 2u : 1u)) break;
+        look(false, sets, waves / sets);
+    }
+    if (chunk_waves) look(true, chunk_waves, 1);
+    return best;
+}
+
 // Units and blocks of the items a launch takes, how their line is cut, and where in it inline items begin; `whole`: no unit is split.
-itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work, bool &whole) {
+itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work, bool &whole, bool known = false) {
     uint32_t longest = 0;
     auto each = [&](uint32_t pad, auto item) {
         uint64_t at = 0, units = 0;
@@ -177,7 +234,7 @@ itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work, bool &whole
             const uint64_t vectors = uint64_t(it[1]) * a.group;
             item(i, at, units);
             if (vectors < a.v_from || vectors > a.v_to) continue;
-            const uint64_t tiles = (vectors + a.tile - 1) / a.tile * a.g.kv_heads;
+            const uint64_t tiles = (vectors + a.tile - 1) / a.tile * (a.apart ? 1 : a.g.kv_heads);
             const uint32_t blocks = (it[0] + it[1] + 31) / 32 - paged_first_block(it[0], a.window);
             units += tiles;
             at += tiles * paged_run(blocks, pad);
@@ -191,6 +248,28 @@ itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work, bool &whole
     // dealt to parts they are few.)
     if (work >= kMostBlocks || units > (1ull << 32) / 512 - 1) return size_overflow(p->err, "blocks of the batch's attention");
     a.units = uint32_t(units);
+    if (a.apart) {
+        const uint32_t room = std::max(1u, kPagedTreesGroups / a.g.kv_heads), share = a.share;
+        a.groups = std::max(room, a.units);
+        whole = a.units >= room;
+        if (whole) a.least = ~0u;
+        if (known) {
+            a.share = a.pad = share;
+            for (uint32_t i = 0; i < kPagedInline; ++i) a.start[i] = a.unit0[i] = ~0u;
+            uint64_t total = 0;
+            each(share, [&](uint32_t i, uint64_t at, uint64_t u) {
+                if (i < a.inline_items) a.start[i] = uint32_t(at), a.unit0[i] = uint32_t(u);
+                total = at;
+            });
+            // (Every unit's run is rounded up by less than a share: what the device counts in 32 bits may then be too much.)
+            if (total >= 2 * kMostBlocks) return size_overflow(p->err, "blocks of the batch's attention");
+            a.total = uint32_t(total);
+            whole = share >= longest;
+        } else {
+            a.share = 0;
+        }
+        return ITAK_OK;
+    }
     // (The kernel of many rows has no line.)
     const PagedCut cut = a.parts ? PagedCut{} : paged_cut(uint32_t(work), a.units, longest, a.groups, a.least);
     whole = cut.pad >= longest;
@@ -206,22 +285,25 @@ itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work, bool &whole
 
 // What a call's attention launches: found out, and its memory had, before the call enqueues anything.
 struct AttnPlan {
-    PagedAttn few{}, many{};
+    PagedAttn few{}, trees{}, many{};
     uint32_t sets = 0;       // of the kernel of few rows; 0: it has no items
     bool merge_few = false;
+    bool has_trees = false, join_trees = false, trees_as_many = false;
     bool has_many = false;
 };
 
-// The partials of both launches lie in one place: they run one after the other.
+// The partials of all launches lie in one place: they run one after the other.
 itak_status workspace(itak_paged *p, AttnPlan &plan, uint32_t dp) {
-    auto slots = [](const PagedAttn &a) { return a.parts ? (a.parts > 1 ? uint64_t(a.units) * a.parts : 0) : uint64_t(a.groups) + a.units; };
-    auto sums = [&](const PagedAttn &a) { return slots(a) * a.tile * dp * sizeof(float); };
+    // (Of the kernel of trees as much as any call of it needs: one that is captured may be planned for other lengths.)
+    auto slots = [](const PagedAttn &a) { return a.apart ? uint64_t(kPagedTreesGroups + a.g.kv_heads) : a.parts ? (a.parts > 1 ? uint64_t(a.units) * a.parts : 0) : uint64_t(a.groups) + a.units; };
+    auto vectors = [&](const PagedAttn &a) { return slots(a) * (a.apart ? 256 : a.tile); };
+    auto sums = [&](const PagedAttn &a) { return vectors(a) * dp * sizeof(float); };
     uint64_t need = 0;
-    for (const PagedAttn *a : {&plan.few, &plan.many}) need = std::max(need, sums(*a) + slots(*a) * a->tile * sizeof(float2));
+    for (const PagedAttn *a : {&plan.few, &plan.trees, &plan.many}) need = std::max(need, sums(*a) + vectors(*a) * sizeof(float2));
     void *ws = p->ws;
     const itak_status st = grow(p, &ws, &p->ws_bytes, need, "split workspace");
     p->ws = static_cast<float *>(ws);
-    for (PagedAttn *a : {&plan.few, &plan.many}) {
+    for (PagedAttn *a : {&plan.few, &plan.trees, &plan.many}) {
         a->ws_acc = p->ws;
         a->ws_ml = reinterpret_cast<float2 *>(reinterpret_cast<unsigned char *>(p->ws) + sums(*a));
     }
@@ -246,7 +328,18 @@ uint32_t chunk_parts(uint32_t units, uint64_t work, uint32_t places) {
 
 // q is as it attends: turned where it has to be.
 itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, const itak_rows &out, float scale, float softcap,
-                           uint64_t window, AttnPlan &plan) {
+                           uint64_t window, AttnPlan &plan, bool for_capture = false) {
+    const bool captures = capturing(p->stream);
+    // A call over a batch without trees has the memory that it would take captured, where it has to be right for trees as well: once a batch.
+    if (p->tree_dev && !p->batch.trees && !captures && !for_capture) {
+        const uint64_t key = q.heads * 4ull + q.elem + 1;
+        if (uint64_t &sized = p->batch.sized[window ? 1 : 0]; sized != key) {
+            AttnPlan other;
+            const itak_status st = plan_attention(p, layer, q, out, scale, softcap, window, other, true);
+            if (st != ITAK_OK) return st;
+            sized = key;
+        }
+    }
     const uint32_t d = uint32_t(p->cfg.head_dim);
     const uint32_t group = uint32_t(q.heads / p->cfg.num_kv_heads);
     PagedAttn &a = plan.few;
@@ -261,7 +354,7 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
     a.group_magic = group > 1 ? uint32_t((1ull << 32) / group + ((1ull << 32) % group != 0)) : 0;
     if (uint64_t(a.rows) * group >= (1ull << 26)) return size_overflow(p->err, "query vectors of the batch");
     // (A call that is being captured is replayed over other batches.)
-    const bool captured = capturing(p->stream);
+    const bool captured = captures || for_capture;
     // A handle that takes trees captures launches that find out whether the batch has them.
     if (p->batch.trees || (captured && p->tree_dev)) a.tree = p->tree_dev;
     if (a.items <= kPagedInline && !captured && !p->batch.on_device) {
@@ -282,11 +375,14 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
     // and 27.8, 64 at 600 47.7 and 26.7), though tiles of four sets of 16 had been made for them.
     const uint32_t few_most = 2 * kPagedSet;
     const bool chunks = paged_chunk_takes(dp, p->cfg.elem, q.elem);
+    // Of a batch whose rows may be trees those of more than few vectors are one launch, of the kernel of trees or of that of many rows.
     uint32_t most_few = 0;
     bool many = false;
     for (uint32_t i = 0; i < a.items; ++i) {
         const uint64_t vectors = uint64_t(p->batch.head[kPagedItem0 + 4 * i + 1]) * group;
-        if (chunks && vectors > few_most)
+        if (a.tree && vectors > few_most)
+            plan.has_trees = true;
+        else if (chunks && vectors > few_most)
             many = true;
         else
             most_few = std::max(most_few, uint32_t(std::min<uint64_t>(vectors, few_most)));
@@ -304,11 +400,25 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
         if (st != ITAK_OK) return st;
         b.parts = chunk_parts(b.units, work, cus * kPagedChunkGroupsPerCu);
     }
+    if (plan.has_trees) {
+        PagedAttn &b = plan.trees = a;
+        b.v_from = few_most + 1, b.v_to = ~0u;
+        b.apart = 1;
+        const TreesCut cut = trees_plan(p->batch, b, paged_trees_waves(dp, p->cfg.elem, q.elem), chunks ? paged_chunk_waves(dp, q.elem) : 0, dp, cus);
+        b.tile = cut.tile, b.share = cut.share;
+        plan.trees_as_many = cut.chunk;
+        b.tile_shift = shift_of(b.tile);
+        b.least = 2;
+        const bool known = !captured && !p->batch.on_device;
+        const itak_status st = count_units(p, b, work, whole, known);
+        if (st != ITAK_OK) return st;
+        plan.join_trees = !whole;
+    }
     if (most_few) {
         plan.sets = most_few <= kPagedSet ? 1 : 2;
         a.tile = plan.sets * kPagedSet;
         a.tile_shift = shift_of(a.tile);
-        a.v_from = 1, a.v_to = chunks ? few_most : ~0u;
+        a.v_from = 1, a.v_to = chunks || a.tree ? few_most : ~0u;
         a.groups = std::min(cus * paged_few_groups_per_cu(dp, p->cfg.elem, q.elem, plan.sets, a.tree != nullptr), kPagedMostParts);
         a.least = 4;
         a.parts = 0;
@@ -317,9 +427,9 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
         plan.merge_few = captured || p->batch.on_device || !whole;
     }
     const itak_status st = workspace(p, plan, dp);
-    if (st == ITAK_OK && captured) {
+    if (st == ITAK_OK && captures) {
         itak_paged::Captured &c = p->captured[a.window ? 1 : 0];
-        c.units = std::max<uint64_t>({c.units, plan.few.units, plan.many.units});
+        c.units = std::max<uint64_t>({c.units, plan.few.units, plan.trees.units, plan.many.units});
         c.window = std::max(c.window, a.window);
         if (a.window && p->tree_dev) c.least_window = c.least_window ? std::min(c.least_window, a.window) : a.window;
     }
@@ -355,12 +465,20 @@ itak_status run_attention(itak_paged *p, uint32_t elem, const AttnPlan &plan) {
         HIP_TRY(p, he, "launch paged attention of few rows");
         if (plan.merge_few) HIP_TRY(p, launch_paged_merge(elem, plan.few, p->stream), "launch the merge of paged attention");
     }
+    if (plan.has_trees) {
+        const bool f16 = p->cfg.elem == ITAK_ELEM_F16, f32 = elem == ITAK_ELEM_F32;
+        const auto launch = plan.trees_as_many ? (f16 ? (f32 ? launch_paged_chunk_tree_f16_f32 : launch_paged_chunk_tree_f16)
+                                                      : (f32 ? launch_paged_chunk_tree_bf16_f32 : launch_paged_chunk_tree_bf16))
+                                               : (f16 ? (f32 ? launch_paged_trees_f16_f32 : launch_paged_trees_f16)
+                                                      : (f32 ? launch_paged_trees_bf16_f32 : launch_paged_trees_bf16));
+        const hipError_t he = launch(plan.trees, p->stream);
+        HIP_TRY(p, he, "launch paged attention of trees");
+        if (plan.join_trees) HIP_TRY(p, launch_paged_join(elem, plan.trees, p->stream), "launch the join of paged attention");
+    }
     if (plan.has_many) {
         const hipError_t he = p->cfg.elem == ITAK_ELEM_F16
-                                  ? (elem == ITAK_ELEM_F32 ? (trees ? launch_paged_chunk_tree_f16_f32 : launch_paged_chunk_f16_f32)
-                                                           : (trees ? launch_paged_chunk_tree_f16 : launch_paged_chunk_f16))(plan.many, p->stream)
-                                  : (elem == ITAK_ELEM_F32 ? (trees ? launch_paged_chunk_tree_bf16_f32 : launch_paged_chunk_bf16_f32)
-                                                           : (trees ? launch_paged_chunk_tree_bf16 : launch_paged_chunk_bf16))(plan.many, p->stream);
+                                  ? (elem == ITAK_ELEM_F32 ? launch_paged_chunk_f16_f32 : launch_paged_chunk_f16)(plan.many, p->stream)
+                                  : (elem == ITAK_ELEM_F32 ? launch_paged_chunk_bf16_f32 : launch_paged_chunk_bf16)(plan.many, p->stream);
         HIP_TRY(p, he, "launch paged attention of many rows");
         if (plan.many.parts > 1) HIP_TRY(p, launch_paged_merge(elem, plan.many, p->stream), "launch the merge of paged attention");
     }
@@ -442,7 +560,7 @@ itak_status set_batch(itak_paged *p, const itak_paged_item *items, uint32_t coun
     PagedBatch &next = p->next;
     const PagedRefusal r = make_paged_batch(p->limits, items, count, pages, page_ids, p->marks, p->stamp, next, p->tree_dev != nullptr);
     if (r.code != ITAK_OK) return set_error(p->err, r.code, r.what, r.a, r.b, 0, 0, "%s", r.text.c_str());
-    next.trees = parents != nullptr, next.on_device = false, next.tree_most = 0;
+    next.trees = parents != nullptr, next.on_device = false, next.tree_most = 0, next.sized[0] = next.sized[1] = 0;
     if (parents) {
         const itak_status st = check_trees(p, items, count, parents, next.rows, next.tree_most);
         if (st != ITAK_OK) return st;

@@ -393,7 +393,7 @@ itak_status itak_paged_set_batch_device(itak_paged *paged, const itak_page_table
         next.head.assign(kPagedItem0, 0);
         next.ids.clear();
         next.items = n, next.rows = uint32_t(all), next.most_rows = most;
-        next.trees = parents_dev != nullptr, next.tree_most = tree_most, next.on_device = true;
+        next.trees = parents_dev != nullptr, next.tree_most = tree_most, next.on_device = true, next.sized[0] = next.sized[1] = 0;
         uint32_t row0 = 0;
         for (uint32_t i = 0; i < n; row0 += rows[i], ++i) {
             const uint32_t words[4] = {uint32_t(most_positions), rows[i], row0, 0};

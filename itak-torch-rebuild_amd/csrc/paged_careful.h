@@ -161,6 +161,19 @@ __device__ __forceinline__ void paged_write_careful(const PagedAttn &a, const Pa
     if (!whole && has_slot && lane == 0) a.ws_ml[slot] = make_float2(m, kCarefulScale<PAGE> == 1.0f ? l : -l);
 }
 
+// The same into a part for the join: the tile's accumulators as the kernels' registers hold them, sets of 32 vectors, 16 bytes of four channels
+// of a vector; `of`: the vector of the tile.
+template <int PAGE, int DP>
+__device__ __forceinline__ void paged_part_careful(const PagedAttn &a, uint64_t slot0, uint32_t of, const float (&acc)[DP / 64], float m, float l) {
+    const uint32_t lane = __lane_id();
+#pragma unroll
+    for (uint32_t c = 0; c < DP / 64; ++c) {
+        const uint32_t ch = 64 * c + lane;
+        a.ws_acc[slot0 * DP + ((of / 32 * (DP / 8) + ch / 8) * 64 + (ch / 4 % 2) * 32 + of % 32) * 4 + ch % 4] = acc[c];
+    }
+    if (lane == 0) a.ws_ml[slot0 + of] = make_float2(m, kCarefulScale<PAGE> == 1.0f ? l : -l);
+}
+
 // Whether any of a workgroup's threads says so; all of them ask.
 __device__ __forceinline__ bool any_of_group(bool mine, uint32_t *lds_word) {
     if (threadIdx.x == 0) *lds_word = 0;

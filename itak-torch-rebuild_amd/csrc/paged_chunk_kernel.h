@@ -26,35 +26,11 @@
 
 #include "lds_grant.h"
 #include "paged_careful.h"
+#include "paged_ring.h"
 
 namespace itak {
 
 namespace {
-
-typedef float floatx16 __attribute__((ext_vector_type(16)));
-typedef short shortx4 __attribute__((ext_vector_type(4)));
-
-template <int PAGE>
-__device__ __forceinline__ floatx16 mfma_32x32x16(u32x4 a, u32x4 b, floatx16 c) {
-    if constexpr (PAGE == ITAK_ELEM_F16)
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bfloat8, a), __builtin_bit_cast(bfloat8, b), c, 0, 0, 0);
-}
-
-// Issued from assembly: the compiler then neither waits for such a load at every LDS read nor needs to, because its only
-// consumer is ordered by the wait and the barrier at the top of each block. It does not look for hazards in there either: a scalar
-// register that vector code wrote (readlane: the address) takes five wait states before a load may read it, m0 one.
-__device__ __forceinline__ void page_to_lds(uint64_t base, uint32_t offset, uint32_t lds_addr) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds_addr) : "memory");
-}
-__device__ __forceinline__ void lane_to_lds(uint64_t address, uint32_t lds_addr) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(address), "s"(lds_addr) : "memory");
-}
-template <int n>
-__device__ __forceinline__ void wait_loads() {  // s_waitcnt vmcnt(n), other counters untouched
-    __builtin_amdgcn_s_waitcnt(0x0f70 | (n & 15) | ((n >> 4) << 14));
-}
 
 // Sub-blocks of 32 keys a stage of the ring holds, and stages.
 constexpr int chunk_subs(int dp) { return dp <= 128 ? 2 : 1; }
@@ -89,13 +65,24 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     const uint32_t d = EXACT ? DP : a.g.head_dim;
 
     // Which tile of which head of which item, and which part of its keys. Parts come slowest and heads fastest: workgroup w runs on
-    // compute die w mod 8, so a die keeps to the keys of few heads, and the tiles that run at a time read them together. Longest first.
-    const uint32_t units = gridDim.x / a.parts;
-    const uint32_t part = blockIdx.x / units, unit = blockIdx.x - part * units;
-    const PagedLine line(a);
+    // compute die w mod 8, so a die keeps to the keys of few heads, and the tiles that run at a time read them together. Longest first. (Of a
+    // batch whose rows may be trees the cut is that of the kernel of trees.)
+    const uint32_t units = TREE ? 1 : gridDim.x / a.parts;
+    const uint32_t part = TREE ? 0 : blockIdx.x / units, unit = blockIdx.x - part * units;
+    PagedLine line(a);
     PagedSpan span;
-    if (!line.find<PagedLine::kUnit>(span, unit)) return;
-    const uint32_t local = unit - span.unit0, turn = local / a.g.kv_heads, head = local - turn * a.g.kv_heads;
+    uint32_t from = 0, head, turn;
+    if constexpr (TREE) {
+        paged_fetch_arguments(a);
+        line.cut();
+        const uint32_t at = blockIdx.x * line.share;
+        if (at >= line.total || !line.find<PagedLine::kBlock>(span, at)) return;
+        turn = span.tiles == 1 ? 0 : (at - span.start) / span.run, from = (at - span.start) - turn * span.run, head = blockIdx.y;
+    } else {
+        if (!line.find<PagedLine::kUnit>(span, unit)) return;
+        const uint32_t local = unit - span.unit0;
+        turn = local / a.g.kv_heads, head = local - turn * a.g.kv_heads;
+    }
     const uint32_t tile = span.tiles - 1 - turn;
     const uint32_t length = span.position + span.rows;
     const uint32_t vectors = span.rows * a.group, v0 = tile * kTile;
@@ -104,9 +91,20 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     // (A row of a tree is turned by less than its number, and may see nothing of the rows before it.)
     const bool trees = TREE && paged_has_trees(a);
     const uint32_t tile_lo = lowest_visible(span.position + (trees ? 0 : first_row), a.window, 0), tile_hi = span.position + last_row + 1;
-    const uint32_t b_first = tile_lo / 32, b_all = (tile_hi + 31) / 32 - b_first, b_part = (b_all + a.parts - 1) / a.parts;
-    const uint32_t kb0 = b_first + min(b_all, part * b_part), kb_end = b_first + min(b_all, part * b_part + b_part);
-    const uint64_t slot0 = uint64_t(unit * a.parts + part) * kTile;
+    uint32_t kb0, kb_end;
+    bool whole;
+    uint64_t slot0;
+    if constexpr (TREE) {
+        whole = span.blocks <= line.share;
+        kb0 = max(span.first + from, tile_lo / 32);
+        kb_end = max(kb0, min(span.first + min(from + line.share, span.blocks), (tile_hi + 31) / 32));
+        slot0 = uint64_t(head * a.groups + blockIdx.x) * kTile;
+    } else {
+        whole = a.parts == 1;
+        const uint32_t b_first = tile_lo / 32, b_all = (tile_hi + 31) / 32 - b_first, b_part = (b_all + a.parts - 1) / a.parts;
+        kb0 = b_first + min(b_all, part * b_part), kb_end = b_first + min(b_all, part * b_part + b_part);
+        slot0 = uint64_t(unit * a.parts + part) * kTile;
+    }
 
     // Positions all of this wavefront's rows see.
     const uint32_t wv0 = v0 + wave * 32;
@@ -446,7 +444,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     }
     // A lane holds of its column channels 32 t + 8 (r / 4) + 4 h + r % 4.
     // (The check comes before the stores: the barriers it takes would wait for them.)
-    const bool whole = a.parts == 1, mine = wv0 + j < vectors;
+    const bool mine = wv0 + j < vectors;
     const uint32_t v = wv0 + j;
     const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
     const float l = __uint_as_float(both[0]) + __uint_as_float(both[1]);
@@ -459,9 +457,12 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     if (any_of_group(mine && to_be_done_over<PAGE>(all), &lds_flag)) {
         paged_careful<PAGE, ELEM, DP, TREE>(a, span, head, v0, min(v0 + kTile, vectors), wave, kWaves, 32 * kb0, 32 * kb_end,
                                       [&](uint32_t v, const float (&acc)[DP / 64], float m, float l) {
-                                          paged_write_careful<PAGE, ELEM, DP>(a, span, head, v, whole, slot0 + v - v0, true, acc, m, l);
+                                          if (TREE && !whole)
+                                              paged_part_careful<PAGE, DP>(a, slot0, v - v0, acc, m, l);
+                                          else
+                                              paged_write_careful<PAGE, ELEM, DP>(a, span, head, v, whole, slot0 + v - v0, true, acc, m, l);
                                       });
-    } else if (mine) {
+    } else if (mine || (TREE && !whole)) {
         if (whole) {
             const float inv = 1.0f / l;
             const uint32_t row = paged_row_of(a, v), hq = head * a.group + v - row * a.group;
@@ -485,11 +486,13 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
                 }
         } else {
             const uint64_t slot = slot0 + (v - v0);
+            // (For the join as the registers hold them, 1 KiB a store; for the merge row by row.)
+            floatx4 *const set_at = reinterpret_cast<floatx4 *>(a.ws_acc + slot0 * DP) + wave * (DP / 8) * 64 + lane;
 #pragma unroll
             for (int t = 0; t < kOut; ++t)
 #pragma unroll
                 for (int r = 0; r < 16; r += 4)
-                    *reinterpret_cast<floatx4 *>(a.ws_acc + slot * DP + 32 * t + 2 * r + 4 * h) =
+                    *(TREE ? set_at + (4 * t + r / 4) * 64 : reinterpret_cast<floatx4 *>(a.ws_acc + slot * DP + 32 * t + 2 * r + 4 * h)) =
                         floatx4{o[t][r], o[t][r + 1], o[t][r + 2], o[t][r + 3]};
             if (h == 0) a.ws_ml[slot] = make_float2(threshold == -INFINITY ? -INFINITY : ref, l);
         }
@@ -504,7 +507,9 @@ hipError_t launch_chunk_kernel(const PagedAttn &a, hipStream_t stream) {
         return hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(chunk_lds(DP)));
     });
     if (granted != hipSuccess) return granted;
-    launch_kernel(Kernel, a.units * a.parts, paged_chunk_waves(DP, ELEM) * 64, chunk_lds(DP), stream, a);
+    // (Workgroups that would find nothing are left out where the batch is known.)
+    const dim3 grid = a.apart ? dim3(a.share ? a.total / a.share : a.groups, a.g.kv_heads) : dim3(a.units * a.parts);
+    launch_kernel(Kernel, grid, paged_chunk_waves(DP, ELEM) * 64, chunk_lds(DP), stream, a);
     return hipGetLastError();
 }
 template <bool TREE, int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP>

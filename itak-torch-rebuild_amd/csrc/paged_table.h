@@ -40,6 +40,7 @@ struct PagedBatch {
     uint32_t most_rows = 0;      // of one
     bool trees = false;          // its rows have records
     uint32_t tree_most = 0;      // rows of its largest tree
+    uint64_t sized[2] = {};      // what attention over it, without a window and with one, has been given a captured call's memory for
     bool on_device = false;      // lengths and tables are the device's: positions in `head` are the most they may be, and there are no ids
 };
 

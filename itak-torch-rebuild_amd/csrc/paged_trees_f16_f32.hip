@@ -1,0 +1,10 @@
+// The kernel of trees over f16 pages, f32 tensors.
+#include "paged_trees_kernel.h"
+
+namespace itak {
+
+hipError_t launch_paged_trees_f16_f32(const PagedAttn &a, hipStream_t stream) {
+    return launch_trees<ITAK_ELEM_F16, ITAK_ELEM_F32, 2, 2>(a, stream);
+}
+
+}  // namespace itak
