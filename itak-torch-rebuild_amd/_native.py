@@ -264,6 +264,7 @@ class NoFront:
 
     step = prep_step = truncate = compute = gqa = staticmethod(lambda *_: -1)
     rotate = set_batch = append = paged_attention = paged_step = staticmethod(lambda *_: -1)
+    set_batch_tree = fit_tables = set_batch_device = batch_rows = accept = keep = staticmethod(lambda *_: -1)
 
 
 def load_front(lib, cache_type):
@@ -284,6 +285,9 @@ def load_front(lib, cache_type):
     front.bind_paged(rows_type, *(C.cast(getattr(lib, name), C.c_void_p).value for name in (
         "itak_rotate_device", "itak_paged_set_batch", "itak_paged_append_device", "itak_paged_attention_device",
         "itak_paged_step_device")))
+    front.bind_trees(*(C.cast(getattr(lib, name), C.c_void_p).value for name in (
+        "itak_paged_set_batch_tree", "itak_paged_fit_tables_device", "itak_paged_set_batch_device", "itak_paged_batch_rows_device",
+        "itak_paged_accept_device", "itak_paged_keep_device")))
     return front
 
 

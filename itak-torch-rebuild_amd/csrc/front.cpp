@@ -38,6 +38,12 @@ decltype(&itak_paged_set_batch) set_batch_fn;
 decltype(&itak_paged_append_device) append_fn;
 decltype(&itak_paged_attention_device) paged_attention_fn;
 decltype(&itak_paged_step_device) paged_step_fn;
+decltype(&itak_paged_set_batch_tree) set_batch_tree_fn;
+decltype(&itak_paged_fit_tables_device) fit_fn;
+decltype(&itak_paged_set_batch_device) set_batch_device_fn;
+decltype(&itak_paged_batch_rows_device) batch_rows_fn;
+decltype(&itak_paged_accept_device) accept_fn;
+decltype(&itak_paged_keep_device) keep_fn;
 PyTypeObject *cache_type;  // hip_compute.KvCache
 PyTypeObject *rows_type;   // paged.Rows
 PyObject *slot_name, *address_name, *rows_name, *channels_name;
@@ -289,8 +295,9 @@ bool bound_type(PyObject *o) {
     if (!PyType_Check(o)) PyErr_SetString(PyExc_TypeError, "a type comes first");
     return PyType_Check(o);
 }
-bool bound_addresses(PyObject *const *a, uint64_t (&at)[5]) {
-    for (int i = 0; i < 5; ++i)
+template <int N>
+bool bound_addresses(PyObject *const *a, uint64_t (&at)[N]) {
+    for (int i = 0; i < N; ++i)
         if (!plain_within(a[i], 64, at[i]) || at[i] == 0) {
             PyErr_SetString(PyExc_TypeError, "an address is an int that is not zero");
             return false;
@@ -325,9 +332,8 @@ PyObject *rotate(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return PyLong_FromLong(st);
 }
 
-// set_batch(paged, items, tables) -> status
-PyObject *set_batch(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    if (!arity(n, 3)) return nullptr;
+// set_batch(paged, items, tables) -> status, and set_batch_tree(paged, items, tables, parents) -> status
+PyObject *set_batch_with(PyObject *const *a, const int32_t *parents, Py_ssize_t parent_count) {
     itak_paged *paged;
     PyObject **item_at, **table_at;
     Py_ssize_t items, tables;
@@ -336,7 +342,7 @@ PyObject *set_batch(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (!plain_ptr(a[0], paged) || !plain_sequence(a[1], item_at, items) || !plain_sequence(a[2], table_at, tables) ||
         items != tables || items > kMostItems)
         return not_plain();
-    uint64_t all = 0;
+    uint64_t all = 0, new_rows = 0;
     for (Py_ssize_t i = 0; i < items; ++i) {
         uint64_t rows;
         Py_ssize_t pages;
@@ -347,7 +353,9 @@ PyObject *set_batch(PyObject *, PyObject *const *a, Py_ssize_t n) {
             return not_plain();
         item[i].rows = uint32_t(rows), item[i].pages = uint32_t(pages);
         all += uint64_t(pages);
+        new_rows += rows;
     }
+    if (parents && uint64_t(parent_count) != new_rows) return not_plain();
     // (A batch of one sequence is read where it lies.)
     uint32_t *joined = nullptr;
     const uint32_t *ids = items && all ? static_cast<const uint32_t *>(run[0]) : nullptr;
@@ -361,9 +369,118 @@ PyObject *set_batch(PyObject *, PyObject *const *a, Py_ssize_t n) {
     }
     itak_status st;
     Py_BEGIN_ALLOW_THREADS
-    st = set_batch_fn(paged, item, uint32_t(items), ids, all);
+    st = parents ? set_batch_tree_fn(paged, item, uint32_t(items), ids, all, parents) : set_batch_fn(paged, item, uint32_t(items), ids, all);
     Py_END_ALLOW_THREADS
     PyMem_Free(joined);
+    return PyLong_FromLong(st);
+}
+PyObject *set_batch(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (!arity(n, 3)) return nullptr;
+    return set_batch_with(a, nullptr, 0);
+}
+PyObject *set_batch_tree(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (!arity(n, 4)) return nullptr;
+    const void *parents;
+    Py_ssize_t count;
+    if (!plain_words(a[3], parents, count) || count == 0 || PyArray_TYPE(reinterpret_cast<PyArrayObject *>(a[3])) != NPY_INT32) return not_plain();
+    return set_batch_with(a, static_cast<const int32_t *>(parents), count);
+}
+
+// Every sequence's rows: a list or tuple of exact ints of 32 bits, as many as the tables have sequences.
+constexpr Py_ssize_t kMostSequences = 1024;
+bool plain_counts(PyObject *o, Py_ssize_t want, uint32_t *counts, uint64_t &sum) {
+    PyObject **at;
+    Py_ssize_t n;
+    if (!plain_sequence(o, at, n) || n != want || n > kMostSequences) return false;
+    sum = 0;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        uint64_t v;
+        if (!plain_within(at[i], 32, v)) return false;
+        counts[i] = uint32_t(v);
+        sum += v;
+    }
+    return true;
+}
+
+// fit_tables(paged, tables, sequences, lengths, rows or None, status) -> status
+PyObject *fit_tables(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (!arity(n, 6)) return nullptr;
+    itak_paged *paged;
+    const itak_page_tables *tables;
+    const int32_t *lengths;
+    int32_t *status;
+    uint64_t sequences, sum;
+    uint32_t counts[kMostSequences];
+    const bool rows = a[4] != Py_None;
+    if (!plain_ptr(a[0], paged) || !plain_ptr(a[1], tables) || !plain_within(a[2], 32, sequences) || !plain_ptr(a[3], lengths) ||
+        !plain_ptr(a[5], status) || (rows && !plain_counts(a[4], Py_ssize_t(sequences), counts, sum)))
+        return not_plain();
+    itak_status st;
+    Py_BEGIN_ALLOW_THREADS
+    st = fit_fn(paged, tables, lengths, rows ? counts : nullptr, status);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(st);
+}
+
+// set_batch_device(paged, tables, sequences, positions, rows, most_positions, parents, status) -> status << 32 | the batch's rows
+PyObject *set_batch_device(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (!arity(n, 8)) return nullptr;
+    itak_paged *paged;
+    const itak_page_tables *tables;
+    const int32_t *positions, *parents;
+    int32_t *status;
+    uint64_t sequences, most, sum = 0;
+    uint32_t counts[kMostSequences];
+    if (!plain_ptr(a[0], paged) || !plain_ptr(a[1], tables) || !plain_within(a[2], 32, sequences) || !plain_ptr(a[3], positions) ||
+        !plain_counts(a[4], Py_ssize_t(sequences), counts, sum) || sum >> 32 || !plain_within(a[5], 64, most) || !plain_ptr(a[6], parents) ||
+        !plain_ptr(a[7], status))
+        return not_plain();
+    itak_status st;
+    Py_BEGIN_ALLOW_THREADS
+    st = set_batch_device_fn(paged, tables, positions, counts, most, parents, status);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLongLong((long long)(uint32_t(st)) << 32 | (long long)sum);
+}
+
+// batch_rows(paged, positions, slots) -> status
+PyObject *batch_rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (!arity(n, 3)) return nullptr;
+    itak_paged *paged;
+    int64_t *positions, *slots;
+    if (!plain_ptr(a[0], paged) || !plain_ptr(a[1], positions) || !plain_ptr(a[2], slots)) return not_plain();
+    itak_status st;
+    Py_BEGIN_ALLOW_THREADS
+    st = batch_rows_fn(paged, positions, slots);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(st);
+}
+
+// accept(paged, tokens, chosen, path, next) -> status
+PyObject *accept(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (!arity(n, 5)) return nullptr;
+    itak_paged *paged;
+    const int32_t *tokens, *chosen;
+    int32_t *path, *next;
+    if (!plain_ptr(a[0], paged) || !plain_ptr(a[1], tokens) || !plain_ptr(a[2], chosen) || !plain_ptr(a[3], path) || !plain_ptr(a[4], next))
+        return not_plain();
+    itak_status st;
+    Py_BEGIN_ALLOW_THREADS
+    st = accept_fn(paged, tokens, chosen, path, next);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(st);
+}
+
+// keep(paged, path, lengths) -> status
+PyObject *keep(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (!arity(n, 3)) return nullptr;
+    itak_paged *paged;
+    const int32_t *path;
+    int32_t *lengths;
+    if (!plain_ptr(a[0], paged) || !plain_ptr(a[1], path) || !plain_ptr(a[2], lengths)) return not_plain();
+    itak_status st;
+    Py_BEGIN_ALLOW_THREADS
+    st = keep_fn(paged, path, lengths);
+    Py_END_ALLOW_THREADS
     return PyLong_FromLong(st);
 }
 
@@ -439,6 +556,20 @@ PyObject *bind_paged(PyObject *, PyObject *const *a, Py_ssize_t n) {
     Py_RETURN_NONE;
 }
 
+// bind_trees(address of the six functions from set_batch_tree's to keep's, in their order)
+PyObject *bind_trees(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (!arity(n, 6)) return nullptr;
+    uint64_t at[6];
+    if (!bound_addresses(a, at)) return nullptr;
+    set_batch_tree_fn = reinterpret_cast<decltype(set_batch_tree_fn)>(uintptr_t(at[0]));
+    fit_fn = reinterpret_cast<decltype(fit_fn)>(uintptr_t(at[1]));
+    set_batch_device_fn = reinterpret_cast<decltype(set_batch_device_fn)>(uintptr_t(at[2]));
+    batch_rows_fn = reinterpret_cast<decltype(batch_rows_fn)>(uintptr_t(at[3]));
+    accept_fn = reinterpret_cast<decltype(accept_fn)>(uintptr_t(at[4]));
+    keep_fn = reinterpret_cast<decltype(keep_fn)>(uintptr_t(at[5]));
+    Py_RETURN_NONE;
+}
+
 // bind(KvCache, address of step's, prep_step's, truncate's, compute's and gqa's function)
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (!arity(n, 6)) return nullptr;
@@ -464,6 +595,9 @@ PyMethodDef methods[] = {method<bind>("bind"), method<step>("step"),       metho
                          method<bind_paged>("bind_paged"), method<rotate>("rotate"), method<set_batch>("set_batch"),
                          method<append>("append"), method<paged_attention>("paged_attention"),
                          method<paged_step>("paged_step"),
+                         method<bind_trees>("bind_trees"), method<set_batch_tree>("set_batch_tree"),
+                         method<fit_tables>("fit_tables"), method<set_batch_device>("set_batch_device"),
+                         method<batch_rows>("batch_rows"), method<accept>("accept"), method<keep>("keep"),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_itak_front", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

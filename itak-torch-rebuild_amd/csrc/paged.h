@@ -140,6 +140,7 @@ hipError_t launch_paged_trees_f16_f32(const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_trees_bf16(const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_trees_bf16_f32(const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_join(uint32_t elem, const PagedAttn &a, hipStream_t stream);
+hipError_t launch_paged_few_join(uint32_t elem, const PagedAttn &a, hipStream_t stream);
 hipError_t launch_paged_merge(uint32_t elem, const PagedAttn &a, hipStream_t stream);
 // head_dim as the kernels hold it.
 __host__ __device__ constexpr uint32_t paged_padded(uint32_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }

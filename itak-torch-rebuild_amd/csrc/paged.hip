@@ -273,7 +273,7 @@ itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work, bool &whole
     // (The kernel of many rows has no line.)
     const PagedCut cut = a.parts ? PagedCut{} : paged_cut(uint32_t(work), a.units, longest, a.groups, a.least);
     whole = cut.pad >= longest;
-    if (!a.inline_items) return ITAK_OK;
+    if (!known) return ITAK_OK;
     a.share = cut.share, a.pad = cut.pad;
     for (uint32_t i = 0; i < kPagedInline; ++i) a.start[i] = a.unit0[i] = ~0u;
     each(cut.pad, [&](uint32_t i, uint64_t at, uint64_t u) {
@@ -357,7 +357,8 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
     const bool captured = captures || for_capture;
     // A handle that takes trees captures launches that find out whether the batch has them.
     if (p->batch.trees || (captured && p->tree_dev)) a.tree = p->tree_dev;
-    if (a.items <= kPagedInline && !captured && !p->batch.on_device) {
+    const bool known = !captured && !p->batch.on_device;
+    if (a.items <= kPagedInline && known) {
         a.inline_items = a.items;
         for (PagedItemWords &w : a.item) w.row0 = ~0u;
         std::memcpy(a.item, p->batch.head.data() + kPagedItem0, a.items * sizeof(PagedItemWords));
@@ -396,7 +397,7 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
         b.tile_shift = shift_of(b.tile);
         b.v_from = few_most + 1, b.v_to = ~0u;
         b.parts = 1;
-        const itak_status st = count_units(p, b, work, whole);
+        const itak_status st = count_units(p, b, work, whole, known);
         if (st != ITAK_OK) return st;
         b.parts = chunk_parts(b.units, work, cus * kPagedChunkGroupsPerCu);
     }
@@ -409,7 +410,6 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
         plan.trees_as_many = cut.chunk;
         b.tile_shift = shift_of(b.tile);
         b.least = 2;
-        const bool known = !captured && !p->batch.on_device;
         const itak_status st = count_units(p, b, work, whole, known);
         if (st != ITAK_OK) return st;
         plan.join_trees = !whole;
@@ -422,9 +422,9 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
         a.groups = std::min(cus * paged_few_groups_per_cu(dp, p->cfg.elem, q.elem, plan.sets, a.tree != nullptr), kPagedMostParts);
         a.least = 4;
         a.parts = 0;
-        const itak_status st = count_units(p, a, work, whole);
+        const itak_status st = count_units(p, a, work, whole, known);
         if (st != ITAK_OK) return st;
-        plan.merge_few = captured || p->batch.on_device || !whole;
+        plan.merge_few = !known || !whole;
     }
     const itak_status st = workspace(p, plan, dp);
     if (st == ITAK_OK && captures) {
@@ -463,7 +463,8 @@ itak_status run_attention(itak_paged *p, uint32_t elem, const AttnPlan &plan) {
                 : (elem == ITAK_ELEM_F32 ? (trees ? launch_paged_few_tree_bf16_f32 : launch_paged_few_bf16_f32)
                                          : (trees ? launch_paged_few_tree_bf16 : launch_paged_few_bf16))(plan.sets, plan.few, p->stream);
         HIP_TRY(p, he, "launch paged attention of few rows");
-        if (plan.merge_few) HIP_TRY(p, launch_paged_merge(elem, plan.few, p->stream), "launch the merge of paged attention");
+        if (plan.merge_few)
+            HIP_TRY(p, (trees ? launch_paged_few_join : launch_paged_merge)(elem, plan.few, p->stream), "launch the merge of paged attention");
     }
     if (plan.has_trees) {
         const bool f16 = p->cfg.elem == ITAK_ELEM_F16, f32 = elem == ITAK_ELEM_F32;
@@ -580,7 +581,10 @@ itak_status set_batch(itak_paged *p, const itak_paged_item *items, uint32_t coun
     while (hi > lo && p->ids_there[hi - 1] == ids[hi - 1]) --hi;
     // What the device has is unknown from the first launch to the last.
     std::copy(ids.begin() + lo, ids.begin() + hi, p->ids_there.begin() + lo);
-    for (uint32_t at = 0; at < head.size();) {
+    const bool sent = parents && next.rows && send_tree_batch(p->batch_dev, p->tree_dev, head, ids_at + lo, ids.data() + lo, hi - lo, parents,
+                                                              next.rows, next.items, p->stream);
+    if (sent) lo = hi;
+    for (uint32_t at = 0; !sent && at < head.size();) {
         const uint32_t n = std::min<uint32_t>(uint32_t(head.size()) - at, kManyWords);
         const uint32_t room = at + n == head.size() ? kManyWords - n : 0;
         const uint32_t m = std::min(room, hi - lo);
@@ -593,7 +597,7 @@ itak_status set_batch(itak_paged *p, const itak_paged_item *items, uint32_t coun
         lo += n;
     }
     hipError_t he = hipSuccess;
-    if (parents && next.rows) {
+    if (parents && next.rows && !sent) {
         uint32_t *const there = p->tree_dev + p->tree_rows * kTreeStride;
         const uint32_t *words = reinterpret_cast<const uint32_t *>(parents);
         for (uint32_t at = 0; at < next.rows; at += kManyWords)
@@ -652,7 +656,7 @@ itak_status itak_paged_create(const itak_paged_config *config, itak_paged **out)
     const DeviceScope scope(config->device);
     he = scope.status();
     p->zeros_at = (p->g.ids_at + p->cfg.max_table_pages + 3) / 4 * 4;
-    const uint64_t words = (p->zeros_at + 4 + config->max_sequences) * sizeof(uint32_t);
+    const uint64_t words = (p->zeros_at + 4 + 2 * uint64_t(config->max_sequences)) * sizeof(uint32_t);
     if (he == hipSuccess) he = hipMalloc(reinterpret_cast<void **>(&p->batch_dev), words);
     if (he == hipSuccess) he = hipMemset(p->batch_dev, 0, words);  // (an empty batch)
     if (he == hipSuccess) p->rows_dev = p->batch_dev + p->zeros_at + 4;

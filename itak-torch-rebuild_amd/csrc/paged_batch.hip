@@ -2,7 +2,7 @@
 // themselves, which take their pages from a free list and give them back.
 //
 // All of it is a few words a sequence and a row; what it costs are launches and, inside one, the trips to memory that wait for one another.
-// A workgroup serves a sequence and finds out for itself what stands before it (a sum over up to 1,024 lengths that lie in the cache),
+// A workgroup serves a sequence and finds out for itself what stands before it (a sum over up to 1,024 lengths),
 // so that a batch is one launch; the free list is one workgroup's, which every sequence's place in it has to pass through.
 #include "paged_handle.h"
 
@@ -22,57 +22,100 @@ __device__ __forceinline__ uint64_t wave_sum(uint64_t x) {
     return x;
 }
 
-// An item's records from its parents; `up`: kTreeRows words of LDS. All of a workgroup's threads ask. False, and nothing written, where they are no tree's: a parent that is no
-// row before and not -1, or more rows than a tree may have that are no chain.
-__device__ __forceinline__ bool make_records(uint32_t *tree, const int32_t *parents, uint32_t rows, uint32_t position, int32_t *up) {
+// The bits that any of a workgroup's threads has; all of them ask. `words`: a word a wavefront, another call's others.
+__device__ __forceinline__ uint32_t any_bits(uint32_t mine, uint32_t *words) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mine |= __shfl_xor(mine, o);
+    if ((threadIdx.x & 63) == 0) words[threadIdx.x / 64] = mine;
+    __syncthreads();
+    uint32_t all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kThreads / 64; ++w) all |= words[w];
+    return all;
+}
+
+// What parents are not: row 0's and so on those of a chain, and of a tree (a row before, or -1).
+constexpr uint32_t kNoChain = 1, kNoTree = 2;
+__device__ __forceinline__ uint32_t parent_is_not(int32_t parent, uint32_t r) {
+    return (parent != int32_t(r) - 1 ? kNoChain : 0) | (parent < -1 || parent >= int32_t(r) ? kNoTree : 0);
+}
+// An item's records from its parents, the threads' rows' in `up` (LDS) where it is a tree; `not_`: what any of them is not, no kNoTree.
+__device__ __forceinline__ void make_records(uint32_t *tree, uint32_t rows, uint32_t position, uint32_t not_, const int32_t *up) {
     const uint32_t tid = threadIdx.x;
-    bool other = false, wrong = false;
-    int32_t mine = 0;
-    for (uint32_t r = tid; r < rows; r += kThreads) {
-        const int32_t parent = parents[r];
-        if (r == tid) mine = parent;
-        other = other || parent != int32_t(r) - 1;
-        wrong = wrong || parent < -1 || parent >= int32_t(r);
-    }
-    if (tid < kTreeRows) up[tid] = mine;
-    if (__syncthreads_or(wrong)) return false;
-    if (!__syncthreads_or(other)) {
-        for (uint32_t r = tid; r < rows; r += kThreads) {
-            tree[uint64_t(r) * kTreeStride + kTreeDepth] = kTreeChain | r;
-            tree[uint64_t(r) * kTreeStride + kTreeParent] = r - 1;
-        }
-        return true;
-    }
-    if (rows > kTreeRows) return false;
-    if (tid < rows) {
+    if (!not_) {
+        for (uint32_t r = tid; r < rows; r += kThreads)
+            *reinterpret_cast<uint2 *>(tree + uint64_t(r) * kTreeStride) = make_uint2(kTreeChain | r, r - 1);
+    } else if (tid < rows) {
         // Upwards from the row: every step goes to a lower row, so there are at most as many steps as rows.
         const uint32_t held = position % 32;
-        uint32_t word[kTreeBlocks], depth = 0;
-#pragma unroll
-        for (uint32_t w = 0; w < kTreeBlocks; ++w) word[w] = w == 0 ? (1u << held) - 1 : 0;
+        uint32_t word[kTreeStride] = {}, depth = 0;
+        word[kTreeParent] = uint32_t(up[tid]);
+        word[kTreeSees] = (1u << held) - 1;
         for (int32_t at = int32_t(tid); at >= 0; at = up[at], ++depth) {
             const uint32_t bit = held + uint32_t(at);
 #pragma unroll
-            for (uint32_t w = 0; w < kTreeBlocks; ++w) word[w] |= bit / 32 == w ? 1u << bit % 32 : 0u;
+            for (uint32_t w = 0; w < kTreeBlocks; ++w) word[kTreeSees + w] |= bit / 32 == w ? 1u << bit % 32 : 0u;
         }
-        uint32_t *const record = tree + uint64_t(tid) * kTreeStride;
-        record[kTreeDepth] = depth - 1;
-        record[kTreeParent] = uint32_t(up[tid]);
+        word[kTreeDepth] = depth - 1;
 #pragma unroll
-        for (uint32_t w = 0; w < kTreeBlocks; ++w) record[kTreeSees + w] = word[w];
+        for (uint32_t w = 0; w < kTreeStride; w += 4)
+            *reinterpret_cast<uint4 *>(tree + uint64_t(tid) * kTreeStride + w) = make_uint4(word[w], word[w + 1], word[w + 2], word[w + 3]);
     }
-    return true;
 }
 
-__global__ __launch_bounds__(kThreads) void paged_records_kernel(const uint32_t *batch, const int32_t *parents, uint32_t *tree) {
+// A batch of trees on its way to the device: its words as those of paged.hip travel, and the parents behind them. A workgroup makes an item's
+// records, and the first stores the words besides.
+template <uint32_t N>
+struct TreeWords {
+    uint32_t *batch, *tree;
+    uint32_t n0;       // words of header and items
+    uint32_t at1, n1;  // page ids, and where they go
+    uint32_t pad;
+    uint32_t w[N];     // and then the parents
+};
+template <uint32_t N>
+__global__ __launch_bounds__(kThreads) void paged_tree_words_kernel(TreeWords<N> a) {
     __shared__ int32_t up[kTreeRows];
-    const uint4 item = *reinterpret_cast<const uint4 *>(batch + kPagedItem0 + 4 * blockIdx.x);
-    (void)make_records(tree + uint64_t(item.z) * kTreeStride, parents + item.z, item.y, item.x, up);
+    __shared__ uint32_t words[kThreads / 64];
+    const uint32_t tid = threadIdx.x;
+    // (The arguments by their address: indexed as a value they would be copied first.)
+    const uint32_t *const w = reinterpret_cast<const uint32_t *>(reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr()) + offsetof(TreeWords<N>, w));
+    const uint32_t *const item = w + kPagedItem0 + 4 * blockIdx.x;
+    if (blockIdx.x == 0)
+        for (uint32_t i = tid; i < a.n0 + a.n1; i += kThreads) a.batch[i < a.n0 ? i : a.at1 + (i - a.n0)] = w[i];
+    if (kPagedItem0 + 4 * blockIdx.x >= a.n0) return;  // (a batch without items)
+    const uint32_t position = item[0], rows = item[1], row0 = item[2];
+    const int32_t *const parents = reinterpret_cast<const int32_t *>(w) + a.n0 + a.n1 + row0;
+    uint32_t not_ = 0;
+    for (uint32_t r = tid; r < rows; r += kThreads) {
+        const int32_t parent = parents[r];
+        if (r == tid && tid < kTreeRows) up[tid] = parent;
+        not_ |= parent_is_not(parent, r);
+    }
+    not_ = any_bits(not_, words);
+    make_records(a.tree + uint64_t(row0) * kTreeStride, rows, position, not_, up);
 }
 
-// Rows of every sequence travel with the launch, or lie at rows_at where they are more.
-constexpr uint32_t kRowsInline = 256;
-struct DeviceBatch {
+__global__ __launch_bounds__(kThreads) void paged_records_kernel(const uint32_t *batch, const int32_t *all_parents, uint32_t *tree) {
+    __shared__ int32_t up[kTreeRows];
+    __shared__ uint32_t words[kThreads / 64];
+    const uint32_t tid = threadIdx.x;
+    const uint4 item = *reinterpret_cast<const uint4 *>(batch + kPagedItem0 + 4 * blockIdx.x);
+    const int32_t *const parents = all_parents + item.z;
+    uint32_t not_ = 0;
+    for (uint32_t r = tid; r < item.y; r += kThreads) {
+        const int32_t parent = parents[r];
+        if (r == tid && tid < kTreeRows) up[tid] = parent;
+        not_ |= parent_is_not(parent, r);
+    }
+    not_ = any_bits(not_, words);
+    make_records(tree + uint64_t(item.z) * kTreeStride, item.y, item.x, not_, up);
+}
+
+// Rows of every sequence, and the first of them among the batch's, travel with the launch, or lie at rows_at where they are more. (Few of them are a
+// form of its own: 2 KiB of arguments cost the host a microsecond.)
+constexpr uint32_t kRowsFew = 16, kRowsInline = 256;
+struct DeviceBatchArgs {
     uint32_t *batch;
     uint32_t *tree;
     const int32_t *parents;    // null: no trees
@@ -81,68 +124,84 @@ struct DeviceBatch {
     uint64_t stride;
     const int32_t *held;       // pages of every sequence
     int32_t *status;           // null: not asked for
-    const uint32_t *rows_at;
+    const uint32_t *rows_at;   // [sequences] rows, [sequences] first rows
     uint32_t sequences, rows;
     uint32_t page_shift;
     uint32_t page_count;
     uint32_t most_positions;
     uint32_t ids_at;
     uint64_t ids_room;
-    uint32_t inline_rows[kRowsInline];
 };
-__device__ __forceinline__ uint32_t rows_of(const DeviceBatch &a, uint32_t i) { return a.rows_at ? a.rows_at[i] : a.inline_rows[i]; }
+template <uint32_t N>
+struct DeviceBatch : DeviceBatchArgs {
+    uint32_t inline_rows[2 * N];
+};
 
-__global__ __launch_bounds__(kThreads) void paged_device_batch_kernel(DeviceBatch a) {
-    __shared__ uint64_t sums[2][kThreads / 64];
+// Lengths, numbers of pages, the first 256 of its page ids and its parents are one trip to memory for a sequence's workgroup.
+template <uint32_t N>
+__global__ __launch_bounds__(kThreads) void paged_device_batch_kernel(DeviceBatch<N> a) {
+    __shared__ uint64_t sums[kThreads / 64];
     __shared__ int32_t up[kTreeRows];
+    __shared__ uint32_t words[kThreads / 64];
     const uint32_t i = blockIdx.x, tid = threadIdx.x;
+    auto rows_of = [&](uint32_t s) { return a.rows_at ? a.rows_at[s] : a.inline_rows[s]; };
+    const uint32_t rows = rows_of(i), row0 = a.rows_at ? a.rows_at[a.sequences + i] : a.inline_rows[N + i];
+    const uint32_t first_id = tid < a.stride ? a.table[i * a.stride + tid] : 0;
+    const int32_t first_parent = a.parents && tid < rows ? a.parents[row0 + tid] : -1;
     // What a sequence's positions are refused for, and the pages that they take otherwise.
-    auto pages_of = [&](uint32_t s, uint32_t rows, uint32_t &pages) {
-        pages = 0;
-        if (!rows) return ITAK_TABLE_OK;
+    auto pages_of = [&](uint32_t s, uint32_t new_rows, uint32_t &pages) {
         const int32_t position = a.positions[s], held = a.held[s];
+        pages = 0;
+        if (!new_rows) return ITAK_TABLE_OK;
         if (position < 0 || uint32_t(position) > a.most_positions) return ITAK_TABLE_POSITION;
-        const uint32_t need = (uint32_t(position) + rows + (1u << a.page_shift) - 1) >> a.page_shift;
+        const uint32_t need = (uint32_t(position) + new_rows + (1u << a.page_shift) - 1) >> a.page_shift;
         if (held < 0 || need > uint32_t(held) || uint32_t(held) > a.stride) return ITAK_TABLE_PAGES;
         pages = need;
         return ITAK_TABLE_OK;
     };
-    uint64_t row0 = 0, id0 = 0;
-    for (uint32_t s = tid; s < i; s += kThreads) {
-        const uint32_t rows = rows_of(a, s);
-        uint32_t pages;
-        (void)pages_of(s, rows, pages);
-        row0 += rows, id0 += pages;
-    }
-    row0 = wave_sum(row0), id0 = wave_sum(id0);
-    if ((tid & 63) == 0) sums[0][tid / 64] = row0, sums[1][tid / 64] = id0;
-    __syncthreads();
-    row0 = id0 = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < kThreads / 64; ++w) row0 += sums[0][w], id0 += sums[1][w];
-    const uint32_t rows = rows_of(a, i);
     uint32_t pages;
     int32_t status = pages_of(i, rows, pages);
-    if (status == ITAK_TABLE_OK && id0 + pages > a.ids_room) status = ITAK_TABLE_ROOM;
     const uint32_t position = status == ITAK_TABLE_OK && rows ? uint32_t(a.positions[i]) : 0;
-    uint32_t *const ids = a.batch + a.ids_at + id0;
-    bool wrong = false;
-    if (status == ITAK_TABLE_OK)
-        for (uint32_t p = tid; p < pages; p += kThreads) {
-            const uint32_t id = a.table[i * a.stride + p];
-            wrong = wrong || id >= a.page_count;
-            ids[p] = id;
-        }
-    if (__syncthreads_or(wrong)) status = ITAK_TABLE_ID;
-    if (a.parents && status == ITAK_TABLE_OK &&
-        !make_records(a.tree + row0 * kTreeStride, a.parents + row0, rows, position, up))
-        status = ITAK_TABLE_PARENTS;
+    uint64_t id0 = 0;
+    for (uint32_t s = tid; s < i; s += kThreads) {
+        uint32_t others;
+        (void)pages_of(s, rows_of(s), others);
+        id0 += others;
+    }
+    id0 = wave_sum(id0);
+    if ((tid & 63) == 0) sums[tid / 64] = id0;
+    uint32_t not_ = 0;
+    constexpr uint32_t kNoPage = 4;
+    if (status == ITAK_TABLE_OK) {
+        for (uint32_t p = tid; p < pages; p += kThreads)
+            if ((p == tid ? first_id : a.table[i * a.stride + p]) >= a.page_count) not_ |= kNoPage;
+        if (a.parents)
+            for (uint32_t r = tid; r < rows; r += kThreads) not_ |= parent_is_not(r == tid ? first_parent : a.parents[row0 + r], r);
+    }
+    up[tid] = first_parent;
+    not_ = any_bits(not_, words);
+    id0 = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kThreads / 64; ++w) id0 += sums[w];
+    if (status == ITAK_TABLE_OK) {
+        if (id0 + pages > a.ids_room)
+            status = ITAK_TABLE_ROOM;
+        else if (not_ & kNoPage)
+            status = ITAK_TABLE_ID;
+        else if ((not_ & kNoTree) || ((not_ & kNoChain) && rows > kTreeRows))
+            status = ITAK_TABLE_PARENTS;
+    }
+    const bool in = status == ITAK_TABLE_OK;
+    if (in) {
+        uint32_t *const ids = a.batch + a.ids_at + id0;
+        for (uint32_t p = tid; p < pages; p += kThreads) ids[p] = p == tid ? first_id : a.table[i * a.stride + p];
+        if (a.parents) make_records(a.tree + uint64_t(row0) * kTreeStride, rows, position, not_ & kNoChain, up);
+    }
     if (tid == 0) {
-        const bool in = status == ITAK_TABLE_OK;
         *reinterpret_cast<uint4 *>(a.batch + kPagedItem0 + 4 * i) =
-            make_uint4(in ? position : 0, in ? rows : 0, uint32_t(row0), a.ids_at + uint32_t(in ? id0 : 0));
+            make_uint4(in ? position : 0, in ? rows : 0, row0, a.ids_at + uint32_t(in ? id0 : 0));
         if (a.status) a.status[i] = status;
-        if (i == 0) a.batch[0] = a.sequences, a.batch[1] = a.rows, a.batch[2] = a.parents ? 1 : 0, a.batch[3] = 0;
+        if (i == 0) *reinterpret_cast<uint4 *>(a.batch) = make_uint4(a.sequences, a.rows, a.parents ? 1 : 0, 0);
     }
 }
 
@@ -174,8 +233,7 @@ __global__ __launch_bounds__(kThreads) void paged_batch_rows_kernel(BatchRows a)
 
 // Page tables that grow and shrink to lengths. Pages given back come onto the free list's end in the order in which taking them from
 // there finds them again; then sequences take theirs from the end, the first ones first.
-constexpr uint32_t kFitThreads = 1024;
-struct FitTables {
+struct FitTablesArgs {
     uint32_t *table;
     uint64_t stride;
     int32_t *held;
@@ -188,9 +246,13 @@ struct FitTables {
     uint32_t page_shift;
     uint32_t page_count;
     uint32_t plus_rows;        // whether rows come on top of the lengths
-    uint32_t inline_rows[kRowsInline];
 };
-// Inclusive sums over the workgroup; `sums` is kFitThreads / 64 words of LDS, which the caller lets go of behind a barrier.
+template <uint32_t N>
+struct FitTables : FitTablesArgs {
+    uint32_t inline_rows[N];
+};
+// Inclusive sums over the workgroup; `sums` is a word a wavefront of LDS, which the caller lets go of behind a barrier.
+template <uint32_t THREADS>
 __device__ __forceinline__ uint64_t scan_all(uint64_t x, uint64_t *sums) {
     const uint32_t lane = __lane_id(), wave = threadIdx.x / 64;
 #pragma unroll
@@ -198,15 +260,19 @@ __device__ __forceinline__ uint64_t scan_all(uint64_t x, uint64_t *sums) {
         const uint64_t y = __shfl_up(x, d);
         x += lane >= uint32_t(d) ? y : 0;
     }
-    if (lane == 63) sums[wave] = x;
-    __syncthreads();
-    for (uint32_t w = 0; w < wave; ++w) x += sums[w];
+    if constexpr (THREADS > 64) {
+        if (lane == 63) sums[wave] = x;
+        __syncthreads();
+        for (uint32_t w = 0; w < wave; ++w) x += sums[w];
+    }
     return x;
 }
-__global__ __launch_bounds__(kFitThreads) void paged_fit_kernel(FitTables a) {
-    __shared__ uint64_t sums[2][kFitThreads / 64];
-    __shared__ uint64_t ends[kFitThreads];   // of every sequence's pages among those that move
-    __shared__ uint32_t from[kFitThreads];   // its first of them
+// THREADS: as many as the sequences, or more: 64 are one wavefront, whose barriers cost nothing.
+template <uint32_t THREADS, uint32_t N>
+__global__ __launch_bounds__(THREADS) void paged_fit_kernel(FitTables<N> a) {
+    __shared__ uint64_t sums[2][THREADS / 64];
+    __shared__ uint64_t ends[THREADS];   // of every sequence's pages among those that move
+    __shared__ uint32_t from[THREADS];   // its first of them
     const uint32_t i = threadIdx.x, n = a.sequences;
     int32_t status = ITAK_TABLE_OK;
     uint32_t held = 0, need = 0;
@@ -225,22 +291,22 @@ __global__ __launch_bounds__(kFitThreads) void paged_fit_kernel(FitTables a) {
     const bool sound = said >= 0 && uint32_t(said) <= a.page_count;
     const uint64_t count = sound ? uint32_t(said) : 0;
     // Back: page `from + k` of a sequence is number `before + k` of all that go, and lies that far from the list's end when they have come.
-    const uint64_t back = need < held ? held - need : 0, back_end = scan_all(back, sums[0]);
+    const uint64_t back = need < held ? held - need : 0, back_end = scan_all<THREADS>(back, sums[0]);
     ends[i] = back_end, from[i] = need;
     __syncthreads();
-    const uint64_t all_back = ends[kFitThreads - 1];
+    const uint64_t all_back = ends[THREADS - 1];
     const bool room = sound && count + all_back <= a.page_count;
     // The sequence that has number x of the pages that move, and which of its own that is.
     auto owner = [&](uint64_t x, uint64_t &own) {
         uint32_t s = 0;
 #pragma unroll
-        for (uint32_t step = kFitThreads / 2; step; step /= 2)
+        for (uint32_t step = THREADS / 2; step; step /= 2)
             if (ends[s + step - 1] <= x) s += step;
         own = x - (s ? ends[s - 1] : 0) + from[s];
         return s;
     };
     if (room)
-        for (uint64_t x = i; x < all_back; x += kFitThreads) {
+        for (uint64_t x = i; x < all_back; x += THREADS) {
             uint64_t own;
             const uint32_t s = owner(x, own);
             a.free_ids[count + all_back - 1 - x] = a.table[s * a.stride + own];
@@ -248,7 +314,7 @@ __global__ __launch_bounds__(kFitThreads) void paged_fit_kernel(FitTables a) {
     __syncthreads();  // (what was given back is there to be taken)
     const uint64_t have_free = count + all_back;
     uint64_t take = room && need > held ? need - held : 0;
-    const uint64_t take_end = scan_all(take, sums[1]);
+    const uint64_t take_end = scan_all<THREADS>(take, sums[1]);
     const bool granted = take_end <= have_free;
     // (Sequences behind one that goes without do so too where they take any: what they would get depends on nobody else's being refused.)
     if (take && !granted) status = ITAK_TABLE_FREE;
@@ -265,8 +331,8 @@ __global__ __launch_bounds__(kFitThreads) void paged_fit_kernel(FitTables a) {
     }
     if (__lane_id() == 0) sums[0][i / 64] = all_taken;
     __syncthreads();
-    for (uint32_t w = 0; w < kFitThreads / 64; ++w) all_taken = sums[0][w] > all_taken ? sums[0][w] : all_taken;
-    for (uint64_t x = i; x < all_taken; x += kFitThreads) {
+    for (uint32_t w = 0; w < THREADS / 64; ++w) all_taken = sums[0][w] > all_taken ? sums[0][w] : all_taken;
+    for (uint64_t x = i; x < all_taken; x += THREADS) {
         uint64_t own;
         const uint32_t s = owner(x, own);
         a.table[s * a.stride + own] = a.free_ids[have_free - 1 - x];
@@ -279,6 +345,24 @@ __global__ __launch_bounds__(kFitThreads) void paged_fit_kernel(FitTables a) {
 }
 
 }  // namespace
+
+template <uint32_t N>
+void send_tree(uint32_t *batch, uint32_t *tree, const std::vector<uint32_t> &head, uint32_t ids_at, const uint32_t *ids, uint32_t id_count,
+               const int32_t *parents, uint32_t rows, uint32_t items, hipStream_t stream) {
+    TreeWords<N> a;
+    a.batch = batch, a.tree = tree, a.n0 = uint32_t(head.size()), a.at1 = ids_at, a.n1 = id_count, a.pad = 0;
+    std::copy(head.begin(), head.end(), a.w);
+    std::copy(ids, ids + id_count, a.w + a.n0);
+    std::copy(parents, parents + rows, reinterpret_cast<int32_t *>(a.w) + a.n0 + id_count);
+    launch_kernel(paged_tree_words_kernel<N>, std::max(1u, items), kThreads, 0, stream, a);
+}
+bool send_tree_batch(uint32_t *batch, uint32_t *tree, const std::vector<uint32_t> &head, uint32_t ids_at, const uint32_t *ids, uint32_t id_count,
+                     const int32_t *parents, uint32_t rows, uint32_t items, hipStream_t stream) {
+    const uint64_t words = head.size() + id_count + rows;
+    if (words > kManyWords) return false;
+    (words <= kFewWords ? send_tree<kFewWords> : send_tree<kManyWords>)(batch, tree, head, ids_at, ids, id_count, parents, rows, items, stream);
+    return true;
+}
 
 hipError_t launch_paged_records(const uint32_t *batch, uint32_t items, const int32_t *parents, uint32_t *tree, hipStream_t stream) {
     launch_kernel(paged_records_kernel, items, kThreads, 0, stream, batch, parents, tree);
@@ -301,17 +385,25 @@ itak_status check_tables(itak_paged *p, const itak_page_tables *t) {
     return ITAK_OK;
 }
 
-// Every sequence's rows: with the launch, or in the handle's memory where they are more than that takes.
-itak_status place_rows(itak_paged *p, const uint32_t *rows, uint32_t n, uint32_t *inline_rows, const uint32_t **rows_at) {
-    *rows_at = nullptr;
-    if (n <= kRowsInline) {
-        std::copy(rows, rows + n, inline_rows);
-        return ITAK_OK;
-    }
-    uint32_t *const there = p->rows_dev;
-    for (uint32_t at = 0; at < n; at += kManyWords) send_words(there, at, rows + at, std::min(n - at, kManyWords), 0, nullptr, 0, p->stream);
-    *rows_at = there;
-    return ITAK_OK;
+// Words of every sequence where they are more than travel with a launch, to the handle's memory, `at` words from its start.
+void place_words(itak_paged *p, const uint32_t *words, uint32_t n, uint32_t at) {
+    for (uint32_t i = 0; i < n; i += kManyWords)
+        send_words(p->rows_dev, at + i, words + i, std::min(n - i, kManyWords), 0, nullptr, 0, p->stream);
+}
+
+template <uint32_t THREADS, uint32_t N>
+void launch_fit(const FitTablesArgs &args, const uint32_t *rows, uint32_t n, hipStream_t stream) {
+    FitTables<N> a;
+    static_cast<FitTablesArgs &>(a) = args;
+    if (rows) std::copy(rows, rows + n, a.inline_rows);
+    launch_kernel(paged_fit_kernel<THREADS, N>, 1, THREADS, 0, stream, a);
+}
+template <uint32_t N>
+void launch_device_batch(const DeviceBatchArgs &args, const uint32_t *rows, const uint32_t *first, uint32_t n, hipStream_t stream) {
+    DeviceBatch<N> a;
+    static_cast<DeviceBatchArgs &>(a) = args;
+    if (rows) std::copy(rows, rows + n, a.inline_rows), std::copy(first, first + n, a.inline_rows + N);
+    launch_kernel(paged_device_batch_kernel<N>, args.sequences, kThreads, 0, stream, a);
 }
 
 }  // namespace
@@ -349,9 +441,12 @@ itak_status itak_paged_fit_tables_device(itak_paged *paged, const itak_page_tabl
     if (!lengths_dev) return invalid_argument(paged->err, "lengths are null");
     const DeviceScope scope(paged->cfg.device);
     HIP_TRY(paged, scope.status(), "set the device");
-    FitTables a{};
-    if (rows) st = place_rows(paged, rows, tables->sequences, a.inline_rows, &a.rows_at);
-    if (st != ITAK_OK) return st;
+    FitTablesArgs a{};
+    const uint32_t n = tables->sequences;
+    if (rows && n > kRowsInline) {
+        place_words(paged, rows, n, 0);
+        a.rows_at = paged->rows_dev;
+    }
     a.table = tables->table, a.stride = tables->stride, a.held = tables->pages;
     a.free_ids = tables->free_ids, a.free_count = tables->free_count;
     a.lengths = lengths_dev, a.status = status_dev;
@@ -359,7 +454,14 @@ itak_status itak_paged_fit_tables_device(itak_paged *paged, const itak_page_tabl
     a.page_shift = paged->g.page_shift;
     a.page_count = uint32_t(paged->cfg.page_count);
     a.plus_rows = rows != nullptr;
-    launch_kernel(paged_fit_kernel, 1, kFitThreads, 0, paged->stream, a);
+    if (n <= 64 && (!rows || n <= kRowsFew))
+        launch_fit<64, kRowsFew>(a, rows, n, paged->stream);
+    else if (n <= 64)
+        launch_fit<64, kRowsInline>(a, rows, n, paged->stream);
+    else if (n <= kRowsInline)
+        launch_fit<256, kRowsInline>(a, rows, n, paged->stream);
+    else
+        launch_fit<1024, kRowsFew>(a, nullptr, n, paged->stream);
     HIP_TRY(paged, hipGetLastError(), "launch the fitting of page tables");
     return ITAK_OK;
 }
@@ -395,18 +497,23 @@ itak_status itak_paged_set_batch_device(itak_paged *paged, const itak_page_table
         next.items = n, next.rows = uint32_t(all), next.most_rows = most;
         next.trees = parents_dev != nullptr, next.tree_most = tree_most, next.on_device = true, next.sized[0] = next.sized[1] = 0;
         uint32_t row0 = 0;
+        paged->first_rows.resize(n);
         for (uint32_t i = 0; i < n; row0 += rows[i], ++i) {
             const uint32_t words[4] = {uint32_t(most_positions), rows[i], row0, 0};
             next.head.insert(next.head.end(), words, words + 4);
+            paged->first_rows[i] = row0;
         }
         next.head[0] = n, next.head[1] = next.rows, next.head[2] = next.trees;
     } catch (const std::bad_alloc &) {
         return invalid_argument(paged->err, "out of host memory");
     }
     if (!paged_replays_hold(paged, paged->next)) return size_overflow(paged->err, "a captured attention over the batch");
-    DeviceBatch a{};
-    st = place_rows(paged, rows, n, a.inline_rows, &a.rows_at);
-    if (st != ITAK_OK) return st;
+    DeviceBatchArgs a{};
+    if (n > kRowsInline) {
+        place_words(paged, rows, n, 0);
+        place_words(paged, paged->first_rows.data(), n, n);
+        a.rows_at = paged->rows_dev;
+    }
     a.batch = paged->batch_dev, a.tree = paged->tree_dev;
     a.parents = parents_dev, a.positions = positions_dev;
     a.table = tables->table, a.stride = tables->stride, a.held = tables->pages;
@@ -419,7 +526,13 @@ itak_status itak_paged_set_batch_device(itak_paged *paged, const itak_page_table
     // (The ids that the device has are the tables' from now on, and of a graph's replays whenever they run.)
     paged->ids_known = false;
     if (capturing(paged->stream)) paged->ids_never_known = true;
-    launch_kernel(paged_device_batch_kernel, n, kThreads, 0, paged->stream, a);
+    const uint32_t *const first = paged->first_rows.data();
+    if (n <= kRowsFew)
+        launch_device_batch<kRowsFew>(a, rows, first, n, paged->stream);
+    else if (n <= kRowsInline)
+        launch_device_batch<kRowsInline>(a, rows, first, n, paged->stream);
+    else
+        launch_device_batch<kRowsFew>(a, nullptr, nullptr, n, paged->stream);
     if (const hipError_t he = hipGetLastError(); he != hipSuccess) {
         paged->batch = PagedBatch{};
         return hip_error(paged->err, he, "launch the making of a batch");

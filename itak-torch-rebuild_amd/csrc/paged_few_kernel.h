@@ -418,7 +418,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
 template <bool TREE, int PAGE, int ELEM, int DP, bool EXACT, int NQ, int NP>
 void launch_few_as(uint32_t sets, const PagedAttn &a, hipStream_t stream) {
     // (Workgroups that would find nothing are left out where the batch is known.)
-    const uint32_t groups = a.inline_items ? (a.total + a.share - 1) / a.share : a.groups;
+    const uint32_t groups = a.share ? (a.total + a.share - 1) / a.share : a.groups;
     if (sets == 1) {
         launch_kernel(paged_few_kernel<PAGE, ELEM, DP, EXACT, NQ, NP, 1, TREE>, groups, kFewWaves * 64, 0, stream, a);
     } else {

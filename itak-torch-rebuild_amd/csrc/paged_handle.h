@@ -36,7 +36,8 @@ struct itak_paged {
     // Of a handle that takes trees: a record for each of up to tree_rows rows (paged_tree.h), then those rows' parents on their way there.
     uint32_t *tree_dev = nullptr;
     uint64_t tree_rows = 0;
-    uint32_t *rows_dev = nullptr;    // every sequence's rows on their way to a batch that the device makes
+    uint32_t *rows_dev = nullptr;    // every sequence's rows, and its first, on their way to a batch that the device makes
+    std::vector<uint32_t> first_rows;
     bool ids_known = true;           // what the device has of page ids is what ids_there says
     bool ids_never_known = false;    // a captured graph may set the batch
     mutable itak::ErrorState err;
@@ -61,7 +62,9 @@ constexpr uint32_t kFewWords = 112, kManyWords = 960;
 void send_words(uint32_t *dst, uint32_t at0, const uint32_t *w0, uint32_t n0, uint32_t at1, const uint32_t *w1, uint32_t n1,
                 hipStream_t stream);
 bool paged_replays_hold(const itak_paged *p, const PagedBatch &batch);
-// paged_batch.hip: the records of a batch whose items and parents the device has.
+// paged_batch.hip: a batch of trees, of few enough words for one launch, and the records of one whose items and parents the device has.
+bool send_tree_batch(uint32_t *batch, uint32_t *tree, const std::vector<uint32_t> &head, uint32_t ids_at, const uint32_t *ids, uint32_t id_count,
+                     const int32_t *parents, uint32_t rows, uint32_t items, hipStream_t stream);
 hipError_t launch_paged_records(const uint32_t *batch, uint32_t items, const int32_t *parents, uint32_t *tree, hipStream_t stream);
 
 }  // namespace itak

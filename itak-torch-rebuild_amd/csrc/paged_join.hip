@@ -158,7 +158,109 @@ void launch(const PagedAttn &a, hipStream_t stream) {
         launch_as<ELEM, 256>(a, stream);
 }
 
+// The partials of the kernel of few rows, which lie vector by vector, where rows are drafted trees: some vectors for every compute unit, of a few
+// parts each. A wavefront serves a vector (paged_merge.hip gives a workgroup to each: 85 rows of 32 heads of 64 10.8 us, and so 5.7).
+template <int ELEM, int DP>
+__global__ __launch_bounds__(kThreads) void paged_few_join_kernel(PagedAttn a) {
+    typedef typename Elem<ELEM>::type T;
+    constexpr uint32_t kQuads = DP / 4, kParts = 64 / kQuads, kAtOnce = 8;  // float4s of a partial, and partials that a wavefront takes at once
+    paged_fetch_arguments(a);
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const uint32_t heads = a.g.kv_heads * a.group, vector = blockIdx.x * (kThreads / 64) + wave;
+    const uint32_t row = vector / heads, hq = vector - row * heads;
+    PagedLine line(a);
+    line.cut();
+    PagedSpan span;
+    if (row >= a.rows || !line.find<PagedLine::kRow>(span, row)) return;
+    const uint32_t head = paged_row_of(a, hq), v = (row - span.row0) * a.group + (hq - head * a.group);
+    const uint32_t tile = v >> a.tile_shift, local = tile * a.g.kv_heads + head, unit = span.unit0 + local;
+    // Slots first .. last of the unit's partials, from slot `unit` on.
+    const uint32_t from = span.start + local * span.run, first = from / line.share, last = (from + span.blocks - 1) / line.share;
+    if (first == last || last + unit >= a.groups + a.units) return;  // written whole
+    const uint32_t parts = last - first + 1;
+    const uint64_t base = uint64_t(unit + first) * a.tile + (v - (tile << a.tile_shift));
+    const uint32_t quad = lane % kQuads, part = lane / kQuads;
+    auto acc_of = [&](uint32_t w) { return *reinterpret_cast<const floatx4 *>(a.ws_acc + (base + uint64_t(w) * a.tile) * DP + quad * 4); };
+    floatx4 early[kAtOnce];
+#pragma unroll
+    for (uint32_t u = 0; u < kAtOnce; ++u) early[u] = acc_of(min(part + u * kParts, parts - 1));
+    // Every lane has every 64th part's maximum and sum; the first ones' stay.
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (lane < parts) ml = a.ws_ml[base + uint64_t(lane) * a.tile];
+    float m = ml.x;
+    for (uint32_t p = lane + 64; p < parts; p += 64) m = fmaxf(m, a.ws_ml[base + uint64_t(p) * a.tile].x);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    // (A maximum of minus infinity: nothing visible, a sum of 0, or scores that are no numbers, which the sum then is.)
+    auto weight_of = [&](float2 x) { return x.x == -INFINITY ? 0.0f : fast_exp2(x.x - m) * (x.y < 0.0f ? kPagedMergeLift : 1.0f); };
+    auto sum_of = [&](float2 x) { return x.x == -INFINITY ? x.y : weight_of(x) * __builtin_fabsf(x.y); };
+    float l = sum_of(ml);
+    for (uint32_t p = lane + 64; p < parts; p += 64) l += sum_of(a.ws_ml[base + uint64_t(p) * a.tile]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+    const float inv = 1.0f / l;
+    floatx4 acc = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t run = 0; run < parts; run += 64) {
+        if (run) {
+            ml = make_float2(-INFINITY, 0.0f);
+            if (run + lane < parts) ml = a.ws_ml[base + uint64_t(run + lane) * a.tile];
+        }
+        const float share = weight_of(ml) * inv;
+        for (uint32_t first_of = 0; first_of < min(64u, parts - run); first_of += kAtOnce * kParts) {
+            if (run + first_of) {
+#pragma unroll
+                for (uint32_t u = 0; u < kAtOnce; ++u) early[u] = acc_of(min(run + first_of + part + u * kParts, parts - 1));
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < kAtOnce; ++u) {
+                const uint32_t w = first_of + part + u * kParts;  // of the run: below 64, or behind the last part
+                const float x = __shfl(share, w & 63);
+                if (w < 64 && run + w < parts) acc += early[u] * x;
+            }
+        }
+    }
+#pragma unroll
+    for (uint32_t o = kQuads; o < 64; o *= 2)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o);
+    const uint32_t c = quad * 4;
+    if (part || c >= a.g.head_dim) return;
+    T *dst = static_cast<T *>(a.out.data) + uint64_t(row) * a.out.row_stride + hq * a.out.head_stride + c;
+    Piece<T, 4> y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y.v[e] = Elem<ELEM>::from_f32(acc[e]);
+    if (a.out_on_16) {
+        *reinterpret_cast<Piece<T, 4> *>(dst) = y;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dst[e] = y.v[e];
+    }
+}
+
+template <int ELEM>
+void launch_few(const PagedAttn &a, hipStream_t stream) {
+    const uint32_t dp = paged_padded(a.g.head_dim), groups = uint32_t((uint64_t(a.rows) * a.g.kv_heads * a.group + 3) / 4);
+    if (dp == 64)
+        launch_kernel(paged_few_join_kernel<ELEM, 64>, groups, kThreads, 0, stream, a);
+    else if (dp == 128)
+        launch_kernel(paged_few_join_kernel<ELEM, 128>, groups, kThreads, 0, stream, a);
+    else
+        launch_kernel(paged_few_join_kernel<ELEM, 256>, groups, kThreads, 0, stream, a);
+}
+
 }  // namespace
+
+hipError_t launch_paged_few_join(uint32_t elem, const PagedAttn &a, hipStream_t stream) {
+    // (One row's or two's vectors would leave most of the device without: a workgroup each.)
+    if (uint64_t(a.rows) * a.g.kv_heads * a.group <= 256) return launch_paged_merge(elem, a, stream);
+    if (elem == ITAK_ELEM_F32)
+        launch_few<ITAK_ELEM_F32>(a, stream);
+    else if (elem == ITAK_ELEM_F16)
+        launch_few<ITAK_ELEM_F16>(a, stream);
+    else
+        launch_few<ITAK_ELEM_BF16>(a, stream);
+    return hipGetLastError();
+}
 
 hipError_t launch_paged_join(uint32_t elem, const PagedAttn &a, hipStream_t stream) {
     if (elem == ITAK_ELEM_F32)

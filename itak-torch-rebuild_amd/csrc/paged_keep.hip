@@ -23,17 +23,29 @@ __device__ __forceinline__ uint32_t rows_end(const uint32_t *batch, uint32_t n, 
 struct Accept {
     const uint32_t *batch;
     const uint32_t *tree;
+    uint64_t tree_rows;
     const int32_t *tokens, *chosen;
     int32_t *path, *next;
     uint32_t rows;
 };
 __global__ __launch_bounds__(64) void paged_accept_kernel(Accept a) {
     constexpr uint32_t kOfLane = kTreeRows / 64;
-    const uint32_t n = min(a.batch[0], gridDim.x), i = blockIdx.x, lane = threadIdx.x;
-    if (i >= n) return;
+    const uint32_t i = blockIdx.x, lane = threadIdx.x;
     const uint4 item = *reinterpret_cast<const uint4 *>(a.batch + kPagedItem0 + 4 * i);
-    const uint32_t row0 = item.z, end = rows_end(a.batch, n, i, a.rows);
+    const uint32_t n = min(a.batch[0], gridDim.x), row0 = item.z;
+    if (i >= n) return;
+    const uint32_t end = rows_end(a.batch, n, i, a.rows);
     const uint32_t rows = row0 < end ? min(item.y, end - row0) : 0;
+    // All of a tree's rows at once. (Those behind it are clamped to the batch's last.)
+    int32_t parent[kOfLane], token[kOfLane], chosen[kOfLane];
+#pragma unroll
+    for (uint32_t k = 0; k < kOfLane; ++k) {
+        parent[k] = -2, token[k] = chosen[k] = 0;
+        if (64 * k >= rows) continue;
+        const uint32_t at = min(row0 + 64 * k + lane, a.rows - 1);
+        parent[k] = int32_t(a.tree[min(uint64_t(at), a.tree_rows - 1) * kTreeStride + kTreeParent]);
+        token[k] = a.tokens[at], chosen[k] = a.chosen[at];
+    }
     const bool chain = !a.batch[2] || (rows && a.tree[uint64_t(row0) * kTreeStride] & kTreeChain);
     uint32_t kept = 0;
     int32_t choice = 0;
@@ -53,13 +65,9 @@ __global__ __launch_bounds__(64) void paged_accept_kernel(Accept a) {
         for (uint32_t r = lane; r < kept; r += 64) a.path[row0 + r] = int32_t(r);
         choice = a.chosen[row0 + last];
     } else if (rows) {
-        int32_t parent[kOfLane], token[kOfLane], chosen[kOfLane];
 #pragma unroll
-        for (uint32_t k = 0; k < kOfLane; ++k) {
-            const uint32_t r = 64 * k + lane, at = row0 + min(r, rows - 1);
-            parent[k] = r < rows ? int32_t(a.tree[uint64_t(at) * kTreeStride + kTreeParent]) : -2;
-            token[k] = a.tokens[at], chosen[k] = a.chosen[at];
-        }
+        for (uint32_t k = 0; k < kOfLane; ++k)
+            if (64 * k + lane >= rows) parent[k] = -2;
         uint32_t at = 0;
         while (true) {  // (a child lies behind its parent: at most as many steps as rows)
             if (lane == 0) a.path[row0 + kept] = int32_t(at);
@@ -95,33 +103,42 @@ constexpr uint32_t kKeepThreads = 256;
 __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(Keep a) {
     constexpr uint32_t kAtOnce = 8;
     __shared__ uint64_t lds_from[kKeepThreads], lds_to[kKeepThreads];
+    __shared__ int32_t lds_path[kKeepThreads];
+    __shared__ uint32_t lds_ids[kKeepThreads / 16 + 1];  // pages of as many rows
     __shared__ uint32_t lds_moves, lds_kept, lds_wrong;
-    const uint32_t n = min(a.batch[0], gridDim.x), i = blockIdx.x, tid = threadIdx.x;
-    if (i >= n) return;
+    const uint32_t i = blockIdx.x, tid = threadIdx.x;
     const uint4 item = *reinterpret_cast<const uint4 *>(a.batch + kPagedItem0 + 4 * i);
+    const uint32_t n = min(a.batch[0], gridDim.x), row0 = item.z;
+    if (i >= n) return;
     const uint32_t end = rows_end(a.batch, n, i, a.rows);
-    const uint32_t rows = item.z < end ? min(item.y, end - item.z) : 0;
+    const uint32_t rows = row0 < end ? min(item.y, end - row0) : 0;
     if (!rows) return;
-    const int32_t *const path = a.path + item.z;
+    // The path and the pages of the rows it may name are one trip, for the first 256 of them.
+    const uint32_t first_page = item.x >> a.g.page_shift, last_page = (item.x + rows - 1) >> a.g.page_shift;
+    lds_path[tid] = a.path[min(row0 + tid, a.rows - 1)];
+    if (tid < kKeepThreads / 16 + 1) lds_ids[tid] = a.batch[item.w + min(first_page + tid, last_page)];
+    auto path_of = [&](uint32_t j) { return j < kKeepThreads ? lds_path[j] : a.path[row0 + j]; };
     // How many are kept, and whether they ascend: looked through before anything moves.
     if (tid == 0) lds_kept = rows, lds_wrong = 0;
     __syncthreads();
     for (uint32_t j = tid; j < rows; j += kKeepThreads)
-        if (path[j] < 0) {
+        if (path_of(j) < 0) {
             atomicMin(&lds_kept, j);
             break;
         }
     __syncthreads();
     const uint32_t kept = lds_kept;
     for (uint32_t j = tid; j < kept; j += kKeepThreads)
-        if (path[j] >= int32_t(rows) || (j && path[j - 1] >= path[j])) lds_wrong = 1;
+        if (path_of(j) >= int32_t(rows) || (j && path_of(j - 1) >= path_of(j))) lds_wrong = 1;
     __syncthreads();
     const bool wrong = lds_wrong != 0;
     if (blockIdx.y == 0 && tid == 0 && a.lengths) a.lengths[i] = wrong ? -1 : int32_t(item.x + kept);
     if (wrong) return;
     const uint32_t mask = (1u << a.g.page_shift) - 1;
     auto place = [&](uint32_t position) {
-        return a.batch[item.w + (position >> a.g.page_shift)] * a.g.page_stride + uint64_t(position & mask) * a.g.head_dim;
+        const uint32_t page = position >> a.g.page_shift;
+        const uint32_t id = position < item.x + kKeepThreads ? lds_ids[page - first_page] : a.batch[item.w + page];
+        return id * a.g.page_stride + uint64_t(position & mask) * a.g.head_dim;
     };
     const uint32_t of_head = a.g.head_dim / 8;
     for (uint32_t j0 = 0; j0 < kept; j0 += kKeepThreads) {
@@ -129,7 +146,7 @@ __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(Keep a) {
         if (tid == 0) lds_moves = 0;
         __syncthreads();
         const uint32_t j = j0 + tid;
-        const uint32_t here = j < kept ? uint32_t(path[j]) : j;
+        const uint32_t here = j < kept ? uint32_t(path_of(j)) : j;
         // (Rows that stay where they are come first: an ascending list that has left its places never comes back to them.)
         const bool moves = here != j;
         if (moves) {
@@ -181,7 +198,7 @@ itak_status itak_paged_accept_device(itak_paged *paged, const int32_t *tokens_de
     if (!tokens_dev || !chosen_dev || !path_dev || !next_dev) return invalid_argument(paged->err, "tokens, chosen, path or next are null");
     const DeviceScope scope(paged->cfg.device);
     HIP_TRY(paged, scope.status(), "set the device");
-    const Accept a{paged->batch_dev, paged->tree_dev, tokens_dev, chosen_dev, path_dev, next_dev, paged->batch.rows};
+    const Accept a{paged->batch_dev, paged->tree_dev, paged->tree_rows, tokens_dev, chosen_dev, path_dev, next_dev, paged->batch.rows};
     launch_kernel(paged_accept_kernel, paged->batch.items, 64, 0, paged->stream, a);
     HIP_TRY(paged, hipGetLastError(), "launch the walk down a tree");
     return ITAK_OK;

@@ -139,11 +139,12 @@ class PageTables:
     """Page tables on the device (itak_page_tables), the caller's memory: of each sequence up to `stride` page ids and how many, and the
     free list."""
 
-    __slots__ = ("raw", "ref", "sequences", "keep")
+    __slots__ = ("raw", "ref", "at", "sequences", "keep")
 
     def __init__(self, table_ptr: int, stride: int, pages_ptr: int, sequences: int, free_ptr: int = 0, free_count_ptr: int = 0, keep=None):
         self.raw = _filled(N.PageTables, table_ptr or None, stride, pages_ptr or None, free_ptr or None, free_count_ptr or None, sequences, 0)
         self.ref = C.byref(self.raw)
+        self.at = C.addressof(self.raw)  # as the front module takes it
         self.sequences = sequences
         self.keep = keep  # what owns the memory
 
@@ -246,7 +247,8 @@ class PagedKv:
                   parents: Optional[Sequence[int]] = None) -> None:
         """The sequences of the next forward: (positions held, new rows) of each, and its page ids in order. `parents` makes the new
         rows trees: of all rows in order the number of the row of the same sequence that it continues, or -1."""
-        status = -1 if parents is not None else hip_compute._front.set_batch(self._hv, items, pages)
+        front = hip_compute._front
+        status = front.set_batch(self._hv, items, pages) if parents is None else front.set_batch_tree(self._hv, items, pages, parents)
         if status >= 0:
             self._done(status)
             self._rows = sum([rows for _, rows in items])
@@ -284,6 +286,10 @@ class PagedKv:
 
     def fit_tables_device(self, tables: PageTables, lengths_ptr: int, rows: Optional[Sequence[int]] = None, status_ptr: int = 0) -> None:
         """Page tables to lengths on the device (int32 [sequences]), and `rows` new rows on top of each: pages from the free list, or back."""
+        status = hip_compute._front.fit_tables(self._hv, tables.at, tables.sequences, lengths_ptr, rows, status_ptr)
+        if status >= 0:
+            self._done(status)
+            return
         words, rows_ptr, named = _words(rows, "I", 0, (1 << 32) - 1, "rows") if rows is not None else (None, None, tables.sequences)
         if named != tables.sequences:
             raise ValueError(f"rows of {named} sequences, tables of {tables.sequences}")
@@ -293,6 +299,12 @@ class PagedKv:
                          status_ptr: int = 0) -> None:
         """The batch from positions (int32 [sequences]), tables and parents (int32 [sum rows]) on the device; `rows` new rows of each sequence,
         behind at most `most_positions`."""
+        done = hip_compute._front.set_batch_device(self._hv, tables.at, tables.sequences, positions_ptr, rows, most_positions, parents_ptr,
+                                                   status_ptr)
+        if done >= 0:
+            self._done(done >> 32)
+            self._rows = done & 0xFFFFFFFF
+            return
         words, rows_ptr, named = _words(rows, "I", 0, (1 << 32) - 1, "rows")
         if named != tables.sequences:
             raise ValueError(f"rows of {named} sequences, tables of {tables.sequences}")
@@ -304,16 +316,20 @@ class PagedKv:
 
     def batch_rows_device(self, positions_ptr: int = 0, slots_ptr: int = 0) -> None:
         """Every row's position in the text and its row of the storage (page * page_rows + row): int64 [rows] each; -1 of rows left out."""
-        self._done(self._lib.itak_paged_batch_rows_device(self._h, positions_ptr or None, slots_ptr or None))
+        status = hip_compute._front.batch_rows(self._hv, positions_ptr, slots_ptr)
+        self._done(status if status >= 0 else self._lib.itak_paged_batch_rows_device(self._h, positions_ptr or None, slots_ptr or None))
 
     def accept_device(self, tokens_ptr: int, chosen_ptr: int, path_ptr: int, next_ptr: int) -> None:
         """The walk down every tree along the tokens chosen: `path` [rows] its row numbers and then -1, `next` [sequences] the choice at its
         end (int32 all)."""
-        self._done(self._lib.itak_paged_accept_device(self._h, tokens_ptr or None, chosen_ptr or None, path_ptr or None, next_ptr or None))
+        status = hip_compute._front.accept(self._hv, tokens_ptr, chosen_ptr, path_ptr, next_ptr)
+        self._done(status if status >= 0 else self._lib.itak_paged_accept_device(self._h, tokens_ptr or None, chosen_ptr or None,
+                                                                                 path_ptr or None, next_ptr or None))
 
     def keep_device(self, path_ptr: int, lengths_ptr: int = 0) -> None:
         """The rows of every path to the sequence's next positions, on all layers; `lengths` [sequences] the positions held then."""
-        self._done(self._lib.itak_paged_keep_device(self._h, path_ptr or None, lengths_ptr or None))
+        status = hip_compute._front.keep(self._hv, path_ptr, lengths_ptr)
+        self._done(status if status >= 0 else self._lib.itak_paged_keep_device(self._h, path_ptr or None, lengths_ptr or None))
 
     def append_device(self, layer: int, k: Rows, v: Rows, rotation: Optional[Rotation] = None) -> None:
         """The batch's new rows into their pages, keys turned by their positions if `rotation` is given."""

@@ -267,6 +267,62 @@ def test_kept_rows(pages, d, kv_heads, page_rows):
     assert torch.equal(cache.storage[:, cache.tables[0]].cpu(), want[:, cache.tables[0]])
 
 
+@pytest.mark.parametrize("sequences", [64, 65, 200])
+def test_walks_and_rows_of_many_sequences(sequences):
+    rng = np.random.RandomState(sequences)
+    new, held = rng.randint(0, 9, sequences).tolist(), rng.randint(0, 40, sequences).tolist()
+    new[0], new[-1] = 8, 8
+    items, parents = list(zip(held, new)), [TC.tree(r, i, 6) if r else [] for i, r in enumerate(new)]
+    cache = PC.Cache(pkg(), [p + r + 1 for p, r in items], layers=2, kv_heads=1, d=8, page_rows=16, max_sequences=sequences, seed=1)
+    cache.paged.enable_trees(sum(new))
+    cache.paged.set_batch(items, cache.tables, TC.flat(parents))
+    tokens, chosen = (rng.randint(0, 2, sum(new)).astype(np.int32) for _ in range(2))
+    path, following, lengths = i32([9] * sum(new)), i32([9] * sequences), i32([9] * sequences)
+    t, c = torch.from_numpy(tokens).cuda(), torch.from_numpy(chosen).cuda()
+    want_path, want_next, want_length, want, first = [], [], [], cache.host.clone(), 0
+    for (p, r), mine, table in zip(items, parents, cache.tables):
+        if r:
+            walk, end = TC.walk(mine, tokens[first:first + r], chosen[first:first + r])
+            for to, one in enumerate(walk):
+                want[:, table[(p + to) // 16], :, :, (p + to) % 16] = cache.host[:, table[(p + one) // 16], :, :, (p + one) % 16]
+            want_path += walk + [-1] * (r - len(walk))
+        want_next.append(int(end) if r else 9)
+        want_length.append(p + len(walk) if r else 9)
+        first += r
+    cache.paged.accept_device(t.data_ptr(), c.data_ptr(), path.data_ptr(), following.data_ptr())
+    cache.paged.keep_device(path.data_ptr(), lengths.data_ptr())
+    torch.cuda.synchronize()
+    assert path.tolist() == want_path and following.tolist() == want_next and lengths.tolist() == want_length
+    assert torch.equal(cache.storage.cpu(), want)
+
+
+def test_both_ways_make_the_same_call(monkeypatch):
+    # Plain arguments go through the compiled front module, every other kind through ctypes.
+    P, got = pkg(), []
+    for way in ("front", "ctypes", "arrays"):
+        with monkeypatch.context() as m:
+            if way == "ctypes":
+                m.setattr(P.hip_compute, "_front", P._native.NoFront)
+            cast = (lambda x: np.asarray(x, np.uint32)) if way == "arrays" else list
+            paged, tables = small(max_sequences=3), Tables(3, 8, 64, 2)
+            paged.enable_trees(20)
+            held, status = i32([5, 30, 0]), i32([7] * 3)
+            parents, chosen = i32([-1, 0, 0, 1, -1, 0, -1]), i32([4, 9, 4, 9, 2, 2, 1])
+            tokens, path, following = i32([1, 3, 4, 9, 5, 2, 0]), i32([7] * 7), i32([7] * 3)
+            places = torch.zeros(2, 7, dtype=torch.int64, device="cuda")
+            paged.fit_tables_device(tables.raw, held.data_ptr(), cast([4, 2, 1]), status.data_ptr())
+            paged.set_batch_device(tables.raw, held.data_ptr(), cast([4, 2, 1]), 30, parents.data_ptr(), status.data_ptr())
+            assert paged._rows == 7
+            paged.batch_rows_device(places[0].data_ptr(), places[1].data_ptr())
+            paged.accept_device(tokens.data_ptr(), chosen.data_ptr(), path.data_ptr(), following.data_ptr())
+            paged.keep_device(path.data_ptr(), held.data_ptr())
+            paged.fit_tables_device(tables.raw, held.data_ptr())
+            torch.cuda.synchronize()
+            got.append([t.tolist() for t in (places, path, following, held, status, *tables.dev)])
+    assert got[0] == got[1] == got[2]
+    assert got[0][0][0] == [5, 6, 6, 7, 30, 31, 0] and got[0][1] == [0, 2, -1, -1, 0, 1, 0] and got[0][2] == [4, 2, 1] and got[0][3] == [7, 32, 1]
+
+
 class Model:
     """What stands around the cache in a round: fixed projections of a token, and what it would choose behind a row of attention outputs."""
 
