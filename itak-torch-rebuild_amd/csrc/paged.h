@@ -82,6 +82,7 @@ struct PagedAttn {
     uint32_t window;
     uint32_t parts;      // kernel of many rows: workgroups a unit is dealt to; 0: the line above
     uint32_t apart;      // kernel of trees: no workgroup has parts of two units (paged_cut_apart), and a unit is a tile of all heads
+    uint32_t across;     // and a head's workgroups
     const void *zeros;   // 16 bytes of them
     uint32_t inline_items; // 0: the batch's are read from device memory
     uint32_t total;      // where the host knows the batch: the line's length, and its cut (else a share of 0)
@@ -193,6 +194,15 @@ __device__ __forceinline__ uint32_t paged_row_of(const PagedAttn &a, uint32_t ve
 
 // Whether the rows of the batch at hand have records. (Of a captured launch the batch may be another than it was captured over.)
 __device__ __forceinline__ bool paged_has_trees(const PagedAttn &a) { return a.inline_items || a.batch[2]; }
+
+// The part and the head of a workgroup of the kernel of trees. Workgroup w runs on compute die w mod 8: a die takes a run of the parts in their order,
+// head by head, so that the tiles that read the same keys share its cache, and short last parts do not meet on one die: 8 trees of 256 rows over 16,384
+// 487 us, and 524 side by side over the dies; 100 rows over 20,000 59 and 62; 4 of 61 rows in a window of 2,048 33 and 31 (the one that loses).
+__device__ __forceinline__ void paged_part_of(const PagedAttn &a, uint32_t &part, uint32_t &head) {
+    const uint32_t w = blockIdx.x + a.across * blockIdx.y, all = a.across * a.g.kv_heads, die = w & 7;
+    const uint32_t at = die * (all >> 3) + min(die, all & 7) + (w >> 3);
+    head = at / a.across, part = at - head * a.across;
+}
 
 // Asks for all of the arguments at once: the compiler asks where it needs them, a trip to memory for every 64 bytes that come
 // first there (of the few rows' kernel four in a row, some 3,000 clocks before the first page id).

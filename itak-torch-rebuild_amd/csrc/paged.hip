@@ -174,7 +174,7 @@ struct TreesCut {
     bool chunk;  // the kernel of many rows
     uint32_t tile, share;
 };
-TreesCut trees_plan(const PagedBatch &batch, const PagedAttn &a, uint32_t waves, uint32_t chunk_waves, uint32_t dp, uint32_t cus) {
+TreesCut trees_plan(const PagedBatch &batch, const PagedAttn &a, uint32_t waves, uint32_t chunk_waves, bool f32, uint32_t dp, uint32_t cus) {
     struct Run {
         uint32_t vectors, blocks;
     };
@@ -192,8 +192,9 @@ TreesCut trees_plan(const PagedBatch &batch, const PagedAttn &a, uint32_t waves,
     double lowest = 1e300;
     auto look = [&](bool chunk, uint32_t sets, uint32_t groups) {
         const uint32_t tile = 32 * sets;
-        // Clocks of a step, of 128 channels: chunks' wavefronts work at their products and their softmax at once.
-        const double step = (chunk ? 1900.0 : 2450.0) * (waves == 8 || chunk ? 1.0 : 0.6) * dp / 128;
+        // Clocks of a step, of 128 channels: chunks' wavefronts work at their products and their softmax at once, and tensors of f32 are several products
+        // each (of chunks, whose tiles are half as large then, about as much in all).
+        const double step = (chunk ? 1900.0 : 2450.0 * (f32 ? 2.2 : 1.0) * (waves == 8 ? 1.0 : 0.6)) * dp / 128;
         for (uint32_t share = longest;;) {
             uint64_t parts = 0, work = 0;
             for (const Run &r : runs) {
@@ -268,6 +269,8 @@ itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work, bool &whole
         } else {
             a.share = 0;
         }
+        // (Workgroups that would find nothing are left out where the batch is known.)
+        a.across = known ? a.total / share : a.groups;
         return ITAK_OK;
     }
     // (The kernel of many rows has no line.)
@@ -405,7 +408,7 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
         PagedAttn &b = plan.trees = a;
         b.v_from = few_most + 1, b.v_to = ~0u;
         b.apart = 1;
-        const TreesCut cut = trees_plan(p->batch, b, paged_trees_waves(dp, p->cfg.elem, q.elem), chunks ? paged_chunk_waves(dp, q.elem) : 0, dp, cus);
+        const TreesCut cut = trees_plan(p->batch, b, paged_trees_waves(dp, p->cfg.elem, q.elem), chunks ? paged_chunk_waves(dp, q.elem) : 0, q.elem == ITAK_ELEM_F32, dp, cus);
         b.tile = cut.tile, b.share = cut.share;
         plan.trees_as_many = cut.chunk;
         b.tile_shift = shift_of(b.tile);

@@ -71,13 +71,14 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     const uint32_t part = TREE ? 0 : blockIdx.x / units, unit = blockIdx.x - part * units;
     PagedLine line(a);
     PagedSpan span;
-    uint32_t from = 0, head, turn;
+    uint32_t nth = 0, from = 0, head, turn;
     if constexpr (TREE) {
         paged_fetch_arguments(a);
         line.cut();
-        const uint32_t at = blockIdx.x * line.share;
+        paged_part_of(a, nth, head);
+        const uint32_t at = nth * line.share;
         if (at >= line.total || !line.find<PagedLine::kBlock>(span, at)) return;
-        turn = span.tiles == 1 ? 0 : (at - span.start) / span.run, from = (at - span.start) - turn * span.run, head = blockIdx.y;
+        turn = span.tiles == 1 ? 0 : (at - span.start) / span.run, from = (at - span.start) - turn * span.run;
     } else {
         if (!line.find<PagedLine::kUnit>(span, unit)) return;
         const uint32_t local = unit - span.unit0;
@@ -98,7 +99,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
         whole = span.blocks <= line.share;
         kb0 = max(span.first + from, tile_lo / 32);
         kb_end = max(kb0, min(span.first + min(from + line.share, span.blocks), (tile_hi + 31) / 32));
-        slot0 = uint64_t(head * a.groups + blockIdx.x) * kTile;
+        slot0 = uint64_t(head * a.groups + nth) * kTile;
     } else {
         whole = a.parts == 1;
         const uint32_t b_first = tile_lo / 32, b_all = (tile_hi + 31) / 32 - b_first, b_part = (b_all + a.parts - 1) / a.parts;
@@ -507,8 +508,7 @@ hipError_t launch_chunk_kernel(const PagedAttn &a, hipStream_t stream) {
         return hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(chunk_lds(DP)));
     });
     if (granted != hipSuccess) return granted;
-    // (Workgroups that would find nothing are left out where the batch is known.)
-    const dim3 grid = a.apart ? dim3(a.share ? a.total / a.share : a.groups, a.g.kv_heads) : dim3(a.units * a.parts);
+    const dim3 grid = a.apart ? dim3(a.across, a.g.kv_heads) : dim3(a.units * a.parts);
     launch_kernel(Kernel, grid, paged_chunk_waves(DP, ELEM) * 64, chunk_lds(DP), stream, a);
     return hipGetLastError();
 }

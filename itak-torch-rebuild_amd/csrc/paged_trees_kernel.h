@@ -54,11 +54,13 @@ __global__ __launch_bounds__(paged_trees_waves(DP, PAGE, ELEM) * 64) void paged_
     const uint32_t d = EXACT ? DP : a.g.head_dim;
     PagedLine line(a);
     line.cut();
-    const uint32_t at = blockIdx.x * line.share;
+    uint32_t nth, head;
+    paged_part_of(a, nth, head);
+    const uint32_t at = nth * line.share;
     PagedSpan span;
     if (at >= line.total || !line.find<PagedLine::kBlock>(span, at)) return;
     const bool trees = paged_has_trees(a);
-    const uint32_t turn = span.tiles == 1 ? 0 : (at - span.start) / span.run, from = (at - span.start) - turn * span.run, head = blockIdx.y;
+    const uint32_t turn = span.tiles == 1 ? 0 : (at - span.start) / span.run, from = (at - span.start) - turn * span.run;
     const uint32_t tile = span.tiles - 1 - turn;  // (the longest first, of a chain)
     const bool whole = span.blocks <= line.share;
     const uint32_t vectors = span.rows * a.group, v0 = tile << a.tile_shift, v_end = min(v0 + a.tile, vectors);
@@ -355,7 +357,7 @@ __global__ __launch_bounds__(paged_trees_waves(DP, PAGE, ELEM) * 64) void paged_
         return make_float2(m, l);
     };
     // A part's place: its workgroup's (a head's side by side); of a vector's channels as the registers of its column hold them.
-    const uint64_t slot0 = uint64_t(head * a.groups + blockIdx.x) * a.tile;
+    const uint64_t slot0 = uint64_t(head * a.groups + nth) * a.tile;
     float *const part = a.ws_acc + slot0 * DP;
     float2 *const part_ml = a.ws_ml + slot0;
     // Whether the part is to be done over.
@@ -471,9 +473,7 @@ hipError_t launch_trees_as(const PagedAttn &a, hipStream_t stream) {
         return hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(trees_lds(DP, kWaves)));
     });
     if (granted != hipSuccess) return granted;
-    // (Workgroups that would find nothing are left out where the batch is known.)
-    const uint32_t groups = a.share ? a.total / a.share : a.groups;
-    launch_kernel(kernel, dim3(groups, a.g.kv_heads), kWaves * 64, trees_lds(DP, kWaves), stream, a);
+    launch_kernel(kernel, dim3(a.across, a.g.kv_heads), kWaves * 64, trees_lds(DP, kWaves), stream, a);
     return hipGetLastError();
 }
 template <int PAGE, int ELEM, int NQ, int NP>
