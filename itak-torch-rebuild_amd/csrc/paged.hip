@@ -170,10 +170,7 @@ uint32_t shift_of(uint32_t power) { return uint32_t(__builtin_ctz(power)); }
 // How a batch whose rows may be trees is cut: by which kernel, the vectors of a tile, and the blocks of a workgroup's part. The cost of a choice is
 // worked out in clocks: of a workgroup what it takes before its first products and behind its last, its steps, or its blocks on their way from L2
 // where that is more, and its partial's way out; of the launch its rounds and, where units are split, the join and the partials' way there and back.
-struct TreesCut {
-    bool chunk;  // the kernel of many rows
-    uint32_t tile, share;
-};
+using TreesCut = PagedBatch::Cut;
 TreesCut trees_plan(const PagedBatch &batch, const PagedAttn &a, uint32_t waves, uint32_t chunk_waves, bool f32, uint32_t dp, uint32_t cus) {
     struct Run {
         uint32_t vectors, blocks;
@@ -188,7 +185,7 @@ TreesCut trees_plan(const PagedBatch &batch, const PagedAttn &a, uint32_t waves,
         runs.push_back({uint32_t(vectors), blocks});
         longest = std::max(longest, blocks), widest = std::max(widest, uint32_t(vectors));
     }
-    TreesCut best{chunk_waves != 0, 32 * (chunk_waves ? chunk_waves : waves), longest};
+    TreesCut best{0, chunk_waves != 0, 32 * (chunk_waves ? chunk_waves : waves), longest};
     double lowest = 1e300;
     auto look = [&](bool chunk, uint32_t sets, uint32_t groups) {
         const uint32_t tile = 32 * sets;
@@ -210,15 +207,15 @@ TreesCut trees_plan(const PagedBatch &batch, const PagedAttn &a, uint32_t waves,
             const double alone = time(share) + beside + partial;
             const double among = double(parts) / cus * (time(double(work) / parts) + beside + partial) + time(share) / 2;
             const double cost = (parts <= cus ? alone : std::max(alone, among)) + (split ? 8000.0 + parts * tile * dp / 500.0 : 0.0);
-            if (cost < lowest) lowest = cost, best = {chunk, tile, share};
+            if (cost < lowest) lowest = cost, best = {0, chunk, tile, share};
             if (share <= 2 || parts > 2 * cus) break;
             // (Shares that are whole steps of the groups.)
             share = std::max<uint32_t>(2, std::min((share - 1) / groups * groups, share * 7 / 8 / groups * groups));
         }
     };
-    // (Eight groups of one set have at least a pair of register quads each to finish.)
-    for (uint32_t sets = dp < 128 ? 2 : 1; sets <= waves; sets *= 2) {
-        if (16 * sets >= widest && sets > (dp < 128 ? 2u : 1u)) break;
+    // (Tiles of one set, each read by itself, were behind those of two: 4 of 16 rows by 4 heads at 1,000 18.4 us and 16.2.)
+    for (uint32_t sets = 2; sets <= waves; sets *= 2) {
+        if (16 * sets >= widest && sets > 2) break;
         look(false, sets, waves / sets);
     }
     if (chunk_waves) look(true, chunk_waves, 1);
@@ -408,7 +405,14 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
         PagedAttn &b = plan.trees = a;
         b.v_from = few_most + 1, b.v_to = ~0u;
         b.apart = 1;
-        const TreesCut cut = trees_plan(p->batch, b, paged_trees_waves(dp, p->cfg.elem, q.elem), chunks ? paged_chunk_waves(dp, q.elem) : 0, q.elem == ITAK_ELEM_F32, dp, cus);
+        // (Once a batch: a layer after another asks the same, and over 256 items the answer takes some tens of microseconds.)
+        TreesCut &cut = p->batch.cuts[a.window ? 1 : 0];
+        const uint64_t key = (uint64_t(q.heads) * 2 + (q.elem == ITAK_ELEM_F32)) << 32 | (a.window ? a.window : 1);
+        if (cut.key != key) {
+            cut = trees_plan(p->batch, b, paged_trees_waves(dp, p->cfg.elem, q.elem), chunks ? paged_chunk_waves(dp, q.elem) : 0,
+                             q.elem == ITAK_ELEM_F32, dp, cus);
+            cut.key = key;
+        }
         b.tile = cut.tile, b.share = cut.share;
         plan.trees_as_many = cut.chunk;
         b.tile_shift = shift_of(b.tile);
@@ -565,6 +569,7 @@ itak_status set_batch(itak_paged *p, const itak_paged_item *items, uint32_t coun
     const PagedRefusal r = make_paged_batch(p->limits, items, count, pages, page_ids, p->marks, p->stamp, next, p->tree_dev != nullptr);
     if (r.code != ITAK_OK) return set_error(p->err, r.code, r.what, r.a, r.b, 0, 0, "%s", r.text.c_str());
     next.trees = parents != nullptr, next.on_device = false, next.tree_most = 0, next.sized[0] = next.sized[1] = 0;
+    next.cuts[0] = next.cuts[1] = {};
     if (parents) {
         const itak_status st = check_trees(p, items, count, parents, next.rows, next.tree_most);
         if (st != ITAK_OK) return st;

@@ -183,6 +183,8 @@ namespace {
 
 itak_status check_kept(itak_paged *p) {
     if (!p->tree_dev) return unsupported(p->err, "a paged cache that takes no trees (itak_paged_enable_trees)");
+    // (Without the sequences that have no rows an item's number is not its sequence's.)
+    if (p->batch.rows && !p->batch.idle_kept) return invalid_argument(p->err, "the batch was set before the paged cache took trees");
     return ITAK_OK;
 }
 

@@ -41,6 +41,13 @@ struct PagedBatch {
     bool trees = false;          // its rows have records
     uint32_t tree_most = 0;      // rows of its largest tree
     uint64_t sized[2] = {};      // what attention over it, without a window and with one, has been given a captured call's memory for
+    // How attention's launch for trees is cut over it, without a window and with one; `key`: what that was found for.
+    struct Cut {
+        uint64_t key = 0;
+        bool chunk = false;      // by the kernel of many rows
+        uint32_t tile = 0, share = 0;
+    } cuts[2];
+    bool idle_kept = false;      // an item's number is its sequence's
     bool on_device = false;      // lengths and tables are the device's: positions in `head` are the most they may be, and there are no ids
 };
 
@@ -110,6 +117,7 @@ inline PagedRefusal make_paged_batch(const PagedLimits &lim, const itak_paged_it
     }
     batch.items = batch.rows = batch.most_rows = 0;
     batch.head.assign(kPagedItem0, 0);
+    batch.idle_kept = keep_idle;
     batch.ids.assign(pages, pages + page_ids);
     uint32_t id = paged_ids_at(lim.max_sequences);
     for (uint32_t i = 0; i < count; id += items[i].pages, ++i) {

@@ -6,7 +6,7 @@
 //
 // A workgroup has one part of one tile (the cut is such that all parts are about of one length). Each of its wavefronts has a set of 32 of the
 // tile's vectors and, as one of `groups` that have the same set, every groups-th block of 32 keys: two wavefronts a SIMD, which fill each other's gaps,
-// whether the tile is one set or eight. The loop is one block long: the products of the scores, the softmax, those of the values. Blocks
+// whether the tile is two sets or eight. The loop is one block long: the products of the scores, the softmax, those of the values. Blocks
 // travel from the pages to LDS without passing through registers, into a ring that is full at the start; layout and operands are those of the
 // kernel of many rows (paged_chunk_kernel.h), whose loop is longer and faster: it takes batches of tiles of 256 vectors. At the end the groups meet in LDS.
 //
@@ -449,10 +449,8 @@ __global__ __launch_bounds__(paged_trees_waves(DP, PAGE, ELEM) * 64) void paged_
         over = finish(std::integral_constant<int, 0>{});
     else if (groups == 2)
         over = finish(std::integral_constant<int, 1>{});
-    else if (groups == 4)
+    else if constexpr (kWaves == 8)
         over = finish(std::integral_constant<int, 2>{});
-    else if constexpr (kQuads >= 16 && kWaves == 8)
-        over = finish(std::integral_constant<int, 3>{});
     if (!over) return;
     paged_careful<PAGE, ELEM, DP, true>(a, span, head, v0, v_end, wave, kWaves, 32 * kb0, 32 * max(kb0, kb_end),
                                         [&](uint32_t u, const float (&sums)[DP / 64], float most, float s) {

@@ -139,13 +139,14 @@ class PageTables:
     """Page tables on the device (itak_page_tables), the caller's memory: of each sequence up to `stride` page ids and how many, and the
     free list."""
 
-    __slots__ = ("raw", "ref", "at", "sequences", "keep")
+    __slots__ = ("raw", "ref", "at", "sequences", "free_words", "keep")
 
     def __init__(self, table_ptr: int, stride: int, pages_ptr: int, sequences: int, free_ptr: int = 0, free_count_ptr: int = 0, keep=None):
         self.raw = _filled(N.PageTables, table_ptr or None, stride, pages_ptr or None, free_ptr or None, free_count_ptr or None, sequences, 0)
         self.ref = C.byref(self.raw)
         self.at = C.addressof(self.raw)  # as the front module takes it
         self.sequences = sequences
+        self.free_words = None  # of the free list, where that is known
         self.keep = keep  # what owns the memory
 
     @staticmethod
@@ -154,10 +155,16 @@ class PageTables:
         for name, t, dims in (("table", table, 2), ("pages", pages, 1), ("free", free, 1), ("free_count", free_count, 1)):
             if t is not None and not (t.is_cuda and str(t.dtype) == "torch.int32" and t.dim() == dims and t.is_contiguous()):
                 raise ValueError(f"PageTables.of: {name} is no dense int32 tensor of {dims} dimensions on a GPU")
+            if t is not None and t.device != table.device:
+                raise ValueError(f"PageTables.of: {name} is on another device than table")
         if pages.shape[0] != table.shape[0]:
             raise ValueError(f"PageTables.of: pages of {pages.shape[0]} sequences, tables of {table.shape[0]}")
-        return PageTables(table.data_ptr(), table.shape[1], pages.data_ptr(), table.shape[0], 0 if free is None else free.data_ptr(),
-                          0 if free_count is None else free_count.data_ptr(), (table, pages, free, free_count))
+        if free_count is not None and free_count.shape[0] != 1:
+            raise ValueError(f"PageTables.of: free_count of {free_count.shape[0]} words")
+        tables = PageTables(table.data_ptr(), table.shape[1], pages.data_ptr(), table.shape[0], 0 if free is None else free.data_ptr(),
+                            0 if free_count is None else free_count.data_ptr(), (table, pages, free, free_count))
+        tables.free_words = None if free is None else free.shape[0]
+        return tables
 
 
 def _words(values, kind: str, low: int, high: int, what: str):
@@ -195,6 +202,7 @@ class PagedKv:
             _raise_last(None)
         self._h, self._hv = handle, handle.value
         self.page_rows = page_rows
+        self.page_count = page_count
         self.head_dim = head_dim
         self._rows = 0  # of the batch
 
@@ -286,6 +294,8 @@ class PagedKv:
 
     def fit_tables_device(self, tables: PageTables, lengths_ptr: int, rows: Optional[Sequence[int]] = None, status_ptr: int = 0) -> None:
         """Page tables to lengths on the device (int32 [sequences]), and `rows` new rows on top of each: pages from the free list, or back."""
+        if tables.free_words is not None and tables.free_words < self.page_count:
+            raise ValueError(f"a free list of {tables.free_words} words for {self.page_count} pages")
         status = hip_compute._front.fit_tables(self._hv, tables.at, tables.sequences, lengths_ptr, rows, status_ptr)
         if status >= 0:
             self._done(status)
