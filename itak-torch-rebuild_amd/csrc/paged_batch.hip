@@ -4,6 +4,7 @@
 // All of it is a few words a sequence and a row; what it costs are launches and, inside one, the trips to memory that wait for one another.
 // A workgroup serves a sequence and finds out for itself what stands before it (a sum over up to 1,024 lengths),
 // so that a batch is one launch; the free list is one workgroup's, which every sequence's place in it has to pass through.
+#include "mfma_common.h"
 #include "paged_handle.h"
 
 #include <algorithm>
@@ -39,28 +40,64 @@ constexpr uint32_t kNoChain = 1, kNoTree = 2;
 __device__ __forceinline__ uint32_t parent_is_not(int32_t parent, uint32_t r) {
     return (parent != int32_t(r) - 1 ? kNoChain : 0) | (parent < -1 || parent >= int32_t(r) ? kNoTree : 0);
 }
-// An item's records from its parents, the threads' rows' in `up` (LDS) where it is a tree; `not_`: what any of them is not, no kNoTree.
+// An item's records from its parents, the threads' rows' in `up` (LDS) where it is a tree; `not_`: what any of them is not, no kNoTree. What a row sees
+// is doubled: its nearest 2^k rows upwards and as many of the row behind them are its nearest 2^(k+1). (The whole launch over 255 rows in one line and one
+// beside took 28.2 us upwards row by row, and 6.2; over 32 5.6 and 2.4; over 256 rows of at most 20 levels 3.2 and 4.6, the one that loses.)
 __device__ __forceinline__ void make_records(uint32_t *tree, uint32_t rows, uint32_t position, uint32_t not_, const int32_t *up) {
+    __shared__ int32_t lds_at[kTreeRows];
+    __shared__ u32x4 lds_sees[2][kTreeRows];
     const uint32_t tid = threadIdx.x;
     if (!not_) {
         for (uint32_t r = tid; r < rows; r += kThreads)
             *reinterpret_cast<uint2 *>(tree + uint64_t(r) * kTreeStride) = make_uint2(kTreeChain | r, r - 1);
-    } else if (tid < rows) {
-        // Upwards from the row: every step goes to a lower row, so there are at most as many steps as rows.
-        const uint32_t held = position % 32;
-        uint32_t word[kTreeStride] = {}, depth = 0;
-        word[kTreeParent] = uint32_t(up[tid]);
-        word[kTreeSees] = (1u << held) - 1;
-        for (int32_t at = int32_t(tid); at >= 0; at = up[at], ++depth) {
-            const uint32_t bit = held + uint32_t(at);
-#pragma unroll
-            for (uint32_t w = 0; w < kTreeBlocks; ++w) word[kTreeSees + w] |= bit / 32 == w ? 1u << bit % 32 : 0u;
-        }
-        word[kTreeDepth] = depth - 1;
-#pragma unroll
-        for (uint32_t w = 0; w < kTreeStride; w += 4)
-            *reinterpret_cast<uint4 *>(tree + uint64_t(tid) * kTreeStride + w) = make_uint4(word[w], word[w + 1], word[w + 2], word[w + 3]);
+        return;
     }
+    constexpr uint32_t kWords = kTreeRows / 32;
+    uint32_t sees[kWords];
+    const int32_t parent = tid < rows ? up[tid] : -1;
+    int32_t at = parent;
+    if (rows <= 64) {
+        // (One wavefront, in its registers.)
+        if (tid >= 64) return;
+        uint64_t mine = 1ull << tid;
+        while (__builtin_amdgcn_ballot_w64(at >= 0) != 0) {
+            const int32_t from = max(at, 0);
+            const uint64_t theirs = __shfl(mine, from);
+            const int32_t next = __shfl(at, from);
+            if (at >= 0) mine |= theirs, at = next;
+        }
+#pragma unroll
+        for (uint32_t w = 0; w < kWords; ++w) sees[w] = w < 2 ? uint32_t(mine >> (32 * w)) : 0;
+    } else {
+#pragma unroll
+        for (uint32_t w = 0; w < kWords; ++w) sees[w] = tid / 32 == w ? 1u << tid % 32 : 0;
+        // (Behind each of the two barriers everybody has read, or written.)
+        while (__syncthreads_or(at >= 0)) {
+            lds_at[tid] = at;
+#pragma unroll
+            for (uint32_t x = 0; x < 2; ++x) lds_sees[x][tid] = u32x4{sees[4 * x], sees[4 * x + 1], sees[4 * x + 2], sees[4 * x + 3]};
+            __syncthreads();
+            if (at < 0) continue;
+#pragma unroll
+            for (uint32_t w = 0; w < kWords; ++w) sees[w] |= lds_sees[w / 4][at][w % 4];
+            at = lds_at[at];
+        }
+    }
+    if (tid >= rows) return;
+    const uint32_t held = position % 32;
+    uint32_t word[kTreeStride] = {}, seen = 0;
+    word[kTreeParent] = uint32_t(parent);
+#pragma unroll
+    for (uint32_t w = 0; w < kTreeBlocks; ++w) {
+        // (Row r is bit held + r.)
+        const uint64_t pair = uint64_t(w < kWords ? sees[w] : 0) << 32 | (w ? sees[w - 1] : 0);
+        word[kTreeSees + w] = uint32_t(pair >> (32 - held)) | (w ? 0 : (1u << held) - 1);
+        seen += w < kWords ? __builtin_popcount(sees[w]) : 0;
+    }
+    word[kTreeDepth] = seen - 1;
+#pragma unroll
+    for (uint32_t w = 0; w < kTreeStride; w += 4)
+        *reinterpret_cast<uint4 *>(tree + uint64_t(tid) * kTreeStride + w) = make_uint4(word[w], word[w + 1], word[w + 2], word[w + 3]);
 }
 
 // A batch of trees on its way to the device: its words as those of paged.hip travel, and the parents behind them. A workgroup makes an item's
@@ -83,8 +120,8 @@ __global__ __launch_bounds__(kThreads) void paged_tree_words_kernel(TreeWords<N>
     const uint32_t *const item = w + kPagedItem0 + 4 * blockIdx.x;
     if (blockIdx.x == 0)
         for (uint32_t i = tid; i < a.n0 + a.n1; i += kThreads) a.batch[i < a.n0 ? i : a.at1 + (i - a.n0)] = w[i];
-    if (kPagedItem0 + 4 * blockIdx.x >= a.n0) return;  // (a batch without items)
     const uint32_t position = item[0], rows = item[1], row0 = item[2];
+    if (kPagedItem0 + 4 * blockIdx.x >= a.n0) return;  // (a batch without items)
     const int32_t *const parents = reinterpret_cast<const int32_t *>(w) + a.n0 + a.n1 + row0;
     uint32_t not_ = 0;
     for (uint32_t r = tid; r < rows; r += kThreads) {
