@@ -161,6 +161,14 @@ __device__ __forceinline__ void paged_write_careful(const PagedAttn &a, const Pa
     if (!whole && has_slot && lane == 0) a.ws_ml[slot] = make_float2(m, kCarefulScale<PAGE> == 1.0f ? l : -l);
 }
 
+// Four channels' sums of a part, written through to the memory where the join's compute dies read them: left in this die's cache, all of them would go out
+// when the launch ends (17 MB, 64 rows of a window of 2,048: 27.2 us a launch and 29.2; past the last-level cache as well, as what is not read
+// again, the launch took as long and the join 6.4 us and 5.8).
+__device__ __forceinline__ void store_part(floatx4 *parts, uint32_t at, floatx4 x) {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(parts, 0, -1, 0x00027000);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), rsrc, at * 16, 0, 16);
+}
+
 // The same into a part for the join: the tile's accumulators as the kernels' registers hold them, sets of 32 vectors, 16 bytes of four channels
 // of a vector; `of`: the vector of the tile.
 template <int PAGE, int DP>

@@ -463,7 +463,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
                                           else
                                               paged_write_careful<PAGE, ELEM, DP>(a, span, head, v, whole, slot0 + v - v0, true, acc, m, l);
                                       });
-    } else if (mine || (TREE && !whole)) {
+    } else if (mine || (TREE && !whole && wv0 < vectors)) {
         if (whole) {
             const float inv = 1.0f / l;
             const uint32_t row = paged_row_of(a, v), hq = head * a.group + v - row * a.group;
@@ -488,13 +488,16 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
         } else {
             const uint64_t slot = slot0 + (v - v0);
             // (For the join as the registers hold them, 1 KiB a store; for the merge row by row.)
-            floatx4 *const set_at = reinterpret_cast<floatx4 *>(a.ws_acc + slot0 * DP) + wave * (DP / 8) * 64 + lane;
 #pragma unroll
             for (int t = 0; t < kOut; ++t)
 #pragma unroll
-                for (int r = 0; r < 16; r += 4)
-                    *(TREE ? set_at + (4 * t + r / 4) * 64 : reinterpret_cast<floatx4 *>(a.ws_acc + slot * DP + 32 * t + 2 * r + 4 * h)) =
-                        floatx4{o[t][r], o[t][r + 1], o[t][r + 2], o[t][r + 3]};
+                for (int r = 0; r < 16; r += 4) {
+                    const floatx4 y = {o[t][r], o[t][r + 1], o[t][r + 2], o[t][r + 3]};
+                    if constexpr (TREE)
+                        store_part(reinterpret_cast<floatx4 *>(a.ws_acc + slot0 * DP), (wave * (DP / 8) + 4 * t + r / 4) * 64 + lane, y);
+                    else
+                        *reinterpret_cast<floatx4 *>(a.ws_acc + slot * DP + 32 * t + 2 * r + 4 * h) = y;
+                }
             if (h == 0) a.ws_ml[slot] = make_float2(threshold == -INFINITY ? -INFINITY : ref, l);
         }
     }

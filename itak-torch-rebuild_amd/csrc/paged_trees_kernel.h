@@ -358,7 +358,7 @@ __global__ __launch_bounds__(paged_trees_waves(DP, PAGE, ELEM) * 64) void paged_
     };
     // A part's place: its workgroup's (a head's side by side); of a vector's channels as the registers of its column hold them.
     const uint64_t slot0 = uint64_t(head * a.groups + nth) * a.tile;
-    float *const part = a.ws_acc + slot0 * DP;
+    floatx4 *const part = reinterpret_cast<floatx4 *>(a.ws_acc + slot0 * DP);
     float2 *const part_ml = a.ws_ml + slot0;
     // Whether the part is to be done over.
     auto asked_over = [&](bool bad) __attribute__((always_inline)) {
@@ -392,9 +392,9 @@ __global__ __launch_bounds__(paged_trees_waves(DP, PAGE, ELEM) * 64) void paged_
 #pragma unroll
                 for (int e = 0; e < 4; ++e) check[e] += EXACT || 8 * (group * kMine + u) + 4 * h < d ? acc[u][e] : 0.0f;
             if (asked_over(wv0 + j < v_end && to_be_done_over<PAGE>((check[0] + check[1]) + (check[2] + check[3])))) return true;
-            floatx4 *const to = reinterpret_cast<floatx4 *>(part) + (uint64_t(set) * kQuads + group * kMine) * 64 + lane;
 #pragma unroll
-            for (uint32_t u = 0; u < kMine; ++u) to[u * 64] = acc[u];
+            for (uint32_t u = 0; u < kMine; ++u)
+                if (wv0 < v_end) store_part(part, (set * kQuads + group * kMine + u) * 64 + lane, acc[u]);
             if (group == 0 && h == 0) part_ml[set * 32 + j] = ml;
         } else {
             const uint32_t ch = lane % kOfRow;
