@@ -189,19 +189,20 @@ TreesCut trees_plan(const PagedBatch &batch, const PagedAttn &a, uint32_t waves,
     double lowest = 1e300;
     auto look = [&](bool chunk, uint32_t sets, uint32_t groups) {
         const uint32_t tile = 32 * sets;
-        // Clocks of a step, of 128 channels: chunks' wavefronts work at their products and their softmax at once, and tensors of f32 are several products
-        // each (of chunks, whose tiles are half as large then, about as much in all).
-        const double step = (chunk ? 1900.0 : 2450.0 * (f32 ? 2.2 : 1.0) * (waves == 8 ? 1.0 : 0.6)) * dp / 128;
+        // Clocks of a step, of 128 channels: chunks' wavefronts work at their products and their softmax at once, four groups send twice the loads of two, and
+        // tensors of f32 are several products each (of chunks, whose tiles are half as large then, about as much in all).
+        const double step = (chunk ? 1900.0 : (groups > 2 ? 3300.0 : 2450.0) * (f32 ? 2.2 : 1.0) * (waves == 8 ? 1.0 : 0.6)) * dp / 128;
         for (uint32_t share = longest;;) {
-            uint64_t parts = 0, work = 0;
+            uint64_t parts = 0, work = 0, once = 0;
             for (const Run &r : runs) {
                 const uint64_t tiles = (r.vectors + tile - 1) / tile;
-                parts += tiles * ((r.blocks + share - 1) / share), work += tiles * r.blocks;
+                parts += tiles * ((r.blocks + share - 1) / share), work += tiles * r.blocks, once += r.blocks;
             }
-            parts *= a.g.kv_heads, work *= a.g.kv_heads;
+            parts *= a.g.kv_heads, work *= a.g.kv_heads, once *= a.g.kv_heads;
             if (parts > kPagedTreesGroups && share != longest) break;
             const bool split = share < longest;
-            const double load = std::max(280.0, 900.0 * std::min(1.0, double(parts) / cus)) * dp / 128;
+            // A block's way: of what no other tile reads at 6.2 TB/s among all.
+            const double load = std::max(280.0, 1420.0 * once / work * std::min(1.0, double(parts) / cus)) * dp / 128;
             auto time = [&](double blocks) { return std::max(std::ceil(blocks / groups) * step, blocks * load); };
             const double beside = chunk ? 13000.0 : 11000.0 + (groups > 1 ? 2000.0 : 1000.0), partial = split ? tile * dp / 16.0 : 0.0;
             const double alone = time(share) + beside + partial;
