@@ -82,7 +82,7 @@ struct PagedAttn {
     uint32_t window;
     uint32_t parts;      // kernel of many rows: workgroups a unit is dealt to; 0: the line above
     uint32_t apart;      // kernel of trees: no workgroup has parts of two units (paged_cut_apart), and a unit is a tile of all heads
-    uint32_t across;     // and a head's workgroups
+    uint32_t across;     // and the grid's workgroups of a head
     const void *zeros;   // 16 bytes of them
     uint32_t inline_items; // 0: the batch's are read from device memory
     uint32_t total;      // where the host knows the batch: the line's length, and its cut (else a share of 0)
@@ -178,10 +178,11 @@ __host__ __device__ inline PagedCut paged_cut(uint32_t total, uint32_t units, ui
     const uint32_t left = groups - units, apart = (total + left - 1) / left, own = apart > least ? apart : least;
     return own <= share + kPagedPart ? PagedCut{own, own} : PagedCut{share, 0};
 }
-// The cut of the kernel of trees, whose workgroups have one part of one unit each: at most `groups` of them, which are at least the units.
+// The cut of the kernel of trees, whose workgroups have one part of one unit each: at most `groups` of them, which are at least the units; shares are
+// multiples of `least`, or units are whole.
 __host__ __device__ inline PagedCut paged_cut_apart(uint32_t total, uint32_t units, uint32_t longest, uint32_t groups, uint32_t least) {
     const uint32_t left = groups > units ? groups - units : 0, even = left ? (total + left - 1) / left : longest;
-    const uint32_t share = even > least ? even : least;
+    const uint32_t share = even > least ? (even + least - 1) / least * least : least;
     return share < longest ? PagedCut{share, share} : PagedCut{longest, longest};
 }
 __host__ __device__ inline uint32_t paged_run(uint32_t blocks, uint32_t pad) { return pad ? (blocks + pad - 1) / pad * pad : blocks; }
@@ -194,15 +195,6 @@ __device__ __forceinline__ uint32_t paged_row_of(const PagedAttn &a, uint32_t ve
 
 // Whether the rows of the batch at hand have records. (Of a captured launch the batch may be another than it was captured over.)
 __device__ __forceinline__ bool paged_has_trees(const PagedAttn &a) { return a.inline_items || a.batch[2]; }
-
-// The part and the head of a workgroup of the kernel of trees. Workgroup w runs on compute die w mod 8: a die takes a run of the parts in their order,
-// head by head, so that the tiles that read the same keys share its cache, and short last parts do not meet on one die: 8 trees of 256 rows over 16,384
-// 487 us, and 524 side by side over the dies; 100 rows over 20,000 59 and 62; 4 of 61 rows in a window of 2,048 33 and 31 (the one that loses).
-__device__ __forceinline__ void paged_part_of(const PagedAttn &a, uint32_t &part, uint32_t &head) {
-    const uint32_t w = blockIdx.x + a.across * blockIdx.y, all = a.across * a.g.kv_heads, die = w & 7;
-    const uint32_t at = die * (all >> 3) + min(die, all & 7) + (w >> 3);
-    head = at / a.across, part = at - head * a.across;
-}
 
 // Asks for all of the arguments at once: the compiler asks where it needs them, a trip to memory for every 64 bytes that come
 // first there (of the few rows' kernel four in a row, some 3,000 clocks before the first page id).
@@ -218,6 +210,7 @@ __device__ __forceinline__ void paged_fetch_arguments(const PagedAttn &a) {
 struct PagedLine {
     const PagedAttn &a;
     uint32_t share = 0, pad = 0, total = 0;
+    uint32_t across = 0;  // of cut_apart
 
     __device__ __forceinline__ explicit PagedLine(const PagedAttn &args) : a(args) {}
     // An item's span, and blocks and units of all of it; none of an item that the launch does not take, and of one beyond the
@@ -278,8 +271,37 @@ struct PagedLine {
             longest = max(longest, s.blocks);
         }
         longest = most_of(longest);
-        const PagedCut c = a.apart ? paged_cut_apart(all, all_units, longest, a.groups, a.least) : paged_cut(all, all_units, longest, a.groups, a.least);
+        const PagedCut c = paged_cut(all, all_units, longest, a.groups, a.least);
         share = c.share, pad = c.pad, total = pad ? share * a.groups : all;  // (of rounded runs: what lies past the last is nobody's)
+    }
+    // The cut of the kernel of trees, and how many workgroups of a head have a part.
+    __device__ __forceinline__ void cut_apart() {
+        if (a.share) {
+            share = a.share, pad = a.pad, total = a.total, across = a.across;
+            return;
+        }
+        const uint32_t n = min(a.batch[0], a.items);
+        uint32_t all = 0, all_units = 0, longest = 0;
+        PagedSpan last{};
+        for (uint32_t at = 0; at < n; at += 64) {
+            uint32_t work, units;
+            last = of_lane(at, n, work, units);
+            all += __builtin_amdgcn_readlane(scan(work), 63);
+            all_units += __builtin_amdgcn_readlane(scan(units), 63);
+            longest = max(longest, last.blocks);
+        }
+        longest = most_of(longest);
+        const PagedCut c = paged_cut_apart(all, all_units, longest, a.groups, a.least);
+        share = c.share, pad = c.pad, total = share * a.groups;
+        if (share == longest) {
+            across = all_units;
+            return;
+        }
+        for (uint32_t at = 0; at < n; at += 64) {
+            uint32_t work, units;
+            if (n > 64) last = of_lane(at, n, work, units);
+            across += __builtin_amdgcn_readlane(scan(last.tiles * ((last.blocks + share - 1) / share)), 63);
+        }
     }
     // The item that block, unit or row x of the line belongs to; none if it is no item's, or of one that the launch does not take.
     enum By { kBlock, kUnit, kRow };
@@ -323,6 +345,18 @@ struct PagedLine {
         return false;
     }
 };
+
+// The part and the head of a workgroup of the kernel of trees. Workgroup w runs on compute die w mod 8: a die takes a run of the parts in their order,
+// head by head, so that the tiles that read the same keys share its cache, and short last parts do not meet on one die: 8 trees of 256 rows over 16,384
+// 487 us, and 524 side by side over the dies; 100 rows over 20,000 59 and 62; 4 of 61 rows in a window of 2,048 33 and 31 (the one that loses).
+// (False: none is left for it. Workgroups without a part come last: on their own dies they would leave the others to share the work.)
+__device__ __forceinline__ bool paged_part_of(const PagedLine &line, uint32_t &part, uint32_t &head) {
+    const uint32_t w = blockIdx.x + line.a.across * blockIdx.y, all = line.across * line.a.g.kv_heads, die = w & 7;
+    const uint32_t at = die * (all >> 3) + min(die, all & 7) + (w >> 3);
+    if (w >= all) return false;
+    head = at / line.across, part = at - head * line.across;
+    return true;
+}
 
 // The batch's item that holds row `row`: its position, first row and table. All lanes ask together.
 __device__ __forceinline__ bool paged_item_of_row(const uint32_t *batch, uint32_t row, uint4 &item) {

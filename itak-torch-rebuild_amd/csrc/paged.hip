@@ -249,8 +249,11 @@ itak_status count_units(itak_paged *p, PagedAttn &a, uint64_t &work, bool &whole
     a.units = uint32_t(units);
     if (a.apart) {
         const uint32_t room = std::max(1u, kPagedTreesGroups / a.g.kv_heads), share = a.share;
-        a.groups = std::max(room, a.units);
-        whole = a.units >= room;
+        // (Where the batch is not known as many workgroups as the cut takes here, and one for every compute unit: for other lengths.)
+        const uint64_t parts = units + (share < longest ? (work + share - 1) / share : 0);
+        const uint64_t asked = known ? room : std::max<uint64_t>(parts, std::max(1u, compute_units()) / a.g.kv_heads);
+        a.groups = std::max(a.units, uint32_t(std::min<uint64_t>(room, asked)));
+        whole = a.groups == a.units;
         if (whole) a.least = ~0u;
         if (known) {
             a.share = a.pad = share;
@@ -417,7 +420,7 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
         b.tile = cut.tile, b.share = cut.share;
         plan.trees_as_many = cut.chunk;
         b.tile_shift = shift_of(b.tile);
-        b.least = 2;
+        b.least = std::max(2u, cut.chunk ? 2u : paged_trees_waves(dp, p->cfg.elem, q.elem) * 32 / cut.tile);  // (a step's blocks)
         const itak_status st = count_units(p, b, work, whole, known);
         if (st != ITAK_OK) return st;
         plan.join_trees = !whole;

@@ -74,8 +74,8 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     uint32_t nth = 0, from = 0, head, turn;
     if constexpr (TREE) {
         paged_fetch_arguments(a);
-        line.cut();
-        paged_part_of(a, nth, head);
+        line.cut_apart();
+        if (!paged_part_of(line, nth, head)) return;
         const uint32_t at = nth * line.share;
         if (at >= line.total || !line.find<PagedLine::kBlock>(span, at)) return;
         turn = span.tiles == 1 ? 0 : (at - span.start) / span.run, from = (at - span.start) - turn * span.run;

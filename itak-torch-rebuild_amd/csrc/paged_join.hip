@@ -27,7 +27,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttn a) {
     const uint32_t joined = SHARED > 1 ? blockIdx.x : blockIdx.x * kWaves + wave, unit = joined >> (a.tile_shift - 2);
     static_assert(kJoined == 4, "a tile is 2^(tile_shift - 2) times that");
     PagedLine line(a);
-    line.cut();
+    line.cut_apart();
     PagedSpan span;
     if (!line.find<PagedLine::kUnit>(span, unit)) return;
     const uint32_t parts = (span.blocks + line.share - 1) / line.share;
@@ -142,7 +142,7 @@ void launch_as(const PagedAttn &a, hipStream_t stream) {
     // The wavefronts of a workgroup share their vectors' parts where those are many and the vectors do not fill the device: 16 sequences' 4,096 wavefronts
     // of up to 8 parts 13.6 us shared and 6.8 each for itself.
     const uint32_t waves = a.units * (a.tile / kJoined);
-    if (a.units * 8 <= a.groups && waves * a.g.kv_heads <= 1024)
+    if (a.units * a.g.kv_heads * 8 <= kPagedTreesGroups && waves * a.g.kv_heads <= 1024)
         launch_kernel(paged_join_kernel<ELEM, DP, 4>, dim3(waves, a.g.kv_heads), kThreads, 0, stream, a);
     else
         launch_kernel(paged_join_kernel<ELEM, DP, 1>, dim3(waves / (kThreads / 64), a.g.kv_heads), kThreads, 0, stream, a);

@@ -53,9 +53,9 @@ __global__ __launch_bounds__(paged_trees_waves(DP, PAGE, ELEM) * 64) void paged_
     const uint32_t h = lane >> 5, j = lane & 31;
     const uint32_t d = EXACT ? DP : a.g.head_dim;
     PagedLine line(a);
-    line.cut();
+    line.cut_apart();
     uint32_t nth, head;
-    paged_part_of(a, nth, head);
+    if (!paged_part_of(line, nth, head)) return;
     const uint32_t at = nth * line.share;
     PagedSpan span;
     if (at >= line.total || !line.find<PagedLine::kBlock>(span, at)) return;

@@ -90,6 +90,44 @@ def test_replays_over_long_chains_beside_trees(tensors, window):
         check_one(cache, items, trees, 2, q, again, kind, window)
 
 
+# More sequences than a wavefront has lanes, in a graph of the batch, its attention and the lengths' own: cut by the device, split and whole, other sequences
+# left out at every replay.
+@pytest.mark.parametrize("kv_heads", [1, 4])
+def test_replays_over_many_sequences(kv_heads):
+    n, nodes, d = 70, 20, 64
+    most = [(37 * s) % 701 for s in range(n)]
+    cache = cache_of([(p, nodes) for p in most], kv_heads=kv_heads, d=d, page_rows=32, max_sequences=n, seed=kv_heads)
+    trees = [TC.tree(nodes, s) for s in range(n)]
+    tables, parents = tables_of(cache), torch.from_numpy(TC.flat(trees)).cuda()
+    q = cache.normal(n * nodes, 4 * kv_heads, d).half()
+    qd, out, held, status = q.cuda(), torch.empty_like(q, device="cuda"), i32(most), i32([9] * n)
+    stream, side, graph = torch.cuda.current_stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+
+    def forward():
+        cache.paged.set_batch_device(tables, held.data_ptr(), [nodes] * n, 700, parents.data_ptr(), status.data_ptr())
+        cache.paged.attention_device(0, view(qd), view(out))
+
+    forward()
+    torch.cuda.synchronize()
+    cache.paged.set_stream(side.cuda_stream)
+    with torch.cuda.graph(graph, stream=side):
+        forward()
+    cache.paged.set_stream(stream.cuda_stream)
+    for turn, shrink in enumerate((1, 2, 50)):
+        now = [-1 if (s + turn) % 9 == 4 else p // shrink for s, p in enumerate(most)]
+        held.copy_(i32(now))
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert status.tolist() == [int(p < 0) for p in now]
+        items = [(max(p, 0), nodes) for p in now]
+        for s in range(turn, n, 9):
+            if now[s] < 0:
+                assert bool((out[s * nodes:(s + 1) * nodes] == 7.0).all())
+            else:
+                check_one(cache, items, trees, s, q, out, "f16")
+
+
 def test_layers_that_differ_over_one_batch():
     # Heads, types and windows in turn, over one batch and each over a batch of its own: the same cut, so the same bits.
     items, trees = [(900, 40), (2500, 21), (64, 5)], [TC.tree(40, 1), TC.tree(21, 2), TC.tree(5, 3)]
