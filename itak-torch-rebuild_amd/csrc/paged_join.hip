@@ -3,7 +3,8 @@
 //
 // A unit's parts lie in consecutive slots, each a tile's accumulators as registers held them: 16 bytes of four channels, 32 vectors side by side. A
 // wavefront serves four vectors, which share their 64 bytes, and has four channels of each in a lane; where parts are many and vectors few the four
-// wavefronts of a workgroup share the parts. Bytes bound it, and below some megabytes the trips: item, maxima and sums, accumulators.
+// wavefronts of a workgroup share the parts. Bytes bound it, and below some megabytes the trips: item, maxima and sums, accumulators (4.4 MB 4.8 us, 33 MB
+// 9.2: 3.6 TB/s).
 #include "paged_mfma.h"
 
 namespace itak {
@@ -159,7 +160,7 @@ void launch(const PagedAttn &a, hipStream_t stream) {
 }
 
 // The partials of the kernel of few rows, which lie vector by vector, where rows are drafted trees: some vectors for every compute unit, of a few
-// parts each. A wavefront serves a vector (paged_merge.hip gives a workgroup to each: 85 rows of 32 heads of 64 10.8 us, and so 5.7).
+// parts each. A wavefront serves a vector (paged_merge.hip gives a workgroup to each: 85 rows of 32 heads of 64 10.8 us, and so 5.0).
 template <int ELEM, int DP>
 __global__ __launch_bounds__(kThreads) void paged_few_join_kernel(PagedAttn a) {
     typedef typename Elem<ELEM>::type T;
