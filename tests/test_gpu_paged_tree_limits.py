@@ -7,7 +7,7 @@ import torch
 import paged_cases as PC
 import tree_cases as TC
 from helpers import pkg, refusal
-from test_gpu_paged_trees import cache_of, view
+from test_gpu_paged_trees import attend, cache_of, view
 
 pytestmark = pytest.mark.gpu
 
@@ -126,6 +126,26 @@ def test_replays_over_many_sequences(kv_heads):
                 assert bool((out[s * nodes:(s + 1) * nodes] == 7.0).all())
             else:
                 check_one(cache, items, trees, s, q, out, "f16")
+
+
+# Query heads of a KV head that are no power of two or the most there may be, and more KV heads than parts leave room for.
+@pytest.mark.parametrize("heads,kv_heads,d,tensors", [(64, 1, 64, "f16"), (33, 1, 128, "f32"), (96, 2, 96, "f16"), (390, 130, 8, "f16"), (64, 1, 256, "f32")])
+def test_many_heads(heads, kv_heads, d, tensors):
+    items = [(1500 if kv_heads < 100 else 90, 1), (31, 13), (0, 2), (130, 5)]
+    trees = [[-1], TC.tree(13, 1), [-1, -1], TC.tree(5, 2)]
+    cache = cache_of(items, kv_heads=kv_heads, d=d, page_rows=32, seed=heads)
+    q, out = attend(cache, items, trees, heads, tensors)
+    stream, side, graph = torch.cuda.current_stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    qd, again = q.cuda(), torch.empty_like(q, device="cuda")
+    cache.paged.set_stream(side.cuda_stream)
+    with torch.cuda.graph(graph, stream=side):
+        cache.paged.attention_device(0, view(qd), view(again))
+    cache.paged.set_stream(stream.cuda_stream)
+    for _ in range(2):
+        again.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        TC.check(cache, 0, items, trees, q, again, tensors)
 
 
 def test_layers_that_differ_over_one_batch():
