@@ -342,22 +342,21 @@ __global__ __launch_bounds__(paged_trees_waves(DP, PAGE, ELEM) * 64) void paged_
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
         __builtin_amdgcn_s_barrier();  // (everybody is done with the ring)
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-        floatx4 *const to = met + wave * kQuads * kTreesQuad + lane;
-#pragma unroll
-        for (int t = 0; t < kOut; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) to[(t * 4 + r) * kTreesQuad] = floatx4{o[t][4 * r], o[t][4 * r + 1], o[t][4 * r + 2], o[t][4 * r + 3]};
     }
-    __syncthreads();
-    // Column c of a set over all groups: its maximum and sum. (A maximum of minus infinity: nothing visible, a sum of 0, or scores that are no
-    // numbers, which the sum then is.)
-    auto weight_of = [&](float2 ml, float m) { return ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - m); };
-    auto all_of = [&](uint32_t c) __attribute__((always_inline)) {
+    // Column c of a set over all its groups: the maximum and sum, and the groups' weights. (A maximum of minus infinity: nothing visible, a sum of 0, or
+    // scores that are no numbers, which the sum then is.)
+    auto all_of = [&](uint32_t c, auto &weights) __attribute__((always_inline)) {
+        constexpr uint32_t kGroups = sizeof(weights) / sizeof(float);
+        float2 ml[kGroups];
         float m = -INFINITY, l = 0.0f;
-        for (uint32_t g = 0; g < groups; ++g) m = fmaxf(m, lds_ml[(g << sets_shift) + set][c].x);
-        for (uint32_t g = 0; g < groups; ++g) {
-            const float2 ml = lds_ml[(g << sets_shift) + set][c];
-            l += ml.x == -INFINITY ? ml.y : weight_of(ml, m) * ml.y;
+#pragma unroll
+        for (uint32_t g = 0; g < kGroups; ++g) ml[g] = lds_ml[(g << sets_shift) + set][c];
+#pragma unroll
+        for (uint32_t g = 0; g < kGroups; ++g) m = fmaxf(m, ml[g].x);
+#pragma unroll
+        for (uint32_t g = 0; g < kGroups; ++g) {
+            weights[g] = ml[g].x == -INFINITY ? 0.0f : fast_exp2(ml[g].x - m);
+            l += ml[g].x == -INFINITY ? ml[g].y : weights[g] * ml[g].y;
         }
         return make_float2(m, l);
     };
@@ -376,14 +375,26 @@ __global__ __launch_bounds__(paged_trees_waves(DP, PAGE, ELEM) * 64) void paged_
     auto finish = [&](auto GROUPS) __attribute__((always_inline)) {
         constexpr uint32_t kGroups = 1u << GROUPS.value, kMine = kQuads / kGroups, kOfRow = DP / 8;
         floatx4 acc[kMine];
-        if (!whole) {
-            const float2 ml = all_of(j);
+        float weights[kGroups];
+        // (Of a split unit a group's own quads stay in its registers.)
+        auto own = [&](uint32_t q) { return floatx4{o[q / 4][4 * (q % 4)], o[q / 4][4 * (q % 4) + 1], o[q / 4][4 * (q % 4) + 2], o[q / 4][4 * (q % 4) + 3]}; };
 #pragma unroll
-            for (uint32_t u = 0; u < kMine; ++u) acc[u] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t q = 0; q < kQuads; ++q)
+            if (whole || q / kMine != group) met[(wave * kQuads + q) * kTreesQuad + lane] = own(q);
+        __syncthreads();
+        if (!whole) {
+            const float2 ml = all_of(j, weights);
+#pragma unroll
+            for (uint32_t g = 0; g < kGroups; ++g)
+                if (g == group) {
+#pragma unroll
+                    for (uint32_t u = 0; u < kMine; ++u) acc[u] = own(g * kMine + u) * weights[g];
+                }
 #pragma unroll
             for (uint32_t g = 0; g < kGroups; ++g) {
+                if (g == group) continue;
                 const uint32_t w = (g << sets_shift) + set;
-                const float weight = weight_of(lds_ml[w][j], ml.x);
+                const float weight = weights[g];
 #pragma unroll
                 for (uint32_t u = 0; u < kMine; ++u) {
                     const floatx4 y = met[(w * kQuads + group * kMine + u) * kTreesQuad + lane];
@@ -408,12 +419,12 @@ __global__ __launch_bounds__(paged_trees_waves(DP, PAGE, ELEM) * 64) void paged_
 #pragma unroll
             for (uint32_t u = 0; u < kMine / 2; ++u) {
                 const uint32_t c = column(u);
-                const float2 ml = all_of(c);
+                const float2 ml = all_of(c, weights);
                 acc[2 * u] = acc[2 * u + 1] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (uint32_t g = 0; g < kGroups; ++g) {
                     const uint32_t w = (g << sets_shift) + set;
-                    const float weight = weight_of(lds_ml[w][c], ml.x);
+                    const float weight = weights[g];
 #pragma unroll
                     for (uint32_t x = 0; x < 2; ++x) {
                         const floatx4 y = met[(w * kQuads + ch) * kTreesQuad + x * 32 + c];
