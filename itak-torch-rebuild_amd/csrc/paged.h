@@ -230,21 +230,16 @@ struct PagedLine {
         }
         return s;
     }
+    // (The items are asked for together with their number, which the lanes behind the last find out later.)
     __device__ __forceinline__ PagedSpan of_lane(uint32_t at, uint32_t n, uint32_t &work, uint32_t &units) const {
-        PagedItemWords w{};
-        const bool there = at + __lane_id() < n;
-        if (there) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(a.batch + kPagedItem0 + 4 * (at + __lane_id()));
-            w.position = x.x, w.rows = x.y, w.row0 = x.z, w.table = x.w;
-        }
-        return span_of(w, there, work, units);
+        const uint4 x = *reinterpret_cast<const uint4 *>(a.batch + kPagedItem0 + 4 * min(at + __lane_id(), a.items - 1));
+        return span_of(PagedItemWords{x.x, x.y, x.z, x.w}, at + __lane_id() < n, work, units);
     }
     static __device__ __forceinline__ uint32_t scan(uint32_t x) {  // inclusive, over the wavefront
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t y = __shfl_up(x, d);
-            x += (__lane_id() >= uint32_t(d)) ? y : 0;
-        }
+#define ITAK_ADD(ctrl, rows) x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), ctrl, rows, 0xf, false))
+        ITAK_ADD(0x111, 0xf), ITAK_ADD(0x112, 0xf), ITAK_ADD(0x114, 0xf), ITAK_ADD(0x118, 0xf);  // (of sixteen lanes)
+        ITAK_ADD(0x142, 0xa), ITAK_ADD(0x143, 0xc);  // (and on to the next sixteen, and thirty-two)
+#undef ITAK_ADD
         return x;
     }
     static __device__ __forceinline__ uint32_t most_of(uint32_t x) {  // over the wavefront
@@ -359,12 +354,15 @@ __device__ __forceinline__ bool paged_part_of(const PagedLine &line, uint32_t &p
 }
 
 // The batch's item that holds row `row`: its position, first row and table. All lanes ask together.
-__device__ __forceinline__ bool paged_item_of_row(const uint32_t *batch, uint32_t row, uint4 &item) {
-    const uint32_t n = batch[0], lane = __lane_id();
+// (The first items are asked for together with their number.)
+__device__ __forceinline__ bool paged_item_of_row(const PagedGeom &g, const uint32_t *batch, uint32_t row, uint4 &item) {
+    const uint32_t lane = __lane_id(), last = (g.ids_at - kPagedItem0) / 4 - 1;
+    auto item_of = [&](uint32_t at) { return *reinterpret_cast<const uint4 *>(batch + kPagedItem0 + 4 * min(at + lane, last)); };
+    uint4 w = item_of(0);
+    const uint32_t n = batch[0];
     for (uint32_t at = 0; at < n; at += 64) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (at + lane < n) w = *reinterpret_cast<const uint4 *>(batch + kPagedItem0 + 4 * (at + lane));
-        const uint64_t mask = __builtin_amdgcn_ballot_w64(row >= w.z && row - w.z < w.y);
+        if (at) w = item_of(at);
+        const uint64_t mask = __builtin_amdgcn_ballot_w64(at + lane < n && row >= w.z && row - w.z < w.y);
         if (mask) {
             const uint32_t l = __builtin_ctzll(mask);
             item.x = __builtin_amdgcn_readlane(w.x, l), item.y = __builtin_amdgcn_readlane(w.y, l);

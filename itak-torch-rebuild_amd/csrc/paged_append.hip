@@ -19,7 +19,7 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedAppend a) {
     __shared__ float2 cs[kMostPairs];
     const uint32_t row = blockIdx.x, tid = threadIdx.x;
     uint4 item;
-    if (!paged_item_of_row(a.batch, row, item)) return;  // (the same for the whole workgroup)
+    if (!paged_item_of_row(a.g, a.batch, row, item)) return;  // (the same for the whole workgroup)
     const uint32_t position = item.x + (row - item.z);
     // (A row of a tree is turned by its depth.)
     const uint32_t turned_by = a.tree && a.batch[2] ? item.x + tree_depth(a.tree[uint64_t(row) * kTreeStride]) : position;
