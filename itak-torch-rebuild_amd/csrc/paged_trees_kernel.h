@@ -16,7 +16,7 @@
 // Measured, 32 query heads over 4 of 128 channels, f16: 16 rows at 4,096 12.3 us (8.4 MB of keys and values), 64 rows at 8,192 23.4 (16.8 MB, 8.6 GFLOP), 4
 // trees of 61 rows in a window of 2,048 26.7 (21 MB, 8.2 GFLOP). Of a part's clocks some 16,000 are its start and end: arguments and item 1,350, page ids
 // and queries 2,900, sending the ring's loads 2,600, the first blocks' way 2,600, the groups' meeting 4,200, the stores 2,000; a step of two blocks takes
-// 2,700, some 850 of them products and softmax.
+// 2,700, some 850 of them products and softmax, where LDS reads and writes take some 1,900; with all keys in the L2 it takes 2,550.
 #pragma once
 
 #include "lds_grant.h"
@@ -41,6 +41,7 @@ __global__ __launch_bounds__(paged_trees_waves(DP, PAGE, ELEM) * 64) void paged_
     typedef typename Elem<ELEM>::type T;
     constexpr int kWaves = paged_trees_waves(DP, PAGE, ELEM), kTile = kWaves * 32;
     constexpr uint32_t kBlocks = trees_blocks(DP, kWaves), kWavesShift = kWaves == 8 ? 3 : 2;
+    static_assert(kBlocks >= kWaves);  // two steps of the most groups
     constexpr int kSteps = DP / 16;               // products of a score tile
     constexpr int kOut = DP / 32;                 // output tiles of 32 channels
     constexpr int kRowBytes = 2 * DP, kBlockBytes = 32 * kRowBytes, kStageBytes = 2 * kBlockBytes;
@@ -216,23 +217,16 @@ __global__ __launch_bounds__(paged_trees_waves(DP, PAGE, ELEM) * 64) void paged_
 #pragma unroll 1
     for (uint32_t n = 0; n < steps; ++n) {
         // This wavefront's loads of the step's blocks have landed; behind the barrier everybody's have, and everybody is done with the step before,
-        // whose places the loads that go out now take. (Where the ring holds one step that is this one, which then has to land.)
+        // whose places the loads that go out now take. (The ring holds two steps or more.)
         const uint32_t upto = min(blocks, (n + 1) << groups_shift);
         wait_for(issued > upto ? issued - upto : 0);
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (n) {
-            const bool now = issued < upto;
+        if (n)
             for (const uint32_t more = min(blocks, issued + groups); issued < more; ++issued) {
                 if ((issued & 63) == 0) ask(kb0 + issued), answer(kb0 + issued);
                 issue(issued);
             }
-            if (now) {
-                wait_loads<0>();
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
-            }
-        }
         // Rows no query of the tile sees may hold anything: their values are zeroed. (Every lane reads and writes.)
         const uint32_t k0 = 32 * (kb0 + (n << groups_shift)), k1 = 32 * (kb0 + upto);
         if (k0 < tile_lo || k1 > tile_hi) {
