@@ -81,8 +81,6 @@ struct PagedAttn {
     float cap_log2;      // cap * log2(e), 0: none
     uint32_t window;
     uint32_t parts;      // kernel of many rows: workgroups a unit is dealt to; 0: the line above
-    uint32_t apart;      // kernel of trees: no workgroup has parts of two units (paged_cut_apart), and a unit is a tile of all heads
-    uint32_t across;     // and the grid's workgroups of a head
     const void *zeros;   // 16 bytes of them
     uint32_t inline_items; // 0: the batch's are read from device memory
     uint32_t total;      // where the host knows the batch: the line's length, and its cut (else a share of 0)
@@ -92,6 +90,8 @@ struct PagedAttn {
     float *ws_acc;       // [slots][tile][padded head_dim]
     float2 *ws_ml;       // [slots][tile]: maximum (log2 domain), sum; negative: of a part that is scaled down by kPagedMergeLift
     const uint32_t *tree; // the rows' records (paged_tree.h): of a batch whose rows may be trees, else null
+    uint32_t apart;      // kernel of trees: no workgroup has parts of two units (paged_cut_apart), and a unit is a tile of all heads
+    uint32_t across;     // and the grid's workgroups of a head
 };
 // Workgroups that may share a unit.
 constexpr uint32_t kPagedMostParts = 1024;
@@ -198,21 +198,25 @@ __device__ __forceinline__ bool paged_has_trees(const PagedAttn &a) { return a.i
 
 // Asks for all of the arguments at once: the compiler asks where it needs them, a trip to memory for every 64 bytes that come
 // first there (of the few rows' kernel four in a row, some 3,000 clocks before the first page id).
+template <bool TREE = false>
 __device__ __forceinline__ void paged_fetch_arguments(const PagedAttn &a) {
     static_assert(sizeof(PagedAttn) <= 9 * 64 && kPagedInline == 8, "a word of every 64 bytes is named");
     asm volatile("" ::"s"(a.batch), "s"(a.layer_base), "s"(a.q.data), "s"(a.out.data), "s"(a.rows), "s"(a.units), "s"(a.v_to), "s"(a.window),
                  "s"(a.zeros), "s"(a.total), "s"(a.item[1].row0), "s"(a.item[5].row0), "s"(a.start[1]), "s"(a.unit0[1]), "s"(a.ws_acc),
-                 "s"(a.ws_ml), "s"(a.tree));
+                 "s"(a.ws_ml));
+    if constexpr (TREE) asm volatile("" ::"s"(a.tree), "s"(a.across));
 }
 
 // The items a launch takes, in order: where their blocks and units lie in the line. Those in memory are looked at 64 at a time, one
 // a lane.
-struct PagedLine {
+// APART: those of the kernel of trees.
+template <bool APART>
+struct PagedLineOf {
     const PagedAttn &a;
     uint32_t share = 0, pad = 0, total = 0;
     uint32_t across = 0;  // of cut_apart
 
-    __device__ __forceinline__ explicit PagedLine(const PagedAttn &args) : a(args) {}
+    __device__ __forceinline__ explicit PagedLineOf(const PagedAttn &args) : a(args) {}
     // An item's span, and blocks and units of all of it; none of an item that the launch does not take, and of one beyond the
     // launch's rows (a batch that is not what a captured launch was made for).
     __device__ __forceinline__ PagedSpan span_of(const PagedItemWords &w, bool there, uint32_t &work, uint32_t &units) const {
@@ -224,7 +228,7 @@ struct PagedLine {
             s.first = paged_first_block(w.position, a.window);
             s.blocks = (w.position + w.rows + 31) / 32 - s.first;
             s.tiles = (vectors + (1u << a.tile_shift) - 1) >> a.tile_shift;
-            units = a.apart ? s.tiles : s.tiles * a.g.kv_heads;
+            units = APART ? s.tiles : s.tiles * a.g.kv_heads;
             s.run = paged_run(s.blocks, pad);
             work = units * s.run;
         }
@@ -341,11 +345,14 @@ struct PagedLine {
     }
 };
 
+using PagedLine = PagedLineOf<false>;
+using PagedTreeLine = PagedLineOf<true>;
+
 // The part and the head of a workgroup of the kernel of trees. Workgroup w runs on compute die w mod 8: a die takes a run of the parts in their order,
 // head by head, so that the tiles that read the same keys share its cache, and short last parts do not meet on one die: 8 trees of 256 rows over 16,384
 // 487 us, and 524 side by side over the dies; 100 rows over 20,000 59 and 62; 4 of 61 rows in a window of 2,048 33 and 31 (the one that loses).
 // (False: none is left for it. Workgroups without a part come last: on their own dies they would leave the others to share the work.)
-__device__ __forceinline__ bool paged_part_of(const PagedLine &line, uint32_t &part, uint32_t &head) {
+__device__ __forceinline__ bool paged_part_of(const PagedTreeLine &line, uint32_t &part, uint32_t &head) {
     const uint32_t w = blockIdx.x + line.a.across * blockIdx.y, all = line.across * line.a.g.kv_heads, die = w & 7;
     const uint32_t at = die * (all >> 3) + min(die, all & 7) + (w >> 3);
     if (w >= all) return false;

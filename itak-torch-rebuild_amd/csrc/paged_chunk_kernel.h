@@ -69,18 +69,19 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     // batch whose rows may be trees the cut is that of the kernel of trees.)
     const uint32_t units = TREE ? 1 : gridDim.x / a.parts;
     const uint32_t part = TREE ? 0 : blockIdx.x / units, unit = blockIdx.x - part * units;
-    PagedLine line(a);
+    typedef PagedLineOf<TREE> Line;
+    Line line(a);
     PagedSpan span;
     uint32_t nth = 0, from = 0, head, turn;
     if constexpr (TREE) {
-        paged_fetch_arguments(a);
+        paged_fetch_arguments<true>(a);
         line.cut_apart();
         if (!paged_part_of(line, nth, head)) return;
         const uint32_t at = nth * line.share;
-        if (at >= line.total || !line.find<PagedLine::kBlock>(span, at)) return;
+        if (at >= line.total || !line.template find<Line::kBlock>(span, at)) return;
         turn = span.tiles == 1 ? 0 : (at - span.start) / span.run, from = (at - span.start) - turn * span.run;
     } else {
-        if (!line.find<PagedLine::kUnit>(span, unit)) return;
+        if (!line.template find<Line::kUnit>(span, unit)) return;
         const uint32_t local = unit - span.unit0;
         turn = local / a.g.kv_heads, head = local - turn * a.g.kv_heads;
     }
@@ -93,15 +94,12 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     const bool trees = TREE && paged_has_trees(a);
     const uint32_t tile_lo = lowest_visible(span.position + (trees ? 0 : first_row), a.window, 0), tile_hi = span.position + last_row + 1;
     uint32_t kb0, kb_end;
-    bool whole;
     uint64_t slot0;
     if constexpr (TREE) {
-        whole = span.blocks <= line.share;
         kb0 = max(span.first + from, tile_lo / 32);
         kb_end = max(kb0, min(span.first + min(from + line.share, span.blocks), (tile_hi + 31) / 32));
         slot0 = uint64_t(head * a.groups + nth) * kTile;
     } else {
-        whole = a.parts == 1;
         const uint32_t b_first = tile_lo / 32, b_all = (tile_hi + 31) / 32 - b_first, b_part = (b_all + a.parts - 1) / a.parts;
         kb0 = b_first + min(b_all, part * b_part), kb_end = b_first + min(b_all, part * b_part + b_part);
         slot0 = uint64_t(unit * a.parts + part) * kTile;
@@ -445,7 +443,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
     }
     // A lane holds of its column channels 32 t + 8 (r / 4) + 4 h + r % 4.
     // (The check comes before the stores: the barriers it takes would wait for them.)
-    const bool mine = wv0 + j < vectors;
+    const bool whole = TREE ? span.blocks <= line.share : a.parts == 1, mine = wv0 + j < vectors;
     const uint32_t v = wv0 + j;
     const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
     const float l = __uint_as_float(both[0]) + __uint_as_float(both[1]);

@@ -69,7 +69,7 @@ __global__ __launch_bounds__(kFewWaves * 64, paged_few_groups_per_cu(DP, PAGE, E
     u32x4 *const lds_q = reinterpret_cast<u32x4 *>(lds);
     auto lds_o = reinterpret_cast<float (*)[kTile][kStride]>(lds);
 
-    paged_fetch_arguments(a);
+    paged_fetch_arguments<TREE>(a);
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const uint32_t g = lane >> 4, i = lane & 15;
     const uint32_t d = EXACT ? DP : a.g.head_dim;

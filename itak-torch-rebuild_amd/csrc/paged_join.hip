@@ -23,14 +23,14 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttn a) {
     const uint32_t of_tile = a.tile / kJoined;  // (a power of two)
     __shared__ float lds_weight[SHARED > 1 ? 1 : kWaves][kPagedTreesGroups][kJoined];
     __shared__ floatx4 lds_acc[SHARED > 1 ? SHARED - 1 : 1][SHARED > 1 ? kOfLane : 1][64];
-    paged_fetch_arguments(a);
+    paged_fetch_arguments<true>(a);
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const uint32_t joined = SHARED > 1 ? blockIdx.x : blockIdx.x * kWaves + wave, unit = joined >> (a.tile_shift - 2);
     static_assert(kJoined == 4, "a tile is 2^(tile_shift - 2) times that");
-    PagedLine line(a);
+    PagedTreeLine line(a);
     line.cut_apart();
     PagedSpan span;
-    if (!line.find<PagedLine::kUnit>(span, unit)) return;
+    if (!line.find<PagedTreeLine::kUnit>(span, unit)) return;
     const uint32_t parts = (span.blocks + line.share - 1) / line.share;
     if (parts <= 1) return;  // written whole
     const uint32_t turn = unit - span.unit0, tile = span.tiles - 1 - turn, head = blockIdx.y;

@@ -54,17 +54,17 @@ __global__ __launch_bounds__(paged_trees_waves(DP, PAGE, ELEM) * 64) void paged_
     __shared__ float2 lds_ml[kWaves][32];
     __shared__ uint32_t lds_flag;
 
-    paged_fetch_arguments(a);
+    paged_fetch_arguments<true>(a);
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const uint32_t h = lane >> 5, j = lane & 31;
     const uint32_t d = EXACT ? DP : a.g.head_dim;
-    PagedLine line(a);
+    PagedTreeLine line(a);
     line.cut_apart();
     uint32_t nth, head;
     if (!paged_part_of(line, nth, head)) return;
     const uint32_t at = nth * line.share;
     PagedSpan span;
-    if (at >= line.total || !line.find<PagedLine::kBlock>(span, at)) return;
+    if (at >= line.total || !line.find<PagedTreeLine::kBlock>(span, at)) return;
     const bool trees = paged_has_trees(a);
     const uint32_t turn = span.tiles == 1 ? 0 : (at - span.start) / span.run, from = (at - span.start) - turn * span.run;
     const uint32_t tile = span.tiles - 1 - turn;  // (the longest first, of a chain)
