@@ -18,14 +18,16 @@ constexpr uint32_t kJoined = 4;  // vectors of a wavefront
 template <int ELEM, int DP, uint32_t SHARED>
 __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttn a) {
     typedef typename Elem<ELEM>::type T;
-    constexpr uint32_t kOfLane = DP / 64, kQuads = DP / 8, kAtOnce = 8 / kOfLane;  // quads of a lane; of a lane of the tile; parts at once
+    constexpr uint32_t kOfLane = DP / 64, kQuads = DP / 8, kAtOnce = (SHARED > 1 ? 16 : 8) / kOfLane;  // quads of a lane; of a lane of the tile; parts at once
     constexpr uint32_t kWaves = kThreads / 64;
     const uint32_t of_tile = a.tile / kJoined;  // (a power of two)
     __shared__ float lds_weight[SHARED > 1 ? 1 : kWaves][kPagedTreesGroups][kJoined];
     __shared__ floatx4 lds_acc[SHARED > 1 ? SHARED - 1 : 1][SHARED > 1 ? kOfLane : 1][64];
     paged_fetch_arguments<true>(a);
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    const uint32_t joined = SHARED > 1 ? blockIdx.x : blockIdx.x * kWaves + wave, unit = joined >> (a.tile_shift - 2);
+    // (Eight vectors share their lines of memory: workgroups on the same compute die, eight apart, have them. A head's are a multiple of sixteen.)
+    const uint32_t beside = (blockIdx.x & ~15u) | (blockIdx.x & 7) << 1 | (blockIdx.x >> 3 & 1);
+    const uint32_t joined = SHARED > 1 ? beside : blockIdx.x * kWaves + wave, unit = joined >> (a.tile_shift - 2);
     static_assert(kJoined == 4, "a tile is 2^(tile_shift - 2) times that");
     PagedTreeLine line(a);
     line.cut_apart();
@@ -50,10 +52,16 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttn a) {
     // The first accumulators are asked for before the maxima are there.
     const uint32_t first = SHARED > 1 ? wave : 0;
     floatx4 early[kAtOnce][kOfLane];
+    // (The second half of them where there are as many.)
+    auto ask = [&](uint32_t p0) __attribute__((always_inline)) {
 #pragma unroll
-    for (uint32_t u = 0; u < kAtOnce; ++u)
+        for (uint32_t u = 0; u < kAtOnce; ++u) {
+            if (u >= kAtOnce / 2 && p0 + kAtOnce / 2 * SHARED >= parts) break;
 #pragma unroll
-        for (uint32_t i = 0; i < kOfLane; ++i) early[u][i] = acc_of(min(first + u * SHARED, parts - 1), i);
+            for (uint32_t i = 0; i < kOfLane; ++i) early[u][i] = acc_of(min(p0 + u * SHARED, parts - 1), i);
+        }
+    };
+    ask(first);
     // A lane has every sixteenth part's maximum and sum of its vector. The first 64 parts' stay in registers.
     constexpr uint32_t kKept = 4;
     float2 ml[kKept];
@@ -90,12 +98,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttn a) {
 #pragma unroll
     for (uint32_t i = 0; i < kOfLane; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t p0 = first; p0 < parts; p0 += kAtOnce * SHARED) {
-        if (p0 != first) {
-#pragma unroll
-            for (uint32_t u = 0; u < kAtOnce; ++u)
-#pragma unroll
-                for (uint32_t i = 0; i < kOfLane; ++i) early[u][i] = acc_of(min(p0 + u * SHARED, parts - 1), i);
-        }
+        if (p0 != first) ask(p0);
 #pragma unroll
         for (uint32_t u = 0; u < kAtOnce; ++u) {
             const uint32_t p = p0 + u * SHARED;
