@@ -3,8 +3,8 @@
 //
 // A unit's parts lie in consecutive slots, each a tile's accumulators as registers held them: 16 bytes of four channels, 32 vectors side by side. A
 // wavefront serves four vectors, which share their 64 bytes, and has four channels of each in a lane; where parts are many and vectors few the four
-// wavefronts of a workgroup share the parts. Bytes bound it, and below some megabytes the trips: item, maxima and sums, accumulators (4.4 MB 4.8 us, 33 MB
-// 9.2: 3.6 TB/s).
+// wavefronts of a workgroup share the parts. Bytes bound it, and below some megabytes the trips: item, maxima and sums, accumulators (4.4 MB 4.0 us, 13.6 MB
+// 5.4, 33 MB 9.0: 3.7 TB/s).
 #include "paged_mfma.h"
 
 namespace itak {
@@ -25,7 +25,8 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttn a) {
     __shared__ floatx4 lds_acc[SHARED > 1 ? SHARED - 1 : 1][SHARED > 1 ? kOfLane : 1][64];
     paged_fetch_arguments<true>(a);
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    // (Eight vectors share their lines of memory: workgroups on the same compute die, eight apart, have them. A head's are a multiple of sixteen.)
+    // (Eight vectors share their lines of memory: workgroups on the same compute die, eight apart, have them; side by side, on two dies, the lines came
+    // twice: 13.6 MB 7.2 us for 5.4. A head's workgroups are a multiple of sixteen.)
     const uint32_t beside = (blockIdx.x & ~15u) | (blockIdx.x & 7) << 1 | (blockIdx.x >> 3 & 1);
     const uint32_t joined = SHARED > 1 ? beside : blockIdx.x * kWaves + wave, unit = joined >> (a.tile_shift - 2);
     static_assert(kJoined == 4, "a tile is 2^(tile_shift - 2) times that");
@@ -163,7 +164,7 @@ void launch(const PagedAttn &a, hipStream_t stream) {
 }
 
 // The partials of the kernel of few rows, which lie vector by vector, where rows are drafted trees: some vectors for every compute unit, of a few
-// parts each. A wavefront serves a vector (paged_merge.hip gives a workgroup to each: 85 rows of 32 heads of 64 10.8 us, and so 5.0).
+// parts each. A wavefront serves a vector (paged_merge.hip gives a workgroup to each: 85 rows of 32 heads of 64 10.8 us, and so 4.6).
 template <int ELEM, int DP>
 __global__ __launch_bounds__(kThreads) void paged_few_join_kernel(PagedAttn a) {
     typedef typename Elem<ELEM>::type T;

@@ -13,8 +13,8 @@
 // A small tile makes small partials and reads the keys once a set: the host weighs the two (trees_plan). Partials are written as the registers hold
 // them, 1 KiB a store (a vector's row at a time they took 1.6 us of a part).
 //
-// Measured, 32 query heads over 4 of 128 channels, f16: 16 rows at 4,096 12.3 us (8.4 MB of keys and values), 64 rows at 8,192 23.4 (16.8 MB, 8.6 GFLOP), 4
-// trees of 61 rows in a window of 2,048 26.7 (21 MB, 8.2 GFLOP). Of a part's clocks some 16,000 are its start and end: arguments and item 1,350, page ids
+// Measured, 32 query heads over 4 of 128 channels, f16: 16 rows at 4,096 12.2 us (8.4 MB of keys and values), 64 rows at 8,192 22.9 (16.8 MB, 8.6 GFLOP), 4
+// trees of 61 rows in a window of 2,048 26.4 (21 MB, 8.2 GFLOP). Of a part's clocks some 16,000 are its start and end: arguments and item 1,350, page ids
 // and queries 2,900, sending the ring's loads 2,600, the first blocks' way 2,600, the groups' meeting 4,200, the stores 2,000; a step of two blocks takes
 // 2,700, some 850 of them products and softmax, where LDS reads and writes take some 1,900; with all keys in the L2 it takes 2,550.
 #pragma once
