@@ -59,7 +59,7 @@ __device__ __forceinline__ void paged_careful(const PagedAttn &a, const PagedSpa
         for (uint32_t u = 0; u < kCareful; ++u) {
             const uint32_t mine = min(v + u, v_end - 1), row = paged_row_of(a, mine), pos = span.position + row;
             if constexpr (TREE) {
-                record[u] = a.tree + uint64_t(span.row0 + row) * kTreeStride;
+                record[u] = a.tree + tree_record_at(trees, span.row0 + row);
                 word[u] = trees ? record[u][kTreeDepth] : kTreeChain | row;
             }
             lo[u] = max(lowest_visible(TREE ? span.position + tree_depth(word[u]) : pos, a.window, 0), key0), hi[u] = min(pos + 1, key1);

@@ -179,7 +179,7 @@ __global__ __launch_bounds__(paged_chunk_waves(DP, ELEM) * 64) void paged_chunk_
         const uint32_t hq = head * a.group + (v < vectors ? v - row * a.group : 0);
         my_pos = span.position + row;
         if constexpr (TREE) {
-            const uint32_t *const record = a.tree + uint64_t(span.row0 + row) * kTreeStride;
+            const uint32_t *const record = a.tree + tree_record_at(trees, span.row0 + row);
             const uint32_t word = trees ? record[kTreeDepth] : kTreeChain | row;
             my_lo = lowest_visible(span.position + tree_depth(word), a.window, 0);
             // (The lanes of the two halves hold the same column: each brings every other word. No lane is turned off.)

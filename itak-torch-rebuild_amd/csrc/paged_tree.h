@@ -24,6 +24,9 @@ constexpr uint32_t kTreeDepth = 0, kTreeParent = 1, kTreeSees = 2, kTreeBlocks =
 constexpr uint32_t kTreeChain = 1u << 31;
 
 ITAK_BOTH uint32_t tree_depth(uint32_t word) { return word & ~kTreeChain; }
+// Where a row's record begins. A batch without records may have more rows than there is room for: where one is read all the same, and
+// what it says not looked at, it is the first.
+ITAK_BOTH uint64_t tree_record_at(bool trees, uint64_t row) { return trees ? row * kTreeStride : 0; }
 
 // Whether the parents of a whole item are those of a chain, and of a tree: every one a row before, or -1.
 inline bool tree_is_chain(const int32_t *parents, uint64_t rows) {

@@ -110,7 +110,7 @@ __global__ __launch_bounds__(paged_trees_waves(DP, PAGE, ELEM) * 64) void paged_
     // A lane's column: its query, and what it sees.
     const uint32_t v = wv0 + j, row = min(paged_row_of(a, v), span.rows - 1);
     const uint32_t hq = head * a.group + (v < vectors ? v - row * a.group : 0);
-    const uint32_t *const record = a.tree + uint64_t(span.row0 + row) * kTreeStride;
+    const uint32_t *const record = a.tree + tree_record_at(trees, span.row0 + row);
     typename QueryRaw<ELEM>::type raw[kSteps];
     {
         const T *src = static_cast<const T *>(a.q.data) + uint64_t(span.row0 + row) * a.q.row_stride + hq * a.q.head_stride;
