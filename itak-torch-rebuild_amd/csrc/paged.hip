@@ -441,6 +441,10 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
         plan.merge_few = !known || !whole;
     }
     const itak_status st = workspace(p, plan, dp);
+    // (A graph looks at all items of the batch that is there when it runs. Sequences without rows are left out of one set here, and count among those of a
+    // handle that takes trees and of a batch that the device makes.)
+    if (captured)
+        for (PagedAttn *b : {&plan.few, &plan.trees, &plan.many}) b->items = p->cfg.max_sequences;
     if (st == ITAK_OK && captures) {
         itak_paged::Captured &c = p->captured[a.window ? 1 : 0];
         c.units = std::max<uint64_t>({c.units, plan.few.units, plan.trees.units, plan.many.units});

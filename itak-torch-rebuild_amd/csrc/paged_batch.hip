@@ -251,21 +251,23 @@ struct BatchRows {
     uint32_t rows;
     int64_t *positions, *slots;
 };
+// (Workgroups that a graph captured may be fewer than the items of the batch that is there when it runs.)
 __global__ __launch_bounds__(kThreads) void paged_batch_rows_kernel(BatchRows a) {
-    const uint32_t n = min(a.batch[0], gridDim.x), i = blockIdx.x;
-    if (i >= n) return;
-    const uint4 item = *reinterpret_cast<const uint4 *>(a.batch + kPagedItem0 + 4 * i);
-    const uint32_t end = min(a.rows, i + 1 < n ? a.batch[kPagedItem0 + 4 * (i + 1) + 2] : a.batch[1]);
+    const uint32_t n = a.batch[0];
     const bool trees = a.tree && a.batch[2];
-    for (uint32_t row = item.z + threadIdx.x; row < end; row += kThreads) {
-        const uint32_t r = row - item.z, place = item.x + r;
-        int64_t position = -1, slot = -1;
-        if (r < item.y) {
-            position = item.x + (trees ? tree_depth(a.tree[uint64_t(row) * kTreeStride]) : r);
-            slot = (int64_t(a.batch[item.w + (place >> a.page_shift)]) << a.page_shift) + (place & ((1u << a.page_shift) - 1));
+    for (uint32_t i = blockIdx.x; i < n; i += gridDim.x) {
+        const uint4 item = *reinterpret_cast<const uint4 *>(a.batch + kPagedItem0 + 4 * i);
+        const uint32_t end = min(a.rows, i + 1 < n ? a.batch[kPagedItem0 + 4 * (i + 1) + 2] : a.batch[1]);
+        for (uint32_t row = item.z + threadIdx.x; row < end; row += kThreads) {
+            const uint32_t r = row - item.z, place = item.x + r;
+            int64_t position = -1, slot = -1;
+            if (r < item.y) {
+                position = item.x + (trees ? tree_depth(a.tree[uint64_t(row) * kTreeStride]) : r);
+                slot = (int64_t(a.batch[item.w + (place >> a.page_shift)]) << a.page_shift) + (place & ((1u << a.page_shift) - 1));
+            }
+            if (a.positions) a.positions[row] = position;
+            if (a.slots) a.slots[row] = slot;
         }
-        if (a.positions) a.positions[row] = position;
-        if (a.slots) a.slots[row] = slot;
     }
 }
 

@@ -51,3 +51,40 @@ def test_captured_prompts_of_more_rows_than_trees_may_have(prompt, kv_heads, hea
         for row in (0, 60, prompt // 2, prompt - 5):  # (some rows of the prompt: all of them in 64 bits take minutes)
             mine = slice(1 + row, 1 + row + 5)
             check_attention(cache, 0, [(40, 0), (100 + row, 5)], q[mine], out[mine], tensors)
+
+
+# A graph looks at all sequences of the batch that is there when it runs, also where it was captured over one without those that have no rows: once trees
+# are taken, and of a batch that the device makes, these count too.
+@pytest.mark.parametrize("later", ["trees are taken", "from the device"])
+@pytest.mark.parametrize("rows,heads", [(1, 4), (20, 8), (300, 4)])
+def test_graphs_captured_over_a_batch_that_left_sequences_out(rows, heads, later):
+    new = [rows, 0, rows, 0, rows]
+    items = list(zip([20, 9, 33, 0, 70], new))
+    cache = PC.Cache(pkg(), [p + r for p, r in items], kv_heads=2, d=64, page_rows=16, seed=rows)
+    q = cache.normal(3 * rows, heads, 64).half()
+    qd = q.cuda()
+    out = torch.zeros_like(qd)
+    positions, slots = (torch.zeros(3 * rows, dtype=torch.int64, device="cuda") for _ in range(2))
+
+    def forward():
+        cache.paged.attention_device(0, view(qd), view(out))
+        cache.paged.batch_rows_device(positions.data_ptr(), slots.data_ptr())
+
+    cache.paged.set_batch(items, cache.tables)
+    forward()
+    graph = captured(cache.paged, forward)
+    if later == "trees are taken":
+        cache.paged.enable_trees(3 * rows)
+        cache.paged.set_batch(items, cache.tables)
+    else:
+        width = max(len(t) for t in cache.tables)
+        tables = pkg().PageTables.of(i32([t + [0] * (width - len(t)) for t in cache.tables]), i32([len(t) for t in cache.tables]))
+        held = i32([p for p, _ in items])
+        cache.paged.set_batch_device(tables, held.data_ptr(), new, 100)
+    for _ in range(3):
+        out.fill_(7.0), positions.fill_(-7), slots.fill_(-7)
+        graph.replay()
+        torch.cuda.synchronize()
+        check_attention(cache, 0, items, q, out, "f16")
+        assert positions.tolist() == [p + r for p, n in items for r in range(n)]
+        assert slots.tolist() == [cache.tables[s][x // 16] * 16 + x % 16 for s, (p, n) in enumerate(items) for x in range(p, p + n)]
