@@ -866,7 +866,8 @@ typedef struct itak_page_tables {
     uint32_t reserved;   /* 0 */
 } itak_page_tables;
 
-/* Makes a paged cache one that takes trees, of up to `most_rows` rows a batch (below 2^24; 52 bytes of device memory each). Once; not while its
+/* Makes a paged cache one that takes trees, of up to `most_rows` rows a batch (below 2^24; 52 bytes of device memory each, and for partial sums
+   (512 + num_kv_heads) * 256 * (4 D + 8) bytes, D = head_dim rounded up to 64, 128 or 256: 69 MB of 4 heads of 128). Once; not while its
    stream is being captured. From then on sequences without rows count among a batch's, and attention that is captured is right for batches with
    trees and without; what was captured before takes every row for one that sees all before it. */
 itak_status itak_paged_enable_trees(itak_paged *paged, uint64_t most_rows);

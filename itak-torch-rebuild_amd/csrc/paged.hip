@@ -49,13 +49,13 @@ void itak::send_words(uint32_t *dst, uint32_t at0, const uint32_t *w0, uint32_t 
 
 namespace {
 
-itak_status grow(itak_paged *p, void **buffer, uint64_t *have, uint64_t need, const char *what) {
+itak_status grow(itak_paged *p, void **buffer, uint64_t *have, uint64_t need, const char *what, bool exactly = false) {
     if (need <= *have) return ITAK_OK;
     if (capturing(p->stream))
         return set_error(p->err, ITAK_CAPACITY_EXCEEDED, what, need, *have, 0, 0,
                          "%s: the call needs %llu bytes and the stream is being captured; make the call once uncaptured first", what,
                          ULL(need));
-    const uint64_t want = std::max<uint64_t>(need + need / 2, 1u << 20);
+    const uint64_t want = exactly ? need : std::max<uint64_t>(need + need / 2, 1u << 20);
     p->buffers.reserve(p->buffers.size() + 1);
     void *at = nullptr;
     HIP_TRY(p, hipMalloc(&at, want), what);
@@ -299,11 +299,14 @@ struct AttnPlan {
     bool has_many = false;
 };
 
+// Vectors' places in the partials of the kernel of trees: as many as any call of it takes, which one has from itak_paged_enable_trees on. (A captured one may be
+// planned for other lengths than the calls before it.)
+uint64_t trees_places(const PagedGeom &g) { return (uint64_t(kPagedTreesGroups) + g.kv_heads) * 256; }
+
 // The partials of all launches lie in one place: they run one after the other.
 itak_status workspace(itak_paged *p, AttnPlan &plan, uint32_t dp) {
-    // (Of the kernel of trees as much as any call of it needs: one that is captured may be planned for other lengths.)
-    auto slots = [](const PagedAttn &a) { return a.apart ? uint64_t(kPagedTreesGroups + a.g.kv_heads) : a.parts ? (a.parts > 1 ? uint64_t(a.units) * a.parts : 0) : uint64_t(a.groups) + a.units; };
-    auto vectors = [&](const PagedAttn &a) { return slots(a) * (a.apart ? 256 : a.tile); };
+    auto slots = [](const PagedAttn &a) { return a.parts ? (a.parts > 1 ? uint64_t(a.units) * a.parts : 0) : uint64_t(a.groups) + a.units; };
+    auto vectors = [&](const PagedAttn &a) { return a.apart ? trees_places(a.g) : slots(a) * a.tile; };
     auto sums = [&](const PagedAttn &a) { return vectors(a) * dp * sizeof(float); };
     uint64_t need = 0;
     for (const PagedAttn *a : {&plan.few, &plan.trees, &plan.many}) need = std::max(need, sums(*a) + vectors(*a) * sizeof(float2));
@@ -335,18 +338,9 @@ uint32_t chunk_parts(uint32_t units, uint64_t work, uint32_t places) {
 
 // q is as it attends: turned where it has to be.
 itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, const itak_rows &out, float scale, float softcap,
-                           uint64_t window, AttnPlan &plan, bool for_capture = false) {
-    const bool captures = capturing(p->stream);
-    // A call over a batch without trees has the memory that it would take captured, where it has to be right for trees as well: once a batch.
-    if (p->tree_dev && !p->batch.trees && !captures && !for_capture) {
-        const uint64_t key = q.heads * 4ull + q.elem + 1;
-        if (uint64_t &sized = p->batch.sized[window ? 1 : 0]; sized != key) {
-            AttnPlan other;
-            const itak_status st = plan_attention(p, layer, q, out, scale, softcap, window, other, true);
-            if (st != ITAK_OK) return st;
-            sized = key;
-        }
-    }
+                           uint64_t window, AttnPlan &plan) {
+    // (A call that is being captured is replayed over other batches.)
+    const bool captured = capturing(p->stream);
     const uint32_t d = uint32_t(p->cfg.head_dim);
     const uint32_t group = uint32_t(q.heads / p->cfg.num_kv_heads);
     PagedAttn &a = plan.few;
@@ -360,8 +354,6 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
     a.group = group;
     a.group_magic = group > 1 ? uint32_t((1ull << 32) / group + ((1ull << 32) % group != 0)) : 0;
     if (uint64_t(a.rows) * group >= (1ull << 26)) return size_overflow(p->err, "query vectors of the batch");
-    // (A call that is being captured is replayed over other batches.)
-    const bool captured = captures || for_capture;
     // A handle that takes trees captures launches that find out whether the batch has them.
     if (p->batch.trees || (captured && p->tree_dev)) a.tree = p->tree_dev;
     const bool known = !captured && !p->batch.on_device;
@@ -445,7 +437,7 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
     // handle that takes trees and of a batch that the device makes.)
     if (captured)
         for (PagedAttn *b : {&plan.few, &plan.trees, &plan.many}) b->items = p->cfg.max_sequences;
-    if (st == ITAK_OK && captures) {
+    if (st == ITAK_OK && captured) {
         itak_paged::Captured &c = p->captured[a.window ? 1 : 0];
         c.units = std::max<uint64_t>({c.units, plan.few.units, plan.trees.units, plan.many.units});
         c.window = std::max(c.window, a.window);
@@ -467,6 +459,14 @@ bool itak::paged_replays_hold(const itak_paged *p, const PagedBatch &batch) {
         if (c.least_window && batch.tree_most > c.least_window) return false;
     }
     return true;
+}
+
+itak_status itak::paged_reserve_trees(itak_paged *p) {
+    void *ws = p->ws;
+    const uint64_t bytes = trees_places(p->g) * (paged_padded(p->g.head_dim) * sizeof(float) + sizeof(float2));
+    const itak_status st = grow(p, &ws, &p->ws_bytes, bytes, "allocate the partials of trees", true);
+    p->ws = static_cast<float *>(ws);
+    return st;
 }
 
 namespace {
@@ -579,7 +579,7 @@ itak_status set_batch(itak_paged *p, const itak_paged_item *items, uint32_t coun
     PagedBatch &next = p->next;
     const PagedRefusal r = make_paged_batch(p->limits, items, count, pages, page_ids, p->marks, p->stamp, next, p->tree_dev != nullptr);
     if (r.code != ITAK_OK) return set_error(p->err, r.code, r.what, r.a, r.b, 0, 0, "%s", r.text.c_str());
-    next.trees = parents != nullptr, next.on_device = false, next.tree_most = 0, next.sized[0] = next.sized[1] = 0;
+    next.trees = parents != nullptr, next.on_device = false, next.tree_most = 0;
     next.cuts[0] = next.cuts[1] = {};
     if (parents) {
         const itak_status st = check_trees(p, items, count, parents, next.rows, next.tree_most);

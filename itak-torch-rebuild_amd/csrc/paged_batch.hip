@@ -458,6 +458,11 @@ itak_status itak_paged_enable_trees(itak_paged *paged, uint64_t most_rows) {
     if (capturing(paged->stream)) return invalid_argument(paged->err, "trees are enabled while the stream is being captured");
     const DeviceScope scope(paged->cfg.device);
     HIP_TRY(paged, scope.status(), "set the device");
+    try {
+        if (const itak_status st = paged_reserve_trees(paged); st != ITAK_OK) return st;
+    } catch (const std::bad_alloc &) {
+        return invalid_argument(paged->err, "out of host memory");
+    }
     const uint64_t words = most_rows * (kTreeStride + 1);
     void *at = nullptr;
     HIP_TRY(paged, hipMalloc(&at, words * sizeof(uint32_t)), "allocate the records of trees");
@@ -535,7 +540,7 @@ itak_status itak_paged_set_batch_device(itak_paged *paged, const itak_page_table
         next.head.assign(kPagedItem0, 0);
         next.ids.clear();
         next.items = n, next.rows = uint32_t(all), next.most_rows = most;
-        next.trees = parents_dev != nullptr, next.tree_most = tree_most, next.on_device = true, next.idle_kept = true, next.sized[0] = next.sized[1] = 0;
+        next.trees = parents_dev != nullptr, next.tree_most = tree_most, next.on_device = true, next.idle_kept = true;
         next.cuts[0] = next.cuts[1] = {};
         uint32_t row0 = 0;
         paged->first_rows.resize(n);

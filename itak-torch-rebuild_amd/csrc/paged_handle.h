@@ -62,6 +62,8 @@ constexpr uint32_t kFewWords = 112, kManyWords = 960;
 void send_words(uint32_t *dst, uint32_t at0, const uint32_t *w0, uint32_t n0, uint32_t at1, const uint32_t *w1, uint32_t n1,
                 hipStream_t stream);
 bool paged_replays_hold(const itak_paged *p, const PagedBatch &batch);
+// The memory that attention over trees may need, captured or not.
+itak_status paged_reserve_trees(itak_paged *p);
 // paged_batch.hip: a batch of trees, of few enough words for one launch, and the records of one whose items and parents the device has.
 bool send_tree_batch(uint32_t *batch, uint32_t *tree, const std::vector<uint32_t> &head, uint32_t ids_at, const uint32_t *ids, uint32_t id_count,
                      const int32_t *parents, uint32_t rows, uint32_t items, hipStream_t stream);

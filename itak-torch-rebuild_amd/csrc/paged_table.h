@@ -40,7 +40,6 @@ struct PagedBatch {
     uint32_t most_rows = 0;      // of one
     bool trees = false;          // its rows have records
     uint32_t tree_most = 0;      // rows of its largest tree
-    uint64_t sized[2] = {};      // what attention over it, without a window and with one, has been given a captured call's memory for
     // How attention's launch for trees is cut over it, without a window and with one; `key`: what that was found for.
     struct Cut {
         uint64_t key = 0;

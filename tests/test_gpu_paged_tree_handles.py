@@ -88,3 +88,30 @@ def test_graphs_captured_over_a_batch_that_left_sequences_out(rows, heads, later
         check_attention(cache, 0, items, q, out, "f16")
         assert positions.tolist() == [p + r for p, n in items for r in range(n)]
         assert slots.tolist() == [cache.tables[s][x // 16] * 16 + x % 16 for s, (p, n) in enumerate(items) for x in range(p, p + n)]
+
+
+def test_a_plain_call_takes_the_memory_that_it_needs_and_a_graph_finds_its_own():
+    # What graphs of trees may need lies there from enable_trees on. (A handle that takes none makes the same call first, so that its kernels are loaded; its
+    # own partials are below 32 MiB.)
+    P, items = pkg(), [(100, 600)]
+    q = torch.randn(600, 8, 128, generator=torch.Generator().manual_seed(1)).half()
+    qd = q.cuda()
+    out = torch.zeros_like(qd)
+    free = lambda: (torch.cuda.synchronize(), torch.cuda.mem_get_info()[0])[1]  # noqa: E731
+    for trees in (False, True):
+        cache = PC.Cache(P, [700], kv_heads=2, d=128, page_rows=64)
+        if trees:
+            cache.paged.enable_trees(8)
+        cache.paged.set_batch(items, cache.tables)
+        before = free()
+        cache.paged.attention_device(0, view(qd), view(out))
+        took = before - free()
+    assert took < 32 << 20, took
+    graph = captured(cache.paged, lambda: cache.paged.attention_device(0, view(qd), view(out)))
+    assert before - free() < (32 << 20) + (64 << 20)  # (the graph's kernels)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_attention(cache, 0, [(100, 5)], q[:5], out[:5], "f16")
+        check_attention(cache, 0, [(695, 5)], q[-5:], out[-5:], "f16")
