@@ -123,6 +123,7 @@ itak_status rewind_range(ErrorState &e, uint64_t layer, uint64_t base, uint64_t 
                      ULL(target), ULL(layer), ULL(base), ULL(appended));
 }
 itak_status hip_error(ErrorState &e, hipError_t code, const char *doing) {
+    (void)hipGetLastError();  // (told here: not to be found by the next call, or by the program's own)
     return set_error(e, ITAK_HIP_ERROR, doing, uint64_t(code), 0, 0, 0, "%s: HIP error %d (%s)",
                      doing, int(code), hipGetErrorString(code));
 }

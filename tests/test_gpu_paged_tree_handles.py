@@ -1,10 +1,10 @@
 """Handles that take trees beside what else a program does with them: plain prompts in graphs that hold more rows than trees may have, sequences
-without rows in graphs from before, what memory calls take and when, and windows that graphs hold trees to."""
+without rows in graphs from before, what memory calls take and when, and calls that are refused."""
 import pytest
 import torch
 
 import paged_cases as PC
-from helpers import pkg
+from helpers import pkg, refusal
 from test_gpu_paged import check_attention
 from test_gpu_paged_trees import view
 
@@ -115,3 +115,24 @@ def test_a_plain_call_takes_the_memory_that_it_needs_and_a_graph_finds_its_own()
         torch.cuda.synchronize()
         check_attention(cache, 0, [(100, 5)], q[:5], out[:5], "f16")
         check_attention(cache, 0, [(695, 5)], q[-5:], out[-5:], "f16")
+
+
+# What a call was refused for it says itself: the next one, of the handle or of the program's own, does not.
+def test_a_call_refused_for_memory_leaves_the_next_alone():
+    P, heads, kv_heads, d, rows = pkg(), 64000, 1000, 8, 1 << 19
+    cache = PC.Cache(P, [40], kv_heads=kv_heads, d=d, page_rows=16, seed=2)
+    rotation = P.Rotation(d)
+    tables = P.PageTables.of(i32([cache.tables[0]]), i32([len(cache.tables[0])]))
+    nowhere, held = i32([-1]), i32([30])
+    x = torch.zeros(8, dtype=torch.float32, device="cuda")
+    cache.paged.set_batch_device(tables, nowhere.data_ptr(), [rows], 30)
+    # (1 TB of turned queries; nothing is launched, so nothing lies behind the pointers.)
+    q, out = P.Rows(x.data_ptr(), "f32", heads), P.Rows(x.data_ptr() + 16, "f32", heads)
+    assert refusal(lambda: cache.paged.attention_device(0, q, out, rotation=rotation)) == "HipError"
+    q = cache.normal(3, kv_heads, d).half()
+    qd = q.cuda()
+    out = torch.zeros_like(qd)
+    cache.paged.set_batch_device(tables, held.data_ptr(), [3], 30)
+    cache.paged.attention_device(0, view(qd), view(out))
+    torch.cuda.synchronize()
+    check_attention(cache, 0, [(30, 3)], q, out, "f16")
