@@ -873,7 +873,8 @@ typedef struct itak_page_tables {
 itak_status itak_paged_enable_trees(itak_paged *paged, uint64_t most_rows);
 /* itak_paged_set_batch with the parents of all new rows in order: [sum rows] in host memory, each -1 or the number of a row before it among its
    own item's. An item whose every row continues the one before is no tree but a chain, of any length; a tree has up to 256 rows. A
-   window of an attention or step over the batch is 0 or at least as long as its largest tree has rows. */
+   window of an attention or step over the batch is 0 or at least as long as its largest tree has rows: a larger tree is refused as ITAK_UNSUPPORTED
+   by that call, and by this one where such a call has been captured since the cache takes trees (its graph may be replayed at any time, also after eager calls). */
 itak_status itak_paged_set_batch_tree(itak_paged *paged, const itak_paged_item *items, uint32_t count, const uint32_t *pages,
                                       uint64_t page_ids, const int32_t *parents);
 /* Page tables to lengths: sequence i gets or gives back pages until it has those of lengths_dev[i] + rows[i] positions (rows: host memory,
@@ -887,8 +888,8 @@ itak_status itak_paged_fit_tables_device(itak_paged *paged, const itak_page_tabl
 /* The batch from positions and tables on the device: sequence i is an item of rows[i] new rows (host memory, [sequences]) behind positions_dev[i],
    parents_dev [sum rows] as for itak_paged_set_batch_tree or NULL. A sequence whose position is below 0 or beyond most_positions, whose table
    has too few pages or names one beyond the pages, or whose parents are no tree's is left out: nothing is written for its rows, in the
-   pages or in outputs. status_dev: [sequences] ITAK_TABLE_*, or NULL. What the host refuses and plans is for most_positions; a window has to be as long
-   as the most rows of an item of up to 256, where there are parents. Pages that take new rows and are named twice are not looked for: such rows are
+   pages or in outputs. status_dev: [sequences] ITAK_TABLE_*, or NULL. What the host refuses and plans is for most_positions; a window, that of a captured call
+   too, has to be as long as the most rows of an item of up to 256, where there are parents. Pages that take new rows and are named twice are not looked for: such rows are
    lost. It may be captured, with the rows of then; a batch that a replay sets is not the one that eager calls after it know, so that
    one is set for those again. */
 itak_status itak_paged_set_batch_device(itak_paged *paged, const itak_page_tables *tables, const int32_t *positions_dev, const uint32_t *rows,

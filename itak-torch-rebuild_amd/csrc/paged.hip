@@ -449,16 +449,18 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
 }  // namespace
 
 // Whether the captured calls' replays over a batch (of as many units) can count their blocks, and whether its trees fit their windows.
-bool itak::paged_replays_hold(const itak_paged *p, const PagedBatch &batch) {
+itak_status itak::paged_replays_hold(const itak_paged *p, const PagedBatch &batch) {
     const std::vector<uint32_t> &head = batch.head;
     for (const itak_paged::Captured &c : p->captured) {
         for (size_t at = kPagedItem0; c.units && at < head.size(); at += 4) {
             const uint32_t blocks = (head[at] + head[at + 1] + 31) / 32 - paged_first_block(head[at], c.window);
-            if (c.units * blocks >= kMostBlocks) return false;
+            if (c.units * blocks >= kMostBlocks) return size_overflow(p->err, "a captured attention over the batch");
         }
-        if (c.least_window && batch.tree_most > c.least_window) return false;
+        if (c.least_window && batch.tree_most > c.least_window)
+            return set_error(p->err, ITAK_UNSUPPORTED, "window", batch.tree_most, c.least_window, 0, 0,
+                             "unsupported: a window of %u over a tree of %u rows (an attention that was captured has it)", c.least_window, batch.tree_most);
     }
-    return true;
+    return ITAK_OK;
 }
 
 itak_status itak::paged_reserve_trees(itak_paged *p) {
@@ -586,7 +588,7 @@ itak_status set_batch(itak_paged *p, const itak_paged_item *items, uint32_t coun
         if (st != ITAK_OK) return st;
         next.head[2] = 1;
     }
-    if (!paged_replays_hold(p, next)) return size_overflow(p->err, "a captured attention over the batch");
+    if (const itak_status st = paged_replays_hold(p, next); st != ITAK_OK) return st;
     const DeviceScope scope(p->cfg.device);
     HIP_TRY(p, scope.status(), "set the device");
     // The items go up every time, page ids where they are not what the device has: of a sequence that grows, one every

@@ -553,7 +553,7 @@ itak_status itak_paged_set_batch_device(itak_paged *paged, const itak_page_table
     } catch (const std::bad_alloc &) {
         return invalid_argument(paged->err, "out of host memory");
     }
-    if (!paged_replays_hold(paged, paged->next)) return size_overflow(paged->err, "a captured attention over the batch");
+    if (st = paged_replays_hold(paged, paged->next); st != ITAK_OK) return st;
     DeviceBatchArgs a{};
     if (n > kRowsInline) {
         place_words(paged, rows, n, 0);

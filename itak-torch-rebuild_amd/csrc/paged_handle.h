@@ -57,11 +57,11 @@ inline bool capturing(hipStream_t stream) {
     return hipStreamIsCapturing(stream, &status) != hipSuccess || status != hipStreamCaptureStatusNone;
 }
 
-// paged.hip: words to dst + at0 and the n1 behind them to dst + at1, and whether captured attention holds over a batch of these words.
+// paged.hip: words to dst + at0 and the n1 behind them to dst + at1, and what a batch of these words is refused for where attention was captured.
 constexpr uint32_t kFewWords = 112, kManyWords = 960;
 void send_words(uint32_t *dst, uint32_t at0, const uint32_t *w0, uint32_t n0, uint32_t at1, const uint32_t *w1, uint32_t n1,
                 hipStream_t stream);
-bool paged_replays_hold(const itak_paged *p, const PagedBatch &batch);
+itak_status paged_replays_hold(const itak_paged *p, const PagedBatch &batch);
 // The memory that attention over trees may need, captured or not.
 itak_status paged_reserve_trees(itak_paged *p);
 // paged_batch.hip: a batch of trees, of few enough words for one launch, and the records of one whose items and parents the device has.

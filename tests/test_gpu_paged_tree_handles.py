@@ -4,9 +4,10 @@ import pytest
 import torch
 
 import paged_cases as PC
+import tree_cases as TC
 from helpers import pkg, refusal
 from test_gpu_paged import check_attention
-from test_gpu_paged_trees import view
+from test_gpu_paged_trees import cache_of, view
 
 pytestmark = pytest.mark.gpu
 
@@ -136,3 +137,31 @@ def test_a_call_refused_for_memory_leaves_the_next_alone():
     cache.paged.attention_device(0, view(qd), view(out))
     torch.cuda.synchronize()
     check_attention(cache, 0, [(30, 3)], q, out, "f16")
+
+
+def test_trees_that_a_graph_has_too_short_a_window_for_are_refused_by_name():
+    items = [(100, 9)]
+    cache = cache_of(items, kv_heads=1, d=64, page_rows=16)
+    q = cache.normal(9, 2, 64).half()
+    qd = q.cuda()
+    out = torch.zeros_like(qd)
+    attend = lambda: cache.paged.attention_device(0, view(qd), view(out), window=8)  # noqa: E731
+    cache.paged.set_batch(items, cache.tables)
+    attend()
+    graph = captured(cache.paged, attend)
+    wide, parents = [-1] + [0] * 8, i32([-1] + [0] * 8)
+    tables, held = pkg().PageTables.of(i32([cache.tables[0]]), i32([len(cache.tables[0])])), i32([100])
+    for call in (lambda: cache.paged.set_batch(items, cache.tables, TC.flat([wide])),
+                 lambda: cache.paged.set_batch_device(tables, held.data_ptr(), [9], 100, parents.data_ptr())):
+        try:
+            call()
+            said = None
+        except pkg().AttentionError as e:
+            said = e.variant, e.message
+        assert said and said[0] == "Unsupported" and "a window of 8" in said[1] and "a tree of 9 rows" in said[1] and "captured" in said[1]
+        out.zero_()
+        graph.replay()  # (over the batch before)
+        torch.cuda.synchronize()
+        check_attention(cache, 0, items, q, out, "f16", window=8)
+    cache.paged.set_batch(items, cache.tables, TC.flat([TC.chain(9)]))
+    cache.paged.set_batch([(100, 8)], cache.tables, TC.flat([wide[:8]]))
