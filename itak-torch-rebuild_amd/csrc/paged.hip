@@ -432,6 +432,15 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
         if (st != ITAK_OK) return st;
         plan.merge_few = !known || !whole;
     }
+    if (const auto &c = p->captured_batch; captured && c.rows) {
+        // (Of batches that graphs set the same as of those that are set from now on: paged_replays_hold.)
+        const uint64_t units = std::max({plan.few.units, plan.trees.units, plan.many.units});
+        if (units * ((c.position + c.rows + 31) / 32 - paged_first_block(c.position, a.window)) >= kMostBlocks)
+            return size_overflow(p->err, "attention over a captured batch");
+        if (a.window && a.window < c.tree_most)
+            return set_error(p->err, ITAK_UNSUPPORTED, "window", c.tree_most, a.window, 0, 0,
+                             "unsupported: a window of %u over a tree of %u rows (of a batch that was captured)", a.window, c.tree_most);
+    }
     const itak_status st = workspace(p, plan, dp);
     // (A graph looks at all items of the batch that is there when it runs. Sequences without rows are left out of one set here, and count among those of a
     // handle that takes trees and of a batch that the device makes.)

@@ -571,7 +571,11 @@ itak_status itak_paged_set_batch_device(itak_paged *paged, const itak_page_table
     a.ids_at = paged->g.ids_at, a.ids_room = paged->cfg.max_table_pages;
     // (The ids that the device has are the tables' from now on, and of a graph's replays whenever they run.)
     paged->ids_known = false;
-    if (capturing(paged->stream)) paged->ids_never_known = true;
+    if (capturing(paged->stream)) {
+        paged->ids_never_known = true;
+        auto &c = paged->captured_batch;
+        c.position = std::max(c.position, uint32_t(most_positions)), c.rows = std::max(c.rows, most), c.tree_most = std::max(c.tree_most, tree_most);
+    }
     const uint32_t *const first = paged->first_rows.data();
     if (n <= kRowsFew)
         launch_device_batch<kRowsFew>(a, rows, first, n, paged->stream);

@@ -33,6 +33,10 @@ struct itak_paged {
         uint64_t units;
         uint32_t window, least_window;
     } captured[2] = {};
+    // What batches that graphs set may hold at most: positions, new rows of an item, rows of a tree.
+    struct {
+        uint32_t position, rows, tree_most;
+    } captured_batch = {};
     // Of a handle that takes trees: a record for each of up to tree_rows rows (paged_tree.h), then those rows' parents on their way there.
     uint32_t *tree_dev = nullptr;
     uint64_t tree_rows = 0;

@@ -165,3 +165,56 @@ def test_trees_that_a_graph_has_too_short_a_window_for_are_refused_by_name():
         check_attention(cache, 0, items, q, out, "f16", window=8)
     cache.paged.set_batch(items, cache.tables, TC.flat([TC.chain(9)]))
     cache.paged.set_batch([(100, 8)], cache.tables, TC.flat([wide[:8]]))
+
+
+# A graph may set a batch that the host does not see: attention that is captured afterwards is refused what it could not do over it.
+def test_attention_captured_behind_a_graph_that_sets_larger_trees():
+    items, star = [(100, 9)], [-1] + [0] * 8
+    cache = cache_of(items, kv_heads=1, d=64, page_rows=16)
+    q = cache.normal(9, 2, 64).half()
+    qd = q.cuda()
+    out = torch.zeros_like(qd)
+    tables, held, parents = pkg().PageTables.of(i32([cache.tables[0]]), i32([len(cache.tables[0])])), i32([100]), i32(star)
+    sets = captured(cache.paged, lambda: cache.paged.set_batch_device(tables, held.data_ptr(), [9], 100, parents.data_ptr()))
+    cache.paged.set_batch(items, cache.tables)
+    said, graphs = [], []
+    for window in (8, 9):
+        attend = lambda: cache.paged.attention_device(0, view(qd), view(out), window=window)  # noqa: E731
+        attend()
+        graphs.append(captured(cache.paged, lambda: said.append(refusal(attend))))
+    assert said == ["Unsupported", None]
+    for _ in range(3):
+        out.zero_()
+        sets.replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        TC.check(cache, 0, items, [star], q, out, "f16", window=9)
+
+
+def test_attention_captured_behind_a_graph_that_sets_more_blocks_than_it_can_count():
+    # 32 heads' 2^25 blocks each at 2^30 positions.
+    P, heads, d, far = pkg(), 32, 8, 1 << 30
+    storage = torch.randn(1, 2, 2, heads, 1024, d, device="cuda").half()
+    paged = P.PagedKv(1, heads, d, page_rows=1024, page_count=2, max_sequences=1, max_table_pages=far // 1024 + 1,
+                      storage_ptr=storage.data_ptr(), storage_bytes=storage.numel() * 2)
+    paged.set_stream(torch.cuda.current_stream().cuda_stream)
+    q = torch.randn(1, heads, d, device="cuda").half()
+    out = torch.zeros_like(q)
+    tables, held = P.PageTables.of(i32([[1]]), i32([1])), i32([900])
+    sets = captured(paged, lambda: paged.set_batch_device(tables, held.data_ptr(), [1], far))
+    paged.set_batch([(900, 1)], [[1]])
+    said, graphs = [], []
+    for window in (0, 64):
+        attend = lambda: paged.attention_device(0, view(q), view(out), window=window)  # noqa: E731
+        attend()
+        graphs.append(captured(paged, lambda: said.append(refusal(attend))))
+    assert said == ["SizeOverflow", None]
+    torch.cuda.synchronize()
+    want = out.clone()
+    for _ in range(3):
+        out.zero_()
+        sets.replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        # (Captured the keys are cut otherwise: two outputs of up to 4 rounded to f16, and weights too.)
+        assert bool(((out - want).abs() <= 2.0 ** -7).all()) and bool(out.any())
