@@ -171,8 +171,8 @@ __global__ __launch_bounds__(kThreads) void paged_few_join_kernel(PagedAttn a) {
     constexpr uint32_t kQuads = DP / 4, kParts = 64 / kQuads, kAtOnce = 8;  // float4s of a partial, and partials that a wavefront takes at once
     paged_fetch_arguments(a);
     const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    const uint32_t heads = a.g.kv_heads * a.group, vector = blockIdx.x * (kThreads / 64) + wave;
-    const uint32_t row = vector / heads, hq = vector - row * heads;
+    // (Four rows of a head: vectors of all rows and heads would be more threads than a launch has in one dimension, 2^26 vectors on.)
+    const uint32_t row = blockIdx.x * (kThreads / 64) + wave, hq = blockIdx.y;
     PagedLine line(a);
     line.cut();
     PagedSpan span;
@@ -244,7 +244,8 @@ __global__ __launch_bounds__(kThreads) void paged_few_join_kernel(PagedAttn a) {
 
 template <int ELEM>
 void launch_few(const PagedAttn &a, hipStream_t stream) {
-    const uint32_t dp = paged_padded(a.g.head_dim), groups = uint32_t((uint64_t(a.rows) * a.g.kv_heads * a.group + 3) / 4);
+    const uint32_t dp = paged_padded(a.g.head_dim), waves = kThreads / 64;
+    const dim3 groups((a.rows + waves - 1) / waves, a.g.kv_heads * a.group);
     if (dp == 64)
         launch_kernel(paged_few_join_kernel<ELEM, 64>, groups, kThreads, 0, stream, a);
     else if (dp == 128)

@@ -218,3 +218,21 @@ def test_attention_captured_behind_a_graph_that_sets_more_blocks_than_it_can_cou
         torch.cuda.synchronize()
         # (Captured the keys are cut otherwise: two outputs of up to 4 rounded to f16, and weights too.)
         assert bool(((out - want).abs() <= 2.0 ** -7).all()) and bool(out.any())
+
+
+def test_joins_of_more_vectors_than_a_launch_has_in_one_dimension():
+    # Of 2^20 rows by 64 heads, all rows but the last are of a sequence that the device leaves out.
+    rows, heads, d = 1 << 20, 64, 8
+    cache = PC.Cache(pkg(), [16, 31], kv_heads=heads, d=d, page_rows=16, seed=4)
+    cache.paged.enable_trees(rows)
+    qd, out = torch.zeros(rows, heads, d, dtype=torch.float16, device="cuda"), torch.full((rows, heads, d), 7.0, dtype=torch.float16, device="cuda")
+    q = cache.normal(1, heads, d).half()
+    qd[-1:] = q.cuda()
+    parents = torch.arange(-1, rows - 1, dtype=torch.int32, device="cuda")
+    parents[-1] = -1
+    tables, held, status = pkg().PageTables.of(i32([[0, 0], cache.tables[1]]), i32([1, 2])), i32([-1, 30]), i32([9, 9])
+    cache.paged.set_batch_device(tables, held.data_ptr(), [rows - 1, 1], 30, parents.data_ptr(), status.data_ptr())
+    cache.paged.attention_device(0, view(qd), view(out))
+    torch.cuda.synchronize()
+    assert status.tolist() == [1, 0] and bool((out[:-1] == 7.0).all())
+    check_attention(cache, 0, [(0, 0), (30, 1)], q, out[-1:], "f16")
