@@ -890,7 +890,7 @@ itak_status itak_paged_fit_tables_device(itak_paged *paged, const itak_page_tabl
    has too few pages or names one beyond the pages, or whose parents are no tree's is left out: nothing is written for its rows, in the
    pages or in outputs. status_dev: [sequences] ITAK_TABLE_*, or NULL. What the host refuses and plans is for most_positions; a window, that of a captured call
    too, has to be as long as the most rows of an item of up to 256, where there are parents. Pages that take new rows and are named twice are not looked for: such rows are
-   lost. It may be captured, with the rows of then, and attention that is captured afterwards is refused what it could not do over such a batch; a batch that a replay sets is not the one that eager calls after it know, so that
+   lost. It may be captured, with the rows of then, and attention that is captured afterwards, in another graph, is refused what it could not do over such a batch; a batch that a replay sets is not the one that eager calls after it know, so that
    one is set for those again. */
 itak_status itak_paged_set_batch_device(itak_paged *paged, const itak_page_tables *tables, const int32_t *positions_dev, const uint32_t *rows,
                                         uint64_t most_positions, const int32_t *parents_dev, int32_t *status_dev);

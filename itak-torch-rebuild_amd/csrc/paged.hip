@@ -432,8 +432,8 @@ itak_status plan_attention(itak_paged *p, uint64_t layer, const itak_rows &q, co
         if (st != ITAK_OK) return st;
         plan.merge_few = !known || !whole;
     }
-    if (const auto &c = p->captured_batch; captured && c.rows) {
-        // (Of batches that graphs set the same as of those that are set from now on: paged_replays_hold.)
+    if (const auto &c = p->captured_batch; captured && c.rows && !(p->batch.capture && p->batch.capture == capture_of(p->stream))) {
+        // (Of batches that other graphs set the same as of those that are set from now on: paged_replays_hold.)
         const uint64_t units = std::max({plan.few.units, plan.trees.units, plan.many.units});
         if (units * ((c.position + c.rows + 31) / 32 - paged_first_block(c.position, a.window)) >= kMostBlocks)
             return size_overflow(p->err, "attention over a captured batch");
@@ -590,7 +590,7 @@ itak_status set_batch(itak_paged *p, const itak_paged_item *items, uint32_t coun
     PagedBatch &next = p->next;
     const PagedRefusal r = make_paged_batch(p->limits, items, count, pages, page_ids, p->marks, p->stamp, next, p->tree_dev != nullptr);
     if (r.code != ITAK_OK) return set_error(p->err, r.code, r.what, r.a, r.b, 0, 0, "%s", r.text.c_str());
-    next.trees = parents != nullptr, next.on_device = false, next.tree_most = 0;
+    next.trees = parents != nullptr, next.on_device = false, next.tree_most = 0, next.capture = 0;
     next.cuts[0] = next.cuts[1] = {};
     if (parents) {
         const itak_status st = check_trees(p, items, count, parents, next.rows, next.tree_most);

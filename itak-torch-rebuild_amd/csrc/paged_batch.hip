@@ -542,6 +542,7 @@ itak_status itak_paged_set_batch_device(itak_paged *paged, const itak_page_table
         next.items = n, next.rows = uint32_t(all), next.most_rows = most;
         next.trees = parents_dev != nullptr, next.tree_most = tree_most, next.on_device = true, next.idle_kept = true;
         next.cuts[0] = next.cuts[1] = {};
+        next.capture = capture_of(paged->stream);
         uint32_t row0 = 0;
         paged->first_rows.resize(n);
         for (uint32_t i = 0; i < n; row0 += rows[i], ++i) {

@@ -61,6 +61,13 @@ inline bool capturing(hipStream_t stream) {
     return hipStreamIsCapturing(stream, &status) != hipSuccess || status != hipStreamCaptureStatusNone;
 }
 
+// Which capture a stream is in: 0 of none.
+inline unsigned long long capture_of(hipStream_t stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    return hipStreamGetCaptureInfo(stream, &status, &id) == hipSuccess && status == hipStreamCaptureStatusActive ? id : 0;
+}
+
 // paged.hip: words to dst + at0 and the n1 behind them to dst + at1, and what a batch of these words is refused for where attention was captured.
 constexpr uint32_t kFewWords = 112, kManyWords = 960;
 void send_words(uint32_t *dst, uint32_t at0, const uint32_t *w0, uint32_t n0, uint32_t at1, const uint32_t *w1, uint32_t n1,

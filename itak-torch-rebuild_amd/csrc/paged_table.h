@@ -47,6 +47,7 @@ struct PagedBatch {
         uint32_t tile = 0, share = 0;
     } cuts[2];
     bool idle_kept = false;      // an item's number is its sequence's
+    uint64_t capture = 0;        // the capture that it was set in
     bool on_device = false;      // lengths and tables are the device's: positions in `head` are the most they may be, and there are no ids
 };
 

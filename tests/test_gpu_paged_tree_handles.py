@@ -236,3 +236,28 @@ def test_joins_of_more_vectors_than_a_launch_has_in_one_dimension():
     torch.cuda.synchronize()
     assert status.tolist() == [1, 0] and bool((out[:-1] == 7.0).all())
     check_attention(cache, 0, [(0, 0), (30, 1)], q, out[-1:], "f16")
+
+
+def test_a_graph_that_sets_its_own_batch_goes_by_it_alone():
+    # Trees of nine rows in a graph without windows, and of eight in another with one of eight.
+    star = [-1] + [0] * 8
+    cache = cache_of([(100, 9)], kv_heads=1, d=64, page_rows=16)
+    q = cache.normal(9, 2, 64).half()
+    qd = q.cuda()
+    outs = [torch.zeros_like(qd) for _ in range(2)]
+    tables, held, parents = pkg().PageTables.of(i32([cache.tables[0]]), i32([len(cache.tables[0])])), i32([100]), i32(star)
+
+    def forward(rows, window):
+        cache.paged.set_batch_device(tables, held.data_ptr(), [rows], 100, parents.data_ptr())
+        cache.paged.attention_device(0, view(qd[:rows]), view(outs[rows - 8][:rows]), window=window)
+
+    forms = (9, 0), (8, 8)
+    for form in forms:
+        forward(*form)
+    graphs = [captured(cache.paged, lambda: forward(*form)) for form in forms]
+    for _ in range(3):
+        for graph, (rows, window) in zip(graphs, forms):
+            outs[rows - 8].zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            TC.check(cache, 0, [(100, rows)], [star[:rows]], q[:rows], outs[rows - 8][:rows], "f16", window=window)
