@@ -534,6 +534,7 @@ itak_status itak_paged_set_batch_device(itak_paged *paged, const itak_page_table
                          "a batch of trees of %llu rows, the paged cache takes %llu", ULL(all), ULL(paged->tree_rows));
     const DeviceScope scope(paged->cfg.device);
     HIP_TRY(paged, scope.status(), "set the device");
+    const bool captured = capturing(paged->stream);
     try {
         // What the host knows of the batch: every sequence at the most positions it may have.
         PagedBatch &next = paged->next;
@@ -542,7 +543,7 @@ itak_status itak_paged_set_batch_device(itak_paged *paged, const itak_page_table
         next.items = n, next.rows = uint32_t(all), next.most_rows = most;
         next.trees = parents_dev != nullptr, next.tree_most = tree_most, next.on_device = true, next.idle_kept = true;
         next.cuts[0] = next.cuts[1] = {};
-        next.capture = capture_of(paged->stream);
+        next.capture = captured ? capture_of(paged->stream) : 0;
         uint32_t row0 = 0;
         paged->first_rows.resize(n);
         for (uint32_t i = 0; i < n; row0 += rows[i], ++i) {
@@ -572,7 +573,7 @@ itak_status itak_paged_set_batch_device(itak_paged *paged, const itak_page_table
     a.ids_at = paged->g.ids_at, a.ids_room = paged->cfg.max_table_pages;
     // (The ids that the device has are the tables' from now on, and of a graph's replays whenever they run.)
     paged->ids_known = false;
-    if (capturing(paged->stream)) {
+    if (captured) {
         paged->ids_never_known = true;
         auto &c = paged->captured_batch;
         c.position = std::max(c.position, uint32_t(most_positions)), c.rows = std::max(c.rows, most), c.tree_most = std::max(c.tree_most, tree_most);
